@@ -97,7 +97,7 @@ def draw(rng):
     dtype = rng.choice(["f32", "bf16", "f16"])
     if op == "bias":
         tokens, degree, heads = _log_int(rng, 1000, 1000000), _log_int(rng, 4, 64), _log_int(rng, 1, 16)
-        while tokens * degree * (8 + 4 * heads) > 400_000_000:
+        while tokens * degree * (8 + 4 * heads) > 350_000_000:
             tokens = tokens * 2 // 3
         buckets = 2 * _log_int(rng, 4, 64)
         return _bias(None, tokens, degree, heads, buckets, buckets * _log_int(rng, 2, 64), dtype,
@@ -112,7 +112,7 @@ def draw(rng):
     group, widths = rng.choice([1, 1, 2, 3, 4, 7, 8, 16]), (width(), width())
     if rng.random() < 0.7:
         widths = (widths[0], widths[0])
-    while sequences * length * heads * (widths[0] + widths[1]) > 400_000_000:
+    while sequences * length * heads * (widths[0] + widths[1]) > 150_000_000:
         if length > sequences:
             length = length * 2 // 3
         else:
