@@ -24,8 +24,12 @@ from autosage_amd import (
     __version__,
     calibrate_full,
     csr_attention_forward,
+    csr_position_bias,
     load_native,
     native_available,
+    paged_attention,
+    paged_cache_read,
+    paged_cache_write,
     sddmm_csr_auto,
     spmm_csr,
     spmm_csr_auto,
@@ -53,8 +57,12 @@ __all__ = [
     "__version__",
     "calibrate_full",
     "csr_attention_forward",
+    "csr_position_bias",
     "load_native",
     "native_available",
+    "paged_attention",
+    "paged_cache_read",
+    "paged_cache_write",
     "sddmm_csr_auto",
     "spmm_csr",
     "spmm_csr_auto",

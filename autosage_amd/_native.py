@@ -30,7 +30,7 @@ from . import _env
 from ._memo import GraphMemo
 
 LIBRARY_NAME = "libautosage_hip.so"
-ABI_VERSION = 11
+ABI_VERSION = 12
 HUB_EXACT = 0
 HUB_SPLIT64 = 1
 # 16-bit feature types of as_spmm_csr_rounded_16 (AS_DTYPE_BF16 / AS_DTYPE_F16)
@@ -190,6 +190,25 @@ _SIGNATURES = {
         _c_int,
         [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_float, _c_ptr,
          _c_size, _c_ptr],
+    ),
+    "as_csr_position_bias": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int, _c_int, _c_ptr],
+    ),
+    "as_csr_position_bias_backward_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "as_csr_position_bias_backward": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int, _c_int, _c_ptr,
+         _c_size, _c_ptr],
+    ),
+    "as_paged_cache_write": (
+        _c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
+    "as_paged_cache_read": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
+    "as_paged_attention_workspace_bytes": (_c_size, [_c_ptr, _c_i64, _c_i64]),
+    "as_paged_attention": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, ctypes.c_float, _c_i64, _c_ptr, _c_i64, _c_ptr,
+         _c_int, _c_i64, _c_int, _c_ptr, _c_size, _c_ptr],
     ),
 }
 
@@ -1521,14 +1540,17 @@ def _register_operators() -> None:
     global _OPS_LIBRARY
     if _OPS_LIBRARY is not None:
         return
+    from . import paged, position
+
     lib = torch.library.Library("autosage", "DEF")
-    for name, (schema, impl) in _SCHEMAS.items():
+    for name, (schema, impl) in {**_SCHEMAS, **position.SCHEMAS, **paged.SCHEMAS}.items():
         lib.define(schema)
         lib.impl(name, impl, "CUDA")
     _OPS_LIBRARY = lib
     from . import _autograd
 
     _autograd.register()
+    position.register_autograd()
 
 
 def load(path: os.PathLike[str] | str) -> None:

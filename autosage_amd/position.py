@@ -1,0 +1,223 @@
+"""Learned bias of the distance between two nodes, by buckets.
+
+Attention over the edges of a CSR graph knows which keys a query sees, not how
+far they are.  ``csr_position_bias`` gives every edge and head a learned number
+for the distance between its two nodes, to be added to the edge scores in front
+of the row softmax; ``paged_attention`` adds the same numbers when the tokens of
+a sequence are answered one at a time.
+
+With ``n`` buckets for one side of the query and ``E = n // 2``, distances below
+``E`` have a bucket each and bucket ``E + j`` begins where
+``(d / E) ** (n - E)`` reaches ``(max_distance / E) ** j``; the last bucket holds
+everything farther.  The borders are found in integers, so that no logarithm's
+last bit decides a bucket.  The reference's attention has no positions.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+from typing import Optional
+
+import torch
+
+from . import _native
+from .ops import load_native, native_load_error, validate_if_requested
+
+MAX_BUCKETS = 256
+_DTYPES = {torch.float32: 0, **_native.DTYPES_16}
+
+
+@functools.lru_cache(maxsize=256)
+def bucket_borders(buckets: int, max_distance: int, bidirectional: bool = True) -> tuple[int, ...]:
+    """The smallest distance of each bucket of one side of the query (half of
+    ``buckets`` with ``bidirectional``, else all of them)."""
+    if not 2 <= buckets <= MAX_BUCKETS:
+        raise ValueError(f"the number of buckets must lie in [2, {MAX_BUCKETS}]")
+    if bidirectional and buckets % 2 != 0:
+        raise ValueError("a bidirectional bias needs an even number of buckets")
+    side = buckets // 2 if bidirectional else buckets
+    exact = side // 2
+    if not max(exact, 1) < max_distance < 2**31:
+        raise ValueError(f"max_distance must lie in ({max(exact, 1)}, 2^31)")
+    if side == 1:
+        return (0,)
+    rest = side - exact
+    borders = list(range(exact + 1))
+    for j in range(1, rest):
+        # the smallest d with d^rest >= exact^(rest - j) * max_distance^j
+        goal = exact ** (rest - j) * max_distance**j
+        low, high = borders[-1], max_distance
+        while low < high:
+            middle = (low + high) // 2
+            if middle**rest >= goal:
+                high = middle
+            else:
+                low = middle + 1
+        borders.append(low)
+    return tuple(borders)
+
+
+@functools.lru_cache(maxsize=256)
+def border_array(buckets: int, max_distance: int, bidirectional: bool):
+    """``bucket_borders`` as the C array of the native calls (host memory)."""
+    borders = bucket_borders(buckets, max_distance, bidirectional)
+    return (ctypes.c_int32 * len(borders))(*borders)
+
+
+def position_buckets(relative: torch.Tensor, buckets: int, max_distance: int, bidirectional: bool) -> torch.Tensor:
+    """The bucket of every (key position - query position)."""
+    borders = torch.tensor(bucket_borders(buckets, max_distance, bidirectional), device=relative.device)
+    distance = relative.abs() if bidirectional else (-relative).clamp_min(0)
+    found = torch.searchsorted(borders, distance, right=True) - 1
+    return found + (relative > 0).long() * (buckets // 2) if bidirectional else found
+
+
+def _check_graph(crow, col, positions, values, heads_dim: str) -> None:
+    if crow.ndim != 1 or col.ndim != 1 or crow.numel() < 1:
+        raise ValueError("crow and col must be one-dimensional")
+    if crow.dtype not in (torch.int32, torch.int64) or col.dtype not in (torch.int32, torch.int64):
+        raise TypeError("crow and col must use integer indices")
+    if values.ndim != 2 or values.size(0 if heads_dim == "grad" else 1) < 1:
+        raise ValueError("table must have shape [buckets, heads]" if heads_dim == "table"
+                         else "grad must have shape [heads, edges]")
+    if not values.is_floating_point():
+        raise TypeError(f"{heads_dim} must use a floating-point dtype")
+    if not (crow.device == col.device == values.device):
+        raise ValueError(f"crow, col, and {heads_dim} must be on the same device")
+    if col.numel() > 0 and crow.numel() < 2:
+        raise ValueError("edges without rows")
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError("positions must use integers")
+        if positions.ndim != 1 or positions.numel() != crow.numel() - 1:
+            raise ValueError("positions must contain one entry per node")
+        if positions.device != crow.device:
+            raise ValueError("positions and crow must be on the same device")
+
+
+def _long(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or (t.dtype == torch.long and t.is_contiguous()) else t.to(torch.long).contiguous()
+
+
+def csr_position_bias_impl(crow, col, positions, table, max_distance, bidirectional):
+    _check_graph(crow, col, positions, table, "table")
+    if table.dtype not in _DTYPES:
+        raise TypeError("the native position bias supports float32, bfloat16 and float16 tables")
+    buckets, heads = table.shape
+    borders = border_array(buckets, max_distance, bool(bidirectional))
+    crow, col, positions, table = _long(crow), _long(col), _long(positions), table.contiguous()
+    nnz = col.numel()
+    out = torch.empty(heads, nnz, dtype=table.dtype, device=table.device)
+    if nnz == 0:
+        return out
+    with _native._on(table.device):
+        status = _native.library().as_csr_position_bias(
+            crow.data_ptr(), col.data_ptr(), _native._ptr(positions), table.data_ptr(), out.data_ptr(),
+            crow.numel() - 1, nnz, heads, buckets, borders, int(bool(bidirectional)), _DTYPES[table.dtype],
+            _native._stream(table.device))
+    _native._raise(status, "autosage::csr_position_bias")
+    return out
+
+
+def csr_position_bias_backward_impl(crow, col, positions, grad, buckets, max_distance, bidirectional):
+    """dL/dtable [buckets, heads] from dL/dbias [heads, edges]."""
+    _check_graph(crow, col, positions, grad, "grad")
+    if grad.dtype not in _DTYPES:
+        raise TypeError("the native position bias supports float32, bfloat16 and float16 tables")
+    if grad.size(1) != col.numel():
+        raise ValueError("grad must have shape [heads, edges]")
+    borders = border_array(buckets, max_distance, bool(bidirectional))
+    crow, col, positions, grad = _long(crow), _long(col), _long(positions), grad.contiguous()
+    heads, nnz = grad.shape
+    table = torch.empty(buckets, heads, dtype=grad.dtype, device=grad.device)
+    lib = _native.library()
+    ws = _native._workspace(lib.as_csr_position_bias_backward_workspace_bytes(nnz, heads, buckets), grad.device)
+    with _native._on(grad.device):
+        status = lib.as_csr_position_bias_backward(
+            crow.data_ptr(), col.data_ptr(), _native._ptr(positions), grad.data_ptr(), table.data_ptr(),
+            crow.numel() - 1, nnz, heads, buckets, borders, int(bool(bidirectional)), _DTYPES[grad.dtype],
+            ws.data_ptr(), ws.numel(), _native._stream(grad.device))
+    _native._raise(status, "autosage::csr_position_bias (backward)")
+    return table
+
+
+SCHEMAS = {
+    "csr_position_bias": (
+        "csr_position_bias(Tensor crow, Tensor col, Tensor? positions, Tensor table, int max_distance, "
+        "bool bidirectional) -> Tensor",
+        csr_position_bias_impl,
+    ),
+    "csr_position_bias_backward": (
+        "csr_position_bias_backward(Tensor crow, Tensor col, Tensor? positions, Tensor grad, int buckets, "
+        "int max_distance, bool bidirectional) -> Tensor",
+        csr_position_bias_backward_impl,
+    ),
+}
+
+
+def _setup(ctx, inputs, output) -> None:
+    crow, col, positions, values = inputs[:4]
+    ctx.save_for_backward(crow, col, positions)
+    ctx.size = values.size(0)
+    ctx.map = (inputs[-2], inputs[-1])
+
+
+def _backward(ctx, grad):
+    crow, col, positions = ctx.saved_tensors
+    if not ctx.needs_input_grad[3]:
+        return None, None, None, None, None, None
+    grad_table = torch.ops.autosage.csr_position_bias_backward(crow, col, positions, grad, ctx.size, *ctx.map)
+    return None, None, None, grad_table, None, None
+
+
+def _backward_of_backward(ctx, grad_table):
+    # the sum over each bucket's edges is linear: its transpose is the lookup
+    crow, col, positions = ctx.saved_tensors
+    if not ctx.needs_input_grad[3]:
+        return None, None, None, None, None, None, None
+    grad = torch.ops.autosage.csr_position_bias(crow, col, positions, grad_table, *ctx.map)
+    return None, None, None, grad, None, None, None
+
+
+def register_autograd() -> None:
+    """Attaches the gradients to the registered operators."""
+    torch.library.register_autograd("autosage::csr_position_bias", _backward, setup_context=_setup)
+    torch.library.register_autograd("autosage::csr_position_bias_backward", _backward_of_backward,
+                                    setup_context=_setup)
+
+
+def _cpu_position_bias(crow, col, positions, table, max_distance, bidirectional) -> torch.Tensor:
+    crow, col = crow.long(), col.long()
+    rows = torch.repeat_interleave(torch.arange(crow.numel() - 1, device=col.device), crow[1:] - crow[:-1])
+    relative = col - rows if positions is None else positions.long()[col] - positions.long()[rows]
+    return table.t()[:, position_buckets(relative, table.size(0), max_distance, bidirectional)]
+
+
+def csr_position_bias(crow, col, table, *, max_distance: int, bidirectional: bool = True,
+                      positions=None) -> torch.Tensor:
+    """The learned bias of every edge: ``out[h, e] = table[bucket, h]`` for the
+    bucket of the position of ``col[e]`` minus that of the edge's row.
+
+    ``table`` is ``[buckets, heads]``, float32, bfloat16 or float16; the result
+    is ``[heads, edges]`` of its dtype, one row for each head's scores, with a
+    gradient for ``table`` (the sum over each bucket's edges, in a fixed order).
+    Node ids are positions unless ``positions`` (one integer per node) gives
+    them.  With ``bidirectional`` half of the buckets are for keys behind the
+    query; without it a key behind the query counts as distance 0."""
+    _check_graph(crow, col, positions, table, "table")
+    max_distance = int(max_distance)
+    bucket_borders(table.size(0), max_distance, bool(bidirectional))
+    if not table.is_cuda:
+        return _cpu_position_bias(crow, col, positions, table, max_distance, bool(bidirectional))
+    if not load_native():
+        raise RuntimeError(f"AutoSAGE CUDA extension is unavailable: {native_load_error()}")
+    crow, col, positions = _long(crow), _long(col), _long(positions)
+    validate_if_requested(crow, col)
+    args = (crow, col, positions, table, max_distance, bool(bidirectional))
+    if torch.is_grad_enabled() and table.requires_grad:
+        return torch.ops.autosage.csr_position_bias(*args)
+    return csr_position_bias_impl(*args)
+
+
+__all__ = ["bucket_borders", "csr_position_bias", "position_buckets"]

@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define AS_ABI_VERSION 11
+#define AS_ABI_VERSION 12
 
 typedef enum as_status {
   AS_OK = 0,
@@ -47,7 +47,8 @@ typedef enum as_status {
 enum {
   AS_DTYPE_F32 = 0,
   AS_DTYPE_BF16 = 1,
-  AS_DTYPE_F16 = 2
+  AS_DTYPE_F16 = 2,
+  AS_DTYPE_E4M3 = 3   /* pages of a quantised key-value cache only */
 };
 
 /* Hub-row strategy for as_spmm_csr_split_f32 (no reference counterpart; the
@@ -707,6 +708,113 @@ int as_induced_sample_fill(const int64_t* crow, const int64_t* col,
 int as_csr_validate(const int64_t* crow, const int64_t* col, int64_t n,
                     int64_t nnz, int64_t n_cols, int32_t* flags,
                     void* stream);
+
+/* ---- Learned bias of the distance between two nodes ------------------------
+ * No reference counterpart (its attention has no positions).
+ *
+ * rel = position of the key (column) - position of the query (row).  One side
+ * has `side` buckets: bucket k begins at the integer distance borders[k]
+ * (host memory; borders[0] = 0, non-descending).  both_sides != 0: buckets =
+ * 2 side, those of keys behind the query (rel > 0) after the others; else
+ * buckets = side and a key behind the query has distance 0.
+ * buckets in [1, 256].
+ *
+ *   out[h, e] = table[bucket(e), h]
+ *   grad_table[b, h] = sum of grad[h, e] over the edges e of bucket b
+ *
+ * table, grad_table [buckets, heads] and out, grad [heads, nnz] are of dtype
+ * AS_DTYPE_F32, _BF16 or _F16; positions int64[n] or NULL (node ids are
+ * positions; the graph then need not be square).  The gradient is summed in a
+ * fixed order, at most 64 numbers in fp32 and the sums of those in fp64. */
+int as_csr_position_bias(const int64_t* crow, const int64_t* col,
+                         const int64_t* positions, const void* table,
+                         void* out, int64_t n, int64_t nnz, int64_t heads,
+                         int64_t buckets, const int32_t* borders,
+                         int both_sides, int dtype, void* stream);
+size_t as_csr_position_bias_backward_workspace_bytes(int64_t nnz,
+                                                     int64_t heads,
+                                                     int64_t buckets);
+int as_csr_position_bias_backward(const int64_t* crow, const int64_t* col,
+                                  const int64_t* positions, const void* grad,
+                                  void* grad_table, int64_t n, int64_t nnz,
+                                  int64_t heads, int64_t buckets,
+                                  const int32_t* borders, int both_sides,
+                                  int dtype, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* ---- Paged key-value cache ---------------------------------------------------
+ * No reference counterpart (its attention is over whole graphs).
+ *
+ * Keys and values lie in pages of page_size tokens, [pages, heads, page_size,
+ * width] with any strides of the first three dimensions (in elements) and rows
+ * that are contiguous.  The pages of sequence b are page_idx[page_ptr[b] ..
+ * page_ptr[b + 1]) in the order of its tokens; a list may hold more pages than
+ * the sequence needs so far, and page_idx more entries than page_ptr's last.
+ * dtype AS_DTYPE_E4M3: 8-bit numbers with one exponent for each token and head
+ * ([pages, heads, page_size], any strides); a held number is code * 2^exponent.
+ * Lists, lengths and ids are checked in the kernels: nothing outside the given
+ * tensors is read or written whatever they hold. */
+typedef struct as_paged_cache {
+  void* key_pages;
+  void* value_pages;
+  int8_t* key_exponents;    /* NULL unless dtype is AS_DTYPE_E4M3 */
+  int8_t* value_exponents;
+  const int64_t* page_ptr;  /* [sequences + 1] */
+  const int64_t* page_idx;  /* [page_idx_len] */
+  int64_t page_idx_len;
+  int64_t sequences;
+  int64_t pages;            /* at least 1 */
+  int64_t page_size;        /* at least 1 */
+  int64_t heads;            /* of keys and values */
+  int64_t key_width;        /* 1 to 256 */
+  int64_t value_width;
+  int64_t key_strides[3];
+  int64_t value_strides[3];
+  int64_t key_exponent_strides[3];
+  int64_t value_exponent_strides[3];
+  int32_t dtype;
+} as_paged_cache;
+
+/* Rows of new tokens into the cache.  key [tokens, heads, key_width] and value
+ * [tokens, heads, value_width] of `dtype` (the cache's, or any where the cache
+ * is e4m3) with strides of their first two dimensions.  Tokens token_ptr[b] ..
+ * token_ptr[b + 1] are those of sequence b, from its position start[b] on;
+ * tokens behind token_ptr[sequences], and tokens without a page, leave the
+ * cache as it is.  A place that two tokens of one call are written to holds
+ * parts of either. */
+int as_paged_cache_write(const as_paged_cache* cache, const void* key,
+                         const int64_t* key_strides, const void* value,
+                         const int64_t* value_strides,
+                         const int64_t* token_ptr, const int64_t* start,
+                         int64_t tokens, int dtype, void* stream);
+
+/* The rows of tokens as they are held, contiguous, in `dtype` (the cache's, or
+ * any where the cache is e4m3; each number is rounded once).  Tokens as for
+ * as_paged_cache_write; those without a sequence or a page are zeros. */
+int as_paged_cache_read(const as_paged_cache* cache, void* key, void* value,
+                        const int64_t* token_ptr, const int64_t* start,
+                        int64_t tokens, int dtype, void* stream);
+
+/* Attention of one new token of every sequence, its last one (position
+ * lengths[b] - 1, which the cache holds), over the last `window` tokens
+ * (0: all).  query [sequences, heads * group, key_width] with strides of its
+ * first two dimensions, out [sequences, heads * group, value_width], both of
+ * `dtype` (the cache's, or any where the cache is e4m3); query head h reads key
+ * head h / group.  table: NULL or [buckets, heads * group] of `dtype`, added to
+ * the scores by the distance to the new token.  lse: NULL or fp32 [sequences,
+ * heads * group], the logarithm of the sum of the exponentials.  max_length: an
+ * upper bound of the lengths if the caller knows one, else -1 (it shapes the
+ * launch; lengths beyond it give NaN).  No token seen: zeros and -inf.  A
+ * length beyond the pages of its list, or a page id outside the cache: NaN. */
+size_t as_paged_attention_workspace_bytes(const as_paged_cache* cache,
+                                          int64_t group, int64_t max_length);
+int as_paged_attention(const as_paged_cache* cache, const void* query,
+                       const int64_t* query_strides, void* out, float* lse,
+                       const int64_t* lengths, int64_t group, float scale,
+                       int64_t window, const void* table, int64_t buckets,
+                       const int32_t* borders, int both_sides,
+                       int64_t max_length, int dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

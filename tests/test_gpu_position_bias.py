@@ -1,0 +1,187 @@
+"""The learned position bias on the GPU against the definition: every value exactly, gradients within their sums."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import autosage_amd
+from tests.gpu_common import case_graph, require_gpu, to_dev
+from tests.paged_common import plain_buckets
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    require_gpu()
+
+
+def _plain(crow, col, buckets, max_distance, bidirectional, positions):
+    rows = np.repeat(np.arange(len(crow) - 1), np.diff(crow))
+    at = np.arange(len(crow) - 1) if positions is None else positions
+    return torch.from_numpy(plain_buckets(at[col] - at[rows], buckets, max_distance, bidirectional))
+
+
+def _check(crow, col, heads, buckets, max_distance, dtype, bidirectional=True, positions=None, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    table = torch.randn(buckets, heads, generator=gen).to(dtype)
+    bucket = _plain(crow, col, buckets, max_distance, bidirectional, positions)
+    d_crow, d_col, d_positions = to_dev(crow, col, positions)
+    d_table = table.cuda().requires_grad_()
+    out = autosage_amd.csr_position_bias(d_crow, d_col, d_table, max_distance=max_distance,
+                                         bidirectional=bidirectional, positions=d_positions)
+    assert out.dtype == dtype and torch.equal(out.detach().cpu(), table.t()[:, bucket])
+    with torch.no_grad():
+        again = autosage_amd.csr_position_bias(d_crow, d_col, d_table, max_distance=max_distance,
+                                               bidirectional=bidirectional, positions=d_positions)
+    assert torch.equal(again, out)
+    grad = torch.randn(heads, len(col), generator=gen).to(dtype)
+    got, = torch.autograd.grad(out, d_table, grad.cuda())
+    want = torch.zeros(buckets, heads, dtype=torch.float64).index_add_(0, bucket, grad.double().t())
+    size = torch.zeros_like(want).index_add_(0, bucket, grad.double().abs().t())
+    # at most 64 terms in a row in fp32, the rest in fp64, one rounding to the type
+    allowed = size * 64 * 2.0**-24 + want.abs() * torch.finfo(dtype).eps / 2 * 1.001 + 1e-30
+    if dtype == torch.float16:
+        allowed = allowed + 2.0**-25
+    assert got.dtype == dtype and bool(((got.double().cpu() - want).abs() <= allowed).all())
+    return got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, degree, hubs, empty", [(1, 1, 0, 0.0), (7, 3, 0, 0.3), (64, 1, 0, 0.0), (700, 20, 3, 0.4),
+                                                       (5000, 9, 2, 0.9)])
+@pytest.mark.parametrize("heads, buckets, max_distance, bidirectional", [
+    (1, 32, 128, True), (5, 32, 128, False), (8, 2, 5, False), (3, 64, 4096, True), (16, 128, 300, True),
+    (2, 256, 2000, False), (4, 10, 6, True)])
+def test_bias_and_gradient(dtype, rows, degree, hubs, empty, heads, buckets, max_distance, bidirectional):
+    crow, col = case_graph(rows, degree, seed=rows, hubs=hubs, hub_degree=min(rows, 600) if hubs else 0, empty=empty)
+    _check(crow, col, heads, buckets, max_distance, dtype, bidirectional)
+
+
+@pytest.mark.parametrize("nnz", [1, 63, 64, 65, 255, 257, 1023, 1025, 4097, 16385, 70001])
+def test_edge_counts_around_the_blocks(nnz):
+    rng = np.random.default_rng(nnz)
+    n = 300
+    crow = np.zeros(n + 1, dtype=np.int64)
+    crow[1:] = np.sort(rng.integers(0, nnz + 1, n))
+    crow[-1] = nnz
+    col = rng.integers(0, n, nnz)
+    for dtype, heads in ((torch.float32, 3), (torch.bfloat16, 5)):
+        _check(crow, col, heads, 32, 100, dtype)
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_positions_of_their_own(index):
+    crow, col = case_graph(900, 12, seed=3, empty=0.2)
+    positions = np.random.default_rng(0).integers(-5000, 5000, 900)
+    _check(crow, col, 4, 32, 128, torch.float32, positions=positions)
+    _check(crow, col, 4, 32, 128, torch.float32, bidirectional=False, positions=positions)
+    d_crow, d_col, d_positions = to_dev(crow, col, positions)
+    table = torch.randn(32, 4, device="cuda")
+    a = autosage_amd.csr_position_bias(d_crow, d_col, table, max_distance=128, positions=d_positions)
+    b = autosage_amd.csr_position_bias(d_crow.to(index), d_col.to(index), table, max_distance=128,
+                                       positions=d_positions.to(index))
+    assert torch.equal(a, b)
+
+
+def test_far_positions_and_every_border():
+    """One row of keys at every distance around the borders, and at distances beyond 32 bits."""
+    near = np.arange(-2100, 2101)
+    far = np.array([2**31 - 1, 2**31, 2**31 + 1, 2**40, 2**61])
+    positions = np.concatenate([[0], near, far, -far])
+    n = len(positions)
+    crow = np.concatenate([[0], np.full(n, n - 1)]).astype(np.int64)
+    col = np.arange(1, n)
+    for buckets, distance, both in ((64, 2000, True), (32, 128, False), (200, 1999, False), (8, 2**31 - 1, True)):
+        _check(crow, col, 2, buckets, distance, torch.float32, both, positions)
+
+
+def test_a_table_with_strides_and_a_gradient_that_is_expanded():
+    crow, col = case_graph(400, 7, seed=5)
+    d_crow, d_col = to_dev(crow, col)
+    base = torch.randn(4, 32, device="cuda", requires_grad=True)
+    out = autosage_amd.csr_position_bias(d_crow, d_col, base.t(), max_distance=64)
+    out.sum().backward()  # an expanded gradient of ones
+    bucket = _plain(crow, col, 32, 64, True, None)
+    assert torch.equal(base.grad.cpu(), torch.bincount(bucket, minlength=32).float().expand(4, 32))
+
+
+def test_second_gradient():
+    crow, col = case_graph(50, 4, seed=6)
+    d_crow, d_col = to_dev(crow, col)
+    table = torch.randn(8, 2, device="cuda", requires_grad=True)
+    weights = torch.randn(2, len(col), device="cuda")
+    out = autosage_amd.csr_position_bias(d_crow, d_col, table, max_distance=9)
+    first, = torch.autograd.grad((out * out * weights).sum(), table, create_graph=True)
+    second, = torch.autograd.grad((first * first).sum(), table)
+    cpu = table.detach().cpu().double().requires_grad_()
+    out = autosage_amd.csr_position_bias(torch.from_numpy(crow), torch.from_numpy(col), cpu, max_distance=9)
+    first, = torch.autograd.grad((out * out * weights.cpu().double()).sum(), cpu, create_graph=True)
+    want, = torch.autograd.grad((first * first).sum(), cpu)
+    assert torch.allclose(second.double().cpu(), want, rtol=1e-4, atol=1e-4)
+
+
+def test_the_same_bits_every_time():
+    crow, col = case_graph(20000, 30, seed=7, hubs=4, hub_degree=5000)
+    one = _check(crow, col, 4, 32, 1000, torch.float32)
+    for _ in range(3):
+        assert torch.equal(_check(crow, col, 4, 32, 1000, torch.float32), one)
+
+
+def test_empty_graph_and_refusals():
+    none = torch.zeros(0, dtype=torch.long, device="cuda")
+    crow = torch.zeros(5, dtype=torch.long, device="cuda")
+    table = torch.randn(8, 3, device="cuda", requires_grad=True)
+    out = autosage_amd.csr_position_bias(crow, none, table, max_distance=9)
+    assert out.shape == (3, 0)
+    out.sum().backward()
+    assert table.grad.shape == (8, 3) and not table.grad.any()
+    with pytest.raises(TypeError):
+        autosage_amd.csr_position_bias(crow, none, table.double(), max_distance=9)
+    with pytest.raises(ValueError):
+        autosage_amd.csr_position_bias(crow, none.cpu(), table, max_distance=9)
+
+
+def test_capture_of_a_training_step():
+    crow, col = case_graph(3000, 20, seed=8, hubs=2, hub_degree=900)
+    d_crow, d_col = to_dev(crow, col)
+    table = torch.randn(32, 4, device="cuda", requires_grad=True)
+    grad = torch.randn(4, len(col), device="cuda")
+
+    def step():
+        out = autosage_amd.csr_position_bias(d_crow, d_col, table, max_distance=128)
+        return out.detach(), torch.autograd.grad(out, table, grad)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(3):
+        with torch.no_grad():
+            table.mul_(1.5)
+            grad.mul_(-0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(captured, step()):
+            assert torch.equal(a, b)
+
+
+def test_another_stream():
+    crow, col = case_graph(3000, 20, seed=9)
+    d_crow, d_col = to_dev(crow, col)
+    table = torch.randn(32, 4, device="cuda")
+    want = autosage_amd.csr_position_bias(d_crow, d_col, table, max_distance=128)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = autosage_amd.csr_position_bias(d_crow, d_col, table, max_distance=128)
+    side.synchronize()
+    assert torch.equal(got, want)

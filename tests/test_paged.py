@@ -1,0 +1,269 @@
+"""The paged cache and its attention on the CPU: results, refusals, and the native library's argument checks."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import autosage_amd
+from autosage_amd import _native
+from autosage_amd.paged import _cache_struct
+from tests.paged_common import E4M3, Cache, assert_attention, plain_attention, quantised_rows
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("window, biased", [(None, False), (5, False), (None, True), (7, True)])
+def test_attention(dtype, quantised, window, biased):
+    cache = Cache([0, 1, 9, 16, 37], 2, 6, 5, 8, dtype, quantised=quantised, seed=1)
+    gen = torch.Generator().manual_seed(2)
+    query = torch.randn(5, 6, 6, generator=gen).to(dtype)
+    bias = {}
+    if biased:
+        bias = {"table": torch.randn(8, 6, generator=gen).to(dtype), "max_distance": 20, "bidirectional": False}
+    want = plain_attention(cache, query, 0.3, window=window, **bias)
+    args, exponents = cache.args("cpu")
+    bias = {"bias_table" if k == "table" else k: v for k, v in bias.items()}
+    out, lse = autosage_amd.paged_attention(query, *args, torch.tensor(cache.lengths), scale=0.3, window=window,
+                                            return_lse=True, **bias, **exponents)
+    assert out.dtype == dtype
+    assert_attention(out, lse, want, dtype=dtype, quantised=quantised, lse_bound=1e-5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantised", [False, True])
+def test_write_then_read(dtype, quantised):
+    cache = Cache([3, 0, 20], 2, 6, 5, 8, dtype, quantised=quantised, seed=3, room=1)
+    (key_pages, value_pages, page_ptr, page_idx), exponents = cache.args("cpu")
+    before = (key_pages.clone(), value_pages.clone())
+    gen = torch.Generator().manual_seed(4)
+    key, value = torch.randn(9, 2, 6, generator=gen).to(dtype), torch.randn(9, 2, 5, generator=gen).to(dtype)
+    token_ptr, start = torch.tensor([0, 5, 5, 7]), torch.tensor([3, 0, 20])
+    autosage_amd.paged_cache_write(key, value, key_pages, value_pages, page_ptr, page_idx, token_ptr, start, **exponents)
+    got = autosage_amd.paged_cache_read(key_pages, value_pages, page_ptr, page_idx, token_ptr, start, 9,
+                                        dtype=dtype, **exponents)
+    for rows, back in zip((key, value), got):
+        want = quantised_rows(rows)[0].to(dtype) if quantised else rows
+        assert torch.equal(back[:7], want[:7]) and not back[7:].any()
+    everything = autosage_amd.paged_cache_read(key_pages, value_pages, page_ptr, page_idx, torch.tensor([0, 3, 3, 23]),
+                                               torch.tensor([0, 0, 0]), 23, dtype=dtype, **exponents)
+    for kind, back in zip(("key", "value"), everything):
+        assert torch.equal(back.double(), torch.cat(cache.rows[kind]).to(dtype).double())
+    # nothing but the written places changed
+    touched = torch.zeros(key_pages.shape[0], 8, dtype=torch.bool)
+    for b, first, count in ((0, 3, 5), (2, 20, 2)):
+        t = first + torch.arange(count)
+        touched[page_idx[page_ptr[b] + t // 8], t % 8] = True
+    for old, new in zip(before, (key_pages, value_pages)):
+        a, b = (x.view(torch.uint8).transpose(1, 2)[~touched] for x in (old, new))
+        assert torch.equal(a, b)
+
+
+def test_quantised_numbers_at_the_edges():
+    """Rows of zeros, of the largest and smallest numbers, of 448 exactly and just above, and what is not finite."""
+    tiny = 2.0**-149
+    rows = torch.tensor([[0.0, -0.0, 0.0], [448.0, 1.0, -3.3], [448.0001, 1.0, 2.0**-9], [3.4e38, -1e38, 1.0],
+                         [tiny, -tiny, 0.0], [2.0**-126, 2.0**-130, 2.0**-140], [17.0, 19.0, 1.0625]])
+    key_pages = torch.zeros(1, 1, 8, 3, dtype=E4M3)
+    value_pages = torch.zeros(1, 1, 8, 3, dtype=E4M3)
+    key_e, value_e = torch.zeros(1, 1, 8, dtype=torch.int8), torch.zeros(1, 1, 8, dtype=torch.int8)
+    lists = (torch.tensor([0, 1]), torch.tensor([0]))
+    span = (torch.tensor([0, 7]), torch.tensor([0]))
+    x = rows[:, None]
+    autosage_amd.paged_cache_write(x, x, key_pages, value_pages, *lists, *span, key_exponents=key_e,
+                                   value_exponents=value_e)
+    back, _ = autosage_amd.paged_cache_read(key_pages, value_pages, *lists, *span, 7, dtype=torch.float32,
+                                            key_exponents=key_e, value_exponents=value_e)
+    values, e = quantised_rows(rows)
+    assert torch.equal(key_e[0, 0, :7].long(), e) and torch.equal(back[:, 0], values.float())
+    assert back[3, 0, 0] == float("inf")  # 3.4e38 is held as 2^128
+    odd = torch.tensor([[float("inf"), 1.0, 300.0], [float("nan"), -float("inf"), 2.0]])[:, None]
+    autosage_amd.paged_cache_write(odd, odd, key_pages, value_pages, *lists, torch.tensor([0, 2]), span[1],
+                                   key_exponents=key_e, value_exponents=value_e)
+    back, _ = autosage_amd.paged_cache_read(key_pages, value_pages, *lists, torch.tensor([0, 2]), span[1], 2,
+                                            dtype=torch.float32, key_exponents=key_e, value_exponents=value_e)
+    assert back[0, 0].isnan().tolist() == [True, False, False] and back[0, 0, 1:].tolist() == [1.0, 288.0]  # steps of 32 from 256 on
+    assert back[1, 0].isnan().tolist() == [True, True, False] and back[1, 0, 2] == 2.0
+
+
+def test_lengths_and_pages_that_do_not_fit():
+    cache = Cache([4, 9, 12], 1, 4, 4, 4, torch.float32, seed=5)
+    (k, v, ptr, idx), _ = cache.args("cpu")
+    query = torch.randn(3, 1, 4)
+    call = autosage_amd.paged_attention
+    good = call(query, k, v, ptr, idx, torch.tensor([4, 9, 12]))
+    out, lse = call(query, k, v, ptr, idx, torch.tensor([5, 9, 12]), return_lse=True)  # one token more than its page holds
+    assert out[0].isnan().all() and lse[0].isnan().all() and torch.equal(out[1:], good[1:])
+    assert call(query, k, v, ptr, idx, torch.tensor([4, 9, 12]), max_length=9)[2].isnan().all()
+    idx = idx.clone()
+    idx[1] = k.size(0)
+    out = call(query, k, v, ptr, idx, torch.tensor([4, 9, 12]))
+    assert out[1].isnan().all() and torch.equal(out[[0, 2]], good[[0, 2]])
+    assert not call(query, k, v, ptr, idx, torch.tensor([0, -3, 0])).any()
+
+
+def test_validation(monkeypatch):
+    cache = Cache([4, 9], 1, 4, 4, 4, torch.float32, seed=6)
+    (k, v, ptr, idx), _ = cache.args("cpu")
+    query, rows = torch.randn(2, 1, 4), torch.randn(2, 1, 4)
+    one = torch.tensor([0, 1, 2])
+    monkeypatch.setenv("AUTOSAGE_VALIDATE", "1")
+    good = torch.tensor([4, 9])
+    autosage_amd.paged_attention(query, k, v, ptr, idx, good)
+    autosage_amd.paged_cache_write(rows, rows, k, v, ptr, idx, one, torch.tensor([3, 9]))
+    bad_idx = idx.clone()
+    bad_idx[0] = -1
+    for args, message in [((ptr + 1, idx, good), "page_ptr"), ((ptr, bad_idx, good), "page ids"),
+                          ((ptr, idx, good + 4), "more tokens"), ((ptr, idx, -good), "negative")]:
+        with pytest.raises(ValueError, match=message):
+            autosage_amd.paged_attention(query, k, v, *args)
+    with pytest.raises(ValueError, match="max_length"):
+        autosage_amd.paged_attention(query, k, v, ptr, idx, good, max_length=8)
+    twice = torch.tensor([0, 0, 1, 2])  # the first page of both lists
+    for token_ptr, start, lists, message in [
+            (torch.tensor([0, 1, 3]), good - 1, (ptr, idx), "token_ptr"), (one, good + 4, (ptr, idx), "more tokens"),
+            (one, torch.tensor([-1, 0]), (ptr, idx), "token_ptr"),
+            (one, torch.tensor([2, 2]), (torch.tensor([0, 1, 4]), twice), "same place")]:
+        with pytest.raises(ValueError, match=message):
+            autosage_amd.paged_cache_write(rows, rows, k, v, *lists, token_ptr, start)
+
+
+def test_refusals():
+    cache = Cache([4, 9], 2, 4, 3, 4, torch.float32, seed=7)
+    (k, v, ptr, idx), _ = cache.args("cpu")
+    coded = Cache([4, 9], 2, 4, 3, 4, torch.float32, quantised=True, seed=7)
+    (ck, cv, _, _), e = coded.args("cpu")
+    query, lengths = torch.randn(2, 4, 4), torch.tensor([4, 9])
+    attention, write, read = autosage_amd.paged_attention, autosage_amd.paged_cache_write, autosage_amd.paged_cache_read
+    key, value = torch.randn(2, 2, 4), torch.randn(2, 2, 3)
+    span = (torch.tensor([0, 1, 2]), torch.tensor([3, 8]))
+    table = torch.randn(8, 4)
+    for error, call in [
+        (ValueError, lambda: attention(query, k[0], v, ptr, idx, lengths)),
+        (ValueError, lambda: attention(query, k, v[:, :1], ptr, idx, lengths)),
+        (TypeError, lambda: attention(query, k, v.half(), ptr, idx, lengths)),
+        (TypeError, lambda: attention(query, k.double(), v.double(), ptr, idx, lengths)),
+        (TypeError, lambda: attention(query.half(), k, v, ptr, idx, lengths)),
+        (ValueError, lambda: attention(query[:, :3], k, v, ptr, idx, lengths)),
+        (ValueError, lambda: attention(query[:, :, :3], k, v, ptr, idx, lengths)),
+        (ValueError, lambda: attention(query[:1], k, v, ptr, idx, lengths)),
+        (ValueError, lambda: attention(query, k, v, ptr, idx, lengths[:1])),
+        (TypeError, lambda: attention(query, k, v, ptr, idx, lengths.float())),
+        (TypeError, lambda: attention(query, k, v, ptr.float(), idx, lengths)),
+        (ValueError, lambda: attention(query, k, v, ptr, idx[None], lengths)),
+        (ValueError, lambda: attention(query, k, v, ptr[:0], idx, lengths)),
+        (ValueError, lambda: attention(query, k, v, ptr, idx, lengths, window=0)),
+        (ValueError, lambda: attention(query, k, v, ptr, idx, lengths, max_length=-1)),
+        (ValueError, lambda: attention(query, k, v, ptr, idx, lengths, max_distance=9)),
+        (ValueError, lambda: attention(query, k, v, ptr, idx, lengths, bias_table=table)),
+        (ValueError, lambda: attention(query, k, v, ptr, idx, lengths, bias_table=table[:, :2], max_distance=9)),
+        (ValueError, lambda: attention(query, k, v, ptr, idx, lengths, bias_table=table[:7], max_distance=9)),
+        (TypeError, lambda: attention(query, k, v, ptr, idx, lengths, bias_table=table.half(), max_distance=9)),
+        (ValueError, lambda: attention(query, k, v, ptr, idx, lengths, **e)),
+        (ValueError, lambda: attention(query, ck, cv, ptr, idx, lengths)),
+        (ValueError, lambda: attention(query, ck, cv, ptr, idx, lengths, key_exponents=e["key_exponents"])),
+        (TypeError, lambda: attention(query, ck, cv, ptr, idx, lengths, key_exponents=e["key_exponents"].int(),
+                                      value_exponents=e["value_exponents"])),
+        (ValueError, lambda: attention(query, ck, cv, ptr, idx, lengths, key_exponents=e["key_exponents"][:1],
+                                       value_exponents=e["value_exponents"])),
+        (ValueError, lambda: attention(query, k.transpose(2, 3), v, ptr, idx, lengths)),
+        (ValueError, lambda: attention(torch.randn(2, 2, 257), torch.randn(4, 2, 4, 257), torch.randn(4, 2, 4, 3), ptr,
+                                       idx, lengths)),
+        (ValueError, lambda: attention(query, k[:0], v[:0], ptr, idx, lengths)),
+        (RuntimeError, lambda: attention(query.clone().requires_grad_(), k, v, ptr, idx, lengths)),
+        (ValueError, lambda: write(key[:1], value, k, v, ptr, idx, *span)),
+        (ValueError, lambda: write(key[:, :1], value, k, v, ptr, idx, *span)),
+        (ValueError, lambda: write(value, key, k, v, ptr, idx, *span)),
+        (TypeError, lambda: write(key.half(), value.half(), k, v, ptr, idx, *span)),
+        (TypeError, lambda: write(key.half(), value, ck, cv, ptr, idx, *span, **e)),
+        (ValueError, lambda: write(key, value, k, v, ptr, idx, span[0][:2], span[1])),
+        (ValueError, lambda: write(key, value, k, v, ptr, idx, span[0], span[1][:1])),
+        (TypeError, lambda: write(key, value, k, v, ptr, idx, span[0].float(), span[1])),
+        (ValueError, lambda: write(key, value, k[:1].expand(4, 2, 4, 4), v[:4], ptr, idx, *span)),
+        (RuntimeError, lambda: write(key.clone().requires_grad_(), value, k, v, ptr, idx, *span)),
+        (ValueError, lambda: read(k, v, ptr, idx, *span, -1)),
+        (TypeError, lambda: read(k, v, ptr, idx, *span, 2, dtype=torch.float16)),
+        (TypeError, lambda: read(ck, cv, ptr, idx, *span, 2, dtype=torch.float64, **e)),
+    ]:
+        with pytest.raises(error):
+            call()
+    with torch.no_grad():
+        attention(query.clone().requires_grad_(), k, v, ptr, idx, lengths)
+
+
+def test_no_sequences_and_no_tokens():
+    cache = Cache([4], 2, 4, 3, 4, torch.float32, seed=8)
+    (k, v, _, idx), _ = cache.args("cpu")
+    none = torch.zeros(0, dtype=torch.long)
+    ptr = torch.zeros(1, dtype=torch.long)
+    assert autosage_amd.paged_attention(torch.zeros(0, 4, 4), k, v, ptr, idx, none).shape == (0, 4, 3)
+    key, value = autosage_amd.paged_cache_read(k, v, ptr, idx, ptr, none, 3)
+    assert key.shape == (3, 2, 4) and value.shape == (3, 2, 3) and not key.any() and not value.any()
+    autosage_amd.paged_cache_write(torch.zeros(0, 2, 4), torch.zeros(0, 2, 3), k, v, ptr, idx, ptr, none)
+
+
+def test_native_argument_checks_come_before_any_launch():
+    path = _native.package_library_path()
+    if not path.exists():
+        pytest.skip("HIP library not built")
+    lib = _native.open_library(path)
+    cache = Cache([4, 9], 2, 4, 3, 4, torch.float32, seed=9)
+    (k, v, ptr, idx), _ = cache.args("cpu")
+
+    def struct(**changes):
+        c = _cache_struct(k, v, ptr, idx, None, None)
+        for name, what in changes.items():
+            setattr(c, name, what)
+        return ctypes.byref(c)
+
+    two = (ctypes.c_int64 * 2)(8, 4)
+    fake = 256
+
+    def attention(c, group=2, dtype=0, window=0, bound=-1, table=None, buckets=0, borders=None, sides=0, ws=fake,
+                  ws_bytes=1 << 30, query=fake):
+        return lib.as_paged_attention(c, query, two, fake, None, fake, group, 1.0, window, table, buckets, borders,
+                                      sides, bound, dtype, ws, ws_bytes, None)
+
+    for status, call, message in [
+        (1, lambda: attention(None), b"null cache pointer"),
+        (1, lambda: attention(struct(dtype=4)), b"the cache's dtype"),
+        (1, lambda: attention(struct(dtype=3)), b"an e4m3 cache has exponents"),
+        (1, lambda: attention(struct(pages=0)), b"a cache has 1 to"),
+        (1, lambda: attention(struct(page_size=0)), b"a cache has 1 to"),
+        (1, lambda: attention(struct(heads=0)), b"heads must lie"),
+        (3, lambda: attention(struct(key_width=257)), b"key and value widths"),
+        (1, lambda: attention(struct(key_pages=None)), b"null pointer argument"),
+        (1, lambda: attention(struct(key_pages=k.data_ptr() + 2)), b"the pages must be aligned"),
+        (1, lambda: attention(struct(), dtype=1), b"a cache that is not quantised"),
+        (1, lambda: attention(struct(), dtype=3), b"dtype must be"),
+        (1, lambda: attention(struct(), group=0), b"query heads must lie"),
+        (1, lambda: attention(struct(), group=40000), b"query heads must lie"),
+        (1, lambda: attention(struct(), window=-1), b"window and max_length"),
+        (1, lambda: attention(struct(), table=fake, buckets=257), b"the number of buckets"),
+        (1, lambda: attention(struct(), table=fake, buckets=3, sides=1), b"two sides need"),
+        (1, lambda: attention(struct(), table=fake, buckets=3), b"null borders"),
+        (1, lambda: attention(struct(), table=fake, buckets=3, borders=(ctypes.c_int32 * 3)(0, 2, 1)), b"borders must"),
+        (4, lambda: attention(struct(), ws=None), b"paged attention needs"),
+        (1, lambda: attention(struct(), query=None), b"null pointer argument"),
+        (0, lambda: attention(struct(sequences=0)), b""),
+        (1, lambda: lib.as_paged_cache_write(struct(), fake, two, fake, two, fake, fake, 2, 2, None), b"a cache that"),
+        (3, lambda: lib.as_paged_cache_write(struct(), fake, two, fake, two, fake, fake, 1 << 50, 0, None), b"too many"),
+        (1, lambda: lib.as_paged_cache_write(struct(), fake, two, None, two, fake, fake, 2, 0, None), b"null pointer"),
+        (1, lambda: lib.as_paged_cache_write(struct(), fake, None, fake, two, fake, fake, 2, 0, None), b"null strides"),
+        (0, lambda: lib.as_paged_cache_write(struct(), fake, two, fake, two, fake, fake, 0, 0, None), b""),
+        (1, lambda: lib.as_paged_cache_read(struct(), fake + 1, fake, fake, fake, 2, 0, None), b"key and value must"),
+        (1, lambda: lib.as_paged_cache_read(struct(sequences=0), fake, fake, fake, fake, 2, 0, None), b"tokens without"),
+        (1, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, 4, 4, 2, 8, None, 0, 0, None), b"null borders"),
+        (1, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, 4, 4, 2, 8, None, 0, 3, None), b"dtype must"),
+        (1, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, 0, 4, 2, 8, None, 0, 0, None), b"edges without"),
+        (1, lambda: lib.as_csr_position_bias(fake, None, None, fake, fake, 4, 4, 2, 8, None, 0, 0, None), b"null pointer"),
+        (4, lambda: lib.as_csr_position_bias_backward(fake, fake, None, fake, fake, 4, 4, 2, 2,
+                                                      (ctypes.c_int32 * 2)(0, 1), 0, 0, fake, 8, None),
+         b"the position bias gradient needs"),
+    ]:
+        assert call() == status, message
+        assert lib.as_last_error().startswith(message), lib.as_last_error()
