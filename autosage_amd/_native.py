@@ -204,7 +204,7 @@ _SIGNATURES = {
     "as_paged_cache_write": (
         _c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
     "as_paged_cache_read": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
-    "as_paged_attention_workspace_bytes": (_c_size, [_c_ptr, _c_i64, _c_i64]),
+    "as_paged_attention_workspace_bytes": (_c_size, [_c_ptr, _c_i64, _c_i64, _c_i64]),
     "as_paged_attention": (
         _c_int,
         [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, ctypes.c_float, _c_i64, _c_ptr, _c_i64, _c_ptr,

@@ -430,12 +430,14 @@ def paged_attention_impl(query, key_pages, value_pages, page_ptr, page_idx, leng
     cache = _cache_struct(key_pages, value_pages, page_ptr, page_idx, key_exponents, value_exponents)
     bound = -1 if max_length is None else int(max_length)
     group = heads_q // key_pages.size(1)
-    ws = _native._workspace(lib.as_paged_attention_workspace_bytes(ctypes.byref(cache), group, bound), query.device)
+    seen = 0 if window is None else int(window)
+    ws = _native._workspace(lib.as_paged_attention_workspace_bytes(ctypes.byref(cache), group, seen, bound),
+                            query.device)
     with _native._on(query.device):
         status = lib.as_paged_attention(
             ctypes.byref(cache), query.data_ptr(), (ctypes.c_int64 * 2)(query.stride(0), query.stride(1)),
             out.data_ptr(), lse.data_ptr() if return_lse else None, lengths.data_ptr(), group, float(scale),
-            0 if window is None else int(window), None if bias_table is None else bias_table.data_ptr(), buckets,
+            seen, None if bias_table is None else bias_table.data_ptr(), buckets,
             borders, int(bool(bidirectional)), bound, _DTYPES[query.dtype], ws.data_ptr(), ws.numel(),
             _native._stream(query.device))
     _native._raise(status, "autosage::paged_attention")

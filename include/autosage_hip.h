@@ -807,7 +807,8 @@ int as_paged_cache_read(const as_paged_cache* cache, void* key, void* value,
  * launch; lengths beyond it give NaN).  No token seen: zeros and -inf.  A
  * length beyond the pages of its list, or a page id outside the cache: NaN. */
 size_t as_paged_attention_workspace_bytes(const as_paged_cache* cache,
-                                          int64_t group, int64_t max_length);
+                                          int64_t group, int64_t window,
+                                          int64_t max_length);
 int as_paged_attention(const as_paged_cache* cache, const void* query,
                        const int64_t* query_strides, void* out, float* lse,
                        const int64_t* lengths, int64_t group, float scale,
