@@ -193,14 +193,13 @@ _SIGNATURES = {
     ),
     "as_csr_position_bias": (
         _c_int,
-        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int, _c_int, _c_ptr],
+        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int, _c_int,
+         _c_ptr, _c_size, _c_ptr],
     ),
+    "as_csr_position_bias_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_int]),
     "as_csr_position_bias_backward_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64]),
     "as_csr_position_bias_backward": (
-        _c_int,
-        [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_ptr, _c_int, _c_int, _c_ptr,
-         _c_size, _c_ptr],
-    ),
+        _c_int, [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_int, _c_ptr, _c_size, _c_ptr]),
     "as_paged_cache_write": (
         _c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),
     "as_paged_cache_read": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_ptr]),

@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
   constexpr int kP = WeightParts<T, C>::value;
   using U = typename Unit<T, C>::type;
 
-  __shared__ int32_t border[kMaxBuckets];
+  __shared__ int32_t border[kMaxBuckets + 1];
   __shared__ float wave_top[kWavesPerBlock][kHeads];
   __shared__ float wave_sum[kWavesPerBlock][kHeads];
   // the bias of the loop, then the waves' sums
@@ -283,7 +283,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
 
   if (a.table != nullptr) {
     const int buckets = map.both_sides ? 2 * map.side : map.side;
-    for (int i = threadIdx.x; i < map.side; i += kBlock) border[i] = map.border[i];
+    stage_borders(border, map);
     for (int i = threadIdx.x; i < buckets * kHeads; i += kBlock) {
       const int hh = i % kHeads < heads_here ? i % kHeads : 0;
       bias[i / kHeads][i % kHeads] =
@@ -478,7 +478,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
 #pragma unroll
         for (int e = 0; e < kOwn; ++e) {
           const int away = seen.end - 1 - (t0 + own_token + e);
-          s2[e] += bias[bucket_of_distance(border, map.side, away < 0 ? 0 : away)][n];
+          s2[e] += bias[bucket_of_distance(border, map, away < 0 ? 0 : away)][n];
         }
       }
     }

@@ -73,18 +73,17 @@ def position_buckets(relative: torch.Tensor, buckets: int, max_distance: int, bi
     return found + (relative > 0).long() * (buckets // 2) if bidirectional else found
 
 
-def _check_graph(crow, col, positions, values, heads_dim: str) -> None:
+def _check(crow, col, positions, table) -> None:
     if crow.ndim != 1 or col.ndim != 1 or crow.numel() < 1:
         raise ValueError("crow and col must be one-dimensional")
     if crow.dtype not in (torch.int32, torch.int64) or col.dtype not in (torch.int32, torch.int64):
         raise TypeError("crow and col must use integer indices")
-    if values.ndim != 2 or values.size(0 if heads_dim == "grad" else 1) < 1:
-        raise ValueError("table must have shape [buckets, heads]" if heads_dim == "table"
-                         else "grad must have shape [heads, edges]")
-    if not values.is_floating_point():
-        raise TypeError(f"{heads_dim} must use a floating-point dtype")
-    if not (crow.device == col.device == values.device):
-        raise ValueError(f"crow, col, and {heads_dim} must be on the same device")
+    if table.ndim != 2 or table.size(1) < 1:
+        raise ValueError("table must have shape [buckets, heads]")
+    if not table.is_floating_point():
+        raise TypeError("table must use a floating-point dtype")
+    if not (crow.device == col.device == table.device):
+        raise ValueError("crow, col, and table must be on the same device")
     if col.numel() > 0 and crow.numel() < 2:
         raise ValueError("edges without rows")
     if positions is not None:
@@ -100,8 +99,9 @@ def _long(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or (t.dtype == torch.long and t.is_contiguous()) else t.to(torch.long).contiguous()
 
 
-def csr_position_bias_impl(crow, col, positions, table, max_distance, bidirectional):
-    _check_graph(crow, col, positions, table, "table")
+def csr_position_bias_impl(crow, col, positions, table, max_distance, bidirectional, keep=True):
+    """(bias [heads, edges], the edges' buckets: one byte each, none without ``keep``)."""
+    _check(crow, col, positions, table)
     if table.dtype not in _DTYPES:
         raise TypeError("the native position bias supports float32, bfloat16 and float16 tables")
     buckets, heads = table.shape
@@ -109,82 +109,87 @@ def csr_position_bias_impl(crow, col, positions, table, max_distance, bidirectio
     crow, col, positions, table = _long(crow), _long(col), _long(positions), table.contiguous()
     nnz = col.numel()
     out = torch.empty(heads, nnz, dtype=table.dtype, device=table.device)
+    # whole words: the last one may reach behind the edges
+    found = torch.empty((nnz + 3) // 4 * 4 if keep else 0, dtype=torch.uint8, device=table.device)
     if nnz == 0:
-        return out
+        return out, found
+    n = crow.numel() - 1
+    lib = _native.library()
+    ws = _native._workspace(lib.as_csr_position_bias_workspace_bytes(n, nnz, int(positions is not None)), table.device)
     with _native._on(table.device):
-        status = _native.library().as_csr_position_bias(
+        status = lib.as_csr_position_bias(
             crow.data_ptr(), col.data_ptr(), _native._ptr(positions), table.data_ptr(), out.data_ptr(),
-            crow.numel() - 1, nnz, heads, buckets, borders, int(bool(bidirectional)), _DTYPES[table.dtype],
-            _native._stream(table.device))
+            found.data_ptr() if keep else None, n, nnz, heads, buckets, borders, int(bool(bidirectional)),
+            _DTYPES[table.dtype], ws.data_ptr(), ws.numel(), _native._stream(table.device))
     _native._raise(status, "autosage::csr_position_bias")
-    return out
+    return out, found
 
 
-def csr_position_bias_backward_impl(crow, col, positions, grad, buckets, max_distance, bidirectional):
-    """dL/dtable [buckets, heads] from dL/dbias [heads, edges]."""
-    _check_graph(crow, col, positions, grad, "grad")
-    if grad.dtype not in _DTYPES:
-        raise TypeError("the native position bias supports float32, bfloat16 and float16 tables")
-    if grad.size(1) != col.numel():
-        raise ValueError("grad must have shape [heads, edges]")
-    borders = border_array(buckets, max_distance, bool(bidirectional))
-    crow, col, positions, grad = _long(crow), _long(col), _long(positions), grad.contiguous()
+def csr_position_bias_backward_impl(found, grad, buckets):
+    """dL/dtable [buckets, heads] from the edges' buckets and dL/dbias [heads, edges]."""
+    if grad.ndim != 2 or grad.size(0) < 1 or found.ndim != 1 or found.numel() != (grad.size(1) + 3) // 4 * 4:
+        raise ValueError("grad must have shape [heads, edges], with a bucket for every edge")
+    if grad.dtype not in _DTYPES or found.dtype != torch.uint8:
+        raise TypeError("the native position bias supports float32, bfloat16 and float16 gradients, and uint8 buckets")
+    if grad.device != found.device:
+        raise ValueError("grad and the buckets must be on the same device")
+    found, grad = found.contiguous(), grad.contiguous()
     heads, nnz = grad.shape
     table = torch.empty(buckets, heads, dtype=grad.dtype, device=grad.device)
     lib = _native.library()
     ws = _native._workspace(lib.as_csr_position_bias_backward_workspace_bytes(nnz, heads, buckets), grad.device)
     with _native._on(grad.device):
         status = lib.as_csr_position_bias_backward(
-            crow.data_ptr(), col.data_ptr(), _native._ptr(positions), grad.data_ptr(), table.data_ptr(),
-            crow.numel() - 1, nnz, heads, buckets, borders, int(bool(bidirectional)), _DTYPES[grad.dtype],
+            found.data_ptr(), grad.data_ptr(), table.data_ptr(), nnz, heads, buckets, _DTYPES[grad.dtype],
             ws.data_ptr(), ws.numel(), _native._stream(grad.device))
     _native._raise(status, "autosage::csr_position_bias (backward)")
     return table
 
 
 SCHEMAS = {
+    # the bias, and the edges' buckets for its gradient
     "csr_position_bias": (
         "csr_position_bias(Tensor crow, Tensor col, Tensor? positions, Tensor table, int max_distance, "
-        "bool bidirectional) -> Tensor",
+        "bool bidirectional) -> (Tensor, Tensor)",
         csr_position_bias_impl,
     ),
     "csr_position_bias_backward": (
-        "csr_position_bias_backward(Tensor crow, Tensor col, Tensor? positions, Tensor grad, int buckets, "
-        "int max_distance, bool bidirectional) -> Tensor",
+        "csr_position_bias_backward(Tensor found, Tensor grad, int buckets) -> Tensor",
         csr_position_bias_backward_impl,
     ),
 }
 
 
 def _setup(ctx, inputs, output) -> None:
-    crow, col, positions, values = inputs[:4]
-    ctx.save_for_backward(crow, col, positions)
-    ctx.size = values.size(0)
-    ctx.map = (inputs[-2], inputs[-1])
+    ctx.buckets = inputs[3].size(0)
+    ctx.save_for_backward(output[1])
+    ctx.mark_non_differentiable(output[1])
+    ctx.set_materialize_grads(False)
 
 
-def _backward(ctx, grad):
-    crow, col, positions = ctx.saved_tensors
-    if not ctx.needs_input_grad[3]:
-        return None, None, None, None, None, None
-    grad_table = torch.ops.autosage.csr_position_bias_backward(crow, col, positions, grad, ctx.size, *ctx.map)
+def _backward(ctx, grad, _):
+    grad_table = None
+    if grad is not None and ctx.needs_input_grad[3]:
+        grad_table = torch.ops.autosage.csr_position_bias_backward(ctx.saved_tensors[0], grad, ctx.buckets)
     return None, None, None, grad_table, None, None
 
 
-def _backward_of_backward(ctx, grad_table):
+def _second_setup(ctx, inputs, output) -> None:
+    ctx.save_for_backward(inputs[0])
+    ctx.edges = inputs[1].size(1)
+
+
+def _second_backward(ctx, grad_table):
     # the sum over each bucket's edges is linear: its transpose is the lookup
-    crow, col, positions = ctx.saved_tensors
-    if not ctx.needs_input_grad[3]:
-        return None, None, None, None, None, None, None
-    grad = torch.ops.autosage.csr_position_bias(crow, col, positions, grad_table, *ctx.map)
-    return None, None, None, grad, None, None, None
+    found = ctx.saved_tensors[0][: ctx.edges].long()
+    return None, grad_table.t()[:, found], None
 
 
 def register_autograd() -> None:
     """Attaches the gradients to the registered operators."""
     torch.library.register_autograd("autosage::csr_position_bias", _backward, setup_context=_setup)
-    torch.library.register_autograd("autosage::csr_position_bias_backward", _backward_of_backward,
-                                    setup_context=_setup)
+    torch.library.register_autograd("autosage::csr_position_bias_backward", _second_backward,
+                                    setup_context=_second_setup)
 
 
 def _cpu_position_bias(crow, col, positions, table, max_distance, bidirectional) -> torch.Tensor:
@@ -205,7 +210,7 @@ def csr_position_bias(crow, col, table, *, max_distance: int, bidirectional: boo
     Node ids are positions unless ``positions`` (one integer per node) gives
     them.  With ``bidirectional`` half of the buckets are for keys behind the
     query; without it a key behind the query counts as distance 0."""
-    _check_graph(crow, col, positions, table, "table")
+    _check(crow, col, positions, table)
     max_distance = int(max_distance)
     bucket_borders(table.size(0), max_distance, bool(bidirectional))
     if not table.is_cuda:
@@ -216,8 +221,8 @@ def csr_position_bias(crow, col, table, *, max_distance: int, bidirectional: boo
     validate_if_requested(crow, col)
     args = (crow, col, positions, table, max_distance, bool(bidirectional))
     if torch.is_grad_enabled() and table.requires_grad:
-        return torch.ops.autosage.csr_position_bias(*args)
-    return csr_position_bias_impl(*args)
+        return torch.ops.autosage.csr_position_bias(*args)[0]
+    return csr_position_bias_impl(*args, keep=False)[0]
 
 
 __all__ = ["bucket_borders", "csr_position_bias", "position_buckets"]

@@ -724,23 +724,29 @@ int as_csr_validate(const int64_t* crow, const int64_t* col, int64_t n,
  *
  * table, grad_table [buckets, heads] and out, grad [heads, nnz] are of dtype
  * AS_DTYPE_F32, _BF16 or _F16; positions int64[n] or NULL (node ids are
- * positions; the graph then need not be square).  The gradient is summed in a
- * fixed order, at most 64 numbers in fp32 and the sums of those in fp64. */
+ * positions; the graph then need not be square).  found: NULL, or room for
+ * nnz bytes rounded up to a multiple of 4 (4-byte aligned), which the forward
+ * call fills with the buckets of the edges and the backward call reads in
+ * place of the graph.  The gradient is summed in a fixed order, at most 64
+ * numbers in fp32 and the sums of those in fp64.  nnz at most 2^30. */
 int as_csr_position_bias(const int64_t* crow, const int64_t* col,
                          const int64_t* positions, const void* table,
-                         void* out, int64_t n, int64_t nnz, int64_t heads,
-                         int64_t buckets, const int32_t* borders,
-                         int both_sides, int dtype, void* stream);
+                         void* out, uint8_t* found, int64_t n, int64_t nnz,
+                         int64_t heads, int64_t buckets,
+                         const int32_t* borders, int both_sides, int dtype,
+                         void* workspace, size_t workspace_bytes,
+                         void* stream);
+/* positions != 0: the call has positions. */
+size_t as_csr_position_bias_workspace_bytes(int64_t n, int64_t nnz,
+                                            int positions);
 size_t as_csr_position_bias_backward_workspace_bytes(int64_t nnz,
                                                      int64_t heads,
                                                      int64_t buckets);
-int as_csr_position_bias_backward(const int64_t* crow, const int64_t* col,
-                                  const int64_t* positions, const void* grad,
-                                  void* grad_table, int64_t n, int64_t nnz,
-                                  int64_t heads, int64_t buckets,
-                                  const int32_t* borders, int both_sides,
-                                  int dtype, void* workspace,
-                                  size_t workspace_bytes, void* stream);
+int as_csr_position_bias_backward(const uint8_t* found, const void* grad,
+                                  void* grad_table, int64_t nnz,
+                                  int64_t heads, int64_t buckets, int dtype,
+                                  void* workspace, size_t workspace_bytes,
+                                  void* stream);
 
 /* ---- Paged key-value cache ---------------------------------------------------
  * No reference counterpart (its attention is over whole graphs).

@@ -100,6 +100,24 @@ def test_far_positions_and_every_border():
         _check(crow, col, 2, buckets, distance, torch.float32, both, positions)
 
 
+@pytest.mark.parametrize("far", [False, True])
+def test_many_nodes_with_positions(far):
+    """Enough nodes for the 32-bit copy of the positions, which one position beyond 32 bits rules out."""
+    n, degree = 600_000, 4
+    rng = np.random.default_rng(11)
+    crow = np.arange(n + 1, dtype=np.int64) * degree
+    col = rng.integers(0, n, n * degree)
+    positions = rng.permutation(n) - 100_000
+    if far:
+        positions[n // 3] = 2**33
+    rel = positions[col] - np.repeat(positions, degree)
+    bucket = torch.from_numpy(plain_buckets(np.clip(rel, -3000, 3000), 32, 2000, True))
+    table = torch.randn(32, 2)
+    d_crow, d_col, d_positions = to_dev(crow, col, positions)
+    out = autosage_amd.csr_position_bias(d_crow, d_col, table.cuda(), max_distance=2000, positions=d_positions)
+    assert torch.equal(out.cpu(), table.t()[:, bucket])
+
+
 def test_a_table_with_strides_and_a_gradient_that_is_expanded():
     crow, col = case_graph(400, 7, seed=5)
     d_crow, d_col = to_dev(crow, col)

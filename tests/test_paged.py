@@ -257,13 +257,25 @@ def test_native_argument_checks_come_before_any_launch():
         (0, lambda: lib.as_paged_cache_write(struct(), fake, two, fake, two, fake, fake, 0, 0, None), b""),
         (1, lambda: lib.as_paged_cache_read(struct(), fake + 1, fake, fake, fake, 2, 0, None), b"key and value must"),
         (1, lambda: lib.as_paged_cache_read(struct(sequences=0), fake, fake, fake, fake, 2, 0, None), b"tokens without"),
-        (1, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, 4, 4, 2, 8, None, 0, 0, None), b"null borders"),
-        (1, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, 4, 4, 2, 8, None, 0, 3, None), b"dtype must"),
-        (1, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, 0, 4, 2, 8, None, 0, 0, None), b"edges without"),
-        (1, lambda: lib.as_csr_position_bias(fake, None, None, fake, fake, 4, 4, 2, 8, None, 0, 0, None), b"null pointer"),
-        (4, lambda: lib.as_csr_position_bias_backward(fake, fake, None, fake, fake, 4, 4, 2, 2,
-                                                      (ctypes.c_int32 * 2)(0, 1), 0, 0, fake, 8, None),
+        (1, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, None, 4, 4, 2, 8, None, 0, 0, fake, 8, None),
+         b"null borders"),
+        (1, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, None, 4, 4, 2, 8, None, 0, 3, fake, 8, None),
+         b"dtype must"),
+        (1, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, None, 0, 4, 2, 8, None, 0, 0, fake, 8, None),
+         b"edges without"),
+        (1, lambda: lib.as_csr_position_bias(fake, None, None, fake, fake, None, 4, 4, 2, 8, None, 0, 0, fake, 8, None),
+         b"null pointer"),
+        (1, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, fake + 1, 4, 4, 2, 8, None, 0, 0, fake, 8, None),
+         b"found must be"),
+        (3, lambda: lib.as_csr_position_bias(fake, fake, None, fake, fake, None, 4, 1 << 31, 2, 8, None, 0, 0, fake, 8, None),
+         b"at most 2^30"),
+        (1, lambda: lib.as_csr_position_bias_backward(None, fake, fake, 4, 2, 2, 0, fake, 1 << 20, None), b"null pointer"),
+        (1, lambda: lib.as_csr_position_bias_backward(fake, fake, fake, 4, 2, 257, 0, fake, 1 << 20, None),
+         b"the number of buckets"),
+        (4, lambda: lib.as_csr_position_bias_backward(fake, fake, fake, 4, 2, 2, 0, fake, 8, None),
          b"the position bias gradient needs"),
+        (0, lambda: lib.as_csr_position_bias(None, None, None, fake, None, None, 0, 0, 2, 2, (ctypes.c_int32 * 2)(0, 1), 0,
+                                             0, fake, 8, None), b""),
     ]:
         assert call() == status, message
         assert lib.as_last_error().startswith(message), lib.as_last_error()
