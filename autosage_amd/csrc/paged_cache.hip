@@ -3,8 +3,14 @@
 // Tokens stand one behind the other, those of sequence b at token_ptr[b] ..
 // token_ptr[b + 1]; the first of them has position start[b] in its sequence.
 // Tokens from token_ptr[sequences] on belong to no sequence: a write leaves the
-// cache alone for them, a read gives zeros.  A copy (with a rounding to 8 bits
-// in a quantised cache): bound by memory, or by the launch for a few tokens.
+// cache alone for them, a read gives zeros.
+//
+// A copy (with a rounding to 8 bits in a quantised cache): bound by memory, or by
+// the launch for a few tokens.  A workgroup takes up to 16 tokens: its first wave
+// finds their places, then its threads move runs of 8 elements, all tokens of one
+// head before the next head, because the tokens of one head are neighbours in a
+// page.  Enough lanes for a row (a power of two) stand together, so that a row's
+// maximum takes a few shuffles.
 #include "paged_common.h"
 
 namespace as {
@@ -16,86 +22,231 @@ struct TokenRows {
   int64_t stride[2];
 };
 
-// The place of a token: page id (< 0: none) and the token's place in the page.
-struct Place {
-  int64_t page;
-  int slot;
+constexpr int kMaxTokens = 16;  // of one workgroup
+constexpr int kElements = 8;    // of one thread
+constexpr int kAhead = 4;       // runs of a thread whose loads are under way at once
+
+struct Places {
+  int32_t page[kMaxTokens];  // < 0: none
+  int32_t slot[kMaxTokens];
 };
-__device__ __forceinline__ Place place_of_token(const PagedCache& c, const int64_t* __restrict__ token_ptr,
-                                                const int64_t* __restrict__ start, int64_t t) {
-  const int64_t b = wave_row_of_edge(token_ptr, c.sequences, t);
-  const int64_t at = t - token_ptr[b];
-  if (at < 0 || t >= token_ptr[b + 1]) return Place{-1, 0};
-  const int64_t position = start[b] + at;
-  const PageList list = page_list(c, static_cast<int>(b));
-  const int64_t k = position / c.page_size;
-  if (position < 0 || k >= list.count) return Place{-1, 0};
-  const int64_t page = c.page_idx[list.begin + k];
-  if (page < 0 || page >= c.pages) return Place{-1, 0};
-  return Place{page, static_cast<int>(position - k * c.page_size)};
+
+// The places of tokens first .. first + count - 1, by the first wave.
+__device__ __forceinline__ void find_places(const PagedCache& c, const int64_t* __restrict__ token_ptr,
+                                            const int64_t* __restrict__ start, int64_t first, int count,
+                                            Places& places) {
+  if (wave_in_block() == 0) {
+    const int64_t row = uniform_i64(wave_row_of_edge(token_ptr, c.sequences, first));
+    const int b = block_edge_rows(token_ptr, c.sequences, first, count, row);
+    const int64_t t = first + lane_id();
+    if (lane_id() < count) {
+      const int64_t at = t - token_ptr[b];
+      const int64_t begin = start[b];
+      const int64_t position = begin + at;
+      const PageList list = page_list(c, b);
+      // no token of the sequence, or a position in front of it or beyond its pages
+      const bool none = at < 0 || t >= token_ptr[b + 1] || begin < -at || begin > INT64_MAX / 2 ||
+                        position >= list.count * c.page_size;
+      int64_t page = -1;
+      int64_t k = 0;
+      if (!none) {
+        k = position / c.page_size;
+        page = c.page_idx[list.begin + k];
+      }
+      places.page[lane_id()] = page < 0 || page >= c.pages ? -1 : static_cast<int32_t>(page);
+      places.slot[lane_id()] = static_cast<int32_t>(none ? 0 : position - k * c.page_size);
+    }
+  }
+  __syncthreads();
 }
 
-// One wave per row of one token, head and tensor.
+// Runs of a row: the last one is moved back to end with the row (elements that
+// two runs share are moved twice), so that only rows of fewer than 8 elements
+// are moved one by one.  The accesses ask for the alignment of one byte: the
+// hardware has no other requirement.
+__device__ __forceinline__ int run_start(int d, int width) {
+  const int last = width > kElements ? width - kElements : 0;
+  return d < last ? d : last;
+}
+template <typename E>
+__device__ __forceinline__ RawVec<kElements * sizeof(E)> load_elements(const E* from, int width) {
+  RawVec<kElements * sizeof(E)> r;
+  if (width >= kElements) {
+    __builtin_memcpy(&r, from, sizeof(r));
+  } else {
+    E part[kElements];
+#pragma unroll
+    for (int i = 0; i < kElements; ++i) part[i] = from[i < width ? i : width - 1];
+    __builtin_memcpy(&r, part, sizeof(r));
+  }
+  return r;
+}
+template <typename E>
+__device__ __forceinline__ void store_elements(E* to, int width, const RawVec<kElements * sizeof(E)>& r) {
+  if (width >= kElements) {
+    __builtin_memcpy(to, &r, sizeof(r));
+  } else {
+    E part[kElements];
+    __builtin_memcpy(part, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < kElements; ++i) {
+      if (i < width) to[i] = part[i];
+    }
+  }
+}
+
+// Lane, token and head of a thread's item.
+struct Item {
+  int run;
+  int token;
+  int head;
+};
+__device__ __forceinline__ Item item_of(int i, int log_runs, int log_tokens) {
+  const int r = i >> log_runs;
+  return Item{i & ((1 << log_runs) - 1), r & ((1 << log_tokens) - 1), r >> log_tokens};
+}
+
+template <typename T, typename C>
+__device__ __forceinline__ void write_rows(const TokenRows& from, const PageTensor& to, const Places& places,
+                                           int64_t first, int count, int heads, int log_runs, int log_tokens) {
+  const int items = heads << (log_runs + log_tokens);
+  for (int i0 = threadIdx.x; i0 < items; i0 += kAhead * kBlock) {
+    RawVec<kElements * sizeof(T)> raw[kAhead];
+    bool active[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const Item it = item_of(i0 + u * kBlock, log_runs, log_tokens);
+      active[u] = it.head < heads && it.token < count && it.run * kElements < to.width && places.page[it.token] >= 0;
+      const T* x = static_cast<const T*>(from.data);
+      if (active[u])
+        raw[u] = load_elements(x + (first + it.token) * from.stride[0] + it.head * from.stride[1] +
+                                   run_start(it.run * kElements, to.width), to.width);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const Item it = item_of(i0 + u * kBlock, log_runs, log_tokens);
+      int64_t page = 0;
+      int64_t slot = 0;
+      if (active[u]) {
+        page = places.page[it.token];
+        slot = places.slot[it.token];
+      }
+      C* y = static_cast<C*>(to.data) + page * to.stride[0] + it.head * to.stride[1] + slot * to.stride[2] +
+             run_start(it.run * kElements, to.width);
+      if constexpr (__is_same(T, C)) {
+        if (active[u]) store_elements(y, to.width, raw[u]);
+      } else {
+        float x[kElements];
+        float largest = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kElements; ++k) {
+          x[k] = active[u] ? Elem<T>::get(raw[u].w, k) : 0.0f;
+          largest = fmaxf(largest, finite(x[k]) ? fabsf(x[k]) : 0.0f);
+        }
+        for (int o = 1; o < 1 << log_runs; o <<= 1) largest = fmaxf(largest, __shfl_xor(largest, o, 64));
+        const int e = row_exponent(largest);
+        const float scale = power_of_two(-e);
+        RawVec<kElements> codes;
+#pragma unroll
+        for (int k = 0; k < kElements / 4; ++k)
+          codes.w[k] = e4m3_pair(x[4 * k] * scale, x[4 * k + 1] * scale) |
+                       e4m3_pair(x[4 * k + 2] * scale, x[4 * k + 3] * scale) << 16;
+        if (active[u]) {
+          store_elements(y, to.width, codes);
+          if (it.run == 0)
+            to.exponents[page * to.exponent_stride[0] + it.head * to.exponent_stride[1] +
+                         slot * to.exponent_stride[2]] = static_cast<int8_t>(e);
+        }
+      }
+    }
+  }
+}
+
+template <typename C, typename T>
+__device__ __forceinline__ void read_rows(const PageTensor& from, const TokenRows& to, const Places& places,
+                                          int64_t first, int count, int heads, int log_runs, int log_tokens) {
+  const int items = heads << (log_runs + log_tokens);
+  for (int i0 = threadIdx.x; i0 < items; i0 += kAhead * kBlock) {
+    RawVec<kElements * sizeof(C)> raw[kAhead];
+    int e[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const Item it = item_of(i0 + u * kBlock, log_runs, log_tokens);
+      e[u] = 0;
+#pragma unroll
+      for (uint32_t& w : raw[u].w) w = 0u;  // zero in every type
+      if (it.head < heads && it.token < count && it.run * kElements < from.width && places.page[it.token] >= 0) {
+        const int64_t page = places.page[it.token];
+        const int64_t slot = places.slot[it.token];
+        raw[u] = load_elements(static_cast<const C*>(from.data) + page * from.stride[0] + it.head * from.stride[1] +
+                                   slot * from.stride[2] + run_start(it.run * kElements, from.width), from.width);
+        if constexpr (!__is_same(T, C))
+          e[u] = from.exponents[page * from.exponent_stride[0] + it.head * from.exponent_stride[1] +
+                                slot * from.exponent_stride[2]];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const Item it = item_of(i0 + u * kBlock, log_runs, log_tokens);
+      if (it.head >= heads || it.token >= count || it.run * kElements >= from.width) continue;
+      T* y = static_cast<T*>(to.data) + (first + it.token) * to.stride[0] + it.head * to.stride[1] +
+             run_start(it.run * kElements, from.width);
+      if constexpr (__is_same(T, C)) {
+        store_elements(y, from.width, raw[u]);
+      } else {
+        T values[kElements];
+#pragma unroll
+        for (int k = 0; k < kElements; ++k)
+          values[k] = rounded<T>(ldexpf(e4m3_value(static_cast<uint8_t>(raw[u].w[k / 4] >> (8 * (k % 4)))), e[u]));
+        RawVec<kElements * sizeof(T)> r;
+        __builtin_memcpy(&r, values, sizeof(r));
+        store_elements(y, from.width, r);
+      }
+    }
+  }
+}
+
+struct RowShape {
+  int log_tokens;
+  int log_key_runs;
+  int log_value_runs;
+};
+
 template <typename T, typename C>
 __global__ __launch_bounds__(kBlock) void paged_write_kernel(PagedCache c, TokenRows key, TokenRows value,
                                                              const int64_t* __restrict__ token_ptr,
-                                                             const int64_t* __restrict__ start, int64_t tokens) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave_in_block();
-  if (row >= tokens * c.heads * 2) return;
-  const bool is_value = row & 1;
-  const int64_t t = (row >> 1) / c.heads;
-  const int h = static_cast<int>((row >> 1) - t * c.heads);
-  const Place place = place_of_token(c, token_ptr, start, t);
-  if (place.page < 0) return;
-  const TokenRows& from = is_value ? value : key;
-  const PageTensor& to = is_value ? c.value : c.key;
-  const T* x = static_cast<const T*>(from.data) + t * from.stride[0] + h * from.stride[1];
-  C* y = static_cast<C*>(to.data) + place.page * to.stride[0] + h * to.stride[1] + place.slot * to.stride[2];
-  if constexpr (__is_same(T, C)) {
-    for (int i = lane_id(); i < to.width; i += kWave) y[i] = x[i];
-  } else {
-    float largest = 0.0f;
-    for (int i = lane_id(); i < to.width; i += kWave) {
-      const float v = Elem<T>::at(x, i);
-      largest = fmaxf(largest, finite(v) ? fabsf(v) : 0.0f);
-    }
-    const int e = row_exponent(wave_max_f32(largest));
-    const float scale = power_of_two(-e);
-    for (int i = lane_id(); i < to.width; i += kWave) {
-      y[i].bits = static_cast<uint8_t>(e4m3_pair(Elem<T>::at(x, i) * scale, 0.0f));
-    }
-    if (lane_id() == 0)
-      to.exponents[place.page * to.exponent_stride[0] + h * to.exponent_stride[1] +
-                   place.slot * to.exponent_stride[2]] = static_cast<int8_t>(e);
-  }
+                                                             const int64_t* __restrict__ start, int64_t tokens,
+                                                             RowShape shape) {
+  __shared__ Places places;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) << shape.log_tokens;
+  const int64_t left = tokens - first;
+  const int count = left < (1 << shape.log_tokens) ? static_cast<int>(left) : 1 << shape.log_tokens;
+  find_places(c, token_ptr, start, first, count, places);
+  write_rows<T, C>(key, c.key, places, first, count, c.heads, shape.log_key_runs, shape.log_tokens);
+  write_rows<T, C>(value, c.value, places, first, count, c.heads, shape.log_value_runs, shape.log_tokens);
 }
 
 template <typename C, typename T>
 __global__ __launch_bounds__(kBlock) void paged_read_kernel(PagedCache c, TokenRows key, TokenRows value,
                                                             const int64_t* __restrict__ token_ptr,
-                                                            const int64_t* __restrict__ start, int64_t tokens) {
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave_in_block();
-  if (row >= tokens * c.heads * 2) return;
-  const bool is_value = row & 1;
-  const int64_t t = (row >> 1) / c.heads;
-  const int h = static_cast<int>((row >> 1) - t * c.heads);
-  const Place place = place_of_token(c, token_ptr, start, t);
-  const PageTensor& from = is_value ? c.value : c.key;
-  const TokenRows& to = is_value ? value : key;
-  T* y = static_cast<T*>(to.data) + t * to.stride[0] + h * to.stride[1];
-  if (place.page < 0) {
-    for (int i = lane_id(); i < from.width; i += kWave) y[i] = T{};
-    return;
-  }
-  const C* x = static_cast<const C*>(from.data) + place.page * from.stride[0] + h * from.stride[1] +
-               place.slot * from.stride[2];
-  if constexpr (__is_same(T, C)) {
-    for (int i = lane_id(); i < from.width; i += kWave) y[i] = x[i];
-  } else {
-    const int e = from.exponents[place.page * from.exponent_stride[0] + h * from.exponent_stride[1] +
-                                 place.slot * from.exponent_stride[2]];
-    for (int i = lane_id(); i < from.width; i += kWave) y[i] = rounded<T>(ldexpf(Elem<C>::at(x, i), e));
-  }
+                                                            const int64_t* __restrict__ start, int64_t tokens,
+                                                            RowShape shape) {
+  __shared__ Places places;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) << shape.log_tokens;
+  const int64_t left = tokens - first;
+  const int count = left < (1 << shape.log_tokens) ? static_cast<int>(left) : 1 << shape.log_tokens;
+  find_places(c, token_ptr, start, first, count, places);
+  read_rows<C, T>(c.key, key, places, first, count, c.heads, shape.log_key_runs, shape.log_tokens);
+  read_rows<C, T>(c.value, value, places, first, count, c.heads, shape.log_value_runs, shape.log_tokens);
+}
+
+// Tokens of a workgroup: 16, fewer while that leaves fewer than 1,024 workgroups.
+RowShape row_shape(const PagedCache& c, int64_t tokens) {
+  RowShape s{};
+  while ((kElements << s.log_key_runs) < c.key.width) ++s.log_key_runs;
+  while ((kElements << s.log_value_runs) < c.value.width) ++s.log_value_runs;
+  while ((2 << s.log_tokens) <= kMaxTokens && tokens >> (s.log_tokens + 1) >= 1024) ++s.log_tokens;
+  return s;
 }
 
 int check_tokens(const PagedCache& c, const void* key, const void* value, const int64_t* token_ptr,
@@ -104,7 +255,7 @@ int check_tokens(const PagedCache& c, const void* key, const void* value, const 
     return fail(AS_ERR_INVALID_ARGUMENT, "dtype must be AS_DTYPE_F32, AS_DTYPE_BF16 or AS_DTYPE_F16");
   if (cache_dtype != AS_DTYPE_E4M3 && cache_dtype != dtype)
     return fail(AS_ERR_INVALID_ARGUMENT, "a cache that is not quantised holds the type of its tokens");
-  if (tokens < 0 || tokens > (int64_t(1) << 40) / c.heads) return fail(AS_ERR_UNSUPPORTED, "too many tokens");
+  if (tokens < 0 || tokens > kMaxBlocksPerLaunch * kMaxTokens) return fail(AS_ERR_UNSUPPORTED, "at most 2^26 tokens");
   if (tokens > 0 && c.sequences < 1) return fail(AS_ERR_INVALID_ARGUMENT, "tokens without sequences");
   if (tokens > 0 && (key == nullptr || value == nullptr || token_ptr == nullptr || start == nullptr))
     return fail(AS_ERR_INVALID_ARGUMENT, "null pointer argument");
@@ -133,14 +284,15 @@ int as_paged_cache_write(const as_paged_cache* cache, const void* key, const int
   if (tokens == 0) return AS_OK;
   const TokenRows k{const_cast<void*>(key), {key_strides[0], key_strides[1]}};
   const TokenRows v{const_cast<void*>(value), {value_strides[0], value_strides[1]}};
-  const dim3 grid(static_cast<unsigned>((tokens * c.heads * 2 + kWavesPerBlock - 1) / kWavesPerBlock));
+  const RowShape shape = row_shape(c, tokens);
+  const dim3 grid(static_cast<unsigned>(((tokens - 1) >> shape.log_tokens) + 1));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
     if (cache->dtype == AS_DTYPE_E4M3) {
-      paged_write_kernel<T, E4m3><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens);
+      paged_write_kernel<T, E4m3><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
     } else {
-      paged_write_kernel<T, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens);
+      paged_write_kernel<T, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
     }
     return check_launch("paged_cache_write");
   });
@@ -155,14 +307,15 @@ int as_paged_cache_read(const as_paged_cache* cache, void* key, void* value, con
   if (tokens == 0) return AS_OK;
   const TokenRows k{key, {int64_t(c.heads) * c.key.width, c.key.width}};
   const TokenRows v{value, {int64_t(c.heads) * c.value.width, c.value.width}};
-  const dim3 grid(static_cast<unsigned>((tokens * c.heads * 2 + kWavesPerBlock - 1) / kWavesPerBlock));
+  const RowShape shape = row_shape(c, tokens);
+  const dim3 grid(static_cast<unsigned>(((tokens - 1) >> shape.log_tokens) + 1));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
     if (cache->dtype == AS_DTYPE_E4M3) {
-      paged_read_kernel<E4m3, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens);
+      paged_read_kernel<E4m3, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
     } else {
-      paged_read_kernel<T, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens);
+      paged_read_kernel<T, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
     }
     return check_launch("paged_cache_read");
   });

@@ -143,6 +143,19 @@ def test_second_gradient():
     assert torch.allclose(second.double().cpu(), want, rtol=1e-4, atol=1e-4)
 
 
+def test_the_registered_operators():
+    crow, col = case_graph(500, 9, seed=12)
+    d_crow, d_col = to_dev(crow, col)
+    table = torch.randn(32, 3, device="cuda", requires_grad=True)
+    weights = torch.randn(3, len(col), device="cuda")
+    gradients = []
+    for out in (autosage_amd.csr_position_bias(d_crow, d_col, table, max_distance=90),
+                torch.ops.autosage.csr_position_bias(d_crow, d_col, None, table, 90, True)[0]):
+        first, = torch.autograd.grad((out * out * weights).sum(), table, create_graph=True)
+        gradients.append((out, first, *torch.autograd.grad((first * first).sum(), table)))
+    assert all(torch.equal(a, b) for a, b in zip(*gradients))
+
+
 def test_the_same_bits_every_time():
     crow, col = case_graph(20000, 30, seed=7, hubs=4, hub_degree=5000)
     one = _check(crow, col, 4, 32, 1000, torch.float32)

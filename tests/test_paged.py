@@ -251,7 +251,7 @@ def test_native_argument_checks_come_before_any_launch():
         (1, lambda: attention(struct(), query=None), b"null pointer argument"),
         (0, lambda: attention(struct(sequences=0)), b""),
         (1, lambda: lib.as_paged_cache_write(struct(), fake, two, fake, two, fake, fake, 2, 2, None), b"a cache that"),
-        (3, lambda: lib.as_paged_cache_write(struct(), fake, two, fake, two, fake, fake, 1 << 50, 0, None), b"too many"),
+        (3, lambda: lib.as_paged_cache_write(struct(), fake, two, fake, two, fake, fake, 1 << 50, 0, None), b"at most 2^26"),
         (1, lambda: lib.as_paged_cache_write(struct(), fake, two, None, two, fake, fake, 2, 0, None), b"null pointer"),
         (1, lambda: lib.as_paged_cache_write(struct(), fake, None, fake, two, fake, fake, 2, 0, None), b"null strides"),
         (0, lambda: lib.as_paged_cache_write(struct(), fake, two, fake, two, fake, fake, 0, 0, None), b""),
