@@ -90,11 +90,11 @@ __device__ __forceinline__ float rounded<float>(float v) {
 }
 template <>
 __device__ __forceinline__ Bf16 rounded<Bf16>(float v) {
-  return Bf16{bf16_bits(v)};
+  return __builtin_bit_cast(Bf16, static_cast<__bf16>(v));  // half to even, in hardware
 }
 template <>
 __device__ __forceinline__ Fp16 rounded<Fp16>(float v) {
-  return Fp16{f16_bits(v)};
+  return __builtin_bit_cast(Fp16, static_cast<_Float16>(v));
 }
 
 // Checks the host's description of a cache and lays it out for the kernels.
