@@ -47,7 +47,29 @@ def _check_rows(name: str, t: torch.Tensor) -> None:
     _require(t.size(-1) == 1 or t.stride(-1) == 1, ValueError, f"the rows of {name} must be contiguous")
 
 
+# Each check asks for everything at once (a call of a few tokens is bound by the
+# host: 10 us of checks one by one, 3 together); only where something is wrong do
+# the conditions run one by one and name the first that fails.
+
+
 def _check_cache(key_pages, value_pages, page_ptr, page_idx, key_exponents, value_exponents) -> None:
+    dtype = key_pages.dtype
+    key_shape, value_shape = key_pages.shape, value_pages.shape
+    if (dtype in _DTYPES and value_pages.dtype is dtype and len(key_shape) == 4 and len(value_shape) == 4
+            and key_shape[:3] == value_shape[:3] and key_pages.numel() > 0 and value_pages.numel() > 0
+            and 1 < key_shape[3] <= MAX_WIDTH and 1 < value_shape[3] <= MAX_WIDTH
+            and key_pages.stride(3) == 1 and value_pages.stride(3) == 1
+            and page_ptr.dtype is torch.long and page_idx.dtype is torch.long and page_ptr.dim() == 1
+            and page_idx.dim() == 1 and page_ptr.numel() >= 1
+            and key_pages.get_device() == value_pages.get_device() == page_ptr.get_device() == page_idx.get_device()):
+        if dtype is not E4M3:
+            if key_exponents is None and value_exponents is None:
+                return
+        elif (key_exponents is not None and value_exponents is not None and key_exponents.dtype is torch.int8
+                and value_exponents.dtype is torch.int8 and key_exponents.shape == key_shape[:3]
+                and value_exponents.shape == key_shape[:3]
+                and key_exponents.get_device() == value_exponents.get_device() == key_pages.get_device()):
+            return
     _require(key_pages.ndim == 4 and value_pages.ndim == 4 and key_pages.shape[:3] == value_pages.shape[:3],
              ValueError, "key_pages and value_pages must have shape [pages, heads, page_size, width]")
     _require(key_pages.dtype in _DTYPES and value_pages.dtype == key_pages.dtype, TypeError,
@@ -76,6 +98,10 @@ def _check_cache(key_pages, value_pages, page_ptr, page_idx, key_exponents, valu
 
 
 def _check_tokens(key_pages, page_ptr, token_ptr, start) -> None:
+    if (token_ptr.dtype is torch.long and start.dtype is torch.long and token_ptr.dim() == 1 and start.dim() == 1
+            and token_ptr.numel() == page_ptr.numel() == start.numel() + 1
+            and token_ptr.get_device() == start.get_device() == key_pages.get_device()):
+        return
     for name, t, more in (("token_ptr", token_ptr, 0), ("start", start, 1)):
         _require(t.dtype in _INTEGERS, TypeError, f"{name} must use integers")
         _require(t.ndim == 1 and t.numel() + more == page_ptr.numel(), ValueError,
@@ -84,6 +110,12 @@ def _check_tokens(key_pages, page_ptr, token_ptr, start) -> None:
 
 
 def _check_new_rows(key, value, key_pages, value_pages) -> None:
+    if (key.dim() == 3 and value.dim() == 3 and key.dtype is value.dtype and key.dtype in _DTYPES
+            and key.dtype is not E4M3 and (key_pages.dtype is key.dtype or key_pages.dtype is E4M3)
+            and key.shape == (value.size(0), key_pages.size(1), key_pages.size(3))
+            and value.shape == (key.size(0), value_pages.size(1), value_pages.size(3))
+            and key.get_device() == value.get_device() == key_pages.get_device()):
+        return
     for name, t, pages in (("key", key, key_pages), ("value", value, value_pages)):
         _require(t.ndim == 3 and t.size(1) == pages.size(1) and t.size(2) == pages.size(3), ValueError,
                  f"{name} must have shape [tokens, heads, width] with the heads and width of {name}_pages")
@@ -115,18 +147,27 @@ class _CacheStruct(ctypes.Structure):
     ]
 
 
+# The same as 64-bit words, which ctypes fills three times as fast.
+_CacheWords = ctypes.c_int64 * (ctypes.sizeof(_CacheStruct) // 8)
 _NO_STRIDES = (0, 0, 0)
 
 
-def _cache_struct(key_pages, value_pages, page_ptr, page_idx, key_exponents, value_exponents) -> _CacheStruct:
+def _cache_struct(key_pages, value_pages, page_ptr, page_idx, key_exponents, value_exponents):
     pages, heads, page_size, width = key_pages.shape
-    coded = key_exponents is not None
-    return _CacheStruct(
-        key_pages.data_ptr(), value_pages.data_ptr(), key_exponents.data_ptr() if coded else None,
-        value_exponents.data_ptr() if coded else None, page_ptr.data_ptr(), page_idx.data_ptr(), page_idx.numel(),
-        page_ptr.numel() - 1, pages, page_size, heads, width, value_pages.size(3), key_pages.stride()[:3],
-        value_pages.stride()[:3], key_exponents.stride() if coded else _NO_STRIDES,
-        value_exponents.stride() if coded else _NO_STRIDES, _DTYPES[key_pages.dtype])
+    key_strides, value_strides = key_pages.stride(), value_pages.stride()
+    if key_exponents is None:
+        key_e = value_e = 0
+        key_e_strides = value_e_strides = _NO_STRIDES
+    else:
+        key_e, value_e = key_exponents.data_ptr(), value_exponents.data_ptr()
+        key_e_strides, value_e_strides = key_exponents.stride(), value_exponents.stride()
+    return _CacheWords(
+        key_pages.data_ptr(), value_pages.data_ptr(), key_e, value_e, page_ptr.data_ptr(), page_idx.data_ptr(),
+        page_idx.numel(), page_ptr.numel() - 1, pages, page_size, heads, width, value_pages.size(3),
+        *key_strides[:3], *value_strides[:3], *key_e_strides, *value_e_strides, _DTYPES[key_pages.dtype])
+
+
+_TwoStrides = ctypes.c_int64 * 2
 
 
 def _long(t: torch.Tensor) -> torch.Tensor:
@@ -220,10 +261,10 @@ def paged_cache_write_impl(key, value, key_pages, value_pages, page_ptr, page_id
     _check_cache(key_pages, value_pages, page_ptr, page_idx, key_exponents, value_exponents)
     _check_tokens(key_pages, page_ptr, token_ptr, start)
     _check_new_rows(key, value, key_pages, value_pages)
-    for name, t in (("key_pages", key_pages), ("value_pages", value_pages), ("key_exponents", key_exponents),
-                    ("value_exponents", value_exponents)):
-        _require(t is None or all(s > 0 for s, n in zip(t.stride(), t.shape) if n > 1), ValueError,
-                 f"{name} must not hold a place twice")
+    for t in (key_pages, value_pages, key_exponents, value_exponents):
+        if t is not None and 0 in t.stride():
+            _require(all(s > 0 for s, n in zip(t.stride(), t.shape) if n > 1), ValueError,
+                     "pages and exponents that are written must not hold a place twice")
     _no_gradient("paged_cache_write", key, value, key_pages, value_pages)
     page_ptr, page_idx, token_ptr, start = _long(page_ptr), _long(page_idx), _long(token_ptr), _long(start)
     tokens = key.size(0)
@@ -245,8 +286,8 @@ def paged_cache_write_impl(key, value, key_pages, value_pages, page_ptr, page_id
     cache = _cache_struct(key_pages, value_pages, page_ptr, page_idx, key_exponents, value_exponents)
     with _native._on(key.device):
         status = lib.as_paged_cache_write(
-            ctypes.byref(cache), key.data_ptr(), (ctypes.c_int64 * 2)(key.stride(0), key.stride(1)), value.data_ptr(),
-            (ctypes.c_int64 * 2)(value.stride(0), value.stride(1)), token_ptr.data_ptr(), start.data_ptr(), tokens,
+            ctypes.byref(cache), key.data_ptr(), _TwoStrides(key.stride(0), key.stride(1)), value.data_ptr(),
+            _TwoStrides(value.stride(0), value.stride(1)), token_ptr.data_ptr(), start.data_ptr(), tokens,
             _DTYPES[key.dtype], _native._stream(key.device))
     _native._raise(status, "autosage::paged_cache_write")
 
@@ -331,6 +372,14 @@ def paged_cache_read(key_pages, value_pages, page_ptr, page_idx, token_ptr, star
 def _check_attention(query, key_pages, lengths, page_ptr, window, bias_table, max_distance, max_length,
                      bidirectional) -> None:
     heads = key_pages.size(1)
+    if (bias_table is None and max_distance is None and window is None and query.dim() == 3
+            and query.size(0) == page_ptr.numel() - 1 == lengths.numel() and query.size(2) == key_pages.size(3)
+            and query.size(1) >= 1 and query.size(1) % heads == 0 and query.dtype in _DTYPES
+            and query.dtype is not E4M3 and (key_pages.dtype is query.dtype or key_pages.dtype is E4M3)
+            and lengths.dtype is torch.long and lengths.dim() == 1
+            and query.get_device() == lengths.get_device() == key_pages.get_device()
+            and (max_length is None or max_length >= 0)):
+        return
     _require(query.ndim == 3 and query.size(0) == page_ptr.numel() - 1 and query.size(2) == key_pages.size(3)
              and query.size(1) >= 1 and query.size(1) % heads == 0, ValueError,
              "query must have shape [sequences, query heads, key width] with a multiple of the cache's heads")
@@ -397,10 +446,10 @@ def _cpu_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, s
     return out.to(query.dtype), lse
 
 
-def paged_attention_impl(query, key_pages, value_pages, page_ptr, page_idx, lengths, scale=1.0, window=None,
+def _attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, scale=1.0, window=None,
                          bias_table=None, max_distance=None, bidirectional=True, max_length=None, key_exponents=None,
                          value_exponents=None, return_lse=False):
-    """(out, lse); lse is empty unless ``return_lse``."""
+    """(out, lse); no lse unless ``return_lse``."""
     _check_cache(key_pages, value_pages, page_ptr, page_idx, key_exponents, value_exponents)
     _check_attention(query, key_pages, lengths, page_ptr, window, bias_table, max_distance, max_length, bidirectional)
     _no_gradient("paged_attention", query, key_pages, value_pages, bias_table)
@@ -414,11 +463,11 @@ def paged_attention_impl(query, key_pages, value_pages, page_ptr, page_idx, leng
         out, lse = _cpu_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, float(scale), window,
                                   bias_table, max_distance, bool(bidirectional), max_length, key_exponents,
                                   value_exponents)
-        return out, lse if return_lse else lse.new_empty(0)
+        return out, lse if return_lse else None
     lib = _need_native()
     sequences, heads_q, _ = query.shape
     out = torch.empty(sequences, heads_q, value_pages.size(3), dtype=query.dtype, device=query.device)
-    lse = torch.empty((sequences, heads_q) if return_lse else 0, dtype=torch.float32, device=query.device)
+    lse = torch.empty(sequences, heads_q, dtype=torch.float32, device=query.device) if return_lse else None
     if sequences == 0:
         return out, lse
     query = _rows(query)
@@ -435,13 +484,19 @@ def paged_attention_impl(query, key_pages, value_pages, page_ptr, page_idx, leng
                             query.device)
     with _native._on(query.device):
         status = lib.as_paged_attention(
-            ctypes.byref(cache), query.data_ptr(), (ctypes.c_int64 * 2)(query.stride(0), query.stride(1)),
-            out.data_ptr(), lse.data_ptr() if return_lse else None, lengths.data_ptr(), group, float(scale),
+            ctypes.byref(cache), query.data_ptr(), _TwoStrides(query.stride(0), query.stride(1)),
+            out.data_ptr(), _native._ptr(lse), lengths.data_ptr(), group, float(scale),
             seen, None if bias_table is None else bias_table.data_ptr(), buckets,
             borders, int(bool(bidirectional)), bound, _DTYPES[query.dtype], ws.data_ptr(), ws.numel(),
             _native._stream(query.device))
     _native._raise(status, "autosage::paged_attention")
     return out, lse
+
+
+def paged_attention_impl(*args, **kwargs):
+    """(out, lse) of the registered operator; lse is empty unless ``return_lse``."""
+    out, lse = _attention(*args, **kwargs)
+    return out, out.new_empty(0, dtype=torch.float32) if lse is None else lse
 
 
 def paged_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, *, scale: float = 1.0,
@@ -466,9 +521,8 @@ def paged_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, 
     page id outside the cache, gives NaN.  ``return_lse`` adds the logarithm of
     the sum of the exponentials, float32 ``[sequences, query heads]``, with which
     results over parts of a sequence can be joined."""
-    out, lse = paged_attention_impl(query, key_pages, value_pages, page_ptr, page_idx, lengths, scale, window,
-                                    bias_table, max_distance, bidirectional, max_length, key_exponents,
-                                    value_exponents, return_lse)
+    out, lse = _attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, scale, window, bias_table,
+                          max_distance, bidirectional, max_length, key_exponents, value_exponents, return_lse)
     return (out, lse) if return_lse else out
 
 

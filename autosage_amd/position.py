@@ -160,6 +160,42 @@ SCHEMAS = {
 }
 
 
+def _bucket_sums(found, grad, buckets):
+    """dL/dtable, with a history where it is differentiated itself."""
+    if torch.is_grad_enabled() and grad.requires_grad:
+        return _BucketSums.apply(grad, found, buckets)
+    return csr_position_bias_backward_impl(found, grad, buckets)
+
+
+# The public function's gradients: the dispatcher's own wrapping of an operator's
+# gradient takes some 100 us a training step, these 50, the kernels 20 (720,000
+# edges, 5 heads).
+class _PositionBias(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, crow, col, positions, max_distance, bidirectional):
+        out, found = csr_position_bias_impl(crow, col, positions, table, max_distance, bidirectional)
+        ctx.save_for_backward(found)
+        ctx.buckets = table.size(0)
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        return _bucket_sums(ctx.saved_tensors[0], grad, ctx.buckets), None, None, None, None, None
+
+
+class _BucketSums(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, grad, found, buckets):
+        ctx.save_for_backward(found)
+        ctx.edges = grad.size(1)
+        return csr_position_bias_backward_impl(found, grad, buckets)
+
+    @staticmethod
+    def backward(ctx, grad_table):
+        # the sum over each bucket's edges is linear: its transpose is the lookup
+        return grad_table.t()[:, ctx.saved_tensors[0][: ctx.edges].long()], None, None
+
+
 def _setup(ctx, inputs, output) -> None:
     ctx.buckets = inputs[3].size(0)
     ctx.save_for_backward(output[1])
@@ -168,44 +204,24 @@ def _setup(ctx, inputs, output) -> None:
 
 
 def _backward(ctx, grad, _):
-    grad_table = None
-    if grad is not None and ctx.needs_input_grad[3]:
-        sums = _BucketSums.apply if torch.is_grad_enabled() else csr_position_bias_backward_impl
-        grad_table = sums(ctx.saved_tensors[0], grad, ctx.buckets)
-    return None, None, None, grad_table, *((None,) * (len(ctx.needs_input_grad) - 4))
+    wanted = grad is not None and ctx.needs_input_grad[3]
+    grad_table = _bucket_sums(ctx.saved_tensors[0], grad, ctx.buckets) if wanted else None
+    return None, None, None, grad_table, None, None
 
 
-def _second_setup(ctx, inputs, output) -> None:
+def _sums_setup(ctx, inputs, output) -> None:
     ctx.save_for_backward(inputs[0])
     ctx.edges = inputs[1].size(1)
 
 
-def _second_backward(ctx, grad_table):
-    # the sum over each bucket's edges is linear: its transpose is the lookup
-    found = ctx.saved_tensors[0][: ctx.edges].long()
-    return None, grad_table.t()[:, found], None
-
-
-# The registered operators' gradients as autograd functions: the dispatcher's own
-# wrapping of a gradient takes some 100 us a training step, the kernels 20 for
-# 720,000 edges and 5 heads.
-class _PositionBias(torch.autograd.Function):
-    forward = staticmethod(csr_position_bias_impl)
-    setup_context = staticmethod(_setup)
-    backward = staticmethod(_backward)
-
-
-class _BucketSums(torch.autograd.Function):
-    forward = staticmethod(csr_position_bias_backward_impl)
-    setup_context = staticmethod(_second_setup)
-    backward = staticmethod(_second_backward)
+def _sums_backward(ctx, grad_table):
+    return None, grad_table.t()[:, ctx.saved_tensors[0][: ctx.edges].long()], None
 
 
 def register_autograd() -> None:
     """Attaches the gradients to the registered operators."""
     torch.library.register_autograd("autosage::csr_position_bias", _backward, setup_context=_setup)
-    torch.library.register_autograd("autosage::csr_position_bias_backward", _second_backward,
-                                    setup_context=_second_setup)
+    torch.library.register_autograd("autosage::csr_position_bias_backward", _sums_backward, setup_context=_sums_setup)
 
 
 def _cpu_position_bias(crow, col, positions, table, max_distance, bidirectional) -> torch.Tensor:
@@ -235,10 +251,9 @@ def csr_position_bias(crow, col, table, *, max_distance: int, bidirectional: boo
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable: {native_load_error()}")
     crow, col, positions = _long(crow), _long(col), _long(positions)
     validate_if_requested(crow, col)
-    args = (crow, col, positions, table, max_distance, bool(bidirectional))
     if torch.is_grad_enabled() and table.requires_grad:
-        return _PositionBias.apply(*args)[0]
-    return csr_position_bias_impl(*args, keep=False)[0]
+        return _PositionBias.apply(table, crow, col, positions, max_distance, bool(bidirectional))
+    return csr_position_bias_impl(crow, col, positions, table, max_distance, bool(bidirectional), keep=False)[0]
 
 
 __all__ = ["bucket_borders", "csr_position_bias", "position_buckets"]

@@ -9,7 +9,7 @@ import torch
 
 import autosage_amd
 from autosage_amd import _native
-from autosage_amd.paged import _cache_struct
+from autosage_amd.paged import _cache_struct, _CacheStruct
 from tests.paged_common import E4M3, Cache, assert_attention, plain_attention, quantised_rows
 
 DTYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -215,7 +215,7 @@ def test_native_argument_checks_come_before_any_launch():
     (k, v, ptr, idx), _ = cache.args("cpu")
 
     def struct(**changes):
-        c = _cache_struct(k, v, ptr, idx, None, None)
+        c = _CacheStruct.from_buffer(_cache_struct(k, v, ptr, idx, None, None))
         for name, what in changes.items():
             setattr(c, name, what)
         return ctypes.byref(c)
