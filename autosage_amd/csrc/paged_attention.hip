@@ -7,9 +7,14 @@
 // Every key and value is read once, from a page and for all query heads that
 // share it: bound by memory from a few thousand tokens on, by the launch below.
 //
-// The work is cut along the tokens into chunks, one workgroup for each chunk
-// and 16 query heads of one key head.  The four waves take turns with tiles of
-// 32 tokens (16 in float32) and keep everything in registers: both products are
+// The work is cut into equal shares: the tiles of 32 tokens of all sequences, one
+// sequence behind the other, are dealt out evenly to the workgroups of 16 query
+// heads of one key head, which find their share from the lengths on the device
+// (the host knows neither the lengths nor, in a captured graph, the batch they
+// belong to).  A share may end inside a sequence and reach over several; each
+// part of a sequence in a share gives a partial result.  One workgroup's four
+// waves take turns with the tiles of a part (16 tokens in float32) and keep
+// everything in registers: both products are
 // matrix instructions of 16 x 16, whose rows are arranged so that the scores
 // come out where the second product wants the weights:
 //
@@ -25,9 +30,10 @@
 // With fewer than 16 heads a key head the other rows of the matrix units are
 // idle, which costs nothing while memory is the bound.  The maximum is the
 // running one, raised only where a score passes it by kSlack, so that most
-// tiles rescale nothing; waves and chunks are joined by (maximum, sum,
-// weighted sum).  In a call whose sequences have one chunk the workgroup
-// writes the result, else a second launch joins the chunks.
+// tiles rescale nothing; waves and parts are joined by (maximum, sum,
+// weighted sum).  A part that is all of a sequence writes the result itself; a
+// second launch joins the parts of the others, and is left out where the host
+// knows that the sequences are short (kSingle tokens: one workgroup each).
 //
 // Precision: 16-bit products are exact in the matrix units and summed in fp32.
 // Weights enter the second product as two 16-bit parts (bf16 keeps 2^-18 of a
@@ -73,15 +79,10 @@ struct AttentionArgs {
   float scale;
   uint32_t page_magic;  // token / page_size = token * page_magic >> (31 + page_shift)
   int page_shift;
-  // Chunks.  Their number is known to the host: per_sequence of them for each
-  // sequence, or (per_sequence = 0) blocks of pages_per_chunk entries of page_idx,
-  // of which sequence b has those from page_ptr[b] / pages_per_chunk + b on.
-  int64_t chunks;
-  int per_sequence;
-  int pages_per_chunk;
-  int chunk_tokens;
-  float2* part_sum;  // [chunks, heads * group] maximum (in powers of two) and sum
-  float* part_out;   // [chunks, heads * group, value width]
+  int shares;         // workgroups of each 16 heads of a key head; 0: one per sequence
+  int2* plan;         // [sequences] of each sequence: its first part's number, and how many it has
+  float2* part_sum;   // [parts, heads * group] maximum (in powers of two) and sum
+  float* part_out;    // [parts, heads * group, value width]
 };
 
 __device__ __forceinline__ int page_of_token(const AttentionArgs& a, int t) {
@@ -103,51 +104,108 @@ __device__ __forceinline__ Seen seen_tokens(const AttentionArgs& a, int b, const
   return Seen{static_cast<int>(begin), static_cast<int>(length), bad};
 }
 
-// Chunk k of a sequence covers chunk_tokens tokens from the 8-aligned start of
-// what is seen (the start itself where pages are no multiple of 8 tokens).
+constexpr int kPiece = 32;  // tokens; what is dealt out
+constexpr int kMinShare = 4;  // pieces of a share at least, one for each wave
+
+// The first token of a sequence's pieces: the 8-aligned start of what is seen (the
+// start itself where pages are no multiple of 8 tokens).
 __device__ __forceinline__ int first_token(const AttentionArgs& a, const Seen& seen) {
   return a.cache.page_size % 8 == 0 ? seen.begin & ~7 : seen.begin;
 }
-__device__ __forceinline__ int chunk_count(const AttentionArgs& a, const Seen& seen) {
+// Every sequence has a piece, so that one without tokens is visited too.
+__device__ __forceinline__ int piece_count(const AttentionArgs& a, const Seen& seen) {
   const int n = seen.end - first_token(a, seen);
-  return n <= 0 ? 0 : (n + a.chunk_tokens - 1) / a.chunk_tokens;
+  return n <= kPiece ? 1 : (n + kPiece - 1) / kPiece;
 }
-__device__ __forceinline__ int64_t first_chunk(const AttentionArgs& a, int b) {
-  if (a.per_sequence > 0) return static_cast<int64_t>(b) * a.per_sequence;
-  const uint32_t begin = static_cast<uint32_t>(page_list(a.cache, b).begin);
-  return static_cast<int64_t>(begin / static_cast<uint32_t>(a.pages_per_chunk)) + b;
+__device__ __forceinline__ int piece_count(const AttentionArgs& a, int b) {
+  const PageList list = page_list(a.cache, b);
+  return piece_count(a, seen_tokens(a, b, list));
 }
-// The sequence of a chunk, by the whole wave: the last whose first chunk is not behind it.
-__device__ __forceinline__ int sequence_of_chunk(const AttentionArgs& a, int64_t chunk) {
-  if (a.per_sequence > 0) return static_cast<int>(static_cast<uint32_t>(chunk) / static_cast<uint32_t>(a.per_sequence));
-  int lo = 0;
-  int hi = a.cache.sequences;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 63) / 64;
-    const int probe = lo + lane_id() * step;
-    const uint64_t below = __ballot(probe < hi && first_chunk(a, probe) <= chunk);
-    if (below != 0) lo += (63 - __builtin_clzll(below)) * step;
-    hi = lo + step < hi ? lo + step : hi;
+
+__device__ __forceinline__ int64_t wave_incl_scan_i64(int64_t v) {
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int64_t t = __shfl_up(v, o, kWave);
+    if (lane_id() >= o) v += t;
   }
-  return lo;
+  return v;
 }
+
+// A workgroup's share: pieces first .. end - 1 of all, `size` of them in every
+// share but the last; sequence b holds the first one and begins at piece `at`.
+struct Share {
+  int64_t first, end, size;
+  int64_t at;
+  int b;
+};
+// By every wave of the workgroup: the sequences' pieces are summed, lane l taking
+// `each` sequences from l * each on, then those of the lane that holds `first`,
+// 64 at a time.
+__device__ __forceinline__ Share share_of(const AttentionArgs& a, int i) {
+  const int n = a.cache.sequences;
+  const int each = (n + kWave - 1) / kWave;
+  int64_t mine = 0;
+  const int from = lane_id() * each;
+  const int to = from + each < n ? from + each : n;
+  for (int b = from; b < to; ++b) mine += piece_count(a, b);
+  const int64_t upto = wave_incl_scan_i64(mine);
+  const int64_t all = __shfl(upto, kWave - 1, kWave);
+  Share s;
+  s.size = (all + a.shares - 1) / a.shares;
+  s.size = s.size < kMinShare ? kMinShare : s.size;
+  s.first = s.size * i;
+  s.end = s.first + s.size < all ? s.first + s.size : all;
+  s.at = 0;
+  s.b = 0;
+  if (s.first >= all) return s;
+  const int holder = 63 - __builtin_clzll(__ballot(upto - mine <= s.first));
+  s.at = __shfl(upto - mine, holder, kWave);
+  s.b = holder * each;
+  for (int b0 = s.b; each > 1; b0 += kWave) {
+    const int b = b0 + lane_id();
+    const int64_t own = b < n ? piece_count(a, b) : 0;
+    const int64_t before = s.at + wave_incl_scan_i64(own) - own;
+    const uint64_t below = __ballot(b < n && before <= s.first);
+    const int last = 63 - __builtin_clzll(below | 1);
+    const int64_t next = __shfl(before + own, kWave - 1, kWave);
+    if (next > s.first || b0 + kWave >= n) {
+      s.at = __shfl(before, last, kWave);
+      s.b = b0 + last;
+      break;
+    }
+    s.at = next;
+  }
+  // the same in every lane
+  s.size = uniform_i64(s.size);
+  s.first = uniform_i64(s.first);
+  s.end = uniform_i64(s.end);
+  s.at = uniform_i64(s.at);
+  s.b = uniform_i32(s.b);
+  return s;
+}
+
+// How a call reaches the rows of its tokens.  kBlocks8: pages are a multiple of 8
+// tokens, so that the blocks of 8 which a lane works on lie in one page each, and
+// the exponents of a page's tokens are neighbours.  kTokens: every token is looked
+// up.  kNarrow: so it is, and rows of fewer than 8 elements are read one at a time.
+enum Mode { kBlocks8, kTokens, kNarrow };
 
 // ---- rows of a page ------------------------------------------------------------
 // A lane reads runs of N neighbouring elements.  Where a row does not fill the
 // kernel's width, a run that would pass its end is moved back to end with it, so
 // that no load needs a guard: the elements it then shares with the run before
 // have zeros on the queries' side of the scores, and are the same columns twice
-// on the values' side.  NARROW: rows of fewer than 8 elements, one at a time.
+// on the values' side.
 __device__ __forceinline__ int run_start(int d, int n, int width) {
   const int last = width > n ? width - n : 0;
   return d < last ? d : last;
 }
 
 // The loads ask for the alignment of one byte: the hardware has no other requirement.
-template <typename C, int N, bool NARROW>
+template <typename C, int N, int MODE>
 __device__ __forceinline__ RawVec<N * sizeof(C)> load_run(const C* __restrict__ row, int start, int width) {
   RawVec<N * sizeof(C)> r;
-  if constexpr (!NARROW) {
+  if constexpr (MODE != kNarrow) {
     __builtin_memcpy(&r, row + start, sizeof(r));
   } else {
     C part[N];
@@ -233,7 +291,7 @@ struct WeightParts {
 
 // ---- one workgroup -----------------------------------------------------------------
 
-template <typename T, typename C, int W, bool NARROW>
+template <typename T, typename C, int W, int MODE>
 __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a, PositionMap map) {
   constexpr bool kF32 = sizeof(C) == 4;
   constexpr bool kCoded = sizeof(C) == 1;
@@ -264,24 +322,57 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
   const int n = lane & 15;
   const int g = lane >> 4;
   const int wave = uniform_i32(wave_in_block());
-  const int64_t chunk = blockIdx.x;
-  const int b = uniform_i32(sequence_of_chunk(a, chunk));
-  const int k = uniform_i32(static_cast<int>(chunk - first_chunk(a, b)));
-  const int h = static_cast<int>(blockIdx.y) / a.head_tiles;
-  const int tile_of_heads = static_cast<int>(blockIdx.y) - h * a.head_tiles;
+  // the heads of a share follow one another: they share its pages
+  const int units = c.heads * a.head_tiles;
+  const int share_index = static_cast<int>(blockIdx.x / static_cast<unsigned>(units));
+  const int unit = static_cast<int>(blockIdx.x) - share_index * units;
+  const int h = unit / a.head_tiles;
+  const int tile_of_heads = unit - h * a.head_tiles;
   const int heads_q = c.heads * a.group;
   const int head0 = h * a.group + tile_of_heads * kHeads;
   const int heads_here = a.group - tile_of_heads * kHeads < kHeads ? a.group - tile_of_heads * kHeads : kHeads;
 
+  Share share{0, 1, 1, 0, share_index};
+  if (a.shares > 0) {
+    share = share_of(a, share_index);
+    if (share.first >= share.end) return;
+  }
+
+  const float to_log2 = a.scale * kLog2e;
+  const C* key_base = static_cast<const C*>(c.key.data) + h * c.key.stride[1];
+  const C* value_base = static_cast<const C*>(c.value.data) + h * c.value.stride[1];
+  const int64_t key_step = c.key.stride[2];
+  const int64_t value_step = c.value.stride[2];
+  // tokens of this lane: the first of those it loads keys of (the other is 4 further), and of those it weighs
+  const int key_token = kF32 ? n : (n >> 2) * 8 + (n & 3);
+  const int own_token = g * kOwn;
+  int value_at[kBlocks];
+#pragma unroll
+  for (int j = 0; j < kBlocks; ++j) value_at[j] = run_start(j * 128 + n * kRun, kRun, c.value.width);
+
+  int64_t at = share.at;
+  for (int b = uniform_i32(share.b); b < c.sequences && at < share.end; ++b) {
   const PageList list = page_list(c, b);
   const Seen seen = seen_tokens(a, b, list);
-  const int count = chunk_count(a, seen);
-  if (k < 0 || (k > 0 && k >= count)) return;  // chunk 0 of a sequence without tokens writes its zeros
-  const int base = first_token(a, seen) + k * a.chunk_tokens;
+  const int pieces = a.shares > 0 ? piece_count(a, seen) : 1;
+  // pieces from .. to - 1 of this sequence are in the share
+  const int from_piece = share.first > at ? static_cast<int>(share.first - at) : 0;
+  const int to_piece = share.end < at + pieces ? static_cast<int>(share.end - at) : pieces;
+  const bool whole = from_piece == 0 && to_piece == pieces;
+  const int64_t part = static_cast<int64_t>(share_index) + b;
+  if (a.shares > 0 && unit == 0 && from_piece == 0 && threadIdx.x == 0)
+    a.plan[b] = make_int2(static_cast<int>(part),
+                          static_cast<int>((at + pieces - 1) / share.size - at / share.size) + 1);
+  at += pieces;
+  const int origin = first_token(a, seen);
+  const int base = origin + from_piece * kPiece;
   const int begin = base > seen.begin ? base : seen.begin;
-  const int end = base + a.chunk_tokens < seen.end ? base + a.chunk_tokens : seen.end;
+  const int stop = a.shares > 0 ? origin + to_piece * kPiece : seen.end;
+  const int end = stop < seen.end ? stop : seen.end;
+  const int64_t* pages = c.page_idx + list.begin;
 
   if (a.table != nullptr) {
+    // once in front of every part: the parts' results lie in the same place
     const int buckets = map.both_sides ? 2 * map.side : map.side;
     stage_borders(border, map);
     for (int i = threadIdx.x; i < buckets * kHeads; i += kBlock) {
@@ -305,7 +396,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
     for (int j = 0; j < kKeyRuns; ++j) {
       const int d = (j * 4 + g) * kKeyRun;
       key_at[j] = run_start(d, kKeyRun, c.key.width);
-      const RawVec<kKeyRun * sizeof(T)> raw = load_run<T, kKeyRun, NARROW>(q_row, key_at[j], c.key.width);
+      const RawVec<kKeyRun * sizeof(T)> raw = load_run<T, kKeyRun, MODE>(q_row, key_at[j], c.key.width);
       key_own[j] = 0;
       float q[kKeyRun];
 #pragma unroll
@@ -328,109 +419,103 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
       }
     }
   }
-  int value_at[kBlocks];
-#pragma unroll
-  for (int j = 0; j < kBlocks; ++j) value_at[j] = run_start(j * 128 + n * kRun, kRun, c.value.width);
-
   f32x4 acc[kValues];
   float top;  // of head n, the same in its four lanes
   float sum;  // of head n and the tokens of this lane
 
-  const float to_log2 = a.scale * kLog2e;
-  const C* key_base = static_cast<const C*>(c.key.data) + h * c.key.stride[1];
-  const C* value_base = static_cast<const C*>(c.value.data) + h * c.value.stride[1];
-  const int8_t* key_e_base = kCoded ? c.key.exponents + h * c.key.exponent_stride[1] : nullptr;
-  const int8_t* value_e_base = kCoded ? c.value.exponents + h * c.value.exponent_stride[1] : nullptr;
-  const int64_t* pages = c.page_idx + list.begin;
-  const bool aligned8 = c.page_size % 8 == 0;
-  // tokens of this lane: the first of those it loads keys of (the other is 4 further), and of those it weighs
-  const int key_token = kF32 ? n : (n >> 2) * 8 + (n & 3);
-  const int own_token = g * kOwn;
+  // What a tile needs from memory.
+  struct Tile {
+    RawVec<kKeyRun * sizeof(C)> key[kKeyRows][kKeyRuns];
+    RawVec<kRun * sizeof(C)> value[kOwn];            // the first block
+    const C* value_row[kBlocks == 1 ? 1 : (MODE == kBlocks8 ? 1 : kOwn)];  // where the others are
+    RawVec<8> key_e, value_e;                        // exponents of the tokens this lane weighs, a byte each
+    uint32_t bad_tokens;                             // tokens whose page is outside the cache, a bit each
+  };
+  const auto is_bad = [&](int64_t id) { return id < 0 || id >= c.pages; };
+  const auto load_rows = [&](Tile& tile, int s, const C* key_row) {
+#pragma unroll
+    for (int j = 0; j < kKeyRuns; ++j) tile.key[s][j] = load_run<C, kKeyRun, MODE>(key_row, key_at[j], c.key.width);
+  };
+  const auto load_tile = [&](Tile& tile, int t0) {
+    if constexpr (MODE == kBlocks8) {
+      // a block behind what is seen stands for its last one
+      const int last = (end - 1) & ~7;
+      int t = (t0 + key_token) & ~7;
+      t = t < last ? t : last;
+      int entry = page_of_token(a, t);
+      int slot = t - entry * c.page_size + (key_token & 7);
+      int64_t page = pages[entry];
+      page = is_bad(page) ? 0 : page;
+      const C* row = key_base + page * c.key.stride[0] + slot * key_step;
+#pragma unroll
+      for (int s = 0; s < kKeyRows; ++s) load_rows(tile, s, row + s * 4 * key_step);
+      t = (t0 + own_token) & ~7;
+      t = t < last ? t : last;
+      entry = page_of_token(a, t);
+      slot = t - entry * c.page_size + (own_token & 7);
+      page = pages[entry];
+      const bool bad = is_bad(page);
+      page = bad ? 0 : page;
+      tile.bad_tokens = bad ? 0xffu : 0u;
+      row = value_base + page * c.value.stride[0] + slot * value_step;
+#pragma unroll
+      for (int e = 0; e < kOwn; ++e) tile.value[e] = load_run<C, kRun, MODE>(row + e * value_step, value_at[0], c.value.width);
+      if constexpr (kBlocks > 1) tile.value_row[0] = row;
+      if constexpr (kCoded) {
+        __builtin_memcpy(&tile.key_e, c.key.exponents + page * c.key.exponent_stride[0] +
+                                          h * c.key.exponent_stride[1] + slot, 8);
+        __builtin_memcpy(&tile.value_e, c.value.exponents + page * c.value.exponent_stride[0] +
+                                            h * c.value.exponent_stride[1] + slot, 8);
+      }
+    } else {
+      const auto place = [&](int t, int& slot, bool& bad) {
+        t = t < end ? t : end - 1;  // a token behind what is seen stands for the last one
+        const int e = page_of_token(a, t);
+        slot = t - e * c.page_size;
+        const int64_t id = pages[e];
+        bad = is_bad(id);
+        return bad ? int64_t(0) : id;
+      };
+      int slot;
+      bool bad;
+#pragma unroll
+      for (int s = 0; s < kKeyRows; ++s) {
+        const int64_t page = place(t0 + key_token + s * 4, slot, bad);
+        load_rows(tile, s, key_base + page * c.key.stride[0] + slot * key_step);
+      }
+      tile.bad_tokens = 0;
+      uint32_t key_e[2] = {0u, 0u};
+      uint32_t value_e[2] = {0u, 0u};
+#pragma unroll
+      for (int e = 0; e < kOwn; ++e) {
+        const int64_t page = place(t0 + own_token + e, slot, bad);
+        if (bad) tile.bad_tokens |= 1u << e;
+        const C* row = value_base + page * c.value.stride[0] + slot * value_step;
+        tile.value[e] = load_run<C, kRun, MODE>(row, value_at[0], c.value.width);
+        if constexpr (kBlocks > 1) tile.value_row[e] = row;
+        if constexpr (kCoded) {
+          key_e[e / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(
+                              c.key.exponents[page * c.key.exponent_stride[0] + h * c.key.exponent_stride[1] +
+                                              slot * c.key.exponent_stride[2]])) << (8 * (e % 4));
+          value_e[e / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(
+                                c.value.exponents[page * c.value.exponent_stride[0] + h * c.value.exponent_stride[1] +
+                                                  slot * c.value.exponent_stride[2]])) << (8 * (e % 4));
+        }
+      }
+      tile.key_e.w[0] = key_e[0];
+      tile.key_e.w[1] = key_e[1];
+      tile.value_e.w[0] = value_e[0];
+      tile.value_e.w[1] = value_e[1];
+    }
+  };
 
   // Infinite numbers: a repeated element of a key times zero, or an infinite value
   // times a part of its weight that is zero, would be NaN where the result is
   // infinite.  A wave that ends with NaN runs again without the former, with the
   // parts of the weights for finite values and one for the others.  (8-bit numbers
   // have no infinities.)
-  for (bool careful = false;; careful = true) {
-#pragma unroll
-  for (int j = 0; j < kValues; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  top = -INFINITY;
-  sum = 0.0f;
-  for (int t0 = base + wave * kTile; t0 < end; t0 += kWavesPerBlock * kTile) {
-    // the rows of the lane's tokens; a token outside what is seen stands for one whose place exists
-    const C* key_row[kKeyRows];
-    const C* value_row[kOwn];
-    const int8_t* key_e_at[kCoded ? kOwn : 1];
-    const int8_t* value_e_at[kCoded ? kOwn : 1];
-    uint32_t bad_tokens = 0;
-    const auto place = [&](int t, int& slot, bool& bad) {
-      const int e = page_of_token(a, t);
-      slot = t - e * c.page_size;
-      const int64_t id = pages[e];
-      bad = id < 0 || id >= c.pages;
-      return bad ? int64_t(0) : id;
-    };
-    if (aligned8) {
-      // blocks of 8 tokens lie in one page
-      const int last = (end - 1) & ~7;
-      int slot;
-      bool bad;
-      int t = (t0 + key_token) & ~7;
-      int64_t page = place(t < last ? t : last, slot, bad);
-#pragma unroll
-      for (int s = 0; s < kKeyRows; ++s)
-        key_row[s] = key_base + page * c.key.stride[0] + (slot + (key_token & 7) + s * 4) * c.key.stride[2];
-      t = (t0 + own_token) & ~7;
-      page = place(t < last ? t : last, slot, bad);
-      slot += own_token & 7;
-      if (bad) bad_tokens = 0xffu;
-#pragma unroll
-      for (int e = 0; e < kOwn; ++e) {
-        value_row[e] = value_base + page * c.value.stride[0] + (slot + e) * c.value.stride[2];
-        if constexpr (kCoded) {
-          key_e_at[e] = key_e_base + page * c.key.exponent_stride[0] + (slot + e) * c.key.exponent_stride[2];
-          value_e_at[e] = value_e_base + page * c.value.exponent_stride[0] + (slot + e) * c.value.exponent_stride[2];
-        }
-      }
-    } else {
-      int slot;
-      bool bad;
-#pragma unroll
-      for (int s = 0; s < kKeyRows; ++s) {
-        const int t = t0 + key_token + s * 4;
-        const int64_t page = place(t < end ? t : end - 1, slot, bad);
-        key_row[s] = key_base + page * c.key.stride[0] + slot * c.key.stride[2];
-      }
-#pragma unroll
-      for (int e = 0; e < kOwn; ++e) {
-        const int t = t0 + own_token + e;
-        const int64_t page = place(t < end ? t : end - 1, slot, bad);
-        if (bad) bad_tokens |= 1u << e;
-        value_row[e] = value_base + page * c.value.stride[0] + slot * c.value.stride[2];
-        if constexpr (kCoded) {
-          key_e_at[e] = key_e_base + page * c.key.exponent_stride[0] + slot * c.key.exponent_stride[2];
-          value_e_at[e] = value_e_base + page * c.value.exponent_stride[0] + slot * c.value.exponent_stride[2];
-        }
-      }
-    }
-
-    RawVec<kKeyRun * sizeof(C)> key_raw[kKeyRows][kKeyRuns];
-#pragma unroll
-    for (int s = 0; s < kKeyRows; ++s) {
-#pragma unroll
-      for (int j = 0; j < kKeyRuns; ++j) key_raw[s][j] = load_run<C, kKeyRun, NARROW>(key_row[s], key_at[j], c.key.width);
-    }
-    RawVec<kRun * sizeof(C)> value_raw[kBlocks][kOwn];
-#pragma unroll
-    for (int e = 0; e < kOwn; ++e) value_raw[0][e] = load_run<C, kRun, NARROW>(value_row[e], value_at[0], c.value.width);
-    int key_e[kOwn], value_e[kOwn];
-#pragma unroll
-    for (int e = 0; e < (kCoded ? kOwn : 0); ++e) {
-      key_e[e] = *key_e_at[e];
-      value_e[e] = *value_e_at[e];
-    }
-
+  bool careful = false;
+  const auto work_on = [&](const Tile& tile, int t0) {
     f32x4 score[kKeyRows];
 #pragma unroll
     for (int s = 0; s < kKeyRows; ++s) {
@@ -440,13 +525,13 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
         if constexpr (kF32) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint32_t w = key_raw[s][j].w[i];
+            uint32_t w = tile.key[s][j].w[i];
             if (careful && !((key_own[j] >> i) & 1)) w = 0u;
             score[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w), q32[j][i], score[s], 0, 0, 0);
           }
         } else {
           uint32_t w[4];
-          to_words<C, 8>(key_raw[s][j], w);
+          to_words<C, 8>(tile.key[s][j], w);
           if (!kCoded && careful) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -466,7 +551,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
 #pragma unroll
     for (int e = 0; e < kOwn; ++e) {
       s2[e] = score[e / 4][e % 4] * to_log2;
-      if constexpr (kCoded) s2[e] = ldexpf(s2[e], key_e[e]);
+      if constexpr (kCoded) s2[e] = ldexpf(s2[e], static_cast<int8_t>(tile.key_e.w[e / 4] >> (8 * (e % 4))));
     }
     if (a.table != nullptr) {
       // every token of the tile farther than the last border: one number a head
@@ -483,12 +568,12 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
       }
     }
     const bool edge = t0 < begin || t0 + kTile > end;
-    if (edge || __any(bad_tokens != 0)) {
+    if (edge || __any(tile.bad_tokens != 0)) {
 #pragma unroll
       for (int e = 0; e < kOwn; ++e) {
         const int t = t0 + own_token + e;
         const bool out_of_sight = t < begin || t >= end;
-        if ((bad_tokens >> e) & 1) s2[e] = NAN;
+        if ((tile.bad_tokens >> e) & 1) s2[e] = NAN;
         if (out_of_sight) s2[e] = -INFINITY;
       }
     }
@@ -516,7 +601,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
     for (int e = 0; e < kOwn; ++e) {
       weight[e] = __builtin_amdgcn_exp2f(s2[e] - from);
       sum += weight[e];
-      if constexpr (kCoded) weight[e] = ldexpf(weight[e], value_e[e]);
+      if constexpr (kCoded) weight[e] = ldexpf(weight[e], static_cast<int8_t>(tile.value_e.w[e / 4] >> (8 * (e % 4))));
     }
     u32x4 w16[kP];
     u32x4 one16;
@@ -539,12 +624,18 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
       }
     }
 
+    RawVec<kRun * sizeof(C)> value[2][kOwn];
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) value[0][e] = tile.value[e];
 #pragma unroll
     for (int jb = 0; jb < kBlocks; ++jb) {
       if (jb + 1 < kBlocks) {
 #pragma unroll
-        for (int e = 0; e < kOwn; ++e)
-          value_raw[jb + 1][e] = load_run<C, kRun, NARROW>(value_row[e], value_at[jb + 1], c.value.width);
+        for (int e = 0; e < kOwn; ++e) {
+          const C* row = MODE == kBlocks8 ? tile.value_row[0] + e * value_step
+                                          : tile.value_row[kBlocks == 1 || MODE == kBlocks8 ? 0 : e];
+          value[(jb + 1) % 2][e] = load_run<C, kRun, MODE>(row, value_at[(jb + 1) % kBlocks], c.value.width);
+        }
       }
       if (edge) {
         // a value out of sight may be anything; its weight is zero, and so has to be the product
@@ -552,7 +643,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
         for (int e = 0; e < kOwn; ++e) {
           const int t = t0 + own_token + e;
 #pragma unroll
-          for (uint32_t& w : value_raw[jb][e].w) w = t < begin || t >= end ? 0u : w;
+          for (uint32_t& w : value[jb % 2][e].w) w = t < begin || t >= end ? 0u : w;
         }
       }
       if constexpr (kF32) {
@@ -561,12 +652,12 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
 #pragma unroll
           for (int j = 0; j < kRun; ++j)
             acc[jb * kRun + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                weight[e], __uint_as_float(value_raw[jb][e].w[j]), acc[jb * kRun + j], 0, 0, 0);
+                weight[e], __uint_as_float(value[jb % 2][e].w[j]), acc[jb * kRun + j], 0, 0, 0);
         }
       } else {
         uint32_t words[8][kRun / 2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to_words<C, kRun>(value_raw[jb][e % kOwn], words[e]);
+        for (int e = 0; e < 8; ++e) to_words<C, kRun>(value[jb % 2][e % kOwn], words[e]);
 #pragma unroll
         for (int j = 0; j < kRun; ++j) {
           u32x4 column;
@@ -588,15 +679,28 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
         }
       }
     }
-  }
-  if (kCoded || careful) break;
-  bool odd = sum != sum;
+  };
+
+  constexpr int kStride = kWavesPerBlock * kTile;
+  for (;; careful = true) {
 #pragma unroll
-  for (int j = 0; j < kValues; ++j) {
+    for (int j = 0; j < kValues; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    top = -INFINITY;
+    sum = 0.0f;
+    int t0 = base + wave * kTile;
+    for (; t0 < end; t0 += kStride) {
+      Tile tile;
+      load_tile(tile, t0);
+      work_on(tile, t0);
+    }
+    if (kCoded || careful) break;
+    bool odd = sum != sum;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) odd = odd || acc[j][i] != acc[j][i];
-  }
-  if (!__any(odd)) break;
+    for (int j = 0; j < kValues; ++j) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) odd = odd || acc[j][i] != acc[j][i];
+    }
+    if (!__any(odd)) break;
   }
 
   // join the waves
@@ -619,13 +723,12 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
 #pragma unroll
       for (int j = 0; j < kValues; ++j) {
         const int d = value_at[j / kRun] + j % kRun;
-        if (!NARROW || d < c.value.width) wave_out[wave][hh][d] = acc[j][i] * f;
+        if (MODE != kNarrow || d < c.value.width) wave_out[wave][hh][d] = acc[j][i] * f;
       }
     }
   }
   __syncthreads();
   const int width = c.value.width;
-  const bool last = count <= 1;  // the whole sequence is here
   for (int i = threadIdx.x; i < heads_here * width; i += kBlock) {
     const int hh = i / width;
     const int d = i - hh * width;
@@ -640,77 +743,88 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
       total += (mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - most)) * wave_sum[w][hh];
       x += wave_out[w][hh][d];
     }
-    if (last) {
+    if (whole) {
       const int64_t row = static_cast<int64_t>(b) * heads_q + head0 + hh;
       const bool none = total == 0.0f;
       static_cast<T*>(a.out)[row * width + d] = rounded<T>(seen.bad ? NAN : (none ? 0.0f : x / total));
       if (a.lse != nullptr && d == 0)
         a.lse[row] = seen.bad ? NAN : (none ? -INFINITY : (most - U::kShift + __builtin_amdgcn_logf(total)) * kLn2);
     } else {
-      const int64_t row = chunk * heads_q + head0 + hh;
+      const int64_t row = part * heads_q + head0 + hh;
       a.part_out[row * width + d] = x;
       if (d == 0) a.part_sum[row] = make_float2(most, total);
     }
   }
+  __syncthreads();  // the next part's results go where these were
+  }
 }
 
-// Joins the chunks of one sequence and query head: one workgroup, whose waves
-// take turns with the chunks and whose lanes hold the width.
+// Joins the parts of one sequence and query head: one workgroup.  Every wave
+// finds the maximum and the sum of all parts, lane l those with index l mod 64;
+// then the waves take turns with the parts, four at once, and the lanes hold the
+// width.
+constexpr int kJoinWaves = 8;
+constexpr int kJoinAhead = 4;
 template <typename T>
-__global__ __launch_bounds__(kBlock) void paged_attention_join_kernel(AttentionArgs a, float shift) {
-  __shared__ float2 wave_sums[kWavesPerBlock];
-  __shared__ float wave_out[kWavesPerBlock][kMaxWidth];
+__global__ __launch_bounds__(kJoinWaves* kWave) void paged_attention_join_kernel(AttentionArgs a, float shift) {
+  __shared__ float wave_out[kJoinWaves][kMaxWidth];
   const PagedCache& c = a.cache;
   const int heads_q = c.heads * a.group;
   const int b = blockIdx.y;
   const int hq = blockIdx.x;
-  const PageList list = page_list(c, b);
-  const Seen seen = seen_tokens(a, b, list);
-  const int count = chunk_count(a, seen);
+  const int64_t first = a.plan[b].x;
+  const int count = a.plan[b].y;
   if (count <= 1) return;
-  const int64_t first = first_chunk(a, b);
   const int lane = lane_id();
-  const int wave = wave_in_block();
+  const int wave = uniform_i32(wave_in_block());
   const int width = c.value.width;
+  const float2* const sums = a.part_sum + first * heads_q + hq;
+  const float* const rows = a.part_out + (first * heads_q + hq) * width;
+  float top = -INFINITY;
+  float sum = 0.0f;
+  for (int k = lane; k < count; k += kWave) {
+    const float2 part = sums[static_cast<int64_t>(k) * heads_q];
+    const float next = fmaxf(top, part.x);
+    const float base = next == -INFINITY ? 0.0f : next;
+    sum = sum * __builtin_amdgcn_exp2f(top - base) + part.y * __builtin_amdgcn_exp2f(part.x - base);
+    top = next;
+  }
+  const float most = wave_max_f32(top);
+  const float base = most == -INFINITY ? 0.0f : most;
+  const float total = wave_sum_f32(sum * __builtin_amdgcn_exp2f(top - base));
+
   constexpr int kParts = kMaxWidth / kWave;
   float acc[kParts];
 #pragma unroll
   for (int i = 0; i < kParts; ++i) acc[i] = 0.0f;
-  float top = -INFINITY;
-  float sum = 0.0f;
-  for (int k = wave; k < count && first + k < a.chunks; k += kWavesPerBlock) {
-    const int64_t row = (first + k) * heads_q + hq;
-    const float2 part = a.part_sum[row];
-    const float next = fmaxf(top, part.x);
-    const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next);
-    const float f = part.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(part.x - next);
-    top = next;
-    sum = sum * keep + part.y * f;
+  for (int k0 = wave; k0 < count; k0 += kJoinWaves * kJoinAhead) {
+    float f[kJoinAhead];
+    float x[kJoinAhead][kParts];
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) {
-      const int d = lane + i * kWave;
-      if (d < width) acc[i] = acc[i] * keep + a.part_out[row * width + d] * f;
+    for (int u = 0; u < kJoinAhead; ++u) {
+      const int k = k0 + u * kJoinWaves;
+      const int64_t at = static_cast<int64_t>(k < count ? k : count - 1) * heads_q;
+      f[u] = k < count ? __builtin_amdgcn_exp2f(sums[at].x - base) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        const int d = lane + i * kWave;
+        x[u][i] = k < count && d < width ? rows[at * width + d] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kJoinAhead; ++u) {
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) acc[i] = fmaf(f[u], x[u][i], acc[i]);
     }
   }
-  if (lane == 0) wave_sums[wave] = make_float2(top, sum);
 #pragma unroll
-  for (int i = 0; i < kParts; ++i) {
-    if (lane + i * kWave < width) wave_out[wave][lane + i * kWave] = acc[i];
-  }
+  for (int i = 0; i < kParts; ++i) wave_out[wave][lane + i * kWave] = acc[i];
   __syncthreads();
   const int d = threadIdx.x;
   if (d >= width) return;
-  float most = wave_sums[0].x;
-#pragma unroll
-  for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_sums[w].x);
-  float total = 0.0f;
   float x = 0.0f;
 #pragma unroll
-  for (int w = 0; w < kWavesPerBlock; ++w) {
-    const float f = wave_sums[w].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wave_sums[w].x - most);
-    total += wave_sums[w].y * f;
-    x += wave_out[w][d] * f;
-  }
+  for (int w = 0; w < kJoinWaves; ++w) x += wave_out[w][d];
   const int64_t row = static_cast<int64_t>(b) * heads_q + hq;
   const bool none = total == 0.0f;
   static_cast<T*>(a.out)[row * width + d] = rounded<T>(none ? 0.0f : x / total);
@@ -720,62 +834,54 @@ __global__ __launch_bounds__(kBlock) void paged_attention_join_kernel(AttentionA
 
 // ---- launch --------------------------------------------------------------------------
 
-// Workgroups that a call is cut into at least, while a chunk keeps kMinChunk tokens.
-constexpr int64_t kTargetBlocks = 2048;
-constexpr int64_t kMinChunk = 128;
-constexpr int64_t kMaxChunk = 4096;
+// Sequences of at most this many tokens have a workgroup each, and no second launch.
+constexpr int64_t kSingle = 512;
 
-struct Split {
-  int64_t chunks;
-  int64_t per_sequence;
-  int64_t pages_per_chunk;
-  int64_t chunk_tokens;
-};
-Split split_of(const as_paged_cache* c, int64_t group, int64_t window, int64_t max_length) {
+// Shares: two workgroups a CU in one round (64 sequences of 4,096 tokens, 8 key
+// heads, bf16: 5.5 TB/s; 5.1 in three rounds); more of them where sequences are
+// many, so that a share is not many short sequences one after another.
+int64_t share_count(const as_paged_cache* c, int64_t group, int64_t window, int64_t max_length) {
   const int64_t units = c->heads * ((group + kHeads - 1) / kHeads);
-  // tokens of one sequence at most, and of all of them
+  // tokens of one sequence at most
   int64_t longest = c->page_idx_len * c->page_size;
   if (max_length >= 0 && max_length < longest) longest = max_length;
-  if (window > 0 && window + 8 < longest) longest = window + 8;
-  if (longest < 1) longest = 1;
-  int64_t all = c->page_idx_len * c->page_size;
-  if (all > longest * c->sequences) all = longest * c->sequences;
-  int64_t tokens = all * units / kTargetBlocks;
-  tokens = tokens < kMinChunk ? kMinChunk : (tokens > kMaxChunk ? kMaxChunk : tokens);
-  tokens = (tokens + kMinChunk - 1) / kMinChunk * kMinChunk;
-  Split s{};
-  const int64_t each = (longest + tokens - 1) / tokens;
-  if (max_length >= 0 || each == 1) {
-    s.per_sequence = each;
-    s.chunk_tokens = tokens;
-    s.chunks = each * c->sequences;
-  } else {
-    s.pages_per_chunk = (tokens + c->page_size - 1) / c->page_size;
-    s.chunk_tokens = s.pages_per_chunk * c->page_size;
-    s.chunks = c->page_idx_len / s.pages_per_chunk + c->sequences;
-  }
-  return s;
+  if (window > 0 && window < longest) longest = window;
+  if (longest <= kSingle) return 0;
+  const int64_t few = 512 / units < 1 ? 1 : 512 / units;
+  const int64_t many = 4096 / units < c->sequences ? 4096 / units : c->sequences;
+  return few > many ? few : many;
 }
 
-size_t part_bytes(const Split& s, int64_t heads_q, int64_t width) {
-  if (s.per_sequence == 1) return 8;
-  return align_up(static_cast<size_t>(s.chunks) * heads_q * sizeof(float2), 256) +
-         static_cast<size_t>(s.chunks) * heads_q * width * sizeof(float);
+struct Workspace {
+  size_t sums, out, bytes;  // where the parts' sums and results begin behind the plan, and the size of all
+};
+Workspace workspace_of(const as_paged_cache* c, int64_t group, int64_t shares) {
+  if (shares == 0) return Workspace{0, 0, 8};
+  const size_t rows = static_cast<size_t>(shares + c->sequences) * c->heads * group;
+  Workspace w;
+  w.sums = align_up(static_cast<size_t>(c->sequences) * sizeof(int2), 256);
+  w.out = w.sums + align_up(rows * sizeof(float2), 256);
+  w.bytes = w.out + rows * c->value_width * sizeof(float);
+  return w;
 }
 
 template <typename T, typename C, int W>
 void launch_width(const AttentionArgs& a, const PositionMap& map, dim3 grid, hipStream_t s) {
-  if (a.cache.key.width >= 8 && a.cache.value.width >= 8) {
-    paged_attention_kernel<T, C, W, false><<<grid, kBlock, 0, s>>>(a, map);
+  const PagedCache& c = a.cache;
+  const bool neighbours = sizeof(C) > 1 || (c.key.exponent_stride[2] == 1 && c.value.exponent_stride[2] == 1);
+  if (c.key.width < 8 || c.value.width < 8) {
+    paged_attention_kernel<T, C, W, kNarrow><<<grid, kBlock, 0, s>>>(a, map);
+  } else if (c.page_size % 8 == 0 && neighbours) {
+    paged_attention_kernel<T, C, W, kBlocks8><<<grid, kBlock, 0, s>>>(a, map);
   } else {
-    paged_attention_kernel<T, C, W, true><<<grid, kBlock, 0, s>>>(a, map);
+    paged_attention_kernel<T, C, W, kTokens><<<grid, kBlock, 0, s>>>(a, map);
   }
 }
 
 template <typename T, typename C>
 int launch_attention(const AttentionArgs& a, const PositionMap& map, hipStream_t s) {
   const int width = a.cache.key.width > a.cache.value.width ? a.cache.key.width : a.cache.value.width;
-  const dim3 grid(static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.cache.heads * a.head_tiles));
+  const dim3 grid(static_cast<unsigned>((a.shares > 0 ? a.shares : a.cache.sequences) * a.cache.heads * a.head_tiles));
   if (width <= 64) {
     launch_width<T, C, 64>(a, map, grid, s);
   } else if (width <= 128) {
@@ -784,10 +890,10 @@ int launch_attention(const AttentionArgs& a, const PositionMap& map, hipStream_t
     launch_width<T, C, 256>(a, map, grid, s);
   }
   if (const int bad = check_launch("paged_attention")) return bad;
-  if (a.per_sequence == 1) return AS_OK;
+  if (a.shares == 0) return AS_OK;
   paged_attention_join_kernel<T><<<dim3(static_cast<unsigned>(a.cache.heads * a.group),
                                        static_cast<unsigned>(a.cache.sequences)),
-                                   kBlock, 0, s>>>(a, Unit<T, C>::type::kShift);
+                                   kJoinWaves * kWave, 0, s>>>(a, Unit<T, C>::type::kShift);
   return check_launch("paged_attention (join)");
 }
 
@@ -803,7 +909,7 @@ size_t as_paged_attention_workspace_bytes(const as_paged_cache* cache, int64_t g
                                           int64_t max_length) {
   PagedCache c;
   if (read_paged_cache(cache, &c) != AS_OK || group < 1) return 8;
-  return part_bytes(split_of(cache, group, window, max_length), cache->heads * group, cache->value_width);
+  return workspace_of(cache, group, share_count(cache, group, window, max_length)).bytes;
 }
 
 int as_paged_attention(const as_paged_cache* cache, const void* query, const int64_t* query_strides, void* out,
@@ -824,13 +930,13 @@ int as_paged_attention(const as_paged_cache* cache, const void* query, const int
   if (table != nullptr) {
     if (const int bad = fill_position_map(&map, borders, buckets, both_sides)) return bad;
   }
-  const Split split = split_of(cache, group, window, max_length);
-  const size_t need = part_bytes(split, cache->heads * group, cache->value_width);
-  if (workspace == nullptr || workspace_bytes < need)
-    return fail(AS_ERR_WORKSPACE, "paged attention needs %zu workspace bytes", need);
+  const int64_t shares = share_count(cache, group, window, max_length);
+  const Workspace parts = workspace_of(cache, group, shares);
+  if (workspace == nullptr || workspace_bytes < parts.bytes)
+    return fail(AS_ERR_WORKSPACE, "paged attention needs %zu workspace bytes", parts.bytes);
   if (a.cache.sequences == 0) return AS_OK;
-  if (a.cache.sequences > 65535 || split.chunks > kMaxBlocksPerLaunch || cache->page_idx_len > INT32_MAX)
-    return fail(AS_ERR_UNSUPPORTED, "at most 65535 sequences, 2^31 - 1 list entries and 2^22 chunks");
+  if (a.cache.sequences > 65535 || group * a.cache.heads * a.cache.sequences > kMaxBlocksPerLaunch)
+    return fail(AS_ERR_UNSUPPORTED, "at most 65535 sequences, and 2^22 query heads of all sequences");
   if (query == nullptr || query_strides == nullptr || out == nullptr || lengths == nullptr)
     return fail(AS_ERR_INVALID_ARGUMENT, "null pointer argument");
   const size_t size = dtype == AS_DTYPE_F32 ? 4 : 2;
@@ -852,14 +958,11 @@ int as_paged_attention(const as_paged_cache* cache, const void* query, const int
   while ((1 << a.page_shift) < a.cache.page_size) ++a.page_shift;
   a.page_magic = static_cast<uint32_t>(((uint64_t(1) << (31 + a.page_shift)) + a.cache.page_size - 1) /
                                        static_cast<uint64_t>(a.cache.page_size));
-  a.chunks = split.chunks;
-  a.per_sequence = static_cast<int>(split.per_sequence);
-  a.pages_per_chunk = static_cast<int>(split.pages_per_chunk);
-  a.chunk_tokens = static_cast<int>(split.chunk_tokens);
-  a.part_sum = static_cast<float2*>(workspace);
-  a.part_out = reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                        align_up(static_cast<size_t>(split.chunks) * cache->heads * group *
-                                                     sizeof(float2), 256));
+  a.shares = static_cast<int>(shares);
+  char* const ws = static_cast<char*>(workspace);
+  a.plan = reinterpret_cast<int2*>(ws);
+  a.part_sum = reinterpret_cast<float2*>(ws + parts.sums);
+  a.part_out = reinterpret_cast<float*>(ws + parts.out);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
