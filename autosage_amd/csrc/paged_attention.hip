@@ -292,7 +292,8 @@ struct WeightParts {
 // ---- one workgroup -----------------------------------------------------------------
 
 template <typename T, typename C, int W, int MODE>
-__global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a, PositionMap map) {
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(W == 256 && MODE != kNarrow ? 2 : 1))) void
+paged_attention_kernel(AttentionArgs a, PositionMap map) {
   constexpr bool kF32 = sizeof(C) == 4;
   constexpr bool kCoded = sizeof(C) == 1;
   constexpr int kTile = kF32 ? 16 : 32;   // tokens of one step of a wave
@@ -303,6 +304,8 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
   constexpr int kValues = W / 16;         // dimensions of the values a lane holds
   constexpr int kRun = kValues < 8 ? kValues : 8;  // of which neighbours
   constexpr int kBlocks = kValues / kRun;
+  // rows of 256 take too many registers to ask for keys and values at once
+  constexpr bool kLater = kBlocks > 1;
   constexpr int kQ = Parts<T, C>::value;
   constexpr int kP = WeightParts<T, C>::value;
   using U = typename Unit<T, C>::type;
@@ -311,9 +314,11 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
   __shared__ float wave_top[kWavesPerBlock][kHeads];
   __shared__ float wave_sum[kWavesPerBlock][kHeads];
   // the bias of the loop, then the waves' sums
-  constexpr int kOutFloats = kWavesPerBlock * kHeads * W;
+  constexpr int kOutWaves = kLater ? 2 : kWavesPerBlock;
+  constexpr int kOutFloats = kOutWaves * kHeads * W;
   constexpr int kBiasFloats = kMaxBuckets * kHeads;
   __shared__ float pool[kOutFloats > kBiasFloats ? kOutFloats : kBiasFloats];
+  __shared__ u32x4 q_shared[kLater ? kKeyRuns : 1][kQ][kLater ? kWave : 1];
   float(*const bias)[kHeads] = reinterpret_cast<float(*)[kHeads]>(pool);
   float(*const wave_out)[kHeads][W] = reinterpret_cast<float(*)[kHeads][W]>(pool);
 
@@ -384,11 +389,11 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
   }
 
   // where the lane's runs of a key begin (lane (n, g): dimensions (j*4 + g) * kKeyRun ..), the queries there
-  // as operand B, and which elements count (bit i: element i is no repetition)
+  // as operand B
   int key_at[kKeyRuns];
-  uint32_t key_own[kKeyRuns];
-  float q32[kF32 ? kKeyRuns : 1][4];
-  u32x4 q16[kF32 ? 1 : kKeyRuns][kQ];
+  // (in LDS with rows of 256: all waves hold the same)
+  u32x4 q_own[kLater ? 1 : kKeyRuns][kQ];
+  const auto q_of = [&](int j, int p) { return kLater ? q_shared[j][p][lane] : q_own[kLater ? 0 : j][p]; };
   {
     const int head = n < heads_here ? n : 0;
     const T* q_row = static_cast<const T*>(a.query) + b * a.query_stride[0] + (head0 + head) * a.query_stride[1];
@@ -397,27 +402,33 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
       const int d = (j * 4 + g) * kKeyRun;
       key_at[j] = run_start(d, kKeyRun, c.key.width);
       const RawVec<kKeyRun * sizeof(T)> raw = load_run<T, kKeyRun, MODE>(q_row, key_at[j], c.key.width);
-      key_own[j] = 0;
       float q[kKeyRun];
 #pragma unroll
       for (int i = 0; i < kKeyRun; ++i) {
         const bool mine = key_at[j] + i >= d && key_at[j] + i < c.key.width;
-        key_own[j] |= mine ? 1u << i : 0u;
         q[i] = mine && n < heads_here ? Elem<T>::get(raw.w, i) : 0.0f;
       }
 #pragma unroll
-      for (int i = 0; i < (kF32 ? 4 : 0); ++i) q32[j][i] = q[i];
+      for (int p = 0; p < kQ; ++p) {
+        u32x4 words;
 #pragma unroll
-      for (int i = 0; i < (kF32 ? 0 : 4); ++i) {
-#pragma unroll
-        for (int p = 0; p < kQ; ++p) {
-          const uint32_t w = U::pack(q[(2 * i) % kKeyRun], q[(2 * i + 1) % kKeyRun]);
-          q16[j][p][i] = w;
-          q[(2 * i) % kKeyRun] -= U::unpack(w)[0];
-          q[(2 * i + 1) % kKeyRun] -= U::unpack(w)[1];
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (kF32) {
+            words[i] = __float_as_uint(q[i]);
+          } else {
+            words[i] = U::pack(q[(2 * i) % kKeyRun], q[(2 * i + 1) % kKeyRun]);
+            q[(2 * i) % kKeyRun] -= U::unpack(words[i])[0];
+            q[(2 * i + 1) % kKeyRun] -= U::unpack(words[i])[1];
+          }
+        }
+        if constexpr (!kLater) {
+          q_own[j][p] = words;
+        } else if (wave == 0) {
+          q_shared[j][p][lane] = words;
         }
       }
     }
+    if constexpr (kLater) __syncthreads();
   }
   f32x4 acc[kValues];
   float top;  // of head n, the same in its four lanes
@@ -426,8 +437,8 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
   // What a tile needs from memory.
   struct Tile {
     RawVec<kKeyRun * sizeof(C)> key[kKeyRows][kKeyRuns];
-    RawVec<kRun * sizeof(C)> value[kOwn];            // the first block
-    const C* value_row[kBlocks == 1 ? 1 : (MODE == kBlocks8 ? 1 : kOwn)];  // where the others are
+    RawVec<kRun * sizeof(C)> value[kLater ? 1 : kOwn];
+    const C* value_row[kLater && MODE != kBlocks8 ? kOwn : 1];  // where they are, for later
     RawVec<8> key_e, value_e;                        // exponents of the tokens this lane weighs, a byte each
     uint32_t bad_tokens;                             // tokens whose page is outside the cache, a bit each
   };
@@ -436,31 +447,42 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
 #pragma unroll
     for (int j = 0; j < kKeyRuns; ++j) tile.key[s][j] = load_run<C, kKeyRun, MODE>(key_row, key_at[j], c.key.width);
   };
-  const auto load_tile = [&](Tile& tile, int t0) {
+  // kBlocks8: the page ids of the blocks of a tile that a lane loads keys of and
+  // weighs, asked for a tile ahead; a block behind what is seen stands for its
+  // last one.
+  const int last = (end - 1) & ~7;
+  const auto key_block = [&](int t0) {
+    const int t = (t0 + key_token) & ~7;
+    return t < last ? t : last;
+  };
+  const auto own_block = [&](int t0) {
+    const int t = (t0 + own_token) & ~7;
+    return t < last ? t : last;
+  };
+  struct Ids {
+    int64_t key, own;
+  };
+  const auto ids_of = [&](int t0) {
+    return Ids{pages[page_of_token(a, key_block(t0))], pages[page_of_token(a, own_block(t0))]};
+  };
+  const auto load_tile = [&](Tile& tile, int t0, const Ids& ids) {
     if constexpr (MODE == kBlocks8) {
-      // a block behind what is seen stands for its last one
-      const int last = (end - 1) & ~7;
-      int t = (t0 + key_token) & ~7;
-      t = t < last ? t : last;
-      int entry = page_of_token(a, t);
-      int slot = t - entry * c.page_size + (key_token & 7);
-      int64_t page = pages[entry];
-      page = is_bad(page) ? 0 : page;
+      int t = key_block(t0);
+      int slot = t - page_of_token(a, t) * c.page_size + (key_token & 7);
+      int64_t page = is_bad(ids.key) ? 0 : ids.key;
       const C* row = key_base + page * c.key.stride[0] + slot * key_step;
 #pragma unroll
       for (int s = 0; s < kKeyRows; ++s) load_rows(tile, s, row + s * 4 * key_step);
-      t = (t0 + own_token) & ~7;
-      t = t < last ? t : last;
-      entry = page_of_token(a, t);
-      slot = t - entry * c.page_size + (own_token & 7);
-      page = pages[entry];
-      const bool bad = is_bad(page);
-      page = bad ? 0 : page;
+      t = own_block(t0);
+      slot = t - page_of_token(a, t) * c.page_size + (own_token & 7);
+      const bool bad = is_bad(ids.own);
+      page = bad ? 0 : ids.own;
       tile.bad_tokens = bad ? 0xffu : 0u;
       row = value_base + page * c.value.stride[0] + slot * value_step;
 #pragma unroll
-      for (int e = 0; e < kOwn; ++e) tile.value[e] = load_run<C, kRun, MODE>(row + e * value_step, value_at[0], c.value.width);
-      if constexpr (kBlocks > 1) tile.value_row[0] = row;
+      for (int e = 0; e < (kLater ? 0 : kOwn); ++e)
+        tile.value[e] = load_run<C, kRun, MODE>(row + e * value_step, value_at[0], c.value.width);
+      tile.value_row[0] = row;
       if constexpr (kCoded) {
         __builtin_memcpy(&tile.key_e, c.key.exponents + page * c.key.exponent_stride[0] +
                                           h * c.key.exponent_stride[1] + slot, 8);
@@ -491,8 +513,11 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
         const int64_t page = place(t0 + own_token + e, slot, bad);
         if (bad) tile.bad_tokens |= 1u << e;
         const C* row = value_base + page * c.value.stride[0] + slot * value_step;
-        tile.value[e] = load_run<C, kRun, MODE>(row, value_at[0], c.value.width);
-        if constexpr (kBlocks > 1) tile.value_row[e] = row;
+        if constexpr (kLater) {
+          tile.value_row[e] = row;
+        } else {
+          tile.value[e] = load_run<C, kRun, MODE>(row, value_at[0], c.value.width);
+        }
         if constexpr (kCoded) {
           key_e[e / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(
                               c.key.exponents[page * c.key.exponent_stride[0] + h * c.key.exponent_stride[1] +
@@ -523,11 +548,12 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
 #pragma unroll
       for (int j = 0; j < kKeyRuns; ++j) {
         if constexpr (kF32) {
+          const u32x4 q = q_of(j, 0);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t w = tile.key[s][j].w[i];
-            if (careful && !((key_own[j] >> i) & 1)) w = 0u;
-            score[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w), q32[j][i], score[s], 0, 0, 0);
+            if (careful && key_at[j] + i < (j * 4 + g) * kKeyRun) w = 0u;
+            score[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w), __uint_as_float(q[i]), score[s], 0, 0, 0);
           }
         } else {
           uint32_t w[4];
@@ -535,14 +561,30 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
           if (!kCoded && careful) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t two = key_own[j] >> (2 * i);
-              w[i] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+              const int repeated = (j * 4 + g) * kKeyRun - key_at[j] - 2 * i;
+              w[i] = repeated <= 0 ? w[i] : (repeated == 1 ? w[i] & 0xffff0000u : 0u);
             }
           }
 #pragma unroll
-          for (int p = 0; p < kQ; ++p) score[s] = U::multiply(u32x4{w[0], w[1], w[2], w[3]}, q16[j][p], score[s]);
+          for (int p = 0; p < kQ; ++p) score[s] = U::multiply(u32x4{w[0], w[1], w[2], w[3]}, q_of(j, p), score[s]);
         }
       }
+    }
+
+    RawVec<kRun * sizeof(C)> value[kBlocks][kOwn];
+    const auto load_values = [&](int jb) {
+#pragma unroll
+      for (int e = 0; e < kOwn; ++e) {
+        const C* row = MODE == kBlocks8 ? tile.value_row[0] + e * value_step
+                                        : tile.value_row[kLater && MODE != kBlocks8 ? e : 0];
+        value[jb][e] = load_run<C, kRun, MODE>(row, value_at[jb], c.value.width);
+      }
+    };
+    if constexpr (kLater) {
+      load_values(0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kOwn; ++e) value[0][e] = tile.value[e];
     }
 
     // scores in powers of two
@@ -624,26 +666,16 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
       }
     }
 
-    RawVec<kRun * sizeof(C)> value[2][kOwn];
-#pragma unroll
-    for (int e = 0; e < kOwn; ++e) value[0][e] = tile.value[e];
 #pragma unroll
     for (int jb = 0; jb < kBlocks; ++jb) {
-      if (jb + 1 < kBlocks) {
-#pragma unroll
-        for (int e = 0; e < kOwn; ++e) {
-          const C* row = MODE == kBlocks8 ? tile.value_row[0] + e * value_step
-                                          : tile.value_row[kBlocks == 1 || MODE == kBlocks8 ? 0 : e];
-          value[(jb + 1) % 2][e] = load_run<C, kRun, MODE>(row, value_at[(jb + 1) % kBlocks], c.value.width);
-        }
-      }
+      if (jb + 1 < kBlocks) load_values(jb + 1);
       if (edge) {
         // a value out of sight may be anything; its weight is zero, and so has to be the product
 #pragma unroll
         for (int e = 0; e < kOwn; ++e) {
           const int t = t0 + own_token + e;
 #pragma unroll
-          for (uint32_t& w : value[jb % 2][e].w) w = t < begin || t >= end ? 0u : w;
+          for (uint32_t& w : value[jb][e].w) w = t < begin || t >= end ? 0u : w;
         }
       }
       if constexpr (kF32) {
@@ -652,12 +684,12 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
 #pragma unroll
           for (int j = 0; j < kRun; ++j)
             acc[jb * kRun + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                weight[e], __uint_as_float(value[jb % 2][e].w[j]), acc[jb * kRun + j], 0, 0, 0);
+                weight[e], __uint_as_float(value[jb][e].w[j]), acc[jb * kRun + j], 0, 0, 0);
         }
       } else {
         uint32_t words[8][kRun / 2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to_words<C, kRun>(value[jb % 2][e % kOwn], words[e]);
+        for (int e = 0; e < 8; ++e) to_words<C, kRun>(value[jb][e % kOwn], words[e]);
 #pragma unroll
         for (int j = 0; j < kRun; ++j) {
           u32x4 column;
@@ -688,9 +720,14 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
     top = -INFINITY;
     sum = 0.0f;
     int t0 = base + wave * kTile;
+    Ids ids{};
+    if (MODE == kBlocks8 && t0 < end) ids = ids_of(t0);
     for (; t0 < end; t0 += kStride) {
+      // the queries in LDS are read for every tile: kept, they would take the registers they are spared
+      if constexpr (kLater) asm volatile("" ::: "memory");
       Tile tile;
-      load_tile(tile, t0);
+      load_tile(tile, t0, ids);
+      if constexpr (MODE == kBlocks8) ids = ids_of(t0 + kStride);
       work_on(tile, t0);
     }
     if (kCoded || careful) break;
@@ -714,18 +751,36 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int hh = g * 4 + i;
-    if (hh < heads_here) {
-      float most = wave_top[0][hh];
+    float most = wave_top[0][hh];
 #pragma unroll
-      for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_top[w][hh]);
-      const float mine = wave_top[wave][hh];
-      const float f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - most);
+    for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_top[w][hh]);
+    const float mine = wave_top[wave][hh];
+    const float f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - most);
+#pragma unroll
+    for (int j = 0; j < kValues; ++j) acc[j][i] *= f;
+  }
+  const auto each_out = [&](auto&& f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int hh = g * 4 + i;
 #pragma unroll
       for (int j = 0; j < kValues; ++j) {
         const int d = value_at[j / kRun] + j % kRun;
-        if (MODE != kNarrow || d < c.value.width) wave_out[wave][hh][d] = acc[j][i] * f;
+        if (hh < heads_here && (MODE != kNarrow || d < c.value.width)) acc[j][i] = f(wave_out[wave % kOutWaves][hh][d], acc[j][i]);
       }
     }
+  };
+  const auto put = [](float& to, float x) { return to = x; };
+  if constexpr (kLater) {
+    // two waves hand their sums to the other two; lanes that hold the same column
+    // read it before either writes
+    if (wave >= kOutWaves) each_out(put);
+    __syncthreads();
+    if (wave < kOutWaves) each_out([](float& to, float x) { return x + to; });
+    __syncthreads();
+    if (wave < kOutWaves) each_out(put);
+  } else {
+    each_out(put);
   }
   __syncthreads();
   const int width = c.value.width;
@@ -741,7 +796,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_kernel(AttentionArgs a
     for (int w = 0; w < kWavesPerBlock; ++w) {
       const float mine = wave_top[w][hh];
       total += (mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - most)) * wave_sum[w][hh];
-      x += wave_out[w][hh][d];
+      if (w < kOutWaves) x += wave_out[w % kOutWaves][hh][d];
     }
     if (whole) {
       const int64_t row = static_cast<int64_t>(b) * heads_q + head0 + hh;
