@@ -313,14 +313,10 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
   __shared__ int32_t border[kMaxBuckets + 1];
   __shared__ float wave_top[kWavesPerBlock][kHeads];
   __shared__ float wave_sum[kWavesPerBlock][kHeads];
-  // the bias of the loop, then the waves' sums
+  __shared__ float bias[kMaxBuckets][kHeads];  // in powers of two, of the keys in front of the query
   constexpr int kOutWaves = kLater ? 2 : kWavesPerBlock;
-  constexpr int kOutFloats = kOutWaves * kHeads * W;
-  constexpr int kBiasFloats = kMaxBuckets * kHeads;
-  __shared__ float pool[kOutFloats > kBiasFloats ? kOutFloats : kBiasFloats];
+  __shared__ float wave_out[kOutWaves][kHeads][W];
   __shared__ u32x4 q_shared[kLater ? kKeyRuns : 1][kQ][kLater ? kWave : 1];
-  float(*const bias)[kHeads] = reinterpret_cast<float(*)[kHeads]>(pool);
-  float(*const wave_out)[kHeads][W] = reinterpret_cast<float(*)[kHeads][W]>(pool);
 
   const PagedCache& c = a.cache;
   const int lane = lane_id();
@@ -337,11 +333,20 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
   const int head0 = h * a.group + tile_of_heads * kHeads;
   const int heads_here = a.group - tile_of_heads * kHeads < kHeads ? a.group - tile_of_heads * kHeads : kHeads;
 
+  if (a.table != nullptr) {
+    stage_borders(border, map);
+    for (int i = threadIdx.x; i < map.side * kHeads; i += kBlock) {
+      const int hh = i % kHeads < heads_here ? i % kHeads : 0;
+      bias[i / kHeads][i % kHeads] =
+          kLog2e * Elem<T>::at(static_cast<const T*>(a.table), static_cast<int64_t>(i / kHeads) * heads_q + head0 + hh);
+    }
+  }
   Share share{0, 1, 1, 0, share_index};
   if (a.shares > 0) {
     share = share_of(a, share_index);
     if (share.first >= share.end) return;
   }
+  if (a.table != nullptr) __syncthreads();
 
   const float to_log2 = a.scale * kLog2e;
   const C* key_base = static_cast<const C*>(c.key.data) + h * c.key.stride[1];
@@ -375,18 +380,6 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
   const int stop = a.shares > 0 ? origin + to_piece * kPiece : seen.end;
   const int end = stop < seen.end ? stop : seen.end;
   const int64_t* pages = c.page_idx + list.begin;
-
-  if (a.table != nullptr) {
-    // once in front of every part: the parts' results lie in the same place
-    const int buckets = map.both_sides ? 2 * map.side : map.side;
-    stage_borders(border, map);
-    for (int i = threadIdx.x; i < buckets * kHeads; i += kBlock) {
-      const int hh = i % kHeads < heads_here ? i % kHeads : 0;
-      bias[i / kHeads][i % kHeads] =
-          kLog2e * Elem<T>::at(static_cast<const T*>(a.table), static_cast<int64_t>(i / kHeads) * heads_q + head0 + hh);
-    }
-    __syncthreads();
-  }
 
   // where the lane's runs of a key begin (lane (n, g): dimensions (j*4 + g) * kKeyRun ..), the queries there
   // as operand B
@@ -814,24 +807,27 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
   }
 }
 
-// Joins the parts of one sequence and query head: one workgroup.  Every wave
+// Joins the parts of a sequence and query head: TEAM waves for each (one where
+// there are many; 2,048 rows of two parts: 6 us, 10 with eight).  Every wave
 // finds the maximum and the sum of all parts, lane l those with index l mod 64;
-// then the waves take turns with the parts, four at once, and the lanes hold the
-// width.
+// then the waves of a team take turns with the parts, four at once, and the lanes
+// hold the width.
 constexpr int kJoinWaves = 8;
 constexpr int kJoinAhead = 4;
-template <typename T>
+template <typename T, int TEAM>
 __global__ __launch_bounds__(kJoinWaves* kWave) void paged_attention_join_kernel(AttentionArgs a, float shift) {
-  __shared__ float wave_out[kJoinWaves][kMaxWidth];
+  __shared__ float wave_out[TEAM][kMaxWidth];
   const PagedCache& c = a.cache;
   const int heads_q = c.heads * a.group;
-  const int b = blockIdx.y;
-  const int hq = blockIdx.x;
+  const int lane = lane_id();
+  const int wave = uniform_i32(wave_in_block()) % TEAM;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kJoinWaves / TEAM) + uniform_i32(wave_in_block()) / TEAM;
+  if (row >= static_cast<int64_t>(c.sequences) * heads_q) return;
+  const int b = static_cast<int>(static_cast<uint32_t>(row) / static_cast<uint32_t>(heads_q));
+  const int hq = static_cast<int>(row) - b * heads_q;
   const int64_t first = a.plan[b].x;
   const int count = a.plan[b].y;
   if (count <= 1) return;
-  const int lane = lane_id();
-  const int wave = uniform_i32(wave_in_block());
   const int width = c.value.width;
   const float2* const sums = a.part_sum + first * heads_q + hq;
   const float* const rows = a.part_out + (first * heads_q + hq) * width;
@@ -852,12 +848,12 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void paged_attention_join_kernel
   float acc[kParts];
 #pragma unroll
   for (int i = 0; i < kParts; ++i) acc[i] = 0.0f;
-  for (int k0 = wave; k0 < count; k0 += kJoinWaves * kJoinAhead) {
+  for (int k0 = wave; k0 < count; k0 += TEAM * kJoinAhead) {
     float f[kJoinAhead];
     float x[kJoinAhead][kParts];
 #pragma unroll
     for (int u = 0; u < kJoinAhead; ++u) {
-      const int k = k0 + u * kJoinWaves;
+      const int k = k0 + u * TEAM;
       const int64_t at = static_cast<int64_t>(k < count ? k : count - 1) * heads_q;
       f[u] = k < count ? __builtin_amdgcn_exp2f(sums[at].x - base) : 0.0f;
 #pragma unroll
@@ -872,18 +868,27 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void paged_attention_join_kernel
       for (int i = 0; i < kParts; ++i) acc[i] = fmaf(f[u], x[u][i], acc[i]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < kParts; ++i) wave_out[wave][lane + i * kWave] = acc[i];
-  __syncthreads();
-  const int d = threadIdx.x;
-  if (d >= width) return;
-  float x = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kJoinWaves; ++w) x += wave_out[w][d];
-  const int64_t row = static_cast<int64_t>(b) * heads_q + hq;
   const bool none = total == 0.0f;
-  static_cast<T*>(a.out)[row * width + d] = rounded<T>(none ? 0.0f : x / total);
-  if (a.lse != nullptr && d == 0)
+  T* const out = static_cast<T*>(a.out) + row * width;
+  if constexpr (TEAM == 1) {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) {
+      const int d = lane + i * kWave;
+      if (d < width) out[d] = rounded<T>(none ? 0.0f : acc[i] / total);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kParts; ++i) wave_out[wave][lane + i * kWave] = acc[i];
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d < width) {
+      float x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < TEAM; ++w) x += wave_out[w][d];
+      out[d] = rounded<T>(none ? 0.0f : x / total);
+    }
+  }
+  if (a.lse != nullptr && wave == 0 && lane == 0)
     a.lse[row] = none ? -INFINITY : (most - shift + __builtin_amdgcn_logf(total)) * kLn2;
 }
 
@@ -911,7 +916,7 @@ struct Workspace {
   size_t sums, out, bytes;  // where the parts' sums and results begin behind the plan, and the size of all
 };
 Workspace workspace_of(const as_paged_cache* c, int64_t group, int64_t shares) {
-  if (shares == 0) return Workspace{0, 0, 8};
+  if (shares == 0) return Workspace{0, 0, 0};
   const size_t rows = static_cast<size_t>(shares + c->sequences) * c->heads * group;
   Workspace w;
   w.sums = align_up(static_cast<size_t>(c->sequences) * sizeof(int2), 256);
@@ -946,9 +951,15 @@ int launch_attention(const AttentionArgs& a, const PositionMap& map, hipStream_t
   }
   if (const int bad = check_launch("paged_attention")) return bad;
   if (a.shares == 0) return AS_OK;
-  paged_attention_join_kernel<T><<<dim3(static_cast<unsigned>(a.cache.heads * a.group),
-                                       static_cast<unsigned>(a.cache.sequences)),
-                                   kJoinWaves * kWave, 0, s>>>(a, Unit<T, C>::type::kShift);
+  const int64_t rows = int64_t(a.cache.sequences) * a.cache.heads * a.group;
+  const float shift = Unit<T, C>::type::kShift;
+  if (rows >= 1024) {
+    paged_attention_join_kernel<T, 1>
+        <<<dim3(static_cast<unsigned>((rows + kJoinWaves - 1) / kJoinWaves)), kJoinWaves * kWave, 0, s>>>(a, shift);
+  } else {
+    paged_attention_join_kernel<T, kJoinWaves>
+        <<<dim3(static_cast<unsigned>(rows)), kJoinWaves * kWave, 0, s>>>(a, shift);
+  }
   return check_launch("paged_attention (join)");
 }
 
@@ -963,7 +974,7 @@ extern "C" {
 size_t as_paged_attention_workspace_bytes(const as_paged_cache* cache, int64_t group, int64_t window,
                                           int64_t max_length) {
   PagedCache c;
-  if (read_paged_cache(cache, &c) != AS_OK || group < 1) return 8;
+  if (read_paged_cache(cache, &c) != AS_OK || group < 1) return 0;
   return workspace_of(cache, group, share_count(cache, group, window, max_length)).bytes;
 }
 
@@ -987,7 +998,7 @@ int as_paged_attention(const as_paged_cache* cache, const void* query, const int
   }
   const int64_t shares = share_count(cache, group, window, max_length);
   const Workspace parts = workspace_of(cache, group, shares);
-  if (workspace == nullptr || workspace_bytes < parts.bytes)
+  if (workspace_bytes < parts.bytes || (parts.bytes > 0 && workspace == nullptr))
     return fail(AS_ERR_WORKSPACE, "paged attention needs %zu workspace bytes", parts.bytes);
   if (a.cache.sequences == 0) return AS_OK;
   if (a.cache.sequences > 65535 || group * a.cache.heads * a.cache.sequences > kMaxBlocksPerLaunch)

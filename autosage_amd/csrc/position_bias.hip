@@ -380,7 +380,7 @@ using namespace as;
 extern "C" {
 
 size_t as_csr_position_bias_workspace_bytes(int64_t n, int64_t nnz, int positions) {
-  if (!positions || n <= 0 || !shorten(n, nnz)) return 8;
+  if (!positions || n <= 0 || !shorten(n, nnz)) return 0;
   return sizeof(int32_t) * (kFitBlocks + static_cast<size_t>(n));
 }
 
@@ -397,7 +397,7 @@ int as_csr_position_bias(const int64_t* crow, const int64_t* col, const int64_t*
   PositionMap map;
   if (const int bad = fill_position_map(&map, borders, buckets, both_sides)) return bad;
   const size_t need = as_csr_position_bias_workspace_bytes(n, nnz, positions != nullptr);
-  if (workspace == nullptr || workspace_bytes < need)
+  if (workspace_bytes < need || (need > 0 && workspace == nullptr))
     return fail(AS_ERR_WORKSPACE, "the position bias needs %zu workspace bytes", need);
   if (nnz == 0) return AS_OK;
   EdgeWalk walk{crow, col, positions, nullptr, nullptr, n, nnz};

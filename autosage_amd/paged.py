@@ -480,14 +480,14 @@ def _attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, scale
     bound = -1 if max_length is None else int(max_length)
     group = heads_q // key_pages.size(1)
     seen = 0 if window is None else int(window)
-    ws = _native._workspace(lib.as_paged_attention_workspace_bytes(ctypes.byref(cache), group, seen, bound),
-                            query.device)
+    ws_bytes = lib.as_paged_attention_workspace_bytes(ctypes.byref(cache), group, seen, bound)
+    ws = _native._workspace(ws_bytes, query.device) if ws_bytes else None
     with _native._on(query.device):
         status = lib.as_paged_attention(
             ctypes.byref(cache), query.data_ptr(), _TwoStrides(query.stride(0), query.stride(1)),
             out.data_ptr(), _native._ptr(lse), lengths.data_ptr(), group, float(scale),
             seen, None if bias_table is None else bias_table.data_ptr(), buckets,
-            borders, int(bool(bidirectional)), bound, _DTYPES[query.dtype], ws.data_ptr(), ws.numel(),
+            borders, int(bool(bidirectional)), bound, _DTYPES[query.dtype], _native._ptr(ws), ws_bytes,
             _native._stream(query.device))
     _native._raise(status, "autosage::paged_attention")
     return out, lse

@@ -115,12 +115,13 @@ def csr_position_bias_impl(crow, col, positions, table, max_distance, bidirectio
         return out, found
     n = crow.numel() - 1
     lib = _native.library()
-    ws = _native._workspace(lib.as_csr_position_bias_workspace_bytes(n, nnz, int(positions is not None)), table.device)
+    ws_bytes = lib.as_csr_position_bias_workspace_bytes(n, nnz, int(positions is not None))
+    ws = _native._workspace(ws_bytes, table.device) if ws_bytes else None
     with _native._on(table.device):
         status = lib.as_csr_position_bias(
             crow.data_ptr(), col.data_ptr(), _native._ptr(positions), table.data_ptr(), out.data_ptr(),
             found.data_ptr() if keep else None, n, nnz, heads, buckets, borders, int(bool(bidirectional)),
-            _DTYPES[table.dtype], ws.data_ptr(), ws.numel(), _native._stream(table.device))
+            _DTYPES[table.dtype], _native._ptr(ws), ws_bytes, _native._stream(table.device))
     _native._raise(status, "autosage::csr_position_bias")
     return out, found
 

@@ -247,7 +247,8 @@ def test_native_argument_checks_come_before_any_launch():
         (1, lambda: attention(struct(), table=fake, buckets=3, sides=1), b"two sides need"),
         (1, lambda: attention(struct(), table=fake, buckets=3), b"null borders"),
         (1, lambda: attention(struct(), table=fake, buckets=3, borders=(ctypes.c_int32 * 3)(0, 2, 1)), b"borders must"),
-        (4, lambda: attention(struct(), ws=None), b"paged attention needs"),
+        (4, lambda: attention(struct(page_idx_len=1 << 20), ws=None), b"paged attention needs"),
+        (4, lambda: attention(struct(page_idx_len=1 << 20), ws_bytes=1000), b"paged attention needs"),
         (1, lambda: attention(struct(), query=None), b"null pointer argument"),
         (0, lambda: attention(struct(sequences=0)), b""),
         (1, lambda: lib.as_paged_cache_write(struct(), fake, two, fake, two, fake, fake, 2, 2, None), b"a cache that"),
