@@ -45,6 +45,8 @@
 // A sequence that sees no token, or only scores of -inf, gives zeros and an
 // lse of -inf.  A length beyond the sequence's pages or max_length makes its
 // results NaN, and so does a page id outside the cache, which is never read.
+#include <cfloat>
+
 #include "paged_common.h"
 #include "position_map.h"
 
@@ -138,42 +140,55 @@ struct Share {
   int64_t at;
   int b;
 };
-// By every wave of the workgroup: the sequences' pieces are summed, lane l taking
-// `each` sequences from l * each on, then those of the lane that holds `first`,
-// 64 at a time.
-__device__ __forceinline__ Share share_of(const AttentionArgs& a, int i) {
+// By the whole workgroup: thread t sums the pieces of `each` sequences from t * each
+// on; then the sequences of the thread that holds `first` are gone through, 64 at
+// a time.  Leaves the workgroup synchronised.
+struct ShareSums {
+  int64_t wave[kWavesPerBlock];
+  int64_t at;
+  int b;
+};
+__device__ __forceinline__ Share share_of(const AttentionArgs& a, int i, ShareSums& sums) {
   const int n = a.cache.sequences;
-  const int each = (n + kWave - 1) / kWave;
+  const int each = (n + kBlock - 1) / kBlock;
+  const int from = threadIdx.x * each;
   int64_t mine = 0;
-  const int from = lane_id() * each;
-  const int to = from + each < n ? from + each : n;
-  for (int b = from; b < to; ++b) mine += piece_count(a, b);
-  const int64_t upto = wave_incl_scan_i64(mine);
-  const int64_t all = __shfl(upto, kWave - 1, kWave);
+#pragma unroll 4
+  for (int j = 0; j < each; ++j) {
+    if (from + j < n) mine += piece_count(a, from + j);
+  }
+  int64_t before = wave_incl_scan_i64(mine) - mine;
+  if (lane_id() == kWave - 1) sums.wave[wave_in_block()] = before + mine;
+  __syncthreads();
+  int64_t all = 0;
+#pragma unroll
+  for (int w = 0; w < kWavesPerBlock; ++w) {
+    if (w < wave_in_block()) before += sums.wave[w];
+    all += sums.wave[w];
+  }
   Share s;
   s.size = (all + a.shares - 1) / a.shares;
   s.size = s.size < kMinShare ? kMinShare : s.size;
   s.first = s.size * i;
   s.end = s.first + s.size < all ? s.first + s.size : all;
-  s.at = 0;
-  s.b = 0;
-  if (s.first >= all) return s;
-  const int holder = 63 - __builtin_clzll(__ballot(upto - mine <= s.first));
-  s.at = __shfl(upto - mine, holder, kWave);
-  s.b = holder * each;
-  for (int b0 = s.b; each > 1; b0 += kWave) {
+  if (before <= s.first && s.first < before + mine) {
+    sums.at = before;
+    sums.b = from;
+  }
+  __syncthreads();
+  s.at = sums.at;
+  s.b = sums.b;
+  for (int b0 = s.b; each > 1 && s.first < all; b0 += kWave) {
     const int b = b0 + lane_id();
     const int64_t own = b < n ? piece_count(a, b) : 0;
-    const int64_t before = s.at + wave_incl_scan_i64(own) - own;
-    const uint64_t below = __ballot(b < n && before <= s.first);
-    const int last = 63 - __builtin_clzll(below | 1);
-    const int64_t next = __shfl(before + own, kWave - 1, kWave);
-    if (next > s.first || b0 + kWave >= n) {
-      s.at = __shfl(before, last, kWave);
+    const int64_t upto = s.at + wave_incl_scan_i64(own);
+    if (__shfl(upto, kWave - 1, kWave) > s.first || b0 + kWave >= n) {
+      const int last = 63 - __builtin_clzll(__ballot(b < n && upto - own <= s.first) | 1);
+      s.at = __shfl(upto - own, last, kWave);
       s.b = b0 + last;
       break;
     }
-    s.at = next;
+    s.at = __shfl(upto, kWave - 1, kWave);
   }
   // the same in every lane
   s.size = uniform_i64(s.size);
@@ -311,6 +326,7 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
   using U = typename Unit<T, C>::type;
 
   __shared__ int32_t border[kMaxBuckets + 1];
+  __shared__ ShareSums share_sums;
   __shared__ float wave_top[kWavesPerBlock][kHeads];
   __shared__ float wave_sum[kWavesPerBlock][kHeads];
   __shared__ float bias[kMaxBuckets][kHeads];  // in powers of two, of the keys in front of the query
@@ -337,16 +353,19 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
     stage_borders(border, map);
     for (int i = threadIdx.x; i < map.side * kHeads; i += kBlock) {
       const int hh = i % kHeads < heads_here ? i % kHeads : 0;
-      bias[i / kHeads][i % kHeads] =
-          kLog2e * Elem<T>::at(static_cast<const T*>(a.table), static_cast<int64_t>(i / kHeads) * heads_q + head0 + hh);
+      const float x = Elem<T>::at(static_cast<const T*>(a.table), static_cast<int64_t>(i / kHeads) * heads_q + head0 + hh);
+      // a mask of the type's lowest number stays a number: a row of such masks has weights
+      const float x2 = kLog2e * x;
+      bias[i / kHeads][i % kHeads] = finite(x) && !finite(x2) ? (x < 0.0f ? -FLT_MAX : FLT_MAX) : x2;
     }
   }
   Share share{0, 1, 1, 0, share_index};
   if (a.shares > 0) {
-    share = share_of(a, share_index);
+    share = share_of(a, share_index, share_sums);
     if (share.first >= share.end) return;
+  } else if (a.table != nullptr) {
+    __syncthreads();
   }
-  if (a.table != nullptr) __syncthreads();
 
   const float to_log2 = a.scale * kLog2e;
   const C* key_base = static_cast<const C*>(c.key.data) + h * c.key.stride[1];
@@ -362,448 +381,448 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
 
   int64_t at = share.at;
   for (int b = uniform_i32(share.b); b < c.sequences && at < share.end; ++b) {
-  const PageList list = page_list(c, b);
-  const Seen seen = seen_tokens(a, b, list);
-  const int pieces = a.shares > 0 ? piece_count(a, seen) : 1;
-  // pieces from .. to - 1 of this sequence are in the share
-  const int from_piece = share.first > at ? static_cast<int>(share.first - at) : 0;
-  const int to_piece = share.end < at + pieces ? static_cast<int>(share.end - at) : pieces;
-  const bool whole = from_piece == 0 && to_piece == pieces;
-  const int64_t part = static_cast<int64_t>(share_index) + b;
-  if (a.shares > 0 && unit == 0 && from_piece == 0 && threadIdx.x == 0)
-    a.plan[b] = make_int2(static_cast<int>(part),
-                          static_cast<int>((at + pieces - 1) / share.size - at / share.size) + 1);
-  at += pieces;
-  const int origin = first_token(a, seen);
-  const int base = origin + from_piece * kPiece;
-  const int begin = base > seen.begin ? base : seen.begin;
-  const int stop = a.shares > 0 ? origin + to_piece * kPiece : seen.end;
-  const int end = stop < seen.end ? stop : seen.end;
-  const int64_t* pages = c.page_idx + list.begin;
+    const PageList list = page_list(c, b);
+    const Seen seen = seen_tokens(a, b, list);
+    const int pieces = a.shares > 0 ? piece_count(a, seen) : 1;
+    // pieces from .. to - 1 of this sequence are in the share
+    const int from_piece = share.first > at ? static_cast<int>(share.first - at) : 0;
+    const int to_piece = share.end < at + pieces ? static_cast<int>(share.end - at) : pieces;
+    const bool whole = from_piece == 0 && to_piece == pieces;
+    const int64_t part = static_cast<int64_t>(share_index) + b;
+    if (a.shares > 0 && unit == 0 && from_piece == 0 && threadIdx.x == 0)
+      a.plan[b] = make_int2(static_cast<int>(part),
+                            static_cast<int>((at + pieces - 1) / share.size - at / share.size) + 1);
+    at += pieces;
+    const int origin = first_token(a, seen);
+    const int base = origin + from_piece * kPiece;
+    const int begin = base > seen.begin ? base : seen.begin;
+    const int stop = a.shares > 0 ? origin + to_piece * kPiece : seen.end;
+    const int end = stop < seen.end ? stop : seen.end;
+    const int64_t* pages = c.page_idx + list.begin;
 
-  // where the lane's runs of a key begin (lane (n, g): dimensions (j*4 + g) * kKeyRun ..), the queries there
-  // as operand B
-  int key_at[kKeyRuns];
-  // (in LDS with rows of 256: all waves hold the same)
-  u32x4 q_own[kLater ? 1 : kKeyRuns][kQ];
-  const auto q_of = [&](int j, int p) { return kLater ? q_shared[j][p][lane] : q_own[kLater ? 0 : j][p]; };
-  {
-    const int head = n < heads_here ? n : 0;
-    const T* q_row = static_cast<const T*>(a.query) + b * a.query_stride[0] + (head0 + head) * a.query_stride[1];
-#pragma unroll
-    for (int j = 0; j < kKeyRuns; ++j) {
-      const int d = (j * 4 + g) * kKeyRun;
-      key_at[j] = run_start(d, kKeyRun, c.key.width);
-      const RawVec<kKeyRun * sizeof(T)> raw = load_run<T, kKeyRun, MODE>(q_row, key_at[j], c.key.width);
-      float q[kKeyRun];
-#pragma unroll
-      for (int i = 0; i < kKeyRun; ++i) {
-        const bool mine = key_at[j] + i >= d && key_at[j] + i < c.key.width;
-        q[i] = mine && n < heads_here ? Elem<T>::get(raw.w, i) : 0.0f;
-      }
-#pragma unroll
-      for (int p = 0; p < kQ; ++p) {
-        u32x4 words;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (kF32) {
-            words[i] = __float_as_uint(q[i]);
-          } else {
-            words[i] = U::pack(q[(2 * i) % kKeyRun], q[(2 * i + 1) % kKeyRun]);
-            q[(2 * i) % kKeyRun] -= U::unpack(words[i])[0];
-            q[(2 * i + 1) % kKeyRun] -= U::unpack(words[i])[1];
-          }
-        }
-        if constexpr (!kLater) {
-          q_own[j][p] = words;
-        } else if (wave == 0) {
-          q_shared[j][p][lane] = words;
-        }
-      }
-    }
-    if constexpr (kLater) __syncthreads();
-  }
-  f32x4 acc[kValues];
-  float top;  // of head n, the same in its four lanes
-  float sum;  // of head n and the tokens of this lane
-
-  // What a tile needs from memory.
-  struct Tile {
-    RawVec<kKeyRun * sizeof(C)> key[kKeyRows][kKeyRuns];
-    RawVec<kRun * sizeof(C)> value[kLater ? 1 : kOwn];
-    const C* value_row[kLater && MODE != kBlocks8 ? kOwn : 1];  // where they are, for later
-    RawVec<8> key_e, value_e;                        // exponents of the tokens this lane weighs, a byte each
-    uint32_t bad_tokens;                             // tokens whose page is outside the cache, a bit each
-  };
-  const auto is_bad = [&](int64_t id) { return id < 0 || id >= c.pages; };
-  const auto load_rows = [&](Tile& tile, int s, const C* key_row) {
-#pragma unroll
-    for (int j = 0; j < kKeyRuns; ++j) tile.key[s][j] = load_run<C, kKeyRun, MODE>(key_row, key_at[j], c.key.width);
-  };
-  // kBlocks8: the page ids of the blocks of a tile that a lane loads keys of and
-  // weighs, asked for a tile ahead; a block behind what is seen stands for its
-  // last one.
-  const int last = (end - 1) & ~7;
-  const auto key_block = [&](int t0) {
-    const int t = (t0 + key_token) & ~7;
-    return t < last ? t : last;
-  };
-  const auto own_block = [&](int t0) {
-    const int t = (t0 + own_token) & ~7;
-    return t < last ? t : last;
-  };
-  struct Ids {
-    int64_t key, own;
-  };
-  const auto ids_of = [&](int t0) {
-    return Ids{pages[page_of_token(a, key_block(t0))], pages[page_of_token(a, own_block(t0))]};
-  };
-  const auto load_tile = [&](Tile& tile, int t0, const Ids& ids) {
-    if constexpr (MODE == kBlocks8) {
-      int t = key_block(t0);
-      int slot = t - page_of_token(a, t) * c.page_size + (key_token & 7);
-      int64_t page = is_bad(ids.key) ? 0 : ids.key;
-      const C* row = key_base + page * c.key.stride[0] + slot * key_step;
-#pragma unroll
-      for (int s = 0; s < kKeyRows; ++s) load_rows(tile, s, row + s * 4 * key_step);
-      t = own_block(t0);
-      slot = t - page_of_token(a, t) * c.page_size + (own_token & 7);
-      const bool bad = is_bad(ids.own);
-      page = bad ? 0 : ids.own;
-      tile.bad_tokens = bad ? 0xffu : 0u;
-      row = value_base + page * c.value.stride[0] + slot * value_step;
-#pragma unroll
-      for (int e = 0; e < (kLater ? 0 : kOwn); ++e)
-        tile.value[e] = load_run<C, kRun, MODE>(row + e * value_step, value_at[0], c.value.width);
-      tile.value_row[0] = row;
-      if constexpr (kCoded) {
-        __builtin_memcpy(&tile.key_e, c.key.exponents + page * c.key.exponent_stride[0] +
-                                          h * c.key.exponent_stride[1] + slot, 8);
-        __builtin_memcpy(&tile.value_e, c.value.exponents + page * c.value.exponent_stride[0] +
-                                            h * c.value.exponent_stride[1] + slot, 8);
-      }
-    } else {
-      const auto place = [&](int t, int& slot, bool& bad) {
-        t = t < end ? t : end - 1;  // a token behind what is seen stands for the last one
-        const int e = page_of_token(a, t);
-        slot = t - e * c.page_size;
-        const int64_t id = pages[e];
-        bad = is_bad(id);
-        return bad ? int64_t(0) : id;
-      };
-      int slot;
-      bool bad;
-#pragma unroll
-      for (int s = 0; s < kKeyRows; ++s) {
-        const int64_t page = place(t0 + key_token + s * 4, slot, bad);
-        load_rows(tile, s, key_base + page * c.key.stride[0] + slot * key_step);
-      }
-      tile.bad_tokens = 0;
-      uint32_t key_e[2] = {0u, 0u};
-      uint32_t value_e[2] = {0u, 0u};
-#pragma unroll
-      for (int e = 0; e < kOwn; ++e) {
-        const int64_t page = place(t0 + own_token + e, slot, bad);
-        if (bad) tile.bad_tokens |= 1u << e;
-        const C* row = value_base + page * c.value.stride[0] + slot * value_step;
-        if constexpr (kLater) {
-          tile.value_row[e] = row;
-        } else {
-          tile.value[e] = load_run<C, kRun, MODE>(row, value_at[0], c.value.width);
-        }
-        if constexpr (kCoded) {
-          key_e[e / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(
-                              c.key.exponents[page * c.key.exponent_stride[0] + h * c.key.exponent_stride[1] +
-                                              slot * c.key.exponent_stride[2]])) << (8 * (e % 4));
-          value_e[e / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(
-                                c.value.exponents[page * c.value.exponent_stride[0] + h * c.value.exponent_stride[1] +
-                                                  slot * c.value.exponent_stride[2]])) << (8 * (e % 4));
-        }
-      }
-      tile.key_e.w[0] = key_e[0];
-      tile.key_e.w[1] = key_e[1];
-      tile.value_e.w[0] = value_e[0];
-      tile.value_e.w[1] = value_e[1];
-    }
-  };
-
-  // Infinite numbers: a repeated element of a key times zero, or an infinite value
-  // times a part of its weight that is zero, would be NaN where the result is
-  // infinite.  A wave that ends with NaN runs again without the former, with the
-  // parts of the weights for finite values and one for the others.  (8-bit numbers
-  // have no infinities.)
-  bool careful = false;
-  const auto work_on = [&](const Tile& tile, int t0) {
-    f32x4 score[kKeyRows];
-#pragma unroll
-    for (int s = 0; s < kKeyRows; ++s) {
-      score[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // where the lane's runs of a key begin (lane (n, g): dimensions (j*4 + g) * kKeyRun ..), the queries there
+    // as operand B
+    int key_at[kKeyRuns];
+    // (in LDS with rows of 256: all waves hold the same)
+    u32x4 q_own[kLater ? 1 : kKeyRuns][kQ];
+    const auto q_of = [&](int j, int p) { return kLater ? q_shared[j][p][lane] : q_own[kLater ? 0 : j][p]; };
+    {
+      const int head = n < heads_here ? n : 0;
+      const T* q_row = static_cast<const T*>(a.query) + b * a.query_stride[0] + (head0 + head) * a.query_stride[1];
 #pragma unroll
       for (int j = 0; j < kKeyRuns; ++j) {
-        if constexpr (kF32) {
-          const u32x4 q = q_of(j, 0);
+        const int d = (j * 4 + g) * kKeyRun;
+        key_at[j] = run_start(d, kKeyRun, c.key.width);
+        const RawVec<kKeyRun * sizeof(T)> raw = load_run<T, kKeyRun, MODE>(q_row, key_at[j], c.key.width);
+        float q[kKeyRun];
+#pragma unroll
+        for (int i = 0; i < kKeyRun; ++i) {
+          const bool mine = key_at[j] + i >= d && key_at[j] + i < c.key.width;
+          q[i] = mine && n < heads_here ? Elem<T>::get(raw.w, i) : 0.0f;
+        }
+#pragma unroll
+        for (int p = 0; p < kQ; ++p) {
+          u32x4 words;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint32_t w = tile.key[s][j].w[i];
-            if (careful && key_at[j] + i < (j * 4 + g) * kKeyRun) w = 0u;
-            score[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w), __uint_as_float(q[i]), score[s], 0, 0, 0);
-          }
-        } else {
-          uint32_t w[4];
-          to_words<C, 8>(tile.key[s][j], w);
-          if (!kCoded && careful) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int repeated = (j * 4 + g) * kKeyRun - key_at[j] - 2 * i;
-              w[i] = repeated <= 0 ? w[i] : (repeated == 1 ? w[i] & 0xffff0000u : 0u);
+            if constexpr (kF32) {
+              words[i] = __float_as_uint(q[i]);
+            } else {
+              words[i] = U::pack(q[(2 * i) % kKeyRun], q[(2 * i + 1) % kKeyRun]);
+              q[(2 * i) % kKeyRun] -= U::unpack(words[i])[0];
+              q[(2 * i + 1) % kKeyRun] -= U::unpack(words[i])[1];
             }
           }
-#pragma unroll
-          for (int p = 0; p < kQ; ++p) score[s] = U::multiply(u32x4{w[0], w[1], w[2], w[3]}, q_of(j, p), score[s]);
+          if constexpr (!kLater) {
+            q_own[j][p] = words;
+          } else if (wave == 0) {
+            q_shared[j][p][lane] = words;
+          }
         }
       }
+      if constexpr (kLater) __syncthreads();
     }
+    f32x4 acc[kValues];
+    float top;  // of head n, the same in its four lanes
+    float sum;  // of head n and the tokens of this lane
 
-    RawVec<kRun * sizeof(C)> value[kBlocks][kOwn];
-    const auto load_values = [&](int jb) {
-#pragma unroll
-      for (int e = 0; e < kOwn; ++e) {
-        const C* row = MODE == kBlocks8 ? tile.value_row[0] + e * value_step
-                                        : tile.value_row[kLater && MODE != kBlocks8 ? e : 0];
-        value[jb][e] = load_run<C, kRun, MODE>(row, value_at[jb], c.value.width);
-      }
+    // What a tile needs from memory.
+    struct Tile {
+      RawVec<kKeyRun * sizeof(C)> key[kKeyRows][kKeyRuns];
+      RawVec<kRun * sizeof(C)> value[kLater ? 1 : kOwn];
+      const C* value_row[kLater && MODE != kBlocks8 ? kOwn : 1];  // where they are, for later
+      RawVec<8> key_e, value_e;                        // exponents of the tokens this lane weighs, a byte each
+      uint32_t bad_tokens;                             // tokens whose page is outside the cache, a bit each
     };
-    if constexpr (kLater) {
-      load_values(0);
-    } else {
+    const auto is_bad = [&](int64_t id) { return id < 0 || id >= c.pages; };
+    const auto load_rows = [&](Tile& tile, int s, const C* key_row) {
 #pragma unroll
-      for (int e = 0; e < kOwn; ++e) value[0][e] = tile.value[e];
-    }
-
-    // scores in powers of two
-    float s2[kOwn];
-    float most = -INFINITY;
+      for (int j = 0; j < kKeyRuns; ++j) tile.key[s][j] = load_run<C, kKeyRun, MODE>(key_row, key_at[j], c.key.width);
+    };
+    // kBlocks8: the page ids of the blocks of a tile that a lane loads keys of and
+    // weighs, asked for a tile ahead; a block behind what is seen stands for its
+    // last one.
+    const int last = (end - 1) & ~7;
+    const auto key_block = [&](int t0) {
+      const int t = (t0 + key_token) & ~7;
+      return t < last ? t : last;
+    };
+    const auto own_block = [&](int t0) {
+      const int t = (t0 + own_token) & ~7;
+      return t < last ? t : last;
+    };
+    struct Ids {
+      int64_t key, own;
+    };
+    const auto ids_of = [&](int t0) {
+      return Ids{pages[page_of_token(a, key_block(t0))], pages[page_of_token(a, own_block(t0))]};
+    };
+    const auto load_tile = [&](Tile& tile, int t0, const Ids& ids) {
+      if constexpr (MODE == kBlocks8) {
+        int t = key_block(t0);
+        int slot = t - page_of_token(a, t) * c.page_size + (key_token & 7);
+        int64_t page = is_bad(ids.key) ? 0 : ids.key;
+        const C* row = key_base + page * c.key.stride[0] + slot * key_step;
 #pragma unroll
-    for (int e = 0; e < kOwn; ++e) {
-      s2[e] = score[e / 4][e % 4] * to_log2;
-      if constexpr (kCoded) s2[e] = ldexpf(s2[e], static_cast<int8_t>(tile.key_e.w[e / 4] >> (8 * (e % 4))));
-    }
-    if (a.table != nullptr) {
-      // every token of the tile farther than the last border: one number a head
-      if (seen.end - t0 - kTile >= border[map.side - 1]) {
-        const float far = bias[map.side - 1][n];
+        for (int s = 0; s < kKeyRows; ++s) load_rows(tile, s, row + s * 4 * key_step);
+        t = own_block(t0);
+        slot = t - page_of_token(a, t) * c.page_size + (own_token & 7);
+        const bool bad = is_bad(ids.own);
+        page = bad ? 0 : ids.own;
+        tile.bad_tokens = bad ? 0xffu : 0u;
+        row = value_base + page * c.value.stride[0] + slot * value_step;
 #pragma unroll
-        for (int e = 0; e < kOwn; ++e) s2[e] += far;
+        for (int e = 0; e < (kLater ? 0 : kOwn); ++e)
+          tile.value[e] = load_run<C, kRun, MODE>(row + e * value_step, value_at[0], c.value.width);
+        tile.value_row[0] = row;
+        if constexpr (kCoded) {
+          __builtin_memcpy(&tile.key_e, c.key.exponents + page * c.key.exponent_stride[0] +
+                                            h * c.key.exponent_stride[1] + slot, 8);
+          __builtin_memcpy(&tile.value_e, c.value.exponents + page * c.value.exponent_stride[0] +
+                                              h * c.value.exponent_stride[1] + slot, 8);
+        }
       } else {
+        const auto place = [&](int t, int& slot, bool& bad) {
+          t = t < end ? t : end - 1;  // a token behind what is seen stands for the last one
+          const int e = page_of_token(a, t);
+          slot = t - e * c.page_size;
+          const int64_t id = pages[e];
+          bad = is_bad(id);
+          return bad ? int64_t(0) : id;
+        };
+        int slot;
+        bool bad;
+#pragma unroll
+        for (int s = 0; s < kKeyRows; ++s) {
+          const int64_t page = place(t0 + key_token + s * 4, slot, bad);
+          load_rows(tile, s, key_base + page * c.key.stride[0] + slot * key_step);
+        }
+        tile.bad_tokens = 0;
+        uint32_t key_e[2] = {0u, 0u};
+        uint32_t value_e[2] = {0u, 0u};
 #pragma unroll
         for (int e = 0; e < kOwn; ++e) {
-          const int away = seen.end - 1 - (t0 + own_token + e);
-          s2[e] += bias[bucket_of_distance(border, map, away < 0 ? 0 : away)][n];
+          const int64_t page = place(t0 + own_token + e, slot, bad);
+          if (bad) tile.bad_tokens |= 1u << e;
+          const C* row = value_base + page * c.value.stride[0] + slot * value_step;
+          if constexpr (kLater) {
+            tile.value_row[e] = row;
+          } else {
+            tile.value[e] = load_run<C, kRun, MODE>(row, value_at[0], c.value.width);
+          }
+          if constexpr (kCoded) {
+            key_e[e / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(
+                                c.key.exponents[page * c.key.exponent_stride[0] + h * c.key.exponent_stride[1] +
+                                                slot * c.key.exponent_stride[2]])) << (8 * (e % 4));
+            value_e[e / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(
+                                  c.value.exponents[page * c.value.exponent_stride[0] + h * c.value.exponent_stride[1] +
+                                                    slot * c.value.exponent_stride[2]])) << (8 * (e % 4));
+          }
+        }
+        tile.key_e.w[0] = key_e[0];
+        tile.key_e.w[1] = key_e[1];
+        tile.value_e.w[0] = value_e[0];
+        tile.value_e.w[1] = value_e[1];
+      }
+    };
+
+    // Infinite numbers: a repeated element of a key times zero, or an infinite value
+    // times a part of its weight that is zero, would be NaN where the result is
+    // infinite.  A wave that ends with NaN runs again without the former, with the
+    // parts of the weights for finite values and one for the others.  (8-bit numbers
+    // have no infinities.)
+    bool careful = false;
+    const auto work_on = [&](const Tile& tile, int t0) {
+      f32x4 score[kKeyRows];
+#pragma unroll
+      for (int s = 0; s < kKeyRows; ++s) {
+        score[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < kKeyRuns; ++j) {
+          if constexpr (kF32) {
+            const u32x4 q = q_of(j, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w = tile.key[s][j].w[i];
+              if (careful && key_at[j] + i < (j * 4 + g) * kKeyRun) w = 0u;
+              score[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w), __uint_as_float(q[i]), score[s], 0, 0, 0);
+            }
+          } else {
+            uint32_t w[4];
+            to_words<C, 8>(tile.key[s][j], w);
+            if (!kCoded && careful) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int repeated = (j * 4 + g) * kKeyRun - key_at[j] - 2 * i;
+                w[i] = repeated <= 0 ? w[i] : (repeated == 1 ? w[i] & 0xffff0000u : 0u);
+              }
+            }
+#pragma unroll
+            for (int p = 0; p < kQ; ++p) score[s] = U::multiply(u32x4{w[0], w[1], w[2], w[3]}, q_of(j, p), score[s]);
+          }
         }
       }
-    }
-    const bool edge = t0 < begin || t0 + kTile > end;
-    if (edge || __any(tile.bad_tokens != 0)) {
+
+      RawVec<kRun * sizeof(C)> value[kBlocks][kOwn];
+      const auto load_values = [&](int jb) {
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) {
+          const C* row = MODE == kBlocks8 ? tile.value_row[0] + e * value_step
+                                          : tile.value_row[kLater && MODE != kBlocks8 ? e : 0];
+          value[jb][e] = load_run<C, kRun, MODE>(row, value_at[jb], c.value.width);
+        }
+      };
+      if constexpr (kLater) {
+        load_values(0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) value[0][e] = tile.value[e];
+      }
+
+      // scores in powers of two
+      float s2[kOwn];
+      float most = -INFINITY;
 #pragma unroll
       for (int e = 0; e < kOwn; ++e) {
-        const int t = t0 + own_token + e;
-        const bool out_of_sight = t < begin || t >= end;
-        if ((tile.bad_tokens >> e) & 1) s2[e] = NAN;
-        if (out_of_sight) s2[e] = -INFINITY;
+        s2[e] = score[e / 4][e % 4] * to_log2;
+        if constexpr (kCoded) s2[e] = ldexpf(s2[e], static_cast<int8_t>(tile.key_e.w[e / 4] >> (8 * (e % 4))));
       }
-    }
+      if (a.table != nullptr) {
+        // every token of the tile farther than the last border: one number a head
+        if (seen.end - t0 - kTile >= border[map.side - 1]) {
+          const float far = bias[map.side - 1][n];
 #pragma unroll
-    for (int e = 0; e < kOwn; ++e) most = fmaxf(most, s2[e]);
-
-    if (__any(most > top + kSlack)) {
-      most = fmaxf(most, __shfl_xor(most, 16, 64));
-      most = fmaxf(most, __shfl_xor(most, 32, 64));
-      const float next = fmaxf(top, most);
-      const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next);
-      top = next;
-      sum *= keep;
-      // lane (n, g) holds the heads g*4 .. g*4+3 of its columns
+          for (int e = 0; e < kOwn; ++e) s2[e] += far;
+        } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float f = __shfl(keep, g * 4 + i, 64);
-#pragma unroll
-        for (int j = 0; j < kValues; ++j) acc[j][i] *= f;
+          for (int e = 0; e < kOwn; ++e) {
+            const int away = seen.end - 1 - (t0 + own_token + e);
+            s2[e] += bias[bucket_of_distance(border, map, away < 0 ? 0 : away)][n];
+          }
+        }
       }
-    }
-    const float from = top == -INFINITY ? 0.0f : top - U::kShift;
-    float weight[kOwn];
-#pragma unroll
-    for (int e = 0; e < kOwn; ++e) {
-      weight[e] = __builtin_amdgcn_exp2f(s2[e] - from);
-      sum += weight[e];
-      if constexpr (kCoded) weight[e] = ldexpf(weight[e], static_cast<int8_t>(tile.value_e.w[e / 4] >> (8 * (e % 4))));
-    }
-    u32x4 w16[kP];
-    u32x4 one16;
-    if (!kF32 && !kCoded && careful) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = weight[(2 * i) % kOwn];
-        const float y = weight[(2 * i + 1) % kOwn];
-        one16[i] = U::pack(x > 0.0f ? 1.0f : x, y > 0.0f ? 1.0f : y);
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < (kF32 ? 0 : kP); ++p) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t w = U::pack(weight[(2 * i) % kOwn], weight[(2 * i + 1) % kOwn]);
-        w16[p][i] = w;
-        weight[(2 * i) % kOwn] -= U::unpack(w)[0];
-        weight[(2 * i + 1) % kOwn] -= U::unpack(w)[1];
-      }
-    }
-
-#pragma unroll
-    for (int jb = 0; jb < kBlocks; ++jb) {
-      if (jb + 1 < kBlocks) load_values(jb + 1);
-      if (edge) {
-        // a value out of sight may be anything; its weight is zero, and so has to be the product
+      const bool edge = t0 < begin || t0 + kTile > end;
+      if (edge || __any(tile.bad_tokens != 0)) {
 #pragma unroll
         for (int e = 0; e < kOwn; ++e) {
           const int t = t0 + own_token + e;
-#pragma unroll
-          for (uint32_t& w : value[jb][e].w) w = t < begin || t >= end ? 0u : w;
+          const bool out_of_sight = t < begin || t >= end;
+          if ((tile.bad_tokens >> e) & 1) s2[e] = NAN;
+          if (out_of_sight) s2[e] = -INFINITY;
         }
       }
-      if constexpr (kF32) {
 #pragma unroll
-        for (int e = 0; e < kOwn; ++e) {
+      for (int e = 0; e < kOwn; ++e) most = fmaxf(most, s2[e]);
+
+      if (__any(most > top + kSlack)) {
+        most = fmaxf(most, __shfl_xor(most, 16, 64));
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        const float next = fmaxf(top, most);
+        const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next);
+        top = next;
+        sum *= keep;
+        // lane (n, g) holds the heads g*4 .. g*4+3 of its columns
 #pragma unroll
-          for (int j = 0; j < kRun; ++j)
-            acc[jb * kRun + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                weight[e], __uint_as_float(value[jb][e].w[j]), acc[jb * kRun + j], 0, 0, 0);
+        for (int i = 0; i < 4; ++i) {
+          const float f = __shfl(keep, g * 4 + i, 64);
+#pragma unroll
+          for (int j = 0; j < kValues; ++j) acc[j][i] *= f;
         }
-      } else {
-        uint32_t words[8][kRun / 2];
+      }
+      const float from = top == -INFINITY ? 0.0f : top - U::kShift;
+      float weight[kOwn];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to_words<C, kRun>(value[jb][e % kOwn], words[e]);
+      for (int e = 0; e < kOwn; ++e) {
+        weight[e] = __builtin_amdgcn_exp2f(s2[e] - from);
+        sum += weight[e];
+        if constexpr (kCoded) weight[e] = ldexpf(weight[e], static_cast<int8_t>(tile.value_e.w[e / 4] >> (8 * (e % 4))));
+      }
+      u32x4 w16[kP];
+      u32x4 one16;
+      if (!kF32 && !kCoded && careful) {
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-          u32x4 column;
+        for (int i = 0; i < 4; ++i) {
+          const float x = weight[(2 * i) % kOwn];
+          const float y = weight[(2 * i + 1) % kOwn];
+          one16[i] = U::pack(x > 0.0f ? 1.0f : x, y > 0.0f ? 1.0f : y);
+        }
+      }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            column[i] = __builtin_amdgcn_perm(words[2 * i + 1][j / 2], words[2 * i][j / 2],
-                                              j % 2 == 0 ? 0x05040100u : 0x07060302u);
-          if (!kCoded && careful) {
-            u32x4 others;
+      for (int p = 0; p < (kF32 ? 0 : kP); ++p) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              others[i] = column[i] ^ U::finite_halves(column[i]);
-              column[i] ^= others[i];
-            }
-            acc[jb * kRun + j] = U::multiply(one16, others, acc[jb * kRun + j]);
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = U::pack(weight[(2 * i) % kOwn], weight[(2 * i + 1) % kOwn]);
+          w16[p][i] = w;
+          weight[(2 * i) % kOwn] -= U::unpack(w)[0];
+          weight[(2 * i + 1) % kOwn] -= U::unpack(w)[1];
+        }
+      }
+
+#pragma unroll
+      for (int jb = 0; jb < kBlocks; ++jb) {
+        if (jb + 1 < kBlocks) load_values(jb + 1);
+        if (edge) {
+          // a value out of sight may be anything; its weight is zero, and so has to be the product
+#pragma unroll
+          for (int e = 0; e < kOwn; ++e) {
+            const int t = t0 + own_token + e;
+#pragma unroll
+            for (uint32_t& w : value[jb][e].w) w = t < begin || t >= end ? 0u : w;
           }
+        }
+        if constexpr (kF32) {
 #pragma unroll
-          for (int p = 0; p < kP; ++p) acc[jb * kRun + j] = U::multiply(w16[p], column, acc[jb * kRun + j]);
+          for (int e = 0; e < kOwn; ++e) {
+#pragma unroll
+            for (int j = 0; j < kRun; ++j)
+              acc[jb * kRun + j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  weight[e], __uint_as_float(value[jb][e].w[j]), acc[jb * kRun + j], 0, 0, 0);
+          }
+        } else {
+          uint32_t words[8][kRun / 2];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) to_words<C, kRun>(value[jb][e % kOwn], words[e]);
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) {
+            u32x4 column;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              column[i] = __builtin_amdgcn_perm(words[2 * i + 1][j / 2], words[2 * i][j / 2],
+                                                j % 2 == 0 ? 0x05040100u : 0x07060302u);
+            if (!kCoded && careful) {
+              u32x4 others;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                others[i] = column[i] ^ U::finite_halves(column[i]);
+                column[i] ^= others[i];
+              }
+              acc[jb * kRun + j] = U::multiply(one16, others, acc[jb * kRun + j]);
+            }
+#pragma unroll
+            for (int p = 0; p < kP; ++p) acc[jb * kRun + j] = U::multiply(w16[p], column, acc[jb * kRun + j]);
+          }
         }
       }
-    }
-  };
+    };
 
-  constexpr int kStride = kWavesPerBlock * kTile;
-  for (;; careful = true) {
+    constexpr int kStride = kWavesPerBlock * kTile;
+    for (;; careful = true) {
 #pragma unroll
-    for (int j = 0; j < kValues; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    top = -INFINITY;
-    sum = 0.0f;
-    int t0 = base + wave * kTile;
-    Ids ids{};
-    if (MODE == kBlocks8 && t0 < end) ids = ids_of(t0);
-    for (; t0 < end; t0 += kStride) {
-      // the queries in LDS are read for every tile: kept, they would take the registers they are spared
-      if constexpr (kLater) asm volatile("" ::: "memory");
-      Tile tile;
-      load_tile(tile, t0, ids);
-      if constexpr (MODE == kBlocks8) ids = ids_of(t0 + kStride);
-      work_on(tile, t0);
+      for (int j = 0; j < kValues; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      top = -INFINITY;
+      sum = 0.0f;
+      int t0 = base + wave * kTile;
+      Ids ids{};
+      if (MODE == kBlocks8 && t0 < end) ids = ids_of(t0);
+      for (; t0 < end; t0 += kStride) {
+        // the queries in LDS are read for every tile: kept, they would take the registers they are spared
+        if constexpr (kLater) asm volatile("" ::: "memory");
+        Tile tile;
+        load_tile(tile, t0, ids);
+        if constexpr (MODE == kBlocks8) ids = ids_of(t0 + kStride);
+        work_on(tile, t0);
+      }
+      if (kCoded || careful) break;
+      bool odd = sum != sum;
+#pragma unroll
+      for (int j = 0; j < kValues; ++j) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd = odd || acc[j][i] != acc[j][i];
+      }
+      if (!__any(odd)) break;
     }
-    if (kCoded || careful) break;
-    bool odd = sum != sum;
-#pragma unroll
-    for (int j = 0; j < kValues; ++j) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) odd = odd || acc[j][i] != acc[j][i];
-    }
-    if (!__any(odd)) break;
-  }
 
-  // join the waves
-  sum += __shfl_xor(sum, 16, 64);
-  sum += __shfl_xor(sum, 32, 64);
-  if (g == 0) {
-    wave_top[wave][n] = top;
-    wave_sum[wave][n] = sum;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int hh = g * 4 + i;
-    float most = wave_top[0][hh];
-#pragma unroll
-    for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_top[w][hh]);
-    const float mine = wave_top[wave][hh];
-    const float f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - most);
-#pragma unroll
-    for (int j = 0; j < kValues; ++j) acc[j][i] *= f;
-  }
-  const auto each_out = [&](auto&& f) {
+    // join the waves
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (g == 0) {
+      wave_top[wave][n] = top;
+      wave_sum[wave][n] = sum;
+    }
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int hh = g * 4 + i;
+      float most = wave_top[0][hh];
 #pragma unroll
-      for (int j = 0; j < kValues; ++j) {
-        const int d = value_at[j / kRun] + j % kRun;
-        if (hh < heads_here && (MODE != kNarrow || d < c.value.width)) acc[j][i] = f(wave_out[wave % kOutWaves][hh][d], acc[j][i]);
+      for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_top[w][hh]);
+      const float mine = wave_top[wave][hh];
+      const float f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - most);
+#pragma unroll
+      for (int j = 0; j < kValues; ++j) acc[j][i] *= f;
+    }
+    const auto each_out = [&](auto&& f) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int hh = g * 4 + i;
+#pragma unroll
+        for (int j = 0; j < kValues; ++j) {
+          const int d = value_at[j / kRun] + j % kRun;
+          if (hh < heads_here && (MODE != kNarrow || d < c.value.width)) acc[j][i] = f(wave_out[wave % kOutWaves][hh][d], acc[j][i]);
+        }
+      }
+    };
+    const auto put = [](float& to, float x) { return to = x; };
+    if constexpr (kLater) {
+      // two waves hand their sums to the other two; lanes that hold the same column
+      // read it before either writes
+      if (wave >= kOutWaves) each_out(put);
+      __syncthreads();
+      if (wave < kOutWaves) each_out([](float& to, float x) { return x + to; });
+      __syncthreads();
+      if (wave < kOutWaves) each_out(put);
+    } else {
+      each_out(put);
+    }
+    __syncthreads();
+    const int width = c.value.width;
+    for (int i = threadIdx.x; i < heads_here * width; i += kBlock) {
+      const int hh = i / width;
+      const int d = i - hh * width;
+      float most = wave_top[0][hh];
+#pragma unroll
+      for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_top[w][hh]);
+      float total = 0.0f;
+      float x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWavesPerBlock; ++w) {
+        const float mine = wave_top[w][hh];
+        total += (mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - most)) * wave_sum[w][hh];
+        if (w < kOutWaves) x += wave_out[w % kOutWaves][hh][d];
+      }
+      if (whole) {
+        const int64_t row = static_cast<int64_t>(b) * heads_q + head0 + hh;
+        const bool none = total == 0.0f;
+        static_cast<T*>(a.out)[row * width + d] = rounded<T>(seen.bad ? NAN : (none ? 0.0f : x / total));
+        if (a.lse != nullptr && d == 0)
+          a.lse[row] = seen.bad ? NAN : (none ? -INFINITY : (most - U::kShift + __builtin_amdgcn_logf(total)) * kLn2);
+      } else {
+        const int64_t row = part * heads_q + head0 + hh;
+        a.part_out[row * width + d] = x;
+        if (d == 0) a.part_sum[row] = make_float2(most, total);
       }
     }
-  };
-  const auto put = [](float& to, float x) { return to = x; };
-  if constexpr (kLater) {
-    // two waves hand their sums to the other two; lanes that hold the same column
-    // read it before either writes
-    if (wave >= kOutWaves) each_out(put);
-    __syncthreads();
-    if (wave < kOutWaves) each_out([](float& to, float x) { return x + to; });
-    __syncthreads();
-    if (wave < kOutWaves) each_out(put);
-  } else {
-    each_out(put);
-  }
-  __syncthreads();
-  const int width = c.value.width;
-  for (int i = threadIdx.x; i < heads_here * width; i += kBlock) {
-    const int hh = i / width;
-    const int d = i - hh * width;
-    float most = wave_top[0][hh];
-#pragma unroll
-    for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_top[w][hh]);
-    float total = 0.0f;
-    float x = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWavesPerBlock; ++w) {
-      const float mine = wave_top[w][hh];
-      total += (mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - most)) * wave_sum[w][hh];
-      if (w < kOutWaves) x += wave_out[w % kOutWaves][hh][d];
-    }
-    if (whole) {
-      const int64_t row = static_cast<int64_t>(b) * heads_q + head0 + hh;
-      const bool none = total == 0.0f;
-      static_cast<T*>(a.out)[row * width + d] = rounded<T>(seen.bad ? NAN : (none ? 0.0f : x / total));
-      if (a.lse != nullptr && d == 0)
-        a.lse[row] = seen.bad ? NAN : (none ? -INFINITY : (most - U::kShift + __builtin_amdgcn_logf(total)) * kLn2);
-    } else {
-      const int64_t row = part * heads_q + head0 + hh;
-      a.part_out[row * width + d] = x;
-      if (d == 0) a.part_sum[row] = make_float2(most, total);
-    }
-  }
-  __syncthreads();  // the next part's results go where these were
+    __syncthreads();  // the next part's results go where these were
   }
 }
 
@@ -1000,6 +1019,7 @@ int as_paged_attention(const as_paged_cache* cache, const void* query, const int
   const Workspace parts = workspace_of(cache, group, shares);
   if (workspace_bytes < parts.bytes || (parts.bytes > 0 && workspace == nullptr))
     return fail(AS_ERR_WORKSPACE, "paged attention needs %zu workspace bytes", parts.bytes);
+  if (!aligned(workspace, 16)) return fail(AS_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
   if (a.cache.sequences == 0) return AS_OK;
   if (a.cache.sequences > 65535 || group * a.cache.heads * a.cache.sequences > kMaxBlocksPerLaunch)
     return fail(AS_ERR_UNSUPPORTED, "at most 65535 sequences, and 2^22 query heads of all sequences");

@@ -36,7 +36,7 @@ struct EdgeWalk {
 // each is gathered a few times (4 heads, with and without it: 1M nodes of 16 edges
 // 136 and 192 us, of 4 edges 55 and 57, of 2 edges 36 and 32; 400,000 of 16 53 and
 // 54, 250,000 of 16 40 and 34).  Positions that do not fit are read as they are.
-constexpr int kFitBlocks = kBlock;
+constexpr int kFitBlocks = 4 * kBlock;
 inline bool shorten(int64_t n, int64_t nnz) { return n > (int64_t(1) << 19) && nnz >= 4 * n; }
 
 __global__ __launch_bounds__(kBlock) void short_positions_kernel(const int64_t* __restrict__ positions,
@@ -176,7 +176,8 @@ __global__ __launch_bounds__(kBlock) void position_bias_kernel(EdgeWalk w, Posit
   }
   bool fits = false;
   if (w.short_positions != nullptr) {
-    fits = __syncthreads_and(w.fits[threadIdx.x]);
+    const int4 four = reinterpret_cast<const int4*>(w.fits)[threadIdx.x];
+    fits = __syncthreads_and(four.x & four.y & four.z & four.w);
   } else {
     __syncthreads();
   }
@@ -188,7 +189,8 @@ __global__ __launch_bounds__(kBlock) void position_bias_kernel(EdgeWalk w, Posit
     const uint32_t k = step_buckets(w, fits, border, map, marks[wave], b, row);
     const int64_t at = b + kRun * lane_id();
     T* to = out + at;
-    if (found != nullptr && at < w.nnz) found[at / kRun] = k;  // the last word may end behind the edges
+    // the last word may end behind the edges
+    if (found != nullptr && at < w.nnz) __builtin_nontemporal_store(k, found + at / kRun);
     const int left = at + kRun <= w.nnz ? kRun : (at < w.nnz ? static_cast<int>(w.nnz - at) : 0);
     for (int h = 0; h < heads; ++h, to += w.nnz) {
       Four<T> four;
@@ -399,6 +401,7 @@ int as_csr_position_bias(const int64_t* crow, const int64_t* col, const int64_t*
   const size_t need = as_csr_position_bias_workspace_bytes(n, nnz, positions != nullptr);
   if (workspace_bytes < need || (need > 0 && workspace == nullptr))
     return fail(AS_ERR_WORKSPACE, "the position bias needs %zu workspace bytes", need);
+  if (!aligned(workspace, 16)) return fail(AS_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
   if (nnz == 0) return AS_OK;
   EdgeWalk walk{crow, col, positions, nullptr, nullptr, n, nnz};
   // a wave takes further steps (which spare it the search for its first row) from 8,192 waves on
@@ -443,8 +446,10 @@ int as_csr_position_bias_backward(const uint8_t* found, const void* grad, void* 
   const size_t need = as_csr_position_bias_backward_workspace_bytes(nnz, heads, buckets);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(AS_ERR_WORKSPACE, "the position bias gradient needs %zu workspace bytes", need);
+  if (!aligned(workspace, 16)) return fail(AS_ERR_INVALID_ARGUMENT, "the workspace must be 16-byte aligned");
   const GradientGrid g = gradient_grid(nnz, heads, buckets);
-  if (g.chunks * heads > kMaxBlocksPerLaunch) return fail(AS_ERR_UNSUPPORTED, "too many edges and heads for one launch");
+  if (g.chunks * heads * g.threads > UINT32_MAX)
+    return fail(AS_ERR_UNSUPPORTED, "too many edges and heads for one launch");
   double* partial = static_cast<double*>(workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_element(dtype, [&](auto e) {

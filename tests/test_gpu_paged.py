@@ -143,6 +143,41 @@ def test_rows_that_the_bias_masks(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("max_length", [None, 60])
+def test_masks_of_the_lowest_number(dtype, max_length):
+    """Scores that are all the type's lowest number have equal weights; beside others they have none."""
+    cache = Cache([7, 60], 1, 32, 32, 8, dtype, seed=23)
+    query = torch.randn(2, 1, 32, dtype=dtype, device="cuda")
+    table = torch.zeros(8, 1, dtype=dtype, device="cuda")
+    table[:7] = torch.finfo(dtype).min  # distances below 14: all of the short one, the last 14 of the long one
+    args, _ = cache.args()
+    out = autosage_amd.paged_attention(query, *args, torch.tensor(cache.lengths).cuda(), scale=0.0, bias_table=table,
+                                       max_distance=20, bidirectional=False, max_length=max_length).double().cpu()
+    rows = [cache.rows["value"][0][:, 0].mean(0), cache.rows["value"][1][:46, 0].mean(0)]
+    eps = torch.finfo(dtype).eps
+    for got, want in zip(out[:, 0], rows):
+        assert torch.allclose(got, want, rtol=eps, atol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("count", [65, 257, 600, 1100])
+@pytest.mark.parametrize("page", [8, 5])
+def test_many_sequences(dtype, count, page):
+    """More sequences than lanes, threads and shares, some without tokens, with and without a bound of their lengths."""
+    gen = torch.Generator().manual_seed(count)
+    lengths = torch.randint(0, 45, (count,), generator=gen).tolist()
+    lengths[count // 2], lengths[0], lengths[-1] = 700, 0, 0
+    cache, query, out, lse = _attend(lengths, 1, 2, 16, 16, page, dtype, seed=count, max_length=None)
+    args, _ = cache.args()
+    again = autosage_amd.paged_attention(query.cuda(), *args, torch.tensor(lengths).cuda(), scale=0.25, max_length=700)
+    assert torch.equal(again, out)
+    short = [min(n, 45) for n in lengths]
+    single = autosage_amd.paged_attention(query.cuda(), *args, torch.tensor(short).cuda(), scale=0.25, max_length=45)
+    keep = [i for i, n in enumerate(lengths) if n <= 45]
+    assert torch.allclose(single[keep].float(), out[keep].float(), rtol=2 * torch.finfo(dtype).eps, atol=1e-6)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_infinite_and_nan_rows_that_are_seen(dtype):
     cache = Cache([40, 40, 40], 1, 32, 32, 8, dtype, seed=9)
     (k, v, ptr, idx), _ = cache.args()
