@@ -216,7 +216,7 @@ __global__ __launch_bounds__(kBlock) void position_bias_kernel(EdgeWalk w, Posit
 // (bucket-major: a wave's columns lie in different banks), so nothing is added
 // atomically and the order of every sum is fixed: the same inputs give the same
 // bits.  (Adding with LDS atomics, which would not wait for the sum to come
-// back, takes 190 cycles a wave here: 365 us where this takes 80, for 16M edges
+// back, takes 190 cycles a wave here: 365 us where this takes 77, for 16M edges
 // and 4 heads.)  A thread reads the sums of its four neighbouring edges at once
 // and puts edges of one bucket together in registers.  It adds at most
 // kMaxSteps * 4 = 64 numbers in fp32; all sums above that are fp64.
