@@ -464,9 +464,9 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
 #pragma unroll
       for (int j = 0; j < kKeyRuns; ++j) tile.key[s][j] = load_run<C, kKeyRun, MODE>(key_row, key_at[j], c.key.width);
     };
-    // kBlocks8: the page ids of the blocks of a tile that a lane loads keys of and
-    // weighs, asked for a tile ahead; a block behind what is seen stands for its
-    // last one.
+    // The page ids of what a lane loads keys of and weighs in a tile: of two blocks
+    // with kBlocks8 (asked for a tile ahead), where a block behind what is seen
+    // stands for its last one, else of every token, where the last token does.
     const int last = (end - 1) & ~7;
     const auto key_block = [&](int t0) {
       const int t = (t0 + key_token) & ~7;
@@ -476,24 +476,37 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
       const int t = (t0 + own_token) & ~7;
       return t < last ? t : last;
     };
+    constexpr bool kIdsAhead = MODE == kBlocks8;
     struct Ids {
-      int64_t key, own;
+      int64_t key[MODE == kBlocks8 ? 1 : kKeyRows];
+      int64_t own[MODE == kBlocks8 ? 1 : kOwn];
     };
+    const auto seen_token = [&](int t) { return t < end ? t : end - 1; };
     const auto ids_of = [&](int t0) {
-      return Ids{pages[page_of_token(a, key_block(t0))], pages[page_of_token(a, own_block(t0))]};
+      Ids ids;
+      if constexpr (MODE == kBlocks8) {
+        ids.key[0] = pages[page_of_token(a, key_block(t0))];
+        ids.own[0] = pages[page_of_token(a, own_block(t0))];
+      } else {
+#pragma unroll
+        for (int s = 0; s < kKeyRows; ++s) ids.key[s] = pages[page_of_token(a, seen_token(t0 + key_token + s * 4))];
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) ids.own[e] = pages[page_of_token(a, seen_token(t0 + own_token + e))];
+      }
+      return ids;
     };
     const auto load_tile = [&](Tile& tile, int t0, const Ids& ids) {
       if constexpr (MODE == kBlocks8) {
         int t = key_block(t0);
         int slot = t - page_of_token(a, t) * c.page_size + (key_token & 7);
-        int64_t page = is_bad(ids.key) ? 0 : ids.key;
+        int64_t page = is_bad(ids.key[0]) ? 0 : ids.key[0];
         const C* row = key_base + page * c.key.stride[0] + slot * key_step;
 #pragma unroll
         for (int s = 0; s < kKeyRows; ++s) load_rows(tile, s, row + s * 4 * key_step);
         t = own_block(t0);
         slot = t - page_of_token(a, t) * c.page_size + (own_token & 7);
-        const bool bad = is_bad(ids.own);
-        page = bad ? 0 : ids.own;
+        const bool bad = is_bad(ids.own[0]);
+        page = bad ? 0 : ids.own[0];
         tile.bad_tokens = bad ? 0xffu : 0u;
         row = value_base + page * c.value.stride[0] + slot * value_step;
 #pragma unroll
@@ -507,27 +520,23 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
                                               h * c.value.exponent_stride[1] + slot, 8);
         }
       } else {
-        const auto place = [&](int t, int& slot, bool& bad) {
-          t = t < end ? t : end - 1;  // a token behind what is seen stands for the last one
-          const int e = page_of_token(a, t);
-          slot = t - e * c.page_size;
-          const int64_t id = pages[e];
-          bad = is_bad(id);
-          return bad ? int64_t(0) : id;
+        const auto slot_of = [&](int t) {
+          t = seen_token(t);
+          return t - page_of_token(a, t) * c.page_size;
         };
-        int slot;
-        bool bad;
 #pragma unroll
         for (int s = 0; s < kKeyRows; ++s) {
-          const int64_t page = place(t0 + key_token + s * 4, slot, bad);
-          load_rows(tile, s, key_base + page * c.key.stride[0] + slot * key_step);
+          const int64_t page = is_bad(ids.key[s]) ? 0 : ids.key[s];
+          load_rows(tile, s, key_base + page * c.key.stride[0] + slot_of(t0 + key_token + s * 4) * key_step);
         }
         tile.bad_tokens = 0;
         uint32_t key_e[2] = {0u, 0u};
         uint32_t value_e[2] = {0u, 0u};
 #pragma unroll
         for (int e = 0; e < kOwn; ++e) {
-          const int64_t page = place(t0 + own_token + e, slot, bad);
+          const bool bad = is_bad(ids.own[e]);
+          const int64_t page = bad ? 0 : ids.own[e];
+          const int slot = slot_of(t0 + own_token + e);
           if (bad) tile.bad_tokens |= 1u << e;
           const C* row = value_base + page * c.value.stride[0] + slot * value_step;
           if constexpr (kLater) {
@@ -738,13 +747,14 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
       sum = 0.0f;
       int t0 = base + wave * kTile;
       Ids ids{};
-      if (MODE == kBlocks8 && t0 < end) ids = ids_of(t0);
+      if (kIdsAhead && t0 < end) ids = ids_of(t0);
       for (; t0 < end; t0 += kStride) {
         // the queries in LDS are read for every tile: kept, they would take the registers they are spared
         if constexpr (kLater) asm volatile("" ::: "memory");
         Tile tile;
+        if constexpr (!kIdsAhead) ids = ids_of(t0);
         load_tile(tile, t0, ids);
-        if constexpr (MODE == kBlocks8) ids = ids_of(t0 + kStride);
+        if constexpr (kIdsAhead) ids = ids_of(t0 + kStride);
         work_on(tile, t0);
       }
       if (kCoded || careful) break;

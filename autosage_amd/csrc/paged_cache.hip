@@ -7,10 +7,11 @@
 //
 // A copy (with a rounding to 8 bits in a quantised cache): bound by memory, or by
 // the launch for a few tokens.  A workgroup takes up to 16 tokens: its first wave
-// finds their places, then its threads move runs of 8 elements, all tokens of one
+// finds their places, then its threads move runs of 8 elements (4 in float32: 16
+// bytes of the tokens' type, so that the lanes of a wave are neighbours), all tokens of one
 // head before the next head, because the tokens of one head are neighbours in a
-// page.  Enough lanes for a row (a power of two) stand together, so that a row's
-// maximum takes a few shuffles.
+// page.  Where a row's maximum is needed its lanes are a power of two, so that it
+// takes a few shuffles; else they are as many as the row has runs.
 #include "paged_common.h"
 
 namespace as {
@@ -23,7 +24,9 @@ struct TokenRows {
 };
 
 constexpr int kMaxTokens = 16;  // of one workgroup
-constexpr int kElements = 8;    // of one thread
+// Elements of one thread, for tokens of T.
+template <typename T>
+constexpr int kElements = sizeof(T) == 4 ? 4 : 8;
 constexpr int kAhead = 4;       // runs of a thread whose loads are under way at once
 
 struct Places {
@@ -61,22 +64,22 @@ __device__ __forceinline__ void find_places(const PagedCache& c, const int64_t* 
 }
 
 // Runs of a row: the last one is moved back to end with the row (elements that
-// two runs share are moved twice), so that only rows of fewer than 8 elements
-// are moved one by one.  The accesses ask for the alignment of one byte: the
+// two runs share are moved twice), so that only the elements of rows that are
+// shorter than a run are moved one by one.  The accesses ask for the alignment of one byte: the
 // hardware has no other requirement.
-__device__ __forceinline__ int run_start(int d, int width) {
-  const int last = width > kElements ? width - kElements : 0;
+__device__ __forceinline__ int run_start(int d, int n, int width) {
+  const int last = width > n ? width - n : 0;
   return d < last ? d : last;
 }
-template <typename E>
-__device__ __forceinline__ RawVec<kElements * sizeof(E)> load_elements(const E* from, int width) {
-  RawVec<kElements * sizeof(E)> r;
-  if (width >= kElements) {
+template <int N, typename E>
+__device__ __forceinline__ RawVec<N * sizeof(E)> load_elements(const E* from, int width) {
+  RawVec<N * sizeof(E)> r;
+  if (width >= N) {
     __builtin_memcpy(&r, from, sizeof(r));
   } else {
-    E part[kElements];
+    E part[N];
 #pragma unroll
-    for (int i = 0; i < kElements; ++i) part[i] = from[i < width ? i : width - 1];
+    for (int i = 0; i < N; ++i) part[i] = from[i < width ? i : width - 1];
     __builtin_memcpy(&r, part, sizeof(r));
   }
   return r;
@@ -84,9 +87,9 @@ __device__ __forceinline__ RawVec<kElements * sizeof(E)> load_elements(const E* 
 typedef uint32_t u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
 // STREAM: past the caches, for what a read gives (48 sequences, 8-bit to fp16: 57 us,
 // 6.0 TB/s; 95 through them).  What is written to the pages stays: attention reads it next.
-template <bool STREAM, typename E>
-__device__ __forceinline__ void store_elements(E* to, int width, const RawVec<kElements * sizeof(E)>& r) {
-  if (width >= kElements) {
+template <bool STREAM, int N, typename E>
+__device__ __forceinline__ void store_elements(E* to, int width, const RawVec<N * sizeof(E)>& r) {
+  if (width >= N) {
     if constexpr (STREAM) {
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof(r)) / 16; ++i)
@@ -96,45 +99,63 @@ __device__ __forceinline__ void store_elements(E* to, int width, const RawVec<kE
       __builtin_memcpy(to, &r, sizeof(r));
     }
   } else {
-    E part[kElements];
+    E part[N];
     __builtin_memcpy(part, &r, sizeof(r));
 #pragma unroll
-    for (int i = 0; i < kElements; ++i) {
+    for (int i = 0; i < N; ++i) {
       if (i < width) to[i] = part[i];
     }
   }
 }
 
-// Lane, token and head of a thread's item.
+// How the items of a tensor's rows are told apart: `runs` for each row (i / runs =
+// i * magic >> (31 + shift) for i < 2^31, as paged attention divides by the page
+// size), then 2^log_tokens tokens of each head.
+struct RowItems {
+  int runs;
+  int shift;
+  uint32_t magic;
+};
+inline RowItems row_items(int width, int elements, bool power_of_two) {
+  RowItems it{};
+  it.runs = (width + elements - 1) / elements;
+  while ((1 << it.shift) < it.runs) ++it.shift;
+  if (power_of_two) it.runs = 1 << it.shift;
+  it.magic = static_cast<uint32_t>(((uint64_t(1) << (31 + it.shift)) + it.runs - 1) / static_cast<uint64_t>(it.runs));
+  return it;
+}
+// Run, token and head of a thread's item.
 struct Item {
   int run;
   int token;
   int head;
 };
-__device__ __forceinline__ Item item_of(int i, int log_runs, int log_tokens) {
-  const int r = i >> log_runs;
-  return Item{i & ((1 << log_runs) - 1), r & ((1 << log_tokens) - 1), r >> log_tokens};
+__device__ __forceinline__ Item item_of(int i, const RowItems& items, int log_tokens) {
+  const int r =
+      static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(i)) * items.magic) >> (31 + items.shift));
+  return Item{i - r * items.runs, r & ((1 << log_tokens) - 1), r >> log_tokens};
 }
 
 template <typename T, typename C>
 __device__ __forceinline__ void write_rows(const TokenRows& from, const PageTensor& to, const Places& places,
-                                           int64_t first, int count, int heads, int log_runs, int log_tokens) {
-  const int items = heads << (log_runs + log_tokens);
+                                           int64_t first, int count, int heads, const RowItems& row, int log_tokens) {
+  constexpr int N = kElements<T>;
+  const int items = (heads << log_tokens) * row.runs;
   for (int i0 = threadIdx.x; i0 < items; i0 += kAhead * kBlock) {
-    RawVec<kElements * sizeof(T)> raw[kAhead];
+    RawVec<N * sizeof(T)> raw[kAhead];
     bool active[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const Item it = item_of(i0 + u * kBlock, log_runs, log_tokens);
-      active[u] = it.head < heads && it.token < count && it.run * kElements < to.width && places.page[it.token] >= 0;
+      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
+      active[u] = it.head < heads && it.token < count && it.run * N < to.width && places.page[it.token] >= 0;
       const T* x = static_cast<const T*>(from.data);
       if (active[u])
-        raw[u] = load_elements(x + (first + it.token) * from.stride[0] + it.head * from.stride[1] +
-                                   run_start(it.run * kElements, to.width), to.width);
+        raw[u] = load_elements<N>(x + (first + it.token) * from.stride[0] + it.head * from.stride[1] +
+                                   run_start(it.run * N, N, to.width), to.width);
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const Item it = item_of(i0 + u * kBlock, log_runs, log_tokens);
+      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
       int64_t page = 0;
       int64_t slot = 0;
       if (active[u]) {
@@ -142,27 +163,27 @@ __device__ __forceinline__ void write_rows(const TokenRows& from, const PageTens
         slot = places.slot[it.token];
       }
       C* y = static_cast<C*>(to.data) + page * to.stride[0] + it.head * to.stride[1] + slot * to.stride[2] +
-             run_start(it.run * kElements, to.width);
+             run_start(it.run * N, N, to.width);
       if constexpr (__is_same(T, C)) {
-        if (active[u]) store_elements<false>(y, to.width, raw[u]);
+        if (active[u]) store_elements<false, N>(y, to.width, raw[u]);
       } else {
-        float x[kElements];
+        float x[N];
         float largest = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kElements; ++k) {
+        for (int k = 0; k < N; ++k) {
           x[k] = active[u] ? Elem<T>::get(raw[u].w, k) : 0.0f;
           largest = fmaxf(largest, finite(x[k]) ? fabsf(x[k]) : 0.0f);
         }
-        for (int o = 1; o < 1 << log_runs; o <<= 1) largest = fmaxf(largest, __shfl_xor(largest, o, 64));
+        for (int o = 1; o < row.runs; o <<= 1) largest = fmaxf(largest, __shfl_xor(largest, o, 64));
         const int e = row_exponent(largest);
         const float scale = power_of_two(-e);
-        RawVec<kElements> codes;
+        RawVec<N> codes;
 #pragma unroll
-        for (int k = 0; k < kElements / 4; ++k)
+        for (int k = 0; k < N / 4; ++k)
           codes.w[k] = e4m3_pair(x[4 * k] * scale, x[4 * k + 1] * scale) |
                        e4m3_pair(x[4 * k + 2] * scale, x[4 * k + 3] * scale) << 16;
         if (active[u]) {
-          store_elements<false>(y, to.width, codes);
+          store_elements<false, N>(y, to.width, codes);
           if (it.run == 0)
             to.exponents[page * to.exponent_stride[0] + it.head * to.exponent_stride[1] +
                          slot * to.exponent_stride[2]] = static_cast<int8_t>(e);
@@ -174,22 +195,23 @@ __device__ __forceinline__ void write_rows(const TokenRows& from, const PageTens
 
 template <typename C, typename T>
 __device__ __forceinline__ void read_rows(const PageTensor& from, const TokenRows& to, const Places& places,
-                                          int64_t first, int count, int heads, int log_runs, int log_tokens) {
-  const int items = heads << (log_runs + log_tokens);
+                                          int64_t first, int count, int heads, const RowItems& row, int log_tokens) {
+  constexpr int N = kElements<T>;
+  const int items = (heads << log_tokens) * row.runs;
   for (int i0 = threadIdx.x; i0 < items; i0 += kAhead * kBlock) {
-    RawVec<kElements * sizeof(C)> raw[kAhead];
+    RawVec<N * sizeof(C)> raw[kAhead];
     int e[kAhead];
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const Item it = item_of(i0 + u * kBlock, log_runs, log_tokens);
+      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
       e[u] = 0;
 #pragma unroll
       for (uint32_t& w : raw[u].w) w = 0u;  // zero in every type
-      if (it.head < heads && it.token < count && it.run * kElements < from.width && places.page[it.token] >= 0) {
+      if (it.head < heads && it.token < count && it.run * N < from.width && places.page[it.token] >= 0) {
         const int64_t page = places.page[it.token];
         const int64_t slot = places.slot[it.token];
-        raw[u] = load_elements(static_cast<const C*>(from.data) + page * from.stride[0] + it.head * from.stride[1] +
-                                   slot * from.stride[2] + run_start(it.run * kElements, from.width), from.width);
+        raw[u] = load_elements<N>(static_cast<const C*>(from.data) + page * from.stride[0] + it.head * from.stride[1] +
+                                   slot * from.stride[2] + run_start(it.run * N, N, from.width), from.width);
         if constexpr (!__is_same(T, C))
           e[u] = from.exponents[page * from.exponent_stride[0] + it.head * from.exponent_stride[1] +
                                 slot * from.exponent_stride[2]];
@@ -197,20 +219,20 @@ __device__ __forceinline__ void read_rows(const PageTensor& from, const TokenRow
     }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
-      const Item it = item_of(i0 + u * kBlock, log_runs, log_tokens);
-      if (it.head >= heads || it.token >= count || it.run * kElements >= from.width) continue;
+      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
+      if (it.head >= heads || it.token >= count || it.run * N >= from.width) continue;
       T* y = static_cast<T*>(to.data) + (first + it.token) * to.stride[0] + it.head * to.stride[1] +
-             run_start(it.run * kElements, from.width);
+             run_start(it.run * N, N, from.width);
       if constexpr (__is_same(T, C)) {
-        store_elements<true>(y, from.width, raw[u]);
+        store_elements<true, N>(y, from.width, raw[u]);
       } else {
-        T values[kElements];
+        T values[N];
 #pragma unroll
-        for (int k = 0; k < kElements; ++k)
+        for (int k = 0; k < N; ++k)
           values[k] = rounded<T>(ldexpf(e4m3_value(static_cast<uint8_t>(raw[u].w[k / 4] >> (8 * (k % 4)))), e[u]));
-        RawVec<kElements * sizeof(T)> r;
+        RawVec<N * sizeof(T)> r;
         __builtin_memcpy(&r, values, sizeof(r));
-        store_elements<true>(y, from.width, r);
+        store_elements<true, N>(y, from.width, r);
       }
     }
   }
@@ -218,8 +240,8 @@ __device__ __forceinline__ void read_rows(const PageTensor& from, const TokenRow
 
 struct RowShape {
   int log_tokens;
-  int log_key_runs;
-  int log_value_runs;
+  RowItems key;
+  RowItems value;
 };
 
 template <typename T, typename C>
@@ -232,8 +254,8 @@ __global__ __launch_bounds__(kBlock) void paged_write_kernel(PagedCache c, Token
   const int64_t left = tokens - first;
   const int count = left < (1 << shape.log_tokens) ? static_cast<int>(left) : 1 << shape.log_tokens;
   find_places(c, token_ptr, start, first, count, places);
-  write_rows<T, C>(key, c.key, places, first, count, c.heads, shape.log_key_runs, shape.log_tokens);
-  write_rows<T, C>(value, c.value, places, first, count, c.heads, shape.log_value_runs, shape.log_tokens);
+  write_rows<T, C>(key, c.key, places, first, count, c.heads, shape.key, shape.log_tokens);
+  write_rows<T, C>(value, c.value, places, first, count, c.heads, shape.value, shape.log_tokens);
 }
 
 template <typename C, typename T>
@@ -246,15 +268,15 @@ __global__ __launch_bounds__(kBlock) void paged_read_kernel(PagedCache c, TokenR
   const int64_t left = tokens - first;
   const int count = left < (1 << shape.log_tokens) ? static_cast<int>(left) : 1 << shape.log_tokens;
   find_places(c, token_ptr, start, first, count, places);
-  read_rows<C, T>(c.key, key, places, first, count, c.heads, shape.log_key_runs, shape.log_tokens);
-  read_rows<C, T>(c.value, value, places, first, count, c.heads, shape.log_value_runs, shape.log_tokens);
+  read_rows<C, T>(c.key, key, places, first, count, c.heads, shape.key, shape.log_tokens);
+  read_rows<C, T>(c.value, value, places, first, count, c.heads, shape.value, shape.log_tokens);
 }
 
 // Tokens of a workgroup: 16, fewer while that leaves fewer than 1,024 workgroups.
-RowShape row_shape(const PagedCache& c, int64_t tokens) {
+RowShape row_shape(const PagedCache& c, int64_t tokens, int elements, bool power_of_two) {
   RowShape s{};
-  while ((kElements << s.log_key_runs) < c.key.width) ++s.log_key_runs;
-  while ((kElements << s.log_value_runs) < c.value.width) ++s.log_value_runs;
+  s.key = row_items(c.key.width, elements, power_of_two);
+  s.value = row_items(c.value.width, elements, power_of_two);
   while ((2 << s.log_tokens) <= kMaxTokens && tokens >> (s.log_tokens + 1) >= 1024) ++s.log_tokens;
   return s;
 }
@@ -294,7 +316,8 @@ int as_paged_cache_write(const as_paged_cache* cache, const void* key, const int
   if (tokens == 0) return AS_OK;
   const TokenRows k{const_cast<void*>(key), {key_strides[0], key_strides[1]}};
   const TokenRows v{const_cast<void*>(value), {value_strides[0], value_strides[1]}};
-  const RowShape shape = row_shape(c, tokens);
+  const RowShape shape = row_shape(c, tokens, dtype == AS_DTYPE_F32 ? kElements<float> : kElements<Bf16>,
+                                   cache->dtype == AS_DTYPE_E4M3);
   const dim3 grid(static_cast<unsigned>(((tokens - 1) >> shape.log_tokens) + 1));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_float_element(dtype, [&](auto e) {
@@ -317,7 +340,7 @@ int as_paged_cache_read(const as_paged_cache* cache, void* key, void* value, con
   if (tokens == 0) return AS_OK;
   const TokenRows k{key, {int64_t(c.heads) * c.key.width, c.key.width}};
   const TokenRows v{value, {int64_t(c.heads) * c.value.width, c.value.width}};
-  const RowShape shape = row_shape(c, tokens);
+  const RowShape shape = row_shape(c, tokens, dtype == AS_DTYPE_F32 ? kElements<float> : kElements<Bf16>, false);
   const dim3 grid(static_cast<unsigned>(((tokens - 1) >> shape.log_tokens) + 1));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_float_element(dtype, [&](auto e) {
