@@ -25,7 +25,7 @@
 //            the same tokens).  Column n of instruction j is dimension n*8 + j of
 //            128, so a lane loads 8 neighbouring numbers of 8 tokens (a row of 128
 //            is one contiguous read of 16 lanes) and turns its 8 x 8 block with
-//            byte permutes: no shared memory, no shuffle.
+//            byte permutes: no shared memory, no shuffle.  (Rows of 64 and 192: 4 numbers.)
 //
 // With fewer than 16 heads a key head the other rows of the matrix units are
 // idle, which costs nothing while memory is the bound.  The maximum is the
@@ -312,7 +312,7 @@ struct WeightParts {
 // ---- one workgroup -----------------------------------------------------------------
 
 template <typename T, typename C, int W, int MODE>
-__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(W == 256 && MODE != kNarrow ? 2 : 1))) void
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(W > 128 && MODE != kNarrow ? 2 : 1))) void
 paged_attention_kernel(AttentionArgs a, PositionMap map) {
   constexpr bool kF32 = sizeof(C) == 4;
   constexpr bool kCoded = sizeof(C) == 1;
@@ -322,9 +322,9 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
   constexpr int kKeyRun = kF32 ? 4 : 8;   // dimensions of a key in one load
   constexpr int kKeyRuns = W / (4 * kKeyRun);
   constexpr int kValues = W / 16;         // dimensions of the values a lane holds
-  constexpr int kRun = kValues < 8 ? kValues : 8;  // of which neighbours
+  constexpr int kRun = kValues % 8 == 0 ? 8 : 4;  // of which neighbours
   constexpr int kBlocks = kValues / kRun;
-  // rows of 256 take too many registers to ask for keys and values at once
+  // rows beyond 128 take too many registers to ask for keys and values at once
   constexpr bool kLater = kBlocks > 1;
   constexpr int kQ = Parts<T, C>::value;
   constexpr int kP = WeightParts<T, C>::value;
@@ -382,7 +382,7 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
   const int own_token = g * kOwn;
   int value_at[kBlocks];
 #pragma unroll
-  for (int j = 0; j < kBlocks; ++j) value_at[j] = run_start(j * 128 + n * kRun, kRun, c.value.width);
+  for (int j = 0; j < kBlocks; ++j) value_at[j] = run_start((j * 16 + n) * kRun, kRun, c.value.width);
 
   int64_t at = share.at;
   for (int b = uniform_i32(share.b); b < c.sequences && at < share.end; ++b) {
@@ -408,7 +408,7 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
     // where the lane's runs of a key begin (lane (n, g): dimensions (j*4 + g) * kKeyRun ..), the queries there
     // as operand B
     int key_at[kKeyRuns];
-    // (in LDS with rows of 256: all waves hold the same)
+    // (in LDS with rows beyond 128: all waves hold the same)
     u32x4 q_own[kLater ? 1 : kKeyRuns][kQ];
     const auto q_of = [&](int j, int p) { return kLater ? q_shared[j][p][lane] : q_own[kLater ? 0 : j][p]; };
     {
@@ -976,10 +976,15 @@ template <typename T, typename C>
 int launch_attention(const AttentionArgs& a, const PositionMap& map, hipStream_t s) {
   const int width = a.cache.key.width > a.cache.value.width ? a.cache.key.width : a.cache.value.width;
   const dim3 grid(static_cast<unsigned>((a.shares > 0 ? a.shares : a.cache.sequences) * a.cache.heads * a.head_tiles));
+  // the narrowest rows that hold both widths: what a row does not fill is loaded and
+  // multiplied all the same (width 160 in float32, 20 sequences to 4,000: 69 us in
+  // rows of 192, 82 in rows of 256; width 144 in 8 bits 31 and 36)
   if (width <= 64) {
     launch_width<T, C, 64>(a, map, grid, s);
   } else if (width <= 128) {
     launch_width<T, C, 128>(a, map, grid, s);
+  } else if (width <= 192) {
+    launch_width<T, C, 192>(a, map, grid, s);
   } else {
     launch_width<T, C, 256>(a, map, grid, s);
   }
