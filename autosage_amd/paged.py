@@ -327,6 +327,7 @@ def paged_cache_read_impl(key_pages, value_pages, page_ptr, page_idx, token_ptr,
         dtype = torch.bfloat16 if coded else key_pages.dtype
     _require(dtype in _DTYPES and dtype != E4M3 and (coded or dtype == key_pages.dtype), TypeError,
              "dtype must be the dtype of the pages (float32, bfloat16 or float16 for float8_e4m3fn pages)")
+    _no_gradient("paged_cache_read", key_pages, value_pages)
     page_ptr, page_idx, token_ptr, start = _long(page_ptr), _long(page_idx), _long(token_ptr), _long(start)
     _validate_call(key_pages, page_ptr, page_idx, token_ptr, start, tokens, False)
     heads, device = key_pages.size(1), key_pages.device

@@ -368,6 +368,43 @@ def test_tokens_without_a_place():
     assert torch.equal(k.nan_to_num(7.0), before.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("quantised", [False, True])
+def test_the_registered_operators(quantised):
+    ops = torch.ops.autosage
+    cache = Cache([9, 30], 2, 24, 16, 8, torch.float16, quantised=quantised, seed=24, room=1)
+    (k, v, ptr, idx), e = cache.args()
+    e = tuple(e.values())
+    rows = [torch.randn(4, 2, w, device="cuda", dtype=torch.float16) for w in (24, 16)]
+    span = (torch.tensor([0, 1, 4]).cuda(), torch.tensor([9, 30]).cuda())
+    query, lengths = torch.randn(2, 4, 24, device="cuda", dtype=torch.float16), torch.tensor([10, 33]).cuda()
+    table = torch.randn(8, 4, device="cuda", dtype=torch.float16)
+    names = dict(zip(("key_exponents", "value_exponents"), e))
+    assert ops.paged_cache_write(*rows, k, v, ptr, idx, *span, *e) is None
+    for a, b in zip(ops.paged_cache_read(k, v, ptr, idx, *span, 4, torch.float16, *e),
+                    autosage_amd.paged_cache_read(k, v, ptr, idx, *span, 4, dtype=torch.float16, **names)):
+        assert torch.equal(a, b) and a.any()
+    out, lse = ops.paged_attention(query, k, v, ptr, idx, lengths, 0.2, 20, table, 15, False, 40, *e, True)
+    want = autosage_amd.paged_attention(query, k, v, ptr, idx, lengths, scale=0.2, window=20, bias_table=table,
+                                        max_distance=15, bidirectional=False, max_length=40, return_lse=True, **names)
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    out, lse = ops.paged_attention(query, k, v, ptr, idx, lengths, **names)
+    assert torch.equal(out, autosage_amd.paged_attention(query, k, v, ptr, idx, lengths, **names)) and lse.numel() == 0
+
+
+def test_32_bit_lists_and_validation(monkeypatch):
+    cache = Cache([9, 30], 2, 24, 16, 8, torch.float16, seed=25)
+    (k, v, ptr, idx), _ = cache.args()
+    query, lengths = torch.randn(2, 4, 24, device="cuda", dtype=torch.float16), torch.tensor([9, 30]).cuda()
+    want = autosage_amd.paged_attention(query, k, v, ptr, idx, lengths)
+    assert torch.equal(autosage_amd.paged_attention(query, k, v, ptr.int(), idx.int(), lengths.int()), want)
+    monkeypatch.setenv("AUTOSAGE_VALIDATE", "1")
+    assert torch.equal(autosage_amd.paged_attention(query, k, v, ptr, idx, lengths), want)
+    with pytest.raises(ValueError, match="page ids"):
+        autosage_amd.paged_attention(query, k, v, ptr, idx + k.size(0), lengths)
+    with pytest.raises(ValueError, match="more tokens"):
+        autosage_amd.paged_attention(query, k, v, ptr, idx, lengths + 30)
+
+
 # ---- together ---------------------------------------------------------------------
 
 

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import autosage_amd
+from autosage_amd.position import position_buckets
 from tests.gpu_common import case_graph, require_gpu, to_dev
 from tests.paged_common import plain_buckets
 
@@ -161,6 +162,27 @@ def test_the_same_bits_every_time():
     one = _check(crow, col, 4, 32, 1000, torch.float32)
     for _ in range(3):
         assert torch.equal(_check(crow, col, 4, 32, 1000, torch.float32), one)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^32 biases: rows of 512 neighbours each, nine heads in 16 bits; the gradient of ones counts edges."""
+    n, degree, heads = (1 << 20) + 3, 512, 9
+    crow = torch.arange(n + 1, device="cuda") * degree
+    step = torch.arange(degree, device="cuda") * 3 - 700
+    col = ((torch.arange(n, device="cuda")[:, None] + step) % n).view(-1)
+    table = torch.randn(32, heads, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    out = autosage_amd.csr_position_bias(crow, col, table, max_distance=600)
+    assert out.numel() > 2**32
+    count = torch.zeros(32, dtype=torch.long)
+    for a in range(0, n, 1 << 18):
+        b = min(a + (1 << 18), n)
+        rel = col.view(n, degree)[a:b] - torch.arange(a, b, device="cuda")[:, None]
+        bucket = position_buckets(rel.flatten(), 32, 600, True)
+        count += torch.bincount(bucket, minlength=32).cpu()
+        for h in (0, heads - 1):
+            assert torch.equal(out[h, a * degree:b * degree], table.detach()[bucket, h])
+    grad, = torch.autograd.grad(out, table, torch.ones_like(out))
+    assert torch.equal(grad.cpu(), count.double().bfloat16()[:, None].expand(32, heads))
 
 
 def test_empty_graph_and_refusals():

@@ -186,6 +186,7 @@ def test_refusals():
         (ValueError, lambda: write(key, value, k[:1].expand(4, 2, 4, 4), v[:4], ptr, idx, *span)),
         (RuntimeError, lambda: write(key.clone().requires_grad_(), value, k, v, ptr, idx, *span)),
         (ValueError, lambda: read(k, v, ptr, idx, *span, -1)),
+        (RuntimeError, lambda: read(k.clone().requires_grad_(), v, ptr, idx, *span, 2)),
         (TypeError, lambda: read(k, v, ptr, idx, *span, 2, dtype=torch.float16)),
         (TypeError, lambda: read(ck, cv, ptr, idx, *span, 2, dtype=torch.float64, **e)),
     ]:
