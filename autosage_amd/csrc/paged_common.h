@@ -77,11 +77,6 @@ __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
 }
 __device__ __forceinline__ float e4m3_value(uint8_t code) { return __builtin_amdgcn_cvt_f32_fp8(code, 0); }
 
-template <>
-struct Elem<E4m3> {
-  __device__ static float at(const E4m3* p, int64_t i) { return e4m3_value(p[i].bits); }
-};
-
 template <typename T>
 __device__ __forceinline__ T rounded(float v);
 template <>

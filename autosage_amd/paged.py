@@ -194,8 +194,7 @@ def _validate_lists(key_pages, page_ptr, page_idx, last) -> None:
 
 
 def _places(page_ptr, page_idx, token_ptr, start, tokens: int, page_size: int):
-    """(sequence tokens are of, their pages, their places there) of the tokens
-    that have one; the first result is their index among the call's tokens."""
+    """(which of the call's tokens have a place, their pages, their places there)."""
     at = torch.arange(tokens, device=start.device)
     counts = token_ptr[1:] - token_ptr[:-1]
     sequence = torch.repeat_interleave(torch.arange(counts.numel(), device=start.device), counts)[:tokens]
