@@ -43,13 +43,17 @@ __device__ __forceinline__ void find_places(const PagedCache& c, const int64_t* 
     const int b = block_edge_rows(token_ptr, c.sequences, first, count, row);
     const int64_t t = first + lane_id();
     if (lane_id() < count) {
-      const int64_t at = t - token_ptr[b];
+      const int64_t own = token_ptr[b];
       const int64_t begin = start[b];
-      const int64_t position = begin + at;
       const PageList list = page_list(c, b);
-      // no token of the sequence, or a position in front of it or beyond its pages
-      const bool none = at < 0 || t >= token_ptr[b + 1] || begin < -at || begin > INT64_MAX / 2 ||
-                        position >= list.count * c.page_size;
+      // A token of the sequence, and a position in front of the sequence or beyond its pages.  `at` stays
+      // below 2^62 + 2^26 and begin below what the pages hold, so that no sum wraps whatever the lists hold.
+      const bool mine = own >= -(int64_t(1) << 62) && own <= t && t < token_ptr[b + 1];
+      const int64_t at = mine ? t - own : 0;
+      const int64_t room = list.count * c.page_size;
+      const bool outside = begin < -at || begin >= room;
+      const int64_t position = mine && !outside ? begin + at : 0;
+      const bool none = !mine || outside || position >= room;
       int64_t page = -1;
       int64_t k = 0;
       if (!none) {

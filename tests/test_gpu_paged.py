@@ -525,3 +525,21 @@ def test_offsets_beyond_32_bits(quantised):
     s = (key.double() * query[0].double()).sum(-1) * width**-0.5
     want = (torch.softmax(s, 0)[..., None] * value.double()).sum(0)
     assert torch.allclose(got[0].double(), want, rtol=2.0**-8, atol=1e-4)
+
+
+def test_token_lists_that_begin_anywhere():
+    """Where a position passes 64 bits there is no place, and the other sequence's tokens keep theirs."""
+    cache = Cache([4, 9], 1, 8, 8, 4, torch.float32, seed=19)
+    rows = torch.randn(6, 1, 8, device="cuda")
+    for own, begin in [(-(2**62) - 10, 2**62 - 1), (-(2**63), 2**62 - 1), (-(2**63), 0), (-(2**62), 2**62),
+                       (-(2**62), 2**63 - 1), (-(2**63), -(2**63)), (-5, -(2**63))]:
+        (k, v, ptr, idx), _ = cache.args()
+        before = k.clone()
+        token_ptr, start = torch.tensor([own, 3, 6]).cuda(), torch.tensor([begin, 5]).cuda()
+        autosage_amd.paged_cache_write(rows, rows, k, v, ptr, idx, token_ptr, start)
+        key, value = autosage_amd.paged_cache_read(k, v, ptr, idx, token_ptr, start, 6)
+        for back in (key, value):
+            assert not back[:3].any() and torch.equal(back[3:], rows[3:])
+        for t in range(5, 8):
+            before[idx[ptr[1] + t // 4], 0, t % 4] = rows[t - 2, 0]
+        assert torch.equal(k.nan_to_num(7.0), before.nan_to_num(7.0))
