@@ -282,6 +282,9 @@ def paged_cache_write_impl(key, value, key_pages, value_pages, page_ptr, page_id
         return
     lib = _need_native()
     key, value = _rows(key), _rows(value)
+    # the kernel writes behind torch's back: a graph that saved the pages has to see that they changed
+    torch.autograd.graph.increment_version([t for t in (key_pages, value_pages, key_exponents, value_exponents)
+                                            if t is not None])
     cache = _cache_struct(key_pages, value_pages, page_ptr, page_idx, key_exponents, value_exponents)
     with _native._on(key.device):
         status = lib.as_paged_cache_write(

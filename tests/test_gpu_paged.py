@@ -543,3 +543,26 @@ def test_token_lists_that_begin_anywhere():
         for t in range(5, 8):
             before[idx[ptr[1] + t // 4], 0, t % 4] = rows[t - 2, 0]
         assert torch.equal(k.nan_to_num(7.0), before.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("registered", [False, True])
+@pytest.mark.parametrize("quantised", [False, True])
+def test_a_write_is_seen_by_autograd(quantised, registered):
+    """What a graph saved of the pages is no longer what it was: backward refuses, as after any write in place."""
+    cache = Cache([4, 9], 1, 8, 8, 4, torch.float32, quantised=quantised, seed=26)
+    (k, v, ptr, idx), e = cache.args()
+    rows = torch.randn(2, 1, 8, device="cuda")
+    span = (torch.tensor([0, 1, 2]).cuda(), torch.tensor([3, 8]).cuda())
+    written = [k, v, *(t for t in e.values() if t is not None)]
+    before = [t._version for t in written]
+    if registered:
+        torch.ops.autosage.paged_cache_write(rows, rows, k, v, ptr, idx, *span, *e.values())
+    else:
+        autosage_amd.paged_cache_write(rows, rows, k, v, ptr, idx, *span, **e)
+    assert all(t._version > old for t, old in zip(written, before))
+    if not quantised:
+        query = torch.ones(8, device="cuda", requires_grad=True)
+        scores = k[0, 0] * query
+        autosage_amd.paged_cache_write(rows, rows, k, v, ptr, idx, *span)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            scores.sum().backward()
