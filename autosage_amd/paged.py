@@ -193,7 +193,7 @@ def _validate_lists(key_pages, page_ptr, page_idx, last) -> None:
              "invalid page lists: a sequence has more tokens than its pages hold")
 
 
-def _places(page_ptr, page_idx, token_ptr, start, tokens: int, page_size: int):
+def _places(page_ptr, page_idx, token_ptr, start, tokens: int, pages: int, page_size: int):
     """(which of the call's tokens have a place, their pages, their places there)."""
     at = torch.arange(tokens, device=start.device)
     counts = token_ptr[1:] - token_ptr[:-1]
@@ -204,7 +204,9 @@ def _places(page_ptr, page_idx, token_ptr, start, tokens: int, page_size: int):
     room = (page_ptr[1:] - page_ptr[:-1])[sequence]
     has_page = (position >= 0) & (entry < room)
     at, position, entry, sequence = at[has_page], position[has_page], entry[has_page], sequence[has_page]
-    return at, page_idx[page_ptr[sequence] + entry], position % page_size
+    page = page_idx[page_ptr[sequence] + entry]
+    inside = (page >= 0) & (page < pages)
+    return at[inside], page[inside], position[inside] % page_size
 
 
 def _validate_call(key_pages, page_ptr, page_idx, token_ptr, start, tokens: int, writes: bool) -> None:
@@ -216,8 +218,8 @@ def _validate_call(key_pages, page_ptr, page_idx, token_ptr, start, tokens: int,
              "invalid tokens: token_ptr must start at 0, not descend and end inside the tokens, start not be negative")
     _validate_lists(key_pages, page_ptr, page_idx, torch.where(counts > 0, start + counts, 0))
     if writes:
-        page_size = key_pages.size(2)
-        _, page, place = _places(page_ptr, page_idx, token_ptr, start, tokens, page_size)
+        pages, page_size = key_pages.size(0), key_pages.size(2)
+        _, page, place = _places(page_ptr, page_idx, token_ptr, start, tokens, pages, page_size)
         _require(torch.unique(page * page_size + place).numel() == page.numel(), ValueError,
                  "invalid page lists: two tokens of one call have the same place")
 
@@ -271,7 +273,8 @@ def paged_cache_write_impl(key, value, key_pages, value_pages, page_ptr, page_id
     if tokens == 0 or page_ptr.numel() == 1:
         return
     if not key.is_cuda:
-        at, page, place = _places(page_ptr, page_idx, token_ptr, start, tokens, key_pages.size(2))
+        at, page, place = _places(page_ptr, page_idx, token_ptr, start, tokens, key_pages.size(0),
+                                  key_pages.size(2))
         for rows, pages, exponents in ((key, key_pages, key_exponents), (value, value_pages, value_exponents)):
             if exponents is None:
                 pages[page, :, place] = rows[at]
@@ -337,7 +340,8 @@ def paged_cache_read_impl(key_pages, value_pages, page_ptr, page_idx, token_ptr,
     if tokens == 0 or page_ptr.numel() == 1 or not key_pages.is_cuda:
         out = [torch.zeros(shape, dtype=dtype, device=device) for shape in shapes]
         if tokens > 0 and page_ptr.numel() > 1:
-            at, page, place = _places(page_ptr, page_idx, token_ptr, start, tokens, key_pages.size(2))
+            at, page, place = _places(page_ptr, page_idx, token_ptr, start, tokens, key_pages.size(0),
+                                      key_pages.size(2))
             for rows, pages, exponents in zip(out, (key_pages, value_pages), (key_exponents, value_exponents)):
                 if coded:
                     codes = pages.view(torch.uint8)[page, :, place].view(E4M3)

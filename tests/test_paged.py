@@ -281,3 +281,23 @@ def test_native_argument_checks_come_before_any_launch():
     ]:
         assert call() == status, message
         assert lib.as_last_error().startswith(message), lib.as_last_error()
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("bad", [-1, 10**6, 2**40, -(2**40)])
+def test_tokens_whose_page_is_outside_the_cache(quantised, bad):
+    """They are not written and read as zeros; the others are."""
+    cache = Cache([4, 9], 1, 8, 8, 4, torch.float32, quantised=quantised, seed=10)
+    (k, v, ptr, idx), e = cache.args("cpu")
+    idx = idx.clone()
+    idx[2] = bad  # tokens 4 to 7 of the second sequence
+    rows = torch.randn(9, 1, 8)
+    before = k.view(torch.uint8).clone()
+    span = (torch.tensor([0, 0, 9]), torch.tensor([0, 0]))
+    autosage_amd.paged_cache_write(rows, rows, k, v, ptr, idx, *span, **e)
+    key, value = autosage_amd.paged_cache_read(k, v, ptr, idx, *span, 9, dtype=torch.float32, **e)
+    want = quantised_rows(rows)[0].float() if quantised else rows
+    for back in (key, value):
+        assert not back[4:8].any() and torch.equal(back[:4], want[:4]) and torch.equal(back[8], want[8])
+    others = [p for p in range(k.size(0)) if p not in (idx[1], idx[3])]
+    assert torch.equal(k.view(torch.uint8)[others], before[others])
