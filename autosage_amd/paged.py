@@ -193,6 +193,13 @@ def _validate_lists(key_pages, page_ptr, page_idx, last) -> None:
              "invalid page lists: a sequence has more tokens than its pages hold")
 
 
+def _page_lists(page_ptr, page_idx):
+    """(begin, number of entries) of every sequence's list, inside ``page_idx`` whatever ``page_ptr`` holds: as the
+    kernels do."""
+    begin = page_ptr[:-1].clamp(0, page_idx.numel())
+    return begin, torch.maximum(page_ptr[1:].clamp_max(page_idx.numel()), begin) - begin
+
+
 def _places(page_ptr, page_idx, token_ptr, start, tokens: int, pages: int, page_size: int):
     """(which of the call's tokens have a place, their pages, their places there)."""
     at = torch.arange(tokens, device=start.device)
@@ -201,10 +208,10 @@ def _places(page_ptr, page_idx, token_ptr, start, tokens: int, pages: int, page_
     at = at[: sequence.numel()]
     position = start[sequence] + at - token_ptr[sequence]
     entry = position // page_size
-    room = (page_ptr[1:] - page_ptr[:-1])[sequence]
-    has_page = (position >= 0) & (entry < room)
+    begin, room = _page_lists(page_ptr, page_idx)
+    has_page = (position >= 0) & (entry < room[sequence])
     at, position, entry, sequence = at[has_page], position[has_page], entry[has_page], sequence[has_page]
-    page = page_idx[page_ptr[sequence] + entry]
+    page = page_idx[begin[sequence] + entry]
     inside = (page >= 0) & (page < pages)
     return at[inside], page[inside], position[inside] % page_size
 
@@ -418,10 +425,11 @@ def _cpu_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, s
     group = heads_q // heads
     out = torch.zeros(sequences, heads_q, value_pages.size(3), dtype=torch.float32)
     lse = torch.full((sequences, heads_q), float("-inf"))
+    begins, rooms = _page_lists(page_ptr, page_idx)
     for b in range(sequences):
         length = max(0, int(lengths[b]))
         first = max(0, length - window) if window else 0
-        mine = page_idx[int(page_ptr[b]):int(page_ptr[b + 1])]
+        mine = page_idx[int(begins[b]):int(begins[b] + rooms[b])]
         short = length > mine.numel() * page_size or (max_length is not None and length > max_length)
         skipped = first // page_size
         mine = mine[skipped: -(-length // page_size)]

@@ -301,3 +301,20 @@ def test_tokens_whose_page_is_outside_the_cache(quantised, bad):
         assert not back[4:8].any() and torch.equal(back[:4], want[:4]) and torch.equal(back[8], want[8])
     others = [p for p in range(k.size(0)) if p not in (idx[1], idx[3])]
     assert torch.equal(k.view(torch.uint8)[others], before[others])
+
+
+def test_lists_outside_the_page_ids():
+    """What a list names outside ``page_idx`` is no page: nothing written, zeros, NaN; a list inside is as it was."""
+    cache = Cache([4, 9], 1, 8, 8, 4, torch.float32, seed=11)
+    (k, v, ptr, idx), _ = cache.args("cpu")
+    query, rows = torch.randn(2, 1, 8), torch.randn(8, 1, 8)
+    lengths, span = torch.tensor([4, 9]), (torch.tensor([0, 4, 8]), torch.tensor([0, 0]))
+    good = autosage_amd.paged_attention(query, k, v, ptr, idx, lengths)
+    before = k.clone()
+    for lists in (ptr + 10**6, ptr - 5, ptr - 10**6, ptr.flip(0), torch.tensor([-4, -3, -1])):
+        assert autosage_amd.paged_attention(query, k, v, lists, idx, lengths).isnan().all()
+        autosage_amd.paged_cache_write(rows, rows, k, v, lists, idx, *span)
+        assert not autosage_amd.paged_cache_read(k, v, lists, idx, *span, 8)[0].any()
+    assert torch.equal(k.nan_to_num(7.0), before.nan_to_num(7.0))
+    one = torch.tensor([-1, 1, 10**6])  # cut to [0, 1) and [1, 4)
+    assert torch.equal(autosage_amd.paged_attention(query, k, v, one, idx, lengths), good)
