@@ -203,10 +203,13 @@ def _page_lists(page_ptr, page_idx):
 def _places(page_ptr, page_idx, token_ptr, start, tokens: int, pages: int, page_size: int):
     """(which of the call's tokens have a place, their pages, their places there)."""
     at = torch.arange(tokens, device=start.device)
-    counts = token_ptr[1:] - token_ptr[:-1]
-    sequence = torch.repeat_interleave(torch.arange(counts.numel(), device=start.device), counts)[:tokens]
-    at = at[: sequence.numel()]
-    position = start[sequence] + at - token_ptr[sequence]
+    sequence = torch.searchsorted(token_ptr, at, right=True) - 1
+    known = (sequence >= 0) & (sequence < start.numel())
+    at, sequence = at[known], sequence[known]
+    # bounds beyond which a sum would pass 64 bits; no sequence has pages there
+    mine = (at < token_ptr[sequence + 1]) & (token_ptr[sequence] >= -(2**62)) & (start[sequence] < 2**62)
+    at, sequence = at[mine], sequence[mine]
+    position = start[sequence] + (at - token_ptr[sequence])
     entry = position // page_size
     begin, room = _page_lists(page_ptr, page_idx)
     has_page = (position >= 0) & (entry < room[sequence])

@@ -318,3 +318,36 @@ def test_lists_outside_the_page_ids():
     assert torch.equal(k.nan_to_num(7.0), before.nan_to_num(7.0))
     one = torch.tensor([-1, 1, 10**6])  # cut to [0, 1) and [1, 4)
     assert torch.equal(autosage_amd.paged_attention(query, k, v, one, idx, lengths), good)
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_rows_in_front_of_the_first_token(quantised):
+    """``token_ptr`` need not begin at 0: rows in front of it are padding, as those behind its end are."""
+    cache = Cache([4, 9], 1, 8, 8, 4, torch.float32, quantised=quantised, seed=12)
+    (k, v, ptr, idx), e = cache.args("cpu")
+    rows = torch.randn(9, 1, 8)
+    span = (torch.tensor([2, 3, 7]), torch.tensor([3, 4]))
+    autosage_amd.paged_cache_write(rows, rows, k, v, ptr, idx, *span, **e)
+    key, value = autosage_amd.paged_cache_read(k, v, ptr, idx, *span, 9, dtype=torch.float32, **e)
+    want = quantised_rows(rows)[0].float() if quantised else rows
+    for back in (key, value):
+        assert torch.equal(back[2:7], want[2:7]) and not back[:2].any() and not back[7:].any()
+    # the tokens in front of those
+    old = autosage_amd.paged_cache_read(k, v, ptr, idx, torch.tensor([0, 3, 7]), torch.tensor([0, 0]), 7,
+                                        dtype=torch.float32, **e)[0].double()
+    assert torch.equal(old, torch.cat([cache.rows["key"][0][:3], cache.rows["key"][1][:4]]).float().double())
+
+
+def test_token_lists_that_begin_anywhere():
+    """Where a position passes 64 bits there is no place, and the other sequence's tokens keep theirs."""
+    cache = Cache([4, 9], 1, 8, 8, 4, torch.float32, seed=19)
+    rows = torch.randn(6, 1, 8)
+    for own, begin in [(-(2**62) - 10, 2**62 - 1), (-(2**63), 2**62 - 1), (-(2**63), 0), (-(2**62), 2**62),
+                       (-(2**62), 2**63 - 1), (-(2**63), -(2**63)), (-5, -(2**63))]:
+        (k, v, ptr, idx), _ = cache.args("cpu")
+        k, v = k.clone(), v.clone()
+        token_ptr, start = torch.tensor([own, 3, 6]), torch.tensor([begin, 5])
+        autosage_amd.paged_cache_write(rows, rows, k, v, ptr, idx, token_ptr, start)
+        key, value = autosage_amd.paged_cache_read(k, v, ptr, idx, token_ptr, start, 6)
+        for back in (key, value):
+            assert not back[:3].any() and torch.equal(back[3:], rows[3:])
