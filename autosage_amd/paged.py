@@ -178,15 +178,18 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.size(-1) == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _validate_lists(key_pages, page_ptr, page_idx, last) -> None:
-    """``AUTOSAGE_VALIDATE=1``: every list is inside ``page_idx``, holds ids of
-    pages and enough of them for ``last`` tokens (one pass, one host sync)."""
+def _validate_lists(key_pages, page_ptr, page_idx, first, last) -> None:
+    """``AUTOSAGE_VALIDATE=1``: every list is inside ``page_idx``, and holds ids of pages where tokens ``first`` to
+    ``last - 1`` are (what else a list has room for may be anything)."""
     pages, page_size = key_pages.size(0), key_pages.size(2)
     counts = page_ptr[1:] - page_ptr[:-1]
-    bad = (page_ptr[:1] != 0).any() | (counts < 0).any() | (page_ptr[-1] > page_idx.numel())
+    bad = (page_ptr[0] < 0) | (counts < 0).any() | (page_ptr[-1] > page_idx.numel())
     _require(not bool(bad), ValueError,
-             "invalid page lists: page_ptr must start at 0, not descend and end inside page_idx")
-    used = page_idx[: int(page_ptr[-1])]
+             "invalid page lists: page_ptr must not be negative, not descend and end inside page_idx")
+    entry = torch.arange(int(page_ptr[0]), int(page_ptr[-1]), device=page_ptr.device)
+    sequence = torch.searchsorted(page_ptr, entry, right=True) - 1
+    at = (entry - page_ptr[sequence]) * page_size
+    used = page_idx[entry[(at + page_size > first[sequence]) & (at < last[sequence])]]
     _require(not bool(((used < 0) | (used >= pages)).any()), ValueError,
              "invalid page lists: page ids must lie in [0, pages)")
     _require(not bool((last > counts * page_size).any()), ValueError,
@@ -223,10 +226,11 @@ def _validate_call(key_pages, page_ptr, page_idx, token_ptr, start, tokens: int,
     if _env.get("AUTOSAGE_VALIDATE") != "1":
         return
     counts = token_ptr[1:] - token_ptr[:-1]
-    bad = (token_ptr[:1] != 0).any() | (counts < 0).any() | (token_ptr[-1] > tokens) | (start < 0).any()
+    bad = (token_ptr[0] < 0) | (counts < 0).any() | (token_ptr[-1] > tokens) | (start < 0).any()
     _require(not bool(bad), ValueError,
-             "invalid tokens: token_ptr must start at 0, not descend and end inside the tokens, start not be negative")
-    _validate_lists(key_pages, page_ptr, page_idx, torch.where(counts > 0, start + counts, 0))
+             "invalid tokens: token_ptr must not be negative, not descend and end inside the tokens, start not be "
+             "negative")
+    _validate_lists(key_pages, page_ptr, page_idx, start, torch.where(counts > 0, start + counts, 0))
     if writes:
         pages, page_size = key_pages.size(0), key_pages.size(2)
         _, page, place = _places(page_ptr, page_idx, token_ptr, start, tokens, pages, page_size)
@@ -473,7 +477,8 @@ def _attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, scale
     _no_gradient("paged_attention", query, key_pages, value_pages, bias_table)
     page_ptr, page_idx, lengths = _long(page_ptr), _long(page_idx), _long(lengths)
     if _env.get("AUTOSAGE_VALIDATE") == "1":
-        _validate_lists(key_pages, page_ptr, page_idx, lengths)
+        first = torch.zeros_like(lengths) if window is None else (lengths - int(window)).clamp_min(0)
+        _validate_lists(key_pages, page_ptr, page_idx, first, lengths)
         _require(not bool((lengths < 0).any()), ValueError, "invalid lengths: they must not be negative")
         _require(max_length is None or not bool((lengths > int(max_length)).any()), ValueError,
                  "invalid lengths: one is beyond max_length")

@@ -351,3 +351,37 @@ def test_token_lists_that_begin_anywhere():
         key, value = autosage_amd.paged_cache_read(k, v, ptr, idx, token_ptr, start, 6)
         for back in (key, value):
             assert not back[:3].any() and torch.equal(back[3:], rows[3:])
+
+
+def test_validation_of_lists_with_room(monkeypatch):
+    """Only the entries that a call reaches have to be pages: a table padded with -1, windows that are past the first
+    pages (given back, or never kept), some of a batch's sequences and rows."""
+    monkeypatch.setenv("AUTOSAGE_VALIDATE", "1")
+    cache = Cache([9, 22], 1, 8, 8, 4, torch.float32, seed=13)
+    (k, v, ptr, idx), _ = cache.args("cpu")
+    query, rows, lengths = torch.randn(2, 1, 8), torch.randn(6, 1, 8), torch.tensor([9, 22])
+    table = torch.full((2, 8), -1)
+    table[0, :3], table[1, :6] = idx[:3], idx[3:]
+    wide = torch.arange(3) * 8
+    attention, write, read = autosage_amd.paged_attention, autosage_amd.paged_cache_write, autosage_amd.paged_cache_read
+    want = attention(query, k, v, ptr, idx, lengths)
+    assert torch.equal(attention(query, k, v, wide, table.flatten(), lengths), want)
+    assert torch.equal(attention(query[1:], k, v, wide[1:], table.flatten(), lengths[1:]), want[1:])
+    write(rows, rows, k, v, wide, table.flatten(), torch.tensor([1, 3, 5]), lengths)
+    back, _ = read(k, v, wide, table.flatten(), torch.tensor([1, 3, 5]), lengths, 6)
+    assert torch.equal(back[1:5], rows[1:5])
+    want = attention(query, k, v, ptr, idx, lengths, window=5)
+    table[0, 0], table[1, :4] = 10**9, -1  # in front of tokens 4 and 17
+    assert torch.equal(attention(query, k, v, wide, table.flatten(), lengths, window=5), want)
+    for bad in (lambda: attention(query, k, v, wide, table.flatten(), lengths, window=6),
+                lambda: attention(query, k, v, wide, table.flatten(), lengths + 4),
+                lambda: read(k, v, wide, table.flatten(), torch.tensor([0, 1, 2]), torch.tensor([3, 17]), 2),
+                lambda: write(rows, rows, k, v, wide, table.flatten(), torch.tensor([0, 2, 4]), torch.tensor([11, 17]))):
+        with pytest.raises(ValueError, match="page ids"):
+            bad()
+    with pytest.raises(ValueError, match="page_ptr"):
+        attention(query, k, v, wide - 1, table.flatten(), lengths)
+    with pytest.raises(ValueError, match="token_ptr"):
+        read(k, v, wide, table.flatten(), torch.tensor([-1, 1, 2]), torch.tensor([4, 17]), 2)
+    with pytest.raises(ValueError, match="more tokens"):
+        attention(query, k, v, wide, table.flatten(), torch.tensor([9, 33]), window=1)
