@@ -122,11 +122,11 @@ def _normalize_csr(crow, col, val, x):
     return crow, col, val, x
 
 
-def validate_if_requested(crow, col) -> None:
+def validate_if_requested(crow, col, n_cols: Optional[int] = None) -> None:
     """Runs ``validate_csr`` on CUDA graphs when ``AUTOSAGE_VALIDATE=1``,
     before any baseline or native gather touches them."""
     if _env.get("AUTOSAGE_VALIDATE") == "1" and crow.is_cuda:
-        validate_csr(crow, col)
+        validate_csr(crow, col, n_cols)
 
 
 def _cpu_spmm(crow, col, val, x) -> torch.Tensor:

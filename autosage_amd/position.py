@@ -25,6 +25,8 @@ from . import _native
 from .ops import load_native, native_load_error, validate_if_requested
 
 MAX_BUCKETS = 256
+# node ids that are positions may be any: rows of a part of a graph see columns of all of it
+_MAX_NODES = 2**62
 _DTYPES = {torch.float32: 0, **_native.DTYPES_16}
 
 
@@ -240,8 +242,8 @@ def csr_position_bias(crow, col, table, *, max_distance: int, bidirectional: boo
     ``table`` is ``[buckets, heads]``, float32, bfloat16 or float16; the result
     is ``[heads, edges]`` of its dtype, one row for each head's scores, with a
     gradient for ``table`` (the sum over each bucket's edges, in a fixed order).
-    Node ids are positions unless ``positions`` (one integer per node) gives
-    them.  With ``bidirectional`` half of the buckets are for keys behind the
+    Node ids are positions (and columns may then lie beyond the rows) unless
+    ``positions`` (one integer per node) gives them.  With ``bidirectional`` half of the buckets are for keys behind the
     query; without it a key behind the query counts as distance 0."""
     _check(crow, col, positions, table)
     max_distance = int(max_distance)
@@ -251,7 +253,7 @@ def csr_position_bias(crow, col, table, *, max_distance: int, bidirectional: boo
     if not load_native():
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable: {native_load_error()}")
     crow, col, positions = _long(crow), _long(col), _long(positions)
-    validate_if_requested(crow, col)
+    validate_if_requested(crow, col, _MAX_NODES if positions is None else None)
     if torch.is_grad_enabled() and table.requires_grad:
         return _PositionBias.apply(table, crow, col, positions, max_distance, bool(bidirectional))
     return csr_position_bias_impl(crow, col, positions, table, max_distance, bool(bidirectional), keep=False)[0]

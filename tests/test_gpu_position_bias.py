@@ -238,3 +238,19 @@ def test_another_stream():
         got = autosage_amd.csr_position_bias(d_crow, d_col, table, max_distance=128)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_columns_beyond_the_rows(monkeypatch):
+    """Without positions a graph need not be square, also where it is validated; with them it has to be."""
+    crow, col = torch.tensor([0, 2, 3]), torch.tensor([0, 9, 2**40])
+    table = torch.randn(8, 2)
+    want = autosage_amd.csr_position_bias(crow, col, table, max_distance=20)
+    for validate in ("0", "1"):
+        monkeypatch.setenv("AUTOSAGE_VALIDATE", validate)
+        got = autosage_amd.csr_position_bias(crow.cuda(), col.cuda(), table.cuda(), max_distance=20)
+        assert torch.equal(got.cpu(), want)
+    with pytest.raises(ValueError, match="CSR"):
+        autosage_amd.csr_position_bias(crow.cuda(), -col.cuda(), table.cuda(), max_distance=20)
+    with pytest.raises(ValueError, match="CSR"):
+        autosage_amd.csr_position_bias(crow.cuda(), col.cuda(), table.cuda(), max_distance=20,
+                                       positions=torch.arange(2).cuda())
