@@ -109,6 +109,7 @@ def csr_position_bias_impl(crow, col, positions, table, max_distance, bidirectio
     buckets, heads = table.shape
     borders = border_array(buckets, max_distance, bool(bidirectional))
     crow, col, positions, table = _long(crow), _long(col), _long(positions), table.contiguous()
+    validate_if_requested(crow, col, _MAX_NODES if positions is None else None)
     nnz = col.numel()
     out = torch.empty(heads, nnz, dtype=table.dtype, device=table.device)
     # whole words: the last one may reach behind the edges
@@ -253,7 +254,6 @@ def csr_position_bias(crow, col, table, *, max_distance: int, bidirectional: boo
     if not load_native():
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable: {native_load_error()}")
     crow, col, positions = _long(crow), _long(col), _long(positions)
-    validate_if_requested(crow, col, _MAX_NODES if positions is None else None)
     if torch.is_grad_enabled() and table.requires_grad:
         return _PositionBias.apply(table, crow, col, positions, max_distance, bool(bidirectional))
     return csr_position_bias_impl(crow, col, positions, table, max_distance, bool(bidirectional), keep=False)[0]

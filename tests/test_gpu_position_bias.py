@@ -254,3 +254,12 @@ def test_columns_beyond_the_rows(monkeypatch):
     with pytest.raises(ValueError, match="CSR"):
         autosage_amd.csr_position_bias(crow.cuda(), col.cuda(), table.cuda(), max_distance=20,
                                        positions=torch.arange(2).cuda())
+
+
+def test_the_registered_operator_is_validated(monkeypatch):
+    crow, col = torch.tensor([0, 2, 3]).cuda(), torch.tensor([0, -1, 1]).cuda()
+    table = torch.randn(8, 2, device="cuda", requires_grad=True)
+    monkeypatch.setenv("AUTOSAGE_VALIDATE", "1")
+    with pytest.raises(ValueError, match="CSR"):
+        torch.ops.autosage.csr_position_bias(crow, col, None, table, 9, True)
+    torch.ops.autosage.csr_position_bias(crow, col.abs(), None, table, 9, True)
