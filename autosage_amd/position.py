@@ -20,6 +20,7 @@ import functools
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .ops import load_native, native_load_error, validate_if_requested
@@ -150,23 +151,44 @@ def csr_position_bias_backward_impl(found, grad, buckets):
     return table
 
 
+def has_tangent(*tensors) -> bool:
+    """Whether one of the tensors carries a forward-mode derivative."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _refuse_tangent(t) -> None:
+    if has_tangent(t):
+        raise RuntimeError("the registered operators of the position bias have no forward-mode derivative: "
+                           "call autosage_amd.csr_position_bias")
+
+
+def _registered(crow, col, positions, table, max_distance, bidirectional):
+    _refuse_tangent(table)
+    return csr_position_bias_impl(crow, col, positions, table, max_distance, bidirectional)
+
+
+def _registered_backward(found, grad, buckets):
+    _refuse_tangent(grad)
+    return csr_position_bias_backward_impl(found, grad, buckets)
+
+
 SCHEMAS = {
     # the bias, and the edges' buckets for its gradient
     "csr_position_bias": (
         "csr_position_bias(Tensor crow, Tensor col, Tensor? positions, Tensor table, int max_distance, "
         "bool bidirectional) -> (Tensor, Tensor)",
-        csr_position_bias_impl,
+        _registered,
     ),
     "csr_position_bias_backward": (
         "csr_position_bias_backward(Tensor found, Tensor grad, int buckets) -> Tensor",
-        csr_position_bias_backward_impl,
+        _registered_backward,
     ),
 }
 
 
 def _bucket_sums(found, grad, buckets):
     """dL/dtable, with a history where it is differentiated itself."""
-    if torch.is_grad_enabled() and grad.requires_grad:
+    if (torch.is_grad_enabled() and grad.requires_grad) or has_tangent(grad):
         return _BucketSums.apply(grad, found, buckets)
     return csr_position_bias_backward_impl(found, grad, buckets)
 
@@ -187,17 +209,53 @@ class _PositionBias(torch.autograd.Function):
         return _bucket_sums(ctx.saved_tensors[0], grad, ctx.buckets), None, None, None, None, None
 
 
+# The same for tables that carry a tangent: torch asks for the context in a call of
+# its own where more than the gradient is defined, which costs the host time that
+# the class above saves.
+class _PositionBiasDual(torch.autograd.Function):
+    @staticmethod
+    def forward(table, crow, col, positions, max_distance, bidirectional):
+        return csr_position_bias_impl(crow, col, positions, table, max_distance, bidirectional)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _setup(ctx, (None, None, None, inputs[0]), output)
+        ctx.save_for_forward(output[1])
+        ctx.edges = output[0].size(1)
+
+    @staticmethod
+    def backward(ctx, grad, _):
+        grad_table = None if grad is None else _bucket_sums(ctx.saved_tensors[0], grad, ctx.buckets)
+        return grad_table, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, table, *_):
+        return _lookup(table, ctx.saved_tensors[0], ctx.edges), None
+
+
 class _BucketSums(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, grad, found, buckets):
-        ctx.save_for_backward(found)
-        ctx.edges = grad.size(1)
+    def forward(grad, found, buckets):
         return csr_position_bias_backward_impl(found, grad, buckets)
 
     @staticmethod
+    def setup_context(ctx, inputs, output):
+        ctx.save_for_backward(inputs[1])
+        ctx.save_for_forward(inputs[1])
+        ctx.edges, ctx.buckets = inputs[0].size(1), inputs[2]
+
+    @staticmethod
     def backward(ctx, grad_table):
-        # the sum over each bucket's edges is linear: its transpose is the lookup
-        return grad_table.t()[:, ctx.saved_tensors[0][: ctx.edges].long()], None, None
+        return _lookup(grad_table, ctx.saved_tensors[0], ctx.edges), None, None
+
+    @staticmethod
+    def jvp(ctx, grad, *_):
+        return _bucket_sums(ctx.saved_tensors[0], grad, ctx.buckets)
+
+
+def _lookup(table, found, edges):
+    """The bias of edges whose buckets are known: linear in the table, and the transpose of the sums."""
+    return table.t()[:, found[:edges].long()]
 
 
 def _setup(ctx, inputs, output) -> None:
@@ -219,7 +277,7 @@ def _sums_setup(ctx, inputs, output) -> None:
 
 
 def _sums_backward(ctx, grad_table):
-    return None, grad_table.t()[:, ctx.saved_tensors[0][: ctx.edges].long()], None
+    return None, _lookup(grad_table, ctx.saved_tensors[0], ctx.edges), None
 
 
 def register_autograd() -> None:
@@ -254,6 +312,8 @@ def csr_position_bias(crow, col, table, *, max_distance: int, bidirectional: boo
     if not load_native():
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable: {native_load_error()}")
     crow, col, positions = _long(crow), _long(col), _long(positions)
+    if has_tangent(table):
+        return _PositionBiasDual.apply(table, crow, col, positions, max_distance, bool(bidirectional))[0]
     if torch.is_grad_enabled() and table.requires_grad:
         return _PositionBias.apply(table, crow, col, positions, max_distance, bool(bidirectional))
     return csr_position_bias_impl(crow, col, positions, table, max_distance, bool(bidirectional), keep=False)[0]

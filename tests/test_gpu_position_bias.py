@@ -263,3 +263,34 @@ def test_the_registered_operator_is_validated(monkeypatch):
     with pytest.raises(ValueError, match="CSR"):
         torch.ops.autosage.csr_position_bias(crow, col, None, table, 9, True)
     torch.ops.autosage.csr_position_bias(crow, col.abs(), None, table, 9, True)
+
+
+def test_forward_mode():
+    """Tangents of the table, and of the gradient that comes back."""
+    crow, col = case_graph(60, 5, seed=13)
+    cpu, gpu = (torch.from_numpy(crow), torch.from_numpy(col)), to_dev(crow, col)
+    gen = torch.Generator().manual_seed(14)
+    table, tangent = torch.randn(8, 2, generator=gen), torch.randn(8, 2, generator=gen)
+    weights, change = torch.randn(2, len(col), generator=gen), torch.randn(2, len(col), generator=gen)
+    fw = torch.autograd.forward_ad
+    results = []
+    for graph, device in ((cpu, "cpu"), (gpu, "cuda")):
+        own = table.clone().to(device).requires_grad_()
+        with fw.dual_level():
+            dual = fw.make_dual(own, tangent.to(device))
+            out = autosage_amd.csr_position_bias(*graph, dual, max_distance=9)
+            first, = torch.autograd.grad((out * out).sum(), own)
+            back, = torch.autograd.grad(autosage_amd.csr_position_bias(*graph, own, max_distance=9), own,
+                                        fw.make_dual(weights.to(device), change.to(device)))
+            results.append([*fw.unpack_dual(out), *fw.unpack_dual(first), *fw.unpack_dual(back)])
+    for a, b in zip(*results):
+        assert a is not None and torch.allclose(a, b.cpu(), rtol=1e-5, atol=1e-5)
+    assert torch.equal(results[0][1], results[1][1].cpu())
+    with fw.dual_level():
+        for grad in (False, True):
+            dual = fw.make_dual(table.cuda().requires_grad_(grad), tangent.cuda())
+            with pytest.raises(RuntimeError):
+                torch.ops.autosage.csr_position_bias(*gpu, None, dual, 9, True)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.ops.autosage.csr_position_bias_backward(torch.zeros(4, dtype=torch.uint8, device="cuda"),
+                                                          fw.make_dual(weights[:, :4].cuda(), change[:, :4].cuda()), 8)
