@@ -30,7 +30,7 @@ import torch
 from . import _env
 from . import _native
 from .ops import load_native, native_load_error
-from .position import border_array, bucket_borders, position_buckets
+from .position import border_array, bucket_borders, has_tangent, position_buckets
 
 E4M3 = torch.float8_e4m3fn
 MAX_WIDTH = 256
@@ -129,6 +129,8 @@ def _check_new_rows(key, value, key_pages, value_pages) -> None:
 def _no_gradient(name: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad()")
+    if has_tangent(*tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 class _CacheStruct(ctypes.Structure):

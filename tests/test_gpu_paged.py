@@ -566,3 +566,24 @@ def test_a_write_is_seen_by_autograd(quantised, registered):
         autosage_amd.paged_cache_write(rows, rows, k, v, ptr, idx, *span)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             scores.sum().backward()
+
+
+def test_forward_mode_is_refused():
+    """By the public functions and the registered operators, whose results would have no tangent."""
+    cache = Cache([4, 9], 1, 8, 8, 4, torch.float32, seed=29)
+    (k, v, ptr, idx), _ = cache.args()
+    coded, e = Cache([4, 9], 1, 8, 8, 4, torch.float32, quantised=True, seed=29).args()
+    query, rows = torch.randn(2, 1, 8, device="cuda"), torch.randn(2, 1, 8, device="cuda")
+    span, lengths = (torch.tensor([0, 1, 2]).cuda(), torch.tensor([3, 8]).cuda()), torch.tensor([4, 9]).cuda()
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+        for of in (autosage_amd, torch.ops.autosage):
+            for call in (lambda: of.paged_attention(dual(query), k, v, ptr, idx, lengths),
+                         lambda: of.paged_attention(dual(query), *coded, lengths, **e),
+                         lambda: of.paged_cache_write(rows, dual(rows), k, v, ptr, idx, *span),
+                         lambda: of.paged_cache_read(k, dual(v), ptr, idx, *span, 2)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+            of.paged_attention(query, *coded, lengths, **e)

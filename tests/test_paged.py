@@ -385,3 +385,23 @@ def test_validation_of_lists_with_room(monkeypatch):
         read(k, v, wide, table.flatten(), torch.tensor([-1, 1, 2]), torch.tensor([4, 17]), 2)
     with pytest.raises(ValueError, match="more tokens"):
         attention(query, k, v, wide, table.flatten(), torch.tensor([9, 33]), window=1)
+
+
+def test_forward_mode_is_refused():
+    cache = Cache([4, 9], 1, 8, 8, 4, torch.float32, seed=14)
+    (k, v, ptr, idx), _ = cache.args("cpu")
+    query, rows, span = torch.randn(2, 1, 8), torch.randn(2, 1, 8), (torch.tensor([0, 1, 2]), torch.tensor([3, 8]))
+    lengths = torch.tensor([4, 9])
+    with torch.autograd.forward_ad.dual_level():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: autosage_amd.paged_attention(dual(query), k, v, ptr, idx, lengths),
+                     lambda: autosage_amd.paged_attention(query, k, dual(v), ptr, idx, lengths),
+                     lambda: autosage_amd.paged_attention(query, k, v, ptr, idx, lengths, max_distance=9,
+                                                          bias_table=dual(torch.randn(8, 1))),
+                     lambda: autosage_amd.paged_cache_write(rows, dual(rows), k, v, ptr, idx, *span),
+                     lambda: autosage_amd.paged_cache_read(dual(k), v, ptr, idx, *span, 2)):
+            with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+                call()
+        autosage_amd.paged_attention(query, k, v, ptr, idx, lengths)
