@@ -26,6 +26,7 @@ from . import _native
 from .ops import load_native, native_load_error, validate_if_requested
 
 MAX_BUCKETS = 256
+_MAX_HEADS = 65535
 # node ids that are positions may be any: rows of a part of a graph see columns of all of it
 _MAX_NODES = 2**62
 _DTYPES = {torch.float32: 0, **_native.DTYPES_16}
@@ -189,9 +190,14 @@ SCHEMAS = {
 }
 
 
+# Inside torch.func's transforms (grad, vmap, jvp and what they make up) tensors are
+# wrapped, and only functions with rules for them reach the kernels.
+_transforms_active = getattr(torch._C, "_are_functorch_transforms_active", lambda: False)
+
+
 def _bucket_sums(found, grad, buckets):
     """dL/dtable, with a history where it is differentiated itself."""
-    if (torch.is_grad_enabled() and grad.requires_grad) or has_tangent(grad):
+    if (torch.is_grad_enabled() and grad.requires_grad) or _transforms_active() or has_tangent(grad):
         return _BucketSums.apply(grad, found, buckets)
     return csr_position_bias_backward_impl(found, grad, buckets)
 
@@ -212,10 +218,10 @@ class _PositionBias(torch.autograd.Function):
         return _bucket_sums(ctx.saved_tensors[0], grad, ctx.buckets), None, None, None, None, None
 
 
-# The same for tables that carry a tangent: torch asks for the context in a call of
-# its own where more than the gradient is defined, which costs the host time that
-# the class above saves.
-class _PositionBiasDual(torch.autograd.Function):
+# The same for every other derivative and torch.func's transforms: torch asks for the
+# context in a call of its own where more than the gradient is defined, which costs
+# the host time that the class above saves.
+class _PositionBiasTransformed(torch.autograd.Function):
     @staticmethod
     def forward(table, crow, col, positions, max_distance, bidirectional):
         return csr_position_bias_impl(crow, col, positions, table, max_distance, bidirectional)
@@ -228,12 +234,23 @@ class _PositionBiasDual(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad, _):
-        grad_table = None if grad is None else _bucket_sums(ctx.saved_tensors[0], grad, ctx.buckets)
+        # apply also unwraps what a transform that is over has saved
+        grad_table = None if grad is None else _BucketSums.apply(grad, ctx.saved_tensors[0], ctx.buckets)
         return grad_table, None, None, None, None, None
 
     @staticmethod
     def jvp(ctx, table, *_):
         return _lookup(table, ctx.saved_tensors[0], ctx.edges), None
+
+    @staticmethod
+    def vmap(info, in_dims, *inputs):
+        table = inputs[0]
+        if in_dims[1:4] != (None, None, None) or info.batch_size * table.size(-1) > _MAX_HEADS:
+            return _one_by_one(_PositionBiasTransformed, info, in_dims, inputs)
+        # the tables' heads side by side
+        table = table.movedim(in_dims[0], 1)
+        out, found = _PositionBiasTransformed.apply(table.flatten(1), *inputs[1:])
+        return (out.unflatten(0, table.shape[1:]), found), (0, None)
 
 
 class _BucketSums(torch.autograd.Function):
@@ -253,7 +270,24 @@ class _BucketSums(torch.autograd.Function):
 
     @staticmethod
     def jvp(ctx, grad, *_):
-        return _bucket_sums(ctx.saved_tensors[0], grad, ctx.buckets)
+        return _BucketSums.apply(grad, ctx.saved_tensors[0], ctx.buckets)
+
+    @staticmethod
+    def vmap(info, in_dims, grad, found, buckets):
+        if in_dims[1] is None:
+            rows = grad.movedim(in_dims[0], 0)
+            if info.batch_size * rows.size(1) <= _MAX_HEADS:
+                return _BucketSums.apply(rows.flatten(0, 1), found, buckets).unflatten(1, rows.shape[:2]), 1
+        return _one_by_one(_BucketSums, info, in_dims, (grad, found, buckets))
+
+
+def _one_by_one(function, info, in_dims, inputs):
+    """The vmap rule of calls that differ in more than their tables: one call each."""
+    results = [function.apply(*(x if d is None else x.select(d, i) for x, d in zip(inputs, in_dims)))
+               for i in range(info.batch_size)]
+    if isinstance(results[0], tuple):
+        return tuple(torch.stack(parts) for parts in zip(*results)), (0,) * len(results[0])
+    return torch.stack(results), 0
 
 
 def _lookup(table, found, edges):
@@ -315,8 +349,8 @@ def csr_position_bias(crow, col, table, *, max_distance: int, bidirectional: boo
     if not load_native():
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable: {native_load_error()}")
     crow, col, positions = _long(crow), _long(col), _long(positions)
-    if has_tangent(table):
-        return _PositionBiasDual.apply(table, crow, col, positions, max_distance, bool(bidirectional))[0]
+    if _transforms_active() or has_tangent(table):
+        return _PositionBiasTransformed.apply(table, crow, col, positions, max_distance, bool(bidirectional))[0]
     if torch.is_grad_enabled() and table.requires_grad:
         return _PositionBias.apply(table, crow, col, positions, max_distance, bool(bidirectional))
     return csr_position_bias_impl(crow, col, positions, table, max_distance, bool(bidirectional), keep=False)[0]

@@ -294,3 +294,32 @@ def test_forward_mode():
         with pytest.raises(RuntimeError, match="forward-mode"):
             torch.ops.autosage.csr_position_bias_backward(torch.zeros(4, dtype=torch.uint8, device="cuda"),
                                                           fw.make_dual(weights[:, :4].cuda(), change[:, :4].cuda()), 8)
+
+
+def test_function_transforms():
+    """torch.func over the GPU's function and the CPU's composition: derivatives, batches of tables and of graphs."""
+    crow, col = case_graph(40, 4, seed=15)
+    gen = torch.Generator().manual_seed(16)
+    table, tables = torch.randn(6, 2, generator=gen), torch.randn(3, 6, 2, generator=gen)
+    weights = torch.randn(2, len(col), generator=gen)
+    positions = torch.randint(-20, 20, (3, 40), generator=gen)
+    f = torch.func
+    results = []
+    for device in ("cpu", "cuda"):
+        graph = [torch.from_numpy(a).to(device) for a in (crow, col)]
+        w, t, ts, at = (x.to(device) for x in (weights, table, tables, positions))
+
+        def bias(table, positions=None):
+            return autosage_amd.csr_position_bias(*graph, table, max_distance=9, positions=positions)
+
+        def loss(table):
+            return (bias(table) ** 3 * w).sum()
+
+        results.append([f.grad(loss)(t), f.vmap(bias)(ts), f.vmap(bias, in_dims=1)(ts.transpose(0, 1)),
+                        f.vmap(f.grad(loss))(ts), f.jacrev(bias)(t), f.jacfwd(bias)(t), f.hessian(loss)(t),
+                        f.jacrev(f.jacrev(loss))(t), f.jvp(bias, (t,), (ts[0],))[1], f.vmap(bias)(ts, at),
+                        f.vmap(f.grad(lambda a, p: (bias(a, p) ** 2 * w).sum()))(ts, at), f.vjp(bias, t)[1](w)[0],
+                        f.vmap(f.vjp(bias, t)[1])(torch.stack([w, 2 * w]))[0]])
+    for a, b in zip(*results):
+        # sums of a few dozen numbers of both devices in float32, in different orders
+        assert a.shape == b.shape and torch.allclose(a, b.cpu(), rtol=1e-4, atol=1e-4)
