@@ -228,9 +228,13 @@ __device__ __forceinline__ RawVec<N * sizeof(C)> load_run(const C* __restrict__ 
   if constexpr (MODE != kNarrow) {
     __builtin_memcpy(&r, row + start, sizeof(r));
   } else {
+    // zeros behind the row: an infinite number there would make NaN of the queries' zeros
     C part[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) part[i] = row[start + i < width ? start + i : width - 1];
+    for (int i = 0; i < N; ++i) {
+      const C x = row[start + i < width ? start + i : width - 1];
+      part[i] = start + i < width ? x : C{};
+    }
     __builtin_memcpy(&r, part, sizeof(r));
   }
   return r;

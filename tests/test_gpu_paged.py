@@ -587,3 +587,31 @@ def test_forward_mode_is_refused():
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     call()
             of.paged_attention(query, *coded, lengths, **e)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [8, 5])
+@pytest.mark.parametrize("width, value_width", [(3, 5), (5, 3), (1, 200), (40, 40), (33, 65), (129, 130), (200, 136),
+                                                (255, 250)])
+@pytest.mark.parametrize("from_end", [1, 3])
+def test_infinite_numbers_at_the_ends_of_rows(dtype, page, width, value_width, from_end):
+    """Rows shorter than a run, rows whose last run is moved back over the one before, and wide ones: a score of -inf is
+    no token, an infinite value makes its own column infinite and no other."""
+    at, value_at = max(width - from_end, 0), max(value_width - from_end, 0)
+    cache = Cache([40, 40, 700], 1, width, value_width, page, dtype, seed=30)
+    (k, v, ptr, idx), _ = cache.args()
+    query = torch.full((3, 1, width), 0.25, dtype=dtype, device="cuda")
+    lengths = torch.tensor(cache.lengths).cuda()
+    want = autosage_amd.paged_attention(query, k, v, ptr, idx, lengths)
+    for b, pages, column, what in ((0, k, at, -torch.inf), (1, v, value_at, torch.inf), (2, k, at, -torch.inf)):
+        pages[idx[ptr[b] + 19 // page], 0, 19 % page, column] = what
+    got = autosage_amd.paged_attention(query, k, v, ptr, idx, lengths)
+    others = [d for d in range(value_width) if d != value_at]
+    assert got[1, 0, value_at] == torch.inf and torch.equal(got[1, 0, others], want[1, 0, others])
+    for b in (0, 2):
+        keep = [t for t in range(cache.lengths[b]) if t != 19]
+        for rows in cache.rows.values():
+            rows[b] = rows[b][keep]
+        cache.lengths[b] -= 1
+    plain = plain_attention(cache, query.cpu(), 1.0)
+    assert_attention(got[[0, 2]], None, [t[[0, 2]] for t in plain], dtype=dtype)
