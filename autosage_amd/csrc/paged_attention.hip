@@ -50,7 +50,6 @@
 // A sequence that sees no token, or only scores of -inf, gives zeros and an
 // lse of -inf.  A length beyond the sequence's pages or max_length makes its
 // results NaN, and so does a page id outside the cache, which is never read.
-#include <cfloat>
 
 #include "paged_common.h"
 #include "position_map.h"
@@ -88,7 +87,7 @@ struct AttentionArgs {
   int page_shift;
   int shares;         // workgroups of each 16 heads of a key head; 0: one per sequence
   int2* plan;         // [sequences] of each sequence: its first part's number, and how many it has
-  float2* part_sum;   // [parts, heads * group] maximum (in powers of two) and sum
+  float2* part_sum;   // [parts, heads * group] maximum and sum
   float* part_out;    // [parts, heads * group, value width]
 };
 
@@ -243,7 +242,7 @@ __device__ __forceinline__ RawVec<N * sizeof(C)> load_run(const C* __restrict__ 
 // ---- element types ---------------------------------------------------------------
 // Word pairs of the 16-bit matrix instructions, and how a cache's words get there.
 struct Bf16Unit {
-  static constexpr float kShift = 0.0f;  // weights are exp2(s - m + kShift)
+  static constexpr float kShift = 0.0f;  // weights are exp2((s - m) * kLog2e + kShift)
   __device__ static f32x4 multiply(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
                                                    0, 0);
@@ -285,9 +284,14 @@ struct Unit<Fp16, Fp16> {
   using type = Fp16Unit;
 };
 
-// A running maximum may stay this far (in powers of two) below a score: weights
-// are then at most 2^4, which costs no bit of fp32 or bf16.
-constexpr float kSlack = 4.0f;
+// A running maximum may stay this far below a score: weights are then at most
+// 2^4, which costs no bit of fp32 or bf16.
+constexpr float kSlack = 4.0f * kLn2;
+
+// exp(d) for the difference d of two scores.  Scores stay as they are and only
+// differences are brought to powers of two: a score of -3e38 (a mask) times kLog2e
+// would be infinite.
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
 // N 16-bit numbers of a cache as words: what it holds, or its codes in bf16.
 template <typename C, int N>
@@ -338,7 +342,7 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
   __shared__ ShareSums share_sums;
   __shared__ float wave_top[kWavesPerBlock][kHeads];
   __shared__ float wave_sum[kWavesPerBlock][kHeads];
-  __shared__ float bias[kMaxBuckets][kHeads];  // in powers of two, of the keys in front of the query
+  __shared__ float bias[kMaxBuckets][kHeads];  // of the keys in front of the query
   constexpr int kOutWaves = kLater ? 2 : kWavesPerBlock;
   __shared__ float wave_out[kOutWaves][kHeads][W];
   __shared__ u32x4 q_shared[kLater ? kKeyRuns : 1][kQ][kLater ? kWave : 1];
@@ -362,10 +366,8 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
     stage_borders(border, map);
     for (int i = threadIdx.x; i < map.side * kHeads; i += kBlock) {
       const int hh = i % kHeads < heads_here ? i % kHeads : 0;
-      const float x = Elem<T>::at(static_cast<const T*>(a.table), static_cast<int64_t>(i / kHeads) * heads_q + head0 + hh);
-      // a mask of the type's lowest number stays a number: a row of such masks has weights
-      const float x2 = kLog2e * x;
-      bias[i / kHeads][i % kHeads] = finite(x) && !finite(x2) ? (x < 0.0f ? -FLT_MAX : FLT_MAX) : x2;
+      bias[i / kHeads][i % kHeads] =
+          Elem<T>::at(static_cast<const T*>(a.table), static_cast<int64_t>(i / kHeads) * heads_q + head0 + hh);
     }
   }
   Share share{0, 1, 1, 0, share_index};
@@ -376,7 +378,6 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
     __syncthreads();
   }
 
-  const float to_log2 = a.scale * kLog2e;
   const C* key_base = static_cast<const C*>(c.key.data) + h * c.key.stride[1];
   const C* value_base = static_cast<const C*>(c.value.data) + h * c.value.stride[1];
   const int64_t key_step = c.key.stride[2];
@@ -617,25 +618,24 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
         for (int e = 0; e < kOwn; ++e) value[0][e] = tile.value[e];
       }
 
-      // scores in powers of two
-      float s2[kOwn];
+      float scores[kOwn];
       float most = -INFINITY;
 #pragma unroll
       for (int e = 0; e < kOwn; ++e) {
-        s2[e] = score[e / 4][e % 4] * to_log2;
-        if constexpr (kCoded) s2[e] = ldexpf(s2[e], static_cast<int8_t>(tile.key_e.w[e / 4] >> (8 * (e % 4))));
+        scores[e] = score[e / 4][e % 4] * a.scale;
+        if constexpr (kCoded) scores[e] = ldexpf(scores[e], static_cast<int8_t>(tile.key_e.w[e / 4] >> (8 * (e % 4))));
       }
       if (a.table != nullptr) {
         // every token of the tile farther than the last border: one number a head
         if (seen.end - t0 - kTile >= border[map.side - 1]) {
           const float far = bias[map.side - 1][n];
 #pragma unroll
-          for (int e = 0; e < kOwn; ++e) s2[e] += far;
+          for (int e = 0; e < kOwn; ++e) scores[e] += far;
         } else {
 #pragma unroll
           for (int e = 0; e < kOwn; ++e) {
             const int away = seen.end - 1 - (t0 + own_token + e);
-            s2[e] += bias[bucket_of_distance(border, map, away < 0 ? 0 : away)][n];
+            scores[e] += bias[bucket_of_distance(border, map, away < 0 ? 0 : away)][n];
           }
         }
       }
@@ -645,18 +645,18 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
         for (int e = 0; e < kOwn; ++e) {
           const int t = t0 + own_token + e;
           const bool out_of_sight = t < begin || t >= end;
-          if ((tile.bad_tokens >> e) & 1) s2[e] = NAN;
-          if (out_of_sight) s2[e] = -INFINITY;
+          if ((tile.bad_tokens >> e) & 1) scores[e] = NAN;
+          if (out_of_sight) scores[e] = -INFINITY;
         }
       }
 #pragma unroll
-      for (int e = 0; e < kOwn; ++e) most = fmaxf(most, s2[e]);
+      for (int e = 0; e < kOwn; ++e) most = fmaxf(most, scores[e]);
 
       if (__any(most > top + kSlack)) {
         most = fmaxf(most, __shfl_xor(most, 16, 64));
         most = fmaxf(most, __shfl_xor(most, 32, 64));
         const float next = fmaxf(top, most);
-        const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next);
+        const float keep = top == -INFINITY ? 0.0f : exp_of(top - next);
         top = next;
         sum *= keep;
         // lane (n, g) holds the heads g*4 .. g*4+3 of its columns
@@ -667,11 +667,11 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
           for (int j = 0; j < kValues; ++j) acc[j][i] *= f;
         }
       }
-      const float from = top == -INFINITY ? 0.0f : top - U::kShift;
+      const float from = top == -INFINITY ? 0.0f : top;
       float weight[kOwn];
 #pragma unroll
       for (int e = 0; e < kOwn; ++e) {
-        weight[e] = __builtin_amdgcn_exp2f(s2[e] - from);
+        weight[e] = __builtin_amdgcn_exp2f(fmaf(scores[e] - from, kLog2e, U::kShift));
         sum += weight[e];
         if constexpr (kCoded) weight[e] = ldexpf(weight[e], static_cast<int8_t>(tile.value_e.w[e / 4] >> (8 * (e % 4))));
       }
@@ -786,7 +786,7 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
 #pragma unroll
       for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_top[w][hh]);
       const float mine = wave_top[wave][hh];
-      const float f = mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - most);
+      const float f = mine == -INFINITY ? 0.0f : exp_of(mine - most);
 #pragma unroll
       for (int j = 0; j < kValues; ++j) acc[j][i] *= f;
     }
@@ -826,7 +826,7 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
 #pragma unroll
       for (int w = 0; w < kWavesPerBlock; ++w) {
         const float mine = wave_top[w][hh];
-        total += (mine == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mine - most)) * wave_sum[w][hh];
+        total += (mine == -INFINITY ? 0.0f : exp_of(mine - most)) * wave_sum[w][hh];
         if (w < kOutWaves) x += wave_out[w % kOutWaves][hh][d];
       }
       if (whole) {
@@ -834,7 +834,7 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
         const bool none = total == 0.0f;
         static_cast<T*>(a.out)[row * width + d] = rounded<T>(seen.bad ? NAN : (none ? 0.0f : x / total));
         if (a.lse != nullptr && d == 0)
-          a.lse[row] = seen.bad ? NAN : (none ? -INFINITY : (most - U::kShift + __builtin_amdgcn_logf(total)) * kLn2);
+          a.lse[row] = seen.bad ? NAN : (none ? -INFINITY : fmaf(__builtin_amdgcn_logf(total) - U::kShift, kLn2, most));
       } else {
         const int64_t row = part * heads_q + head0 + hh;
         a.part_out[row * width + d] = x;
@@ -875,12 +875,12 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void paged_attention_join_kernel
     const float2 part = sums[static_cast<int64_t>(k) * heads_q];
     const float next = fmaxf(top, part.x);
     const float base = next == -INFINITY ? 0.0f : next;
-    sum = sum * __builtin_amdgcn_exp2f(top - base) + part.y * __builtin_amdgcn_exp2f(part.x - base);
+    sum = sum * exp_of(top - base) + part.y * exp_of(part.x - base);
     top = next;
   }
   const float most = wave_max_f32(top);
   const float base = most == -INFINITY ? 0.0f : most;
-  const float total = wave_sum_f32(sum * __builtin_amdgcn_exp2f(top - base));
+  const float total = wave_sum_f32(sum * exp_of(top - base));
 
   constexpr int kParts = kMaxWidth / kWave;
   float acc[kParts];
@@ -893,7 +893,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void paged_attention_join_kernel
     for (int u = 0; u < kJoinAhead; ++u) {
       const int k = k0 + u * TEAM;
       const int64_t at = static_cast<int64_t>(k < count ? k : count - 1) * heads_q;
-      f[u] = k < count ? __builtin_amdgcn_exp2f(sums[at].x - base) : 0.0f;
+      f[u] = k < count ? exp_of(sums[at].x - base) : 0.0f;
 #pragma unroll
       for (int i = 0; i < kParts; ++i) {
         const int d = lane + i * kWave;
@@ -927,7 +927,7 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void paged_attention_join_kernel
     }
   }
   if (a.lse != nullptr && wave == 0 && lane == 0)
-    a.lse[row] = none ? -INFINITY : (most - shift + __builtin_amdgcn_logf(total)) * kLn2;
+    a.lse[row] = none ? -INFINITY : fmaf(__builtin_amdgcn_logf(total) - shift, kLn2, most);
 }
 
 // ---- launch --------------------------------------------------------------------------

@@ -615,3 +615,46 @@ def test_infinite_numbers_at_the_ends_of_rows(dtype, page, width, value_width, f
         cache.lengths[b] -= 1
     plain = plain_attention(cache, query.cpu(), 1.0)
     assert_attention(got[[0, 2]], None, [t[[0, 2]] for t in plain], dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("max_length", [None, 700])
+@pytest.mark.parametrize("quantised", [False, True])
+def test_two_masks_and_their_lse(dtype, max_length, quantised):
+    """-3e38 beside the type's lowest number: tokens of the former have all of the weight, and the logarithm of the sum
+    is the mask's number.  A score times log2(e) would be infinite for either."""
+    cache = Cache([7, 2, 700], 1, 32, 32, 8, dtype, quantised=quantised, seed=27)
+    query = torch.randn(3, 1, 32, dtype=dtype, device="cuda")
+    table = torch.full((8, 1), torch.finfo(dtype).min, dtype=dtype)
+    table[:3] = -3e38  # distances 0 to 2
+    args, e = cache.args()
+    out, lse = autosage_amd.paged_attention(query, *args, torch.tensor(cache.lengths).cuda(), scale=0.0, return_lse=True,
+                                            bias_table=table.cuda(), max_distance=20, bidirectional=False,
+                                            max_length=max_length, **e)
+    for b, n in enumerate(cache.lengths):
+        rows = cache.rows["value"][b][max(n - 3, 0):, 0]
+        # equal weights: three fp32 terms and a quotient, bf16 parts of a weight of 1 are exact; one rounding to the type
+        allowed = rows.abs().mean(0) * 2.0**-21 + rows.mean(0).abs() * torch.finfo(dtype).eps / 2 * (1 + 2.0**-10)
+        assert bool(((out[b, 0].double().cpu() - rows.mean(0)).abs() <= allowed).all())
+        # log(3) is nothing beside 3e38
+        assert lse[b, 0].item() == table[0, 0].item()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scores_near_the_largest_number(dtype):
+    """Finite scores of up to 3e38 in both signs: the largest takes all of the weight."""
+    for page, most in ((8, 5), (8, 690), (5, 300)):
+        cache = Cache([700], 1, 8, 8, page, dtype, seed=31)
+        (k, v, ptr, idx), _ = cache.args()
+        rows = torch.zeros(700, 1, 8, dtype=dtype, device="cuda")
+        rows[:, 0, 0] = torch.linspace(-3e19, 2.9e19, 700, device="cuda").to(dtype)
+        rows[most, 0, 0] = 3e19
+        values = torch.randn(700, 1, 8, device="cuda").to(dtype)
+        span, lengths = (torch.tensor([0, 700]).cuda(), torch.tensor([0]).cuda()), torch.tensor([700]).cuda()
+        autosage_amd.paged_cache_write(rows, values, k, v, ptr, idx, *span)
+        query = torch.full((1, 1, 8), 1e19, dtype=dtype, device="cuda")
+        out, lse = autosage_amd.paged_attention(query, k, v, ptr, idx, lengths, return_lse=True)
+        assert torch.equal(out[0], values[most])
+        # one product, exact in fp32 for bf16, rounded once for float32 (and once by the scale of 1)
+        want = float(rows[most, 0, 0].double() * query[0, 0, 0].double())
+        assert abs(lse[0, 0].item() / want - 1) <= 2.0**-23
