@@ -439,8 +439,10 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
               words[i] = __float_as_uint(q[i]);
             } else {
               words[i] = U::pack(q[(2 * i) % kKeyRun], q[(2 * i + 1) % kKeyRun]);
-              q[(2 * i) % kKeyRun] -= U::unpack(words[i])[0];
-              q[(2 * i + 1) % kKeyRun] -= U::unpack(words[i])[1];
+              // what the next part holds; nothing is left of an infinite number
+              const f32x2 held = U::unpack(words[i]);
+              q[(2 * i) % kKeyRun] = finite(held[0]) ? q[(2 * i) % kKeyRun] - held[0] : 0.0f;
+              q[(2 * i + 1) % kKeyRun] = finite(held[1]) ? q[(2 * i + 1) % kKeyRun] - held[1] : 0.0f;
             }
           }
           if constexpr (!kLater) {

@@ -541,7 +541,8 @@ def paged_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, 
     sequences be answered in one launch.
 
     Scores, softmax and sums are float32 and the result is rounded once to the
-    dtype of ``query``.  A sequence without tokens, or with scores of -inf alone,
+    dtype of ``query``.  (Over 8-bit pages a query is multiplied with the codes,
+    so that finite numbers beyond 2^111 may give infinite scores.)  A sequence without tokens, or with scores of -inf alone,
     gives zeros; a length beyond ``max_length`` or the sequence's pages, or a
     page id outside the cache, gives NaN.  ``return_lse`` adds the logarithm of
     the sum of the exponentials, float32 ``[sequences, query heads]``, with which

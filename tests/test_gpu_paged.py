@@ -658,3 +658,22 @@ def test_scores_near_the_largest_number(dtype):
         # one product, exact in fp32 for bf16, rounded once for float32 (and once by the scale of 1)
         want = float(rows[most, 0, 0].double() * query[0, 0, 0].double())
         assert abs(lse[0, 0].item() / want - 1) <= 2.0**-23
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("width, page", [(32, 8), (5, 8), (200, 8), (64, 5)])
+def test_infinite_queries(dtype, quantised, width, page):
+    """Scores of -inf alone are no token at all: zeros.  A score of +inf makes its head NaN, and no other."""
+    cache = Cache([40, 700], 1, width, width, page, dtype, quantised=quantised, seed=32)
+    (k, v, ptr, idx), e = cache.args()
+    rows = torch.randn(740, 1, width, device="cuda").to(dtype)
+    rows[:, :, 2] = rows[:, :, 2].abs() + 1
+    span, lengths = (torch.tensor([0, 40, 740]).cuda(), torch.tensor([0, 0]).cuda()), torch.tensor([40, 700]).cuda()
+    autosage_amd.paged_cache_write(rows, rows, k, v, ptr, idx, *span, **e)
+    query = torch.randn(2, 3, width, device="cuda").to(dtype)
+    want = autosage_amd.paged_attention(query, k, v, ptr, idx, lengths, scale=0.1, **e)
+    query[:, 0, 2], query[:, 2, 2] = -torch.inf, torch.inf
+    out, lse = autosage_amd.paged_attention(query, k, v, ptr, idx, lengths, scale=0.1, return_lse=True, **e)
+    assert not out[:, 0].any() and bool((lse[:, 0] == -torch.inf).all())
+    assert torch.equal(out[:, 1], want[:, 1]) and out[:, 2].isnan().all()
