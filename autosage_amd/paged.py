@@ -325,7 +325,9 @@ def paged_cache_write(key, value, key_pages, value_pages, page_ptr, page_idx, to
     page_size]``): a row is held as codes and the exponent of the smallest power
     of two that brings its largest magnitude to 448, so that scaling is exact
     and every number is off by at most 1/16 of itself or half the smallest
-    code; infinities and NaN become NaN.
+    code; infinities and NaN become NaN.  That 1/16 may pass the largest number
+    of a type: what is 63,488 or more may be held as 65,536, which a read in
+    float16 gives as infinity (and 3.3e38 as 2^128, infinite in every type).
 
     A token whose place has no page is not written.  Two tokens of one call must
     not share a place (``AUTOSAGE_VALIDATE=1`` checks it, with the lists)."""
@@ -383,7 +385,8 @@ def paged_cache_read(key_pages, value_pages, page_ptr, page_idx, token_ptr, star
     rows of the result; rows behind ``token_ptr[-1]``, and tokens without a page,
     are zeros.  ``float8_e4m3fn`` pages give the numbers they stand for in
     ``dtype`` (default bfloat16, which holds them exactly unless they are below
-    its smallest number), other pages their own dtype."""
+    its smallest number; infinite where they are beyond its largest), other pages
+    their own dtype."""
     return paged_cache_read_impl(key_pages, value_pages, page_ptr, page_idx, token_ptr, start, tokens, dtype,
                                  key_exponents, value_exponents)
 

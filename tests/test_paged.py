@@ -405,3 +405,16 @@ def test_forward_mode_is_refused():
             with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
                 call()
         autosage_amd.paged_attention(query, k, v, ptr, idx, lengths)
+
+
+def test_8_bit_numbers_beyond_the_largest_of_a_type():
+    """As documented: held as 65,536, which float16 has not; the largest number that stays below is off by 1/16."""
+    k, v = torch.zeros(1, 1, 4, 2, dtype=E4M3), torch.zeros(1, 1, 4, 2, dtype=E4M3)
+    names = {f"{n}_exponents": torch.zeros(1, 1, 4, dtype=torch.int8) for n in ("key", "value")}
+    lists = (torch.tensor([0, 1]), torch.tensor([0]), torch.tensor([0, 3]), torch.tensor([0]))
+    rows = torch.tensor([[65504.0, 1.0], [63488.0, -63456.0], [-63456.0, 57344.0]], dtype=torch.float16)[:, None]
+    autosage_amd.paged_cache_write(rows, rows, k, v, *lists, **names)
+    for dtype, want in ((torch.float16, [[torch.inf, 1.0], [torch.inf, -61440.0], [-61440.0, 57344.0]]),
+                        (torch.bfloat16, [[65536.0, 1.0], [65536.0, -61440.0], [-61440.0, 57344.0]])):
+        back, _ = autosage_amd.paged_cache_read(k, v, *lists, 3, dtype=dtype, **names)
+        assert back[:, 0].tolist() == want
