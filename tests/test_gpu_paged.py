@@ -677,3 +677,83 @@ def test_infinite_queries(dtype, quantised, width, page):
     out, lse = autosage_amd.paged_attention(query, k, v, ptr, idx, lengths, scale=0.1, return_lse=True, **e)
     assert not out[:, 0].any() and bool((lse[:, 0] == -torch.inf).all())
     assert torch.equal(out[:, 1], want[:, 1]) and out[:, 2].isnan().all()
+
+
+# ---- paths between the others ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("page", [16, 12])
+@pytest.mark.parametrize("window, bias", [(1501, None), (None, (32, 128, False)), (1003, (32, 4000, True))])
+def test_windows_and_biases_of_sequences_in_shares(dtype, quantised, page, window, bias):
+    """Parts begin inside a sequence at any token, near to the query and far."""
+    _attend([3000, 1, 0, 1700, 64, 2999], 2, 2, 32, 32, page, dtype, quantised=quantised, window=window, bias=bias,
+            max_length=None, seed=33)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("quantised", [False, True])
+@pytest.mark.parametrize("page", [12, 1])
+@pytest.mark.parametrize("width, value_width", [(128, 128), (200, 136), (256, 255), (5, 200), (100, 3), (250, 1)])
+def test_tokens_looked_up_one_by_one(dtype, quantised, page, width, value_width):
+    _attend([1, 50, 140, 700], 2, 2, width, value_width, page, dtype, quantised=quantised, max_length=None, seed=width)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width, value_width", [(64, 64), (200, 136), (5, 3)])
+def test_exponents_that_are_not_neighbours(dtype, width, value_width):
+    """Exponents with the tokens of a page outermost: written, read and attended to as those with them innermost."""
+    lengths = [5, 40, 90]
+    cache = Cache(lengths, 2, width, value_width, 16, dtype, quantised=True, seed=34)
+    (k, v, ptr, idx), e = cache.args()
+    turned = {name: t.permute(2, 0, 1).contiguous().permute(1, 2, 0) for name, t in e.items()}
+    gen = torch.Generator().manual_seed(35)
+    rows = [torch.randn(135, 2, w, generator=gen).to(dtype).cuda() for w in (width, value_width)]
+    span = (torch.tensor([0, 5, 45, 135]).cuda(), torch.zeros(3, dtype=torch.long, device="cuda"))
+    results = []
+    for names in (e, turned):
+        pages = [torch.zeros_like(k.view(torch.uint8)).view(E4M3), torch.zeros_like(v.view(torch.uint8)).view(E4M3)]
+        autosage_amd.paged_cache_write(*rows, *pages, ptr, idx, *span, **names)
+        results.append([*(p.view(torch.uint8) for p in pages), *names.values(),
+                        *autosage_amd.paged_cache_read(*pages, ptr, idx, *span, 135, dtype=dtype, **names)])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    # the attention over them, looked up one by one
+    cache.rows = {kind: [t.double().cpu() for t in results[1][at].split(lengths)] for kind, at in (("key", 4), ("value", 5))}
+    query = torch.randn(3, 4, width, generator=gen).to(dtype)
+    for bound in (90, None):
+        out, lse = autosage_amd.paged_attention(query.cuda(), *pages, ptr, idx, torch.tensor(lengths).cuda(), scale=0.1,
+                                                return_lse=True, max_length=bound, **turned)
+        assert_attention(out, lse, plain_attention(cache, query, 0.1), dtype=dtype, quantised=True, lse_bound=2e-4)
+
+
+@pytest.mark.parametrize("quantised", [False, True])
+def test_places_beyond_32_bits(quantised):
+    """A cache of more than 2^32 elements, against the pages themselves: the sequence has the pages at the end and those
+    whose offsets are the same in 32 bits."""
+    dtype = E4M3 if quantised else torch.bfloat16
+    heads, page, width = 8, 64, 128
+    wrap = (1 << 32) // (heads * page * width)
+    k, v = (torch.empty(wrap + 40, heads, page, width, dtype=dtype, device="cuda") for _ in range(2))
+    e = [torch.zeros(wrap + 40, heads, page, dtype=torch.int8, device="cuda") for _ in range(2)] if quantised else []
+    names = dict(zip(("key_exponents", "value_exponents"), e))
+    idx = torch.tensor([wrap + 39, 39, wrap + 37, 37, wrap // 2 + 37]).cuda()
+    ptr, lengths = torch.tensor([0, 5]).cuda(), torch.tensor([320]).cuda()
+    gen = torch.Generator().manual_seed(36)
+    rows = torch.randn(320, heads, width, generator=gen).bfloat16()
+    span = (torch.tensor([0, 320]).cuda(), torch.tensor([0]).cuda())
+    autosage_amd.paged_cache_write(rows.cuda(), -rows.cuda(), k, v, ptr, idx, *span, **names)
+    held, exponents = quantised_rows(rows) if quantised else (rows.double(), None)
+    for pages, sign, of in ((k, 1, 0), (v, -1, 1)):
+        there = pages[idx].transpose(1, 2).reshape(320, heads, width).double().cpu()
+        if quantised:
+            assert torch.equal(e[of][idx].transpose(1, 2).reshape(320, heads).long().cpu(), exponents)
+            there = torch.ldexp(there, exponents[..., None])
+        assert torch.equal(there, sign * held)
+    key, value = autosage_amd.paged_cache_read(k, v, ptr, idx, *span, 320, dtype=torch.bfloat16, **names)
+    assert torch.equal(key.double().cpu(), held) and torch.equal(value.double().cpu(), -held)
+    cache = Cache([1], heads, width, width, page, torch.bfloat16)
+    cache.lengths, cache.rows = [320], {"key": [held], "value": [-held]}
+    query = torch.randn(1, heads, width, generator=gen).bfloat16()
+    out, lse = autosage_amd.paged_attention(query.cuda(), k, v, ptr, idx, lengths, scale=0.1, return_lse=True, **names)
+    assert_attention(out, lse, plain_attention(cache, query, 0.1), dtype=torch.bfloat16, quantised=quantised, lse_bound=2e-4)
