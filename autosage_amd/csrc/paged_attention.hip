@@ -1019,7 +1019,7 @@ extern "C" {
 size_t as_paged_attention_workspace_bytes(const as_paged_cache* cache, int64_t group, int64_t window,
                                           int64_t max_length) {
   PagedCache c;
-  if (read_paged_cache(cache, &c) != AS_OK || group < 1) return 0;
+  if (read_paged_cache(cache, &c) != AS_OK || group < 1 || group > 65535 / c.heads) return 0;
   return workspace_of(cache, group, share_count(cache, group, window, max_length)).bytes;
 }
 
@@ -1034,7 +1034,7 @@ int as_paged_attention(const as_paged_cache* cache, const void* query, const int
     return fail(AS_ERR_INVALID_ARGUMENT, "dtype must be AS_DTYPE_F32, AS_DTYPE_BF16 or AS_DTYPE_F16");
   if (cache->dtype != AS_DTYPE_E4M3 && cache->dtype != dtype)
     return fail(AS_ERR_INVALID_ARGUMENT, "a cache that is not quantised holds the type of the queries");
-  if (group < 1 || group * a.cache.heads > 65535)
+  if (group < 1 || group > 65535 / a.cache.heads)
     return fail(AS_ERR_INVALID_ARGUMENT, "query heads must lie in [1, 65535]");
   if (window < 0 || max_length < -1) return fail(AS_ERR_INVALID_ARGUMENT, "window and max_length must be positive");
   PositionMap map{};

@@ -418,3 +418,21 @@ def test_8_bit_numbers_beyond_the_largest_of_a_type():
                         (torch.bfloat16, [[65536.0, 1.0], [65536.0, -61440.0], [-61440.0, 57344.0]])):
         back, _ = autosage_amd.paged_cache_read(k, v, *lists, 3, dtype=dtype, **names)
         assert back[:, 0].tolist() == want
+
+
+def test_native_groups_whose_product_passes_64_bits():
+    path = _native.package_library_path()
+    if not path.exists():
+        pytest.skip("HIP library not built")
+    lib = _native.open_library(path)
+    cache = Cache([4, 9], 4, 4, 3, 4, torch.float32, seed=9)
+    (k, v, ptr, idx), _ = cache.args("cpu")
+    c = _CacheStruct.from_buffer(_cache_struct(k, v, ptr, idx, None, None))
+    c.sequences = 0  # nothing is launched
+    two = (ctypes.c_int64 * 2)(8, 4)
+    for group, status in ((2**62, 1), (2**62 + 1, 1), (16384, 1), (16383, 0)):
+        assert lib.as_paged_attention(ctypes.byref(c), 256, two, 256, None, 256, group, 1.0, 0, None, 0, None, 0, -1, 0,
+                                      256, 1 << 50, None) == status
+        if status:
+            assert lib.as_last_error().startswith(b"query heads must lie")
+            assert lib.as_paged_attention_workspace_bytes(ctypes.byref(c), group, 0, -1) == 0
