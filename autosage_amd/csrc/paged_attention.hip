@@ -934,12 +934,16 @@ __global__ __launch_bounds__(kJoinWaves* kWave) void paged_attention_join_kernel
 
 // ---- launch --------------------------------------------------------------------------
 
-// Sequences of at most this many tokens have a workgroup each, and no second launch.
+// Sequences of at most this many tokens have a workgroup each, and no second launch
+// (8 key heads of 128 for 32, bf16, one launch and two: one sequence of 256 tokens 9.7
+// and 12.8 us, of 512 12.0 and 12.9, of 1,024 16.7 and 13.0; 8 of 512 12.2 and 13.1, of
+// 1,024 18.2 and 16.8; 64 of 512 26 and 30, of 1,024 46 and 49).
 constexpr int64_t kSingle = 512;
 
 // Shares: two workgroups a CU in one round (64 sequences of 4,096 tokens, 8 key
-// heads, bf16: 5.5 TB/s; 5.1 in three rounds); more of them where sequences are
-// many, so that a share is not many short sequences one after another.
+// heads, bf16: 5.5 TB/s; 5.1 in three rounds), also where sequences are many and
+// short: 1,000 of 50 to 700 tokens 331 us, 375 with eight times the shares; 20,000
+// of up to 520, one key head, 468 and 899; 2,000 of up to 9 197 and 231.
 int64_t share_count(const as_paged_cache* c, int64_t group, int64_t window, int64_t max_length) {
   const int64_t units = c->heads * ((group + kHeads - 1) / kHeads);
   // tokens of one sequence at most
@@ -947,9 +951,7 @@ int64_t share_count(const as_paged_cache* c, int64_t group, int64_t window, int6
   if (max_length >= 0 && max_length < longest) longest = max_length;
   if (window > 0 && window < longest) longest = window;
   if (longest <= kSingle) return 0;
-  const int64_t few = 512 / units < 1 ? 1 : 512 / units;
-  const int64_t many = 4096 / units < c->sequences ? 4096 / units : c->sequences;
-  return few > many ? few : many;
+  return 512 / units < 1 ? 1 : 512 / units;
 }
 
 struct Workspace {

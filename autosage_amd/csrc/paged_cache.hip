@@ -276,7 +276,10 @@ __global__ __launch_bounds__(kBlock) void paged_read_kernel(PagedCache c, TokenR
   read_rows<C, T>(c.value, value, places, first, count, c.heads, shape.value, shape.log_tokens);
 }
 
-// Tokens of a workgroup: 16, fewer while that leaves fewer than 1,024 workgroups.
+// Tokens of a workgroup: 16, fewer while that leaves fewer than 1,024 workgroups
+// (writes of 2,048 tokens, 8 heads of 128, bf16: 7.1 us; 7.8 with down to 256
+// workgroups, 9.0 with 4,096; of 8,192 tokens 12.7, 15.4 and 17.7; of 32,768 tokens
+// 44.6, 44.7 and 40.7; reads alike).
 RowShape row_shape(const PagedCache& c, int64_t tokens, int elements, bool power_of_two) {
   RowShape s{};
   s.key = row_items(c.key.width, elements, power_of_two);
