@@ -2,8 +2,8 @@
 //
 // Tokens stand one behind the other, those of sequence b at token_ptr[b] ..
 // token_ptr[b + 1]; the first of them has position start[b] in its sequence.
-// Tokens from token_ptr[sequences] on belong to no sequence: a write leaves the
-// cache alone for them, a read gives zeros.
+// Tokens in front of token_ptr[0] and from token_ptr[sequences] on belong to no
+// sequence: a write leaves the cache alone for them, a read gives zeros.
 //
 // A copy (with a rounding to 8 bits in a quantised cache): bound by memory, or by
 // the launch for a few tokens.  A workgroup takes up to 16 tokens: its first wave

@@ -319,8 +319,8 @@ def paged_cache_write(key, value, key_pages, value_pages, page_ptr, page_idx, to
 
     ``key`` ``[tokens, heads, key width]`` and ``value`` ``[tokens, heads, value
     width]`` hold the tokens of sequence ``b`` at ``token_ptr[b]:token_ptr[b +
-    1]``; the first of them is token ``start[b]`` of its sequence.  Rows behind
-    ``token_ptr[-1]`` are padding.  Pages of ``torch.float8_e4m3fn`` come with
+    1]``; the first of them is token ``start[b]`` of its sequence.  Rows in front of
+    ``token_ptr[0]`` and behind ``token_ptr[-1]`` are padding.  Pages of ``torch.float8_e4m3fn`` come with
     ``key_exponents`` and ``value_exponents`` (int8, ``[pages, heads,
     page_size]``): a row is held as codes and the exponent of the smallest power
     of two that brings its largest magnitude to 448, so that scaling is exact
@@ -382,8 +382,8 @@ def paged_cache_read(key_pages, value_pages, page_ptr, page_idx, token_ptr, star
     """(key, value) of a run of tokens of every sequence, ``[tokens, heads,
     width]``: those of sequence ``b`` are its tokens from ``start[b]`` on and
     stand at ``token_ptr[b]:token_ptr[b + 1]``.  ``tokens`` is the number of
-    rows of the result; rows behind ``token_ptr[-1]``, and tokens without a page,
-    are zeros.  ``float8_e4m3fn`` pages give the numbers they stand for in
+    rows of the result; rows of no sequence, and tokens without a page, are
+    zeros.  ``float8_e4m3fn`` pages give the numbers they stand for in
     ``dtype`` (default bfloat16, which holds them exactly unless they are below
     its smallest number; infinite where they are beyond its largest), other pages
     their own dtype."""
@@ -431,7 +431,7 @@ def _check_attention(query, key_pages, lengths, page_ptr, window, bias_table, ma
 
 def _cpu_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, scale, window, bias_table, max_distance,
                    bidirectional, max_length, key_exponents, value_exponents):
-    """One sequence after another in float32 (float64 stays what it is)."""
+    """One sequence after another, in float32."""
     sequences, heads_q, _ = query.shape
     heads, page_size = key_pages.size(1), key_pages.size(2)
     group = heads_q // heads

@@ -339,7 +339,7 @@ def csr_position_bias(crow, col, table, *, max_distance: int, bidirectional: boo
     is ``[heads, edges]`` of its dtype, one row for each head's scores, with a
     gradient for ``table`` (the sum over each bucket's edges, in a fixed order).
     Node ids are positions (and columns may then lie beyond the rows) unless
-    ``positions`` (one integer per node) gives them.  With ``bidirectional`` half of the buckets are for keys behind the
+    ``positions`` (one integer per node, within +-2^62) gives them.  With ``bidirectional`` half of the buckets are for keys behind the
     query; without it a key behind the query counts as distance 0."""
     _check(crow, col, positions, table)
     max_distance = int(max_distance)

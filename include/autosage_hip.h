@@ -723,8 +723,8 @@ int as_csr_validate(const int64_t* crow, const int64_t* col, int64_t n,
  *   grad_table[b, h] = sum of grad[h, e] over the edges e of bucket b
  *
  * table, grad_table [buckets, heads] and out, grad [heads, nnz] are of dtype
- * AS_DTYPE_F32, _BF16 or _F16; positions int64[n] or NULL (node ids are
- * positions; the graph then need not be square).  found: NULL, or room for
+ * AS_DTYPE_F32, _BF16 or _F16; positions int64[n], within +-2^62, or NULL (node
+ * ids are positions; the graph then need not be square).  found: NULL, or room for
  * nnz bytes rounded up to a multiple of 4 (4-byte aligned), which the forward
  * call fills with the buckets of the edges and the backward call reads in
  * place of the graph.  The gradient is summed in a fixed order, at most 64
@@ -785,8 +785,8 @@ typedef struct as_paged_cache {
  * [tokens, heads, value_width] of `dtype` (the cache's, or any where the cache
  * is e4m3) with strides of their first two dimensions.  Tokens token_ptr[b] ..
  * token_ptr[b + 1] are those of sequence b, from its position start[b] on;
- * tokens behind token_ptr[sequences], and tokens without a page, leave the
- * cache as it is.  A place that two tokens of one call are written to holds
+ * tokens in front of token_ptr[0], behind token_ptr[sequences] or without a
+ * page leave the cache as it is.  A place that two tokens of one call are written to holds
  * parts of either. */
 int as_paged_cache_write(const as_paged_cache* cache, const void* key,
                          const int64_t* key_strides, const void* value,
