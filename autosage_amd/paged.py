@@ -232,7 +232,8 @@ def _validate_call(key_pages, page_ptr, page_idx, token_ptr, start, tokens: int,
     _require(not bool(bad), ValueError,
              "invalid tokens: token_ptr must not be negative, not descend and end inside the tokens, start not be "
              "negative")
-    _validate_lists(key_pages, page_ptr, page_idx, start, torch.where(counts > 0, start + counts, 0))
+    last = torch.where(counts > 0, start.clamp_max(2**62) + counts, 0)  # the sum stays below 2^63
+    _validate_lists(key_pages, page_ptr, page_idx, start, last)
     if writes:
         pages, page_size = key_pages.size(0), key_pages.size(2)
         _, page, place = _places(page_ptr, page_idx, token_ptr, start, tokens, pages, page_size)

@@ -436,3 +436,13 @@ def test_native_groups_whose_product_passes_64_bits():
         if status:
             assert lib.as_last_error().startswith(b"query heads must lie")
             assert lib.as_paged_attention_workspace_bytes(ctypes.byref(c), group, 0, -1) == 0
+
+
+def test_validation_of_starts_whose_sum_passes_64_bits(monkeypatch):
+    monkeypatch.setenv("AUTOSAGE_VALIDATE", "1")
+    cache = Cache([4, 9], 1, 4, 4, 4, torch.float32, seed=15)
+    (k, v, ptr, idx), _ = cache.args("cpu")
+    rows, one = torch.randn(2, 1, 4), torch.tensor([0, 1, 2])
+    for start in (2**63 - 1, 2**62, 2**40):
+        with pytest.raises(ValueError, match="more tokens"):
+            autosage_amd.paged_cache_write(rows, rows, k, v, ptr, idx, one, torch.tensor([start, 3]))
