@@ -323,3 +323,21 @@ def test_function_transforms():
     for a, b in zip(*results):
         # sums of a few dozen numbers of both devices in float32, in different orders
         assert a.shape == b.shape and torch.allclose(a, b.cpu(), rtol=1e-4, atol=1e-4)
+
+
+def test_batches_of_more_heads_than_one_call_takes():
+    crow, col = case_graph(6, 2, seed=17)
+    gen = torch.Generator().manual_seed(18)
+    tables, weights = torch.randn(2, 4, 40000, generator=gen), torch.randn(40000, len(col), generator=gen)
+    results = []
+    for device in ("cpu", "cuda"):
+        graph = [torch.from_numpy(a).to(device) for a in (crow, col)]
+        ts, w = tables.to(device), weights.to(device)
+
+        def bias(table):
+            return autosage_amd.csr_position_bias(*graph, table, max_distance=9)
+
+        results.append([torch.func.vmap(bias)(ts), torch.func.vmap(torch.func.grad(lambda t: (bias(t) * w).sum()))(ts)])
+    assert torch.equal(results[0][0], results[1][0].cpu())
+    # sums of at most a dozen numbers of a few units in float32
+    assert torch.allclose(results[0][1], results[1][1].cpu(), rtol=1e-5, atol=1e-5)
