@@ -29,7 +29,10 @@ from autosage_amd import (
     native_available,
     paged_attention,
     paged_cache_read,
+    paged_cache_resize,
     paged_cache_write,
+    rotary_frequencies,
+    rotary_positions,
     sddmm_csr_auto,
     spmm_csr,
     spmm_csr_auto,
@@ -62,7 +65,10 @@ __all__ = [
     "native_available",
     "paged_attention",
     "paged_cache_read",
+    "paged_cache_resize",
     "paged_cache_write",
+    "rotary_frequencies",
+    "rotary_positions",
     "sddmm_csr_auto",
     "spmm_csr",
     "spmm_csr_auto",

@@ -30,7 +30,7 @@ from . import _env
 from ._memo import GraphMemo
 
 LIBRARY_NAME = "libautosage_hip.so"
-ABI_VERSION = 12
+ABI_VERSION = 13
 HUB_EXACT = 0
 HUB_SPLIT64 = 1
 # 16-bit feature types of as_spmm_csr_rounded_16 (AS_DTYPE_BF16 / AS_DTYPE_F16)
@@ -208,6 +208,17 @@ _SIGNATURES = {
         _c_int,
         [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, ctypes.c_float, _c_i64, _c_ptr, _c_i64, _c_ptr,
          _c_int, _c_i64, _c_int, _c_ptr, _c_size, _c_ptr],
+    ),
+    "as_paged_cache_resize": (
+        _c_int,
+        [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64,
+         _c_i64, _c_ptr, _c_size, _c_ptr],
+    ),
+    "as_paged_cache_resize_workspace_bytes": (_c_size, [_c_i64]),
+    "as_rotary_positions": (
+        _c_int,
+        [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_int,
+         _c_int, ctypes.c_float, _c_int, _c_ptr],
     ),
 }
 
@@ -1539,10 +1550,11 @@ def _register_operators() -> None:
     global _OPS_LIBRARY
     if _OPS_LIBRARY is not None:
         return
-    from . import paged, position
+    from . import paged, paged_lists, position, rotary
 
     lib = torch.library.Library("autosage", "DEF")
-    for name, (schema, impl) in {**_SCHEMAS, **position.SCHEMAS, **paged.SCHEMAS}.items():
+    for name, (schema, impl) in {**_SCHEMAS, **position.SCHEMAS, **paged.SCHEMAS, **paged_lists.SCHEMAS,
+                                 **rotary.SCHEMAS}.items():
         lib.define(schema)
         lib.impl(name, impl, "CUDA")
     _OPS_LIBRARY = lib
@@ -1550,6 +1562,7 @@ def _register_operators() -> None:
 
     _autograd.register()
     position.register_autograd()
+    rotary.register_autograd()
 
 
 def load(path: os.PathLike[str] | str) -> None:

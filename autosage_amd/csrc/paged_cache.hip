@@ -242,6 +242,132 @@ __device__ __forceinline__ void read_rows(const PageTensor& from, const TokenRow
   }
 }
 
+// 4-bit numbers: a lane has 8 elements of a row (16 bytes of a 16-bit type, 4 of codes)
+// and four lanes share an exponent, so that neighbouring lanes are neighbours on both
+// sides and a group's maximum takes two shuffles.  Rows are cut at whole groups; what
+// passes a row's end counts as zeros and is not stored.
+constexpr int kPairRun = 8;
+inline RowItems pair_items(int width) { return row_items((width + kGroup - 1) / kGroup * (kGroup / kPairRun), 1, false); }
+
+template <typename E, int N>
+__device__ __forceinline__ RawVec<N * sizeof(E)> load_up_to(const E* from, int left) {
+  RawVec<N * sizeof(E)> r;
+  if (left >= N) {
+    __builtin_memcpy(&r, from, sizeof(r));
+  } else {
+    E part[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i] = i < left ? from[i] : E{};
+    __builtin_memcpy(&r, part, sizeof(r));
+  }
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void write_rows_e2m1(const TokenRows& from, const PageTensor& to, const Places& places,
+                                                int64_t first, int count, int heads, const RowItems& row,
+                                                int log_tokens) {
+  constexpr int N = kPairRun;
+  const int items = (heads << log_tokens) * row.runs;
+  for (int i0 = threadIdx.x; i0 < items; i0 += kAhead * kBlock) {
+    RawVec<N * sizeof(T)> raw[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
+#pragma unroll
+      for (uint32_t& w : raw[u].w) w = 0u;
+      if (it.head < heads && it.token < count && places.page[it.token] >= 0 && it.run * N < to.width)
+        raw[u] = load_up_to<T, N>(static_cast<const T*>(from.data) + (first + it.token) * from.stride[0] +
+                                      it.head * from.stride[1] + it.run * N, to.width - it.run * N);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
+      float x[N];
+      float largest = 0.0f;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        x[k] = Elem<T>::get(raw[u].w, k);
+        largest = fmaxf(largest, finite(x[k]) ? fabsf(x[k]) : INFINITY);
+      }
+      largest = fmaxf(largest, __shfl_xor(largest, 1, 64));
+      largest = fmaxf(largest, __shfl_xor(largest, 2, 64));
+      const bool odd = !finite(largest);
+      const int e = odd ? kNanExponent : group_exponent(largest);
+      const float scale = odd ? 0.0f : group_unscale(e);
+      uint32_t codes = 0u;
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] = odd ? 0.0f : x[k] * scale;
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], 1.0f, 0);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], 1.0f, 1);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], 1.0f, 2);
+      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], 1.0f, 3);
+      if (it.head < heads && it.token < count && places.page[it.token] >= 0 && it.run * N < to.width) {
+        const int64_t page = places.page[it.token];
+        const int64_t slot = places.slot[it.token];
+        uint8_t* y = static_cast<uint8_t*>(to.data) + page * to.stride[0] + it.head * to.stride[1] +
+                     slot * to.stride[2] + it.run * (N / 2);
+        if (to.width - it.run * N >= N) {
+          __builtin_memcpy(y, &codes, 4);
+        } else {
+#pragma unroll
+          for (int k = 0; k < N / 2; ++k) {
+            if (it.run * N + 2 * k < to.width) y[k] = static_cast<uint8_t>(codes >> (8 * k));
+          }
+        }
+        if (it.run % (kGroup / N) == 0)
+          reinterpret_cast<uint8_t*>(to.exponents)[page * to.exponent_stride[0] + it.head * to.exponent_stride[1] +
+                                                   slot * to.exponent_stride[2] + it.run / (kGroup / N)] =
+              static_cast<uint8_t>(e);
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void read_rows_e2m1(const PageTensor& from, const TokenRows& to, const Places& places,
+                                               int64_t first, int count, int heads, const RowItems& row,
+                                               int log_tokens) {
+  constexpr int N = kPairRun;
+  const int items = (heads << log_tokens) * row.runs;
+  for (int i0 = threadIdx.x; i0 < items; i0 += kAhead * kBlock) {
+    RawVec<4> raw[kAhead];
+    int e[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
+      raw[u].w[0] = 0u;
+      e[u] = 0;
+      if (it.head < heads && it.token < count && places.page[it.token] >= 0 && it.run * N < from.width) {
+        const int64_t page = places.page[it.token];
+        const int64_t slot = places.slot[it.token];
+        raw[u] = load_up_to<uint8_t, 4>(static_cast<const uint8_t*>(from.data) + page * from.stride[0] +
+                                            it.head * from.stride[1] + slot * from.stride[2] + it.run * (N / 2),
+                                        from.width / 2 - it.run * (N / 2));
+        e[u] = reinterpret_cast<const uint8_t*>(
+            from.exponents)[page * from.exponent_stride[0] + it.head * from.exponent_stride[1] +
+                            slot * from.exponent_stride[2] + it.run / (kGroup / N)];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
+      if (it.head >= heads || it.token >= count || it.run * N >= from.width) continue;
+      const float scale = group_scale(e[u]);
+      float x[N];
+      pairs_to_floats(raw[u].w[0], x);
+      T values[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) values[k] = rounded<T>(x[k] * scale);
+      T* y = static_cast<T*>(to.data) + (first + it.token) * to.stride[0] + it.head * to.stride[1] + it.run * N;
+      RawVec<N * sizeof(T)> r;
+      __builtin_memcpy(&r, values, sizeof(r));
+      // a row's last run may be a part of one
+      store_elements<true, N>(y, from.width - it.run * N, r);
+    }
+  }
+}
+
 struct RowShape {
   int log_tokens;
   RowItems key;
@@ -276,14 +402,45 @@ __global__ __launch_bounds__(kBlock) void paged_read_kernel(PagedCache c, TokenR
   read_rows<C, T>(c.value, value, places, first, count, c.heads, shape.value, shape.log_tokens);
 }
 
+template <typename T>
+__global__ __launch_bounds__(kBlock) void paged_write_e2m1_kernel(PagedCache c, TokenRows key, TokenRows value,
+                                                                  const int64_t* __restrict__ token_ptr,
+                                                                  const int64_t* __restrict__ start, int64_t tokens,
+                                                                  RowShape shape) {
+  __shared__ Places places;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) << shape.log_tokens;
+  const int64_t left = tokens - first;
+  const int count = left < (1 << shape.log_tokens) ? static_cast<int>(left) : 1 << shape.log_tokens;
+  find_places(c, token_ptr, start, first, count, places);
+  write_rows_e2m1<T>(key, c.key, places, first, count, c.heads, shape.key, shape.log_tokens);
+  write_rows_e2m1<T>(value, c.value, places, first, count, c.heads, shape.value, shape.log_tokens);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void paged_read_e2m1_kernel(PagedCache c, TokenRows key, TokenRows value,
+                                                                 const int64_t* __restrict__ token_ptr,
+                                                                 const int64_t* __restrict__ start, int64_t tokens,
+                                                                 RowShape shape) {
+  __shared__ Places places;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) << shape.log_tokens;
+  const int64_t left = tokens - first;
+  const int count = left < (1 << shape.log_tokens) ? static_cast<int>(left) : 1 << shape.log_tokens;
+  find_places(c, token_ptr, start, first, count, places);
+  read_rows_e2m1<T>(c.key, key, places, first, count, c.heads, shape.key, shape.log_tokens);
+  read_rows_e2m1<T>(c.value, value, places, first, count, c.heads, shape.value, shape.log_tokens);
+}
+
 // Tokens of a workgroup: 16, fewer while that leaves fewer than 1,024 workgroups
 // (writes of 2,048 tokens, 8 heads of 128, bf16: 7.1 us; 7.8 with down to 256
 // workgroups, 9.0 with 4,096; of 8,192 tokens 12.7, 15.4 and 17.7; of 32,768 tokens
 // 44.6, 44.7 and 40.7; reads alike).
-RowShape row_shape(const PagedCache& c, int64_t tokens, int elements, bool power_of_two) {
+RowShape row_shape(const PagedCache& c, int64_t tokens, int cache_dtype, int dtype, bool write) {
   RowShape s{};
-  s.key = row_items(c.key.width, elements, power_of_two);
-  s.value = row_items(c.value.width, elements, power_of_two);
+  const int elements = dtype == AS_DTYPE_F32 ? kElements<float> : kElements<Bf16>;
+  const bool power_of_two = write && cache_dtype == AS_DTYPE_E4M3;
+  const bool pairs = cache_dtype == AS_DTYPE_E2M1;
+  s.key = pairs ? pair_items(c.key.width) : row_items(c.key.width, elements, power_of_two);
+  s.value = pairs ? pair_items(c.value.width) : row_items(c.value.width, elements, power_of_two);
   while ((2 << s.log_tokens) <= kMaxTokens && tokens >> (s.log_tokens + 1) >= 1024) ++s.log_tokens;
   return s;
 }
@@ -292,7 +449,7 @@ int check_tokens(const PagedCache& c, const void* key, const void* value, const 
                  const int64_t* start, int64_t tokens, int cache_dtype, int dtype) {
   if (dtype != AS_DTYPE_F32 && dtype != AS_DTYPE_BF16 && dtype != AS_DTYPE_F16)
     return fail(AS_ERR_INVALID_ARGUMENT, "dtype must be AS_DTYPE_F32, AS_DTYPE_BF16 or AS_DTYPE_F16");
-  if (cache_dtype != AS_DTYPE_E4M3 && cache_dtype != dtype)
+  if (!is_coded(cache_dtype) && cache_dtype != dtype)
     return fail(AS_ERR_INVALID_ARGUMENT, "a cache that is not quantised holds the type of its tokens");
   if (tokens < 0 || tokens > kMaxBlocksPerLaunch * kMaxTokens) return fail(AS_ERR_UNSUPPORTED, "at most 2^26 tokens");
   if (tokens > 0 && c.sequences < 1) return fail(AS_ERR_INVALID_ARGUMENT, "tokens without sequences");
@@ -323,13 +480,14 @@ int as_paged_cache_write(const as_paged_cache* cache, const void* key, const int
   if (tokens == 0) return AS_OK;
   const TokenRows k{const_cast<void*>(key), {key_strides[0], key_strides[1]}};
   const TokenRows v{const_cast<void*>(value), {value_strides[0], value_strides[1]}};
-  const RowShape shape = row_shape(c, tokens, dtype == AS_DTYPE_F32 ? kElements<float> : kElements<Bf16>,
-                                   cache->dtype == AS_DTYPE_E4M3);
+  const RowShape shape = row_shape(c, tokens, cache->dtype, dtype, true);
   const dim3 grid(static_cast<unsigned>(((tokens - 1) >> shape.log_tokens) + 1));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
-    if (cache->dtype == AS_DTYPE_E4M3) {
+    if (cache->dtype == AS_DTYPE_E2M1) {
+      paged_write_e2m1_kernel<T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
+    } else if (cache->dtype == AS_DTYPE_E4M3) {
       paged_write_kernel<T, E4m3><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
     } else {
       paged_write_kernel<T, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
@@ -347,12 +505,14 @@ int as_paged_cache_read(const as_paged_cache* cache, void* key, void* value, con
   if (tokens == 0) return AS_OK;
   const TokenRows k{key, {int64_t(c.heads) * c.key.width, c.key.width}};
   const TokenRows v{value, {int64_t(c.heads) * c.value.width, c.value.width}};
-  const RowShape shape = row_shape(c, tokens, dtype == AS_DTYPE_F32 ? kElements<float> : kElements<Bf16>, false);
+  const RowShape shape = row_shape(c, tokens, cache->dtype, dtype, false);
   const dim3 grid(static_cast<unsigned>(((tokens - 1) >> shape.log_tokens) + 1));
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
-    if (cache->dtype == AS_DTYPE_E4M3) {
+    if (cache->dtype == AS_DTYPE_E2M1) {
+      paged_read_e2m1_kernel<T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
+    } else if (cache->dtype == AS_DTYPE_E4M3) {
       paged_read_kernel<E4m3, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
     } else {
       paged_read_kernel<T, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);

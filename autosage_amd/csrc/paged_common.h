@@ -1,5 +1,5 @@
-// The paged key-value cache on the device: which page holds a token, and the
-// 8-bit numbers of a cache that is quantised as it is written.
+// The paged key-value cache on the device: which page holds a token, and the 8-bit
+// and 4-bit numbers of a cache that is quantised as it is written.
 #pragma once
 
 #include "as_device.h"
@@ -7,17 +7,20 @@
 #include "elem16.h"
 
 namespace as {
-namespace {
 
 // 8-bit elements: sign, 4 bits of exponent, 3 of fraction, no infinities.
 struct E4m3 {
+  uint8_t bits;
+};
+// Two 4-bit elements, the first in the low bits: sign, 2 bits of exponent, 1 of fraction.
+struct E2m1Pair {
   uint8_t bits;
 };
 
 // One of the two page tensors [pages, heads, page_size, width], rows unit-stride.
 struct PageTensor {
   void* data;
-  int8_t* exponents;  // [pages, heads, page_size], null unless the elements are e4m3
+  int8_t* exponents;  // e4m3: [pages, heads, page_size]; e2m1: [pages, heads, page_size, ceil(width / 32)], else null
   int64_t stride[3];
   int64_t exponent_stride[3];
   int width;
@@ -34,6 +37,8 @@ struct PagedCache {
   int page_size;
   int heads;
 };
+
+namespace {
 
 // The page list of sequence b, inside page_idx whatever page_ptr holds.
 struct PageList {
@@ -77,6 +82,40 @@ __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
 }
 __device__ __forceinline__ float e4m3_value(uint8_t code) { return __builtin_amdgcn_cvt_f32_fp8(code, 0); }
 
+// ---- 4-bit numbers ------------------------------------------------------------
+// Every 32 neighbouring numbers of a row (fewer at its end) are held as codes and a
+// byte e + 127: 2^e is the smallest power of two (not below 2^-127) with
+// max|x| <= 6 * 2^e, 6 being the largest e2m1 number, and x * 2^-e is rounded to
+// 0, 1/2, 1, 3/2, 2, 3, 4, 6, half to the even code.  The byte 255 makes all of its
+// numbers NaN: that is how a group is held that has a number which is not finite.
+constexpr int kGroup = 32;
+constexpr int kNanExponent = 255;
+
+// The byte of a finite maximum, from its bits: 6 = 1.5 * 2^2.
+__device__ __forceinline__ int group_exponent(float largest) {
+  const uint32_t u = __float_as_uint(largest);
+  int e = static_cast<int>(u >> 23) - 2;
+  if ((u & 0x7fffffu) > 0x400000u) ++e;
+  return e < 0 ? 0 : e;
+}
+// 2^(e - 127), NaN for 255.
+__device__ __forceinline__ float group_scale(int e) {
+  return __uint_as_float(e == 0 ? 0x00400000u : (e == kNanExponent ? 0x7fc00000u : static_cast<uint32_t>(e) << 23));
+}
+// The 8 numbers of a word of codes, exactly.
+__device__ __forceinline__ void pairs_to_floats(uint32_t codes, float (&x)[8]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 0);
+  const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 1);
+  const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 2);
+  const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 3);
+  x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1], x[4] = c[0], x[5] = c[1], x[6] = d[0], x[7] = d[1];
+}
+// 2^(127 - e) for e < 255.
+__device__ __forceinline__ float group_unscale(int e) {
+  return __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+}
+
 template <typename T>
 __device__ __forceinline__ T rounded(float v);
 template <>
@@ -95,10 +134,13 @@ __device__ __forceinline__ Fp16 rounded<Fp16>(float v) {
 // Checks the host's description of a cache and lays it out for the kernels.
 constexpr int64_t kMaxWidth = 256;
 
+// Whether a cache of this type is quantised as it is written.
+inline bool is_coded(int dtype) { return dtype == AS_DTYPE_E4M3 || dtype == AS_DTYPE_E2M1; }
+
 inline int read_paged_cache(const as_paged_cache* c, PagedCache* out) {
   if (c == nullptr) return fail(AS_ERR_INVALID_ARGUMENT, "null cache pointer");
-  if (c->dtype < AS_DTYPE_F32 || c->dtype > AS_DTYPE_E4M3)
-    return fail(AS_ERR_INVALID_ARGUMENT, "the cache's dtype must be AS_DTYPE_F32, _BF16, _F16 or _E4M3");
+  if ((c->dtype < AS_DTYPE_F32 || c->dtype > AS_DTYPE_E4M3) && c->dtype != AS_DTYPE_E2M1)
+    return fail(AS_ERR_INVALID_ARGUMENT, "the cache's dtype must be AS_DTYPE_F32, _BF16, _F16, _E4M3 or _E2M1");
   if (c->sequences < 0 || c->sequences > INT32_MAX || c->page_idx_len < 0)
     return fail(AS_ERR_INVALID_ARGUMENT, "sequences and page lists must have non-negative 32-bit sizes");
   if (c->pages < 1 || c->pages > INT32_MAX || c->page_size < 1 || c->page_size > (1 << 20))
@@ -109,9 +151,11 @@ inline int read_paged_cache(const as_paged_cache* c, PagedCache* out) {
   if (c->key_pages == nullptr || c->value_pages == nullptr || c->page_ptr == nullptr ||
       (c->page_idx_len > 0 && c->page_idx == nullptr))
     return fail(AS_ERR_INVALID_ARGUMENT, "null pointer argument");
-  const bool coded = c->dtype == AS_DTYPE_E4M3;
+  const bool coded = is_coded(c->dtype);
   if (coded != (c->key_exponents != nullptr) || coded != (c->value_exponents != nullptr))
-    return fail(AS_ERR_INVALID_ARGUMENT, "an e4m3 cache has exponents, any other has none");
+    return fail(AS_ERR_INVALID_ARGUMENT, "an e4m3 cache has exponents, and so has an e2m1 cache, any other has none");
+  if (c->dtype == AS_DTYPE_E2M1 && (c->key_width % 2 != 0 || c->value_width % 2 != 0))
+    return fail(AS_ERR_UNSUPPORTED, "an e2m1 cache holds rows of an even width");
   const size_t size = c->dtype == AS_DTYPE_F32 ? 4 : (coded ? 1 : 2);
   if (!aligned(c->key_pages, size) || !aligned(c->value_pages, size))
     return fail(AS_ERR_INVALID_ARGUMENT, "the pages must be aligned to their elements");

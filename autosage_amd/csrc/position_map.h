@@ -14,7 +14,6 @@
 #include "as_internal.h"
 
 namespace as {
-namespace {
 
 constexpr int kMaxBuckets = 256;
 
@@ -27,6 +26,8 @@ struct PositionMap {
   float log_exact;      // an estimate of the others: exact + (log2 d - log_exact) * per_log
   float per_log;
 };
+
+namespace {
 
 inline int fill_position_map(PositionMap* map, const int32_t* borders, int64_t buckets, int both_sides) {
   if (buckets < 1 || buckets > kMaxBuckets)

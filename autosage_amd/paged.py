@@ -33,8 +33,13 @@ from .ops import load_native, native_load_error
 from .position import border_array, bucket_borders, has_tangent, position_buckets
 
 E4M3 = torch.float8_e4m3fn
+E2M1 = torch.float4_e2m1fn_x2  # two numbers in a byte
+E8M0 = torch.float8_e8m0fnu
+GROUP = 32  # numbers of a row of E2M1 that share an exponent
 MAX_WIDTH = 256
-_DTYPES = {torch.float32: 0, **_native.DTYPES_16, E4M3: 3}
+_ROW_DTYPES = {torch.float32: 0, **_native.DTYPES_16}
+_DTYPES = {**_ROW_DTYPES, E4M3: 3, E2M1: 5}
+_CODED = (E4M3, E2M1)
 _INTEGERS = (torch.int32, torch.int64)
 
 
@@ -47,6 +52,16 @@ def _check_rows(name: str, t: torch.Tensor) -> None:
     _require(t.size(-1) == 1 or t.stride(-1) == 1, ValueError, f"the rows of {name} must be contiguous")
 
 
+def _width(pages: torch.Tensor) -> int:
+    """Numbers in a row."""
+    return pages.size(3) * 2 if pages.dtype is E2M1 else pages.size(3)
+
+
+def _exponent_shape(pages: torch.Tensor) -> tuple:
+    shape = tuple(pages.shape[:3])
+    return (*shape, (pages.size(3) + GROUP // 2 - 1) // (GROUP // 2)) if pages.dtype is E2M1 else shape
+
+
 # Each check asks for everything at once (a call of a few tokens is bound by the
 # host: 10 us of checks one by one, 3 together); only where something is wrong do
 # the conditions run one by one and name the first that fails.
@@ -55,39 +70,47 @@ def _check_rows(name: str, t: torch.Tensor) -> None:
 def _check_cache(key_pages, value_pages, page_ptr, page_idx, key_exponents, value_exponents) -> None:
     dtype = key_pages.dtype
     key_shape, value_shape = key_pages.shape, value_pages.shape
+    widest = MAX_WIDTH // 2 if dtype is E2M1 else MAX_WIDTH
     if (dtype in _DTYPES and value_pages.dtype is dtype and len(key_shape) == 4 and len(value_shape) == 4
             and key_shape[:3] == value_shape[:3] and key_pages.numel() > 0 and value_pages.numel() > 0
-            and 1 < key_shape[3] <= MAX_WIDTH and 1 < value_shape[3] <= MAX_WIDTH
+            and 1 < key_shape[3] <= widest and 1 < value_shape[3] <= widest
             and key_pages.stride(3) == 1 and value_pages.stride(3) == 1
             and page_ptr.dtype is torch.long and page_idx.dtype is torch.long and page_ptr.dim() == 1
             and page_idx.dim() == 1 and page_ptr.numel() >= 1
             and key_pages.get_device() == value_pages.get_device() == page_ptr.get_device() == page_idx.get_device()):
-        if dtype is not E4M3:
+        if dtype not in _CODED:
             if key_exponents is None and value_exponents is None:
                 return
-        elif (key_exponents is not None and value_exponents is not None and key_exponents.dtype is torch.int8
-                and value_exponents.dtype is torch.int8 and key_exponents.shape == key_shape[:3]
-                and value_exponents.shape == key_shape[:3]
+        elif (key_exponents is not None and value_exponents is not None
+                and key_exponents.dtype is value_exponents.dtype is (torch.int8 if dtype is E4M3 else E8M0)
+                and key_exponents.shape == _exponent_shape(key_pages)
+                and value_exponents.shape == _exponent_shape(value_pages)
+                and (dtype is E4M3 or (key_exponents.stride(3) == 1 and value_exponents.stride(3) == 1))
                 and key_exponents.get_device() == value_exponents.get_device() == key_pages.get_device()):
             return
     _require(key_pages.ndim == 4 and value_pages.ndim == 4 and key_pages.shape[:3] == value_pages.shape[:3],
              ValueError, "key_pages and value_pages must have shape [pages, heads, page_size, width]")
     _require(key_pages.dtype in _DTYPES and value_pages.dtype == key_pages.dtype, TypeError,
-             "key_pages and value_pages must both use float32, bfloat16, float16 or float8_e4m3fn")
+             "key_pages and value_pages must both use float32, bfloat16, float16, float8_e4m3fn or float4_e2m1fn_x2")
     _require(min(key_pages.shape) >= 1 and min(value_pages.shape) >= 1, ValueError,
              "a cache has at least one page, head, token and number")
-    _require(key_pages.size(3) <= MAX_WIDTH and value_pages.size(3) <= MAX_WIDTH, ValueError,
+    _require(_width(key_pages) <= MAX_WIDTH and _width(value_pages) <= MAX_WIDTH, ValueError,
              f"key and value widths must be at most {MAX_WIDTH}")
     _check_rows("key_pages", key_pages)
     _check_rows("value_pages", value_pages)
-    coded = key_pages.dtype == E4M3
-    for name, exponents in (("key_exponents", key_exponents), ("value_exponents", value_exponents)):
+    coded = key_pages.dtype in _CODED
+    for name, exponents, pages in (("key_exponents", key_exponents, key_pages),
+                                   ("value_exponents", value_exponents, value_pages)):
         _require((exponents is not None) == coded, ValueError,
-                 "key_exponents and value_exponents belong to float8_e4m3fn pages, and to no others")
+                 "key_exponents and value_exponents belong to float8_e4m3fn and float4_e2m1fn_x2 pages, and to no others")
         if coded:
-            _require(exponents.dtype == torch.int8, TypeError, f"{name} must use int8")
-            _require(exponents.shape == key_pages.shape[:3], ValueError,
-                     f"{name} must have shape [pages, heads, page_size]")
+            few = pages.dtype == E2M1
+            _require(exponents.dtype == (E8M0 if few else torch.int8), TypeError,
+                     f"{name} must use {'float8_e8m0fnu' if few else 'int8'}")
+            _require(exponents.shape == _exponent_shape(pages), ValueError,
+                     f"{name} must have shape [pages, heads, page_size" + (", width / 32 rounded up]" if few else "]"))
+            if few:
+                _check_rows(name, exponents)
             _require(exponents.device == key_pages.device, ValueError, f"{name} must be on the pages' device")
     for name, t in (("page_ptr", page_ptr), ("page_idx", page_idx)):
         _require(t.dtype in _INTEGERS, TypeError, f"{name} must use integers")
@@ -110,20 +133,20 @@ def _check_tokens(key_pages, page_ptr, token_ptr, start) -> None:
 
 
 def _check_new_rows(key, value, key_pages, value_pages) -> None:
-    if (key.dim() == 3 and value.dim() == 3 and key.dtype is value.dtype and key.dtype in _DTYPES
-            and key.dtype is not E4M3 and (key_pages.dtype is key.dtype or key_pages.dtype is E4M3)
-            and key.shape == (value.size(0), key_pages.size(1), key_pages.size(3))
-            and value.shape == (key.size(0), value_pages.size(1), value_pages.size(3))
+    if (key.dim() == 3 and value.dim() == 3 and key.dtype is value.dtype and key.dtype in _ROW_DTYPES
+            and (key_pages.dtype is key.dtype or key_pages.dtype in _CODED)
+            and key.shape == (value.size(0), key_pages.size(1), _width(key_pages))
+            and value.shape == (key.size(0), value_pages.size(1), _width(value_pages))
             and key.get_device() == value.get_device() == key_pages.get_device()):
         return
     for name, t, pages in (("key", key, key_pages), ("value", value, value_pages)):
-        _require(t.ndim == 3 and t.size(1) == pages.size(1) and t.size(2) == pages.size(3), ValueError,
+        _require(t.ndim == 3 and t.size(1) == pages.size(1) and t.size(2) == _width(pages), ValueError,
                  f"{name} must have shape [tokens, heads, width] with the heads and width of {name}_pages")
         _require(t.device == pages.device, ValueError, f"{name} must be on the cache's device")
     _require(key.size(0) == value.size(0), ValueError, "key and value must have the same number of tokens")
-    _require(key.dtype == value.dtype and key.dtype in _DTYPES and key.dtype != E4M3
-             and key_pages.dtype in (key.dtype, E4M3), TypeError,
-             "key and value must both use the dtype of the pages (float32, bfloat16 or float16 for float8_e4m3fn pages)")
+    _require(key.dtype == value.dtype and key.dtype in _ROW_DTYPES and key_pages.dtype in (key.dtype, *_CODED),
+             TypeError, "key and value must both use the dtype of the pages (float32, bfloat16 or float16 for "
+             "float8_e4m3fn and float4_e2m1fn_x2 pages)")
 
 
 def _no_gradient(name: str, *tensors) -> None:
@@ -156,16 +179,17 @@ _NO_STRIDES = (0, 0, 0)
 
 def _cache_struct(key_pages, value_pages, page_ptr, page_idx, key_exponents, value_exponents):
     pages, heads, page_size, width = key_pages.shape
+    widths = (2 * width, 2 * value_pages.size(3)) if key_pages.dtype is E2M1 else (width, value_pages.size(3))
     key_strides, value_strides = key_pages.stride(), value_pages.stride()
     if key_exponents is None:
         key_e = value_e = 0
         key_e_strides = value_e_strides = _NO_STRIDES
     else:
         key_e, value_e = key_exponents.data_ptr(), value_exponents.data_ptr()
-        key_e_strides, value_e_strides = key_exponents.stride(), value_exponents.stride()
+        key_e_strides, value_e_strides = key_exponents.stride()[:3], value_exponents.stride()[:3]
     return _CacheWords(
         key_pages.data_ptr(), value_pages.data_ptr(), key_e, value_e, page_ptr.data_ptr(), page_idx.data_ptr(),
-        page_idx.numel(), page_ptr.numel() - 1, pages, page_size, heads, width, value_pages.size(3),
+        page_idx.numel(), page_ptr.numel() - 1, pages, page_size, heads, *widths,
         *key_strides[:3], *value_strides[:3], *key_e_strides, *value_e_strides, _DTYPES[key_pages.dtype])
 
 
@@ -248,7 +272,7 @@ def _need_native() -> ctypes.CDLL:
 
 
 # ---------------------------------------------------------------------------
-# 8-bit numbers
+# 8-bit and 4-bit numbers
 
 
 def _quantise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -268,6 +292,49 @@ def _quantise(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def _values(codes: torch.Tensor, exponents: torch.Tensor) -> torch.Tensor:
     half = exponents.to(torch.int32)[..., None] // 2
     return torch.ldexp(torch.ldexp(codes.float(), half), exponents.to(torch.int32)[..., None] - half)
+
+
+def _quantise_pairs(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes, two in a byte, exponents + 127) of 4-bit numbers, as bytes: 2^e is the smallest power of two, not below
+    2^-127, that brings the largest magnitude of 32 numbers to 6; a group with a number that is not finite is held as
+    NaN (255)."""
+    width = x.size(-1)
+    x = torch.nn.functional.pad(x.float(), (0, -width % GROUP)).unflatten(-1, (-1, GROUP))
+    finite = x.isfinite().all(-1, keepdim=True)
+    x = torch.where(finite, x, 0.0)
+    mantissa, exponent = torch.frexp(x.abs().amax(-1, keepdim=True))
+    exponent = torch.where(mantissa == 0, -127, exponent - 3 + (mantissa > 0.75).to(torch.int32)).clamp_min(-127)
+    size = torch.ldexp(x.abs(), -exponent)
+    # half to the even code
+    code = ((size > 0.25).int() + (size >= 0.75) + (size > 1.25) + (size >= 1.75) + (size > 2.5) + (size >= 3.5)
+            + (size > 5.0) + 8 * x.signbit()).to(torch.uint8).flatten(-2)[..., :width]
+    return code[..., ::2] | code[..., 1::2] << 4, torch.where(finite, exponent + 127, 255).squeeze(-1).to(torch.uint8)
+
+
+def _pair_values(codes: torch.Tensor, exponents: torch.Tensor) -> torch.Tensor:
+    sizes = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device=codes.device)
+    numbers = torch.cat((sizes, -sizes))[torch.stack((codes & 15, codes >> 4), -1).flatten(-2).long()]
+    exponent = exponents.repeat_interleave(GROUP, -1)[..., :numbers.size(-1)].int()
+    return torch.where(exponent == 255, float("nan"), torch.ldexp(numbers, exponent - 127))
+
+
+def _put_rows(rows: torch.Tensor, pages: torch.Tensor, exponents: Optional[torch.Tensor], page, place) -> None:
+    if exponents is None:
+        pages[page, :, place] = rows
+        return
+    codes, scale = (_quantise_pairs if pages.dtype == E2M1 else _quantise)(rows)
+    pages.view(torch.uint8)[page, :, place] = codes.view(torch.uint8)
+    exponents.view(scale.dtype)[page, :, place] = scale
+
+
+def _held_rows(pages: torch.Tensor, exponents: Optional[torch.Tensor], *index) -> torch.Tensor:
+    """What the places of an index hold, in float32 where they are coded."""
+    if exponents is None:
+        return pages[index]
+    codes = pages.view(torch.uint8)[index]
+    if pages.dtype == E2M1:
+        return _pair_values(codes, exponents.view(torch.uint8)[index])
+    return _values(codes.view(E4M3), exponents[index])
 
 
 # ---------------------------------------------------------------------------
@@ -293,12 +360,7 @@ def paged_cache_write_impl(key, value, key_pages, value_pages, page_ptr, page_id
         at, page, place = _places(page_ptr, page_idx, token_ptr, start, tokens, key_pages.size(0),
                                   key_pages.size(2))
         for rows, pages, exponents in ((key, key_pages, key_exponents), (value, value_pages, value_exponents)):
-            if exponents is None:
-                pages[page, :, place] = rows[at]
-            else:
-                codes, scale = _quantise(rows[at])
-                pages.view(torch.uint8)[page, :, place] = codes.view(torch.uint8)
-                exponents[page, :, place] = scale
+            _put_rows(rows[at], pages, exponents, page, place)
         return
     lib = _need_native()
     key, value = _rows(key), _rows(value)
@@ -330,6 +392,14 @@ def paged_cache_write(key, value, key_pages, value_pages, page_ptr, page_idx, to
     of a type: what is 63,488 or more may be held as 65,536, which a read in
     float16 gives as infinity (and 3.3e38 as 2^128, infinite in every type).
 
+    Pages of ``torch.float4_e2m1fn_x2`` (``[pages, heads, page_size, width / 2]``, two numbers in a byte,
+    the first in its low bits; widths are even) come with exponents of ``torch.float8_e8m0fnu``,
+    ``[pages, heads, page_size, ceil(width / 32)]``, contiguous in the last dimension: one
+    power of two for each 32 neighbouring numbers of a row, the smallest that brings the largest of
+    them to 6; the numbers divided by it are rounded to 0, 1/2, 1, 3/2, 2, 3, 4 or 6, half to
+    the even code. A number is off by at most a fifth of itself, or a quarter of its group's power
+    of two where that is more. A group with a number that is not finite is NaN as a whole.
+
     A token whose place has no page is not written.  Two tokens of one call must
     not share a place (``AUTOSAGE_VALIDATE=1`` checks it, with the lists)."""
     paged_cache_write_impl(key, value, key_pages, value_pages, page_ptr, page_idx, token_ptr, start, key_exponents,
@@ -346,27 +416,24 @@ def paged_cache_read_impl(key_pages, value_pages, page_ptr, page_idx, token_ptr,
     _check_tokens(key_pages, page_ptr, token_ptr, start)
     tokens = int(tokens)
     _require(tokens >= 0, ValueError, "tokens must not be negative")
-    coded = key_pages.dtype == E4M3
+    coded = key_pages.dtype in _CODED
     if dtype is None:
         dtype = torch.bfloat16 if coded else key_pages.dtype
-    _require(dtype in _DTYPES and dtype != E4M3 and (coded or dtype == key_pages.dtype), TypeError,
-             "dtype must be the dtype of the pages (float32, bfloat16 or float16 for float8_e4m3fn pages)")
+    _require(dtype in _ROW_DTYPES and (coded or dtype == key_pages.dtype), TypeError,
+             "dtype must be the dtype of the pages (float32, bfloat16 or float16 for float8_e4m3fn and "
+             "float4_e2m1fn_x2 pages)")
     _no_gradient("paged_cache_read", key_pages, value_pages)
     page_ptr, page_idx, token_ptr, start = _long(page_ptr), _long(page_idx), _long(token_ptr), _long(start)
     _validate_call(key_pages, page_ptr, page_idx, token_ptr, start, tokens, False)
     heads, device = key_pages.size(1), key_pages.device
-    shapes = [(tokens, heads, pages.size(3)) for pages in (key_pages, value_pages)]
+    shapes = [(tokens, heads, _width(pages)) for pages in (key_pages, value_pages)]
     if tokens == 0 or page_ptr.numel() == 1 or not key_pages.is_cuda:
         out = [torch.zeros(shape, dtype=dtype, device=device) for shape in shapes]
         if tokens > 0 and page_ptr.numel() > 1:
             at, page, place = _places(page_ptr, page_idx, token_ptr, start, tokens, key_pages.size(0),
                                       key_pages.size(2))
             for rows, pages, exponents in zip(out, (key_pages, value_pages), (key_exponents, value_exponents)):
-                if coded:
-                    codes = pages.view(torch.uint8)[page, :, place].view(E4M3)
-                    rows[at] = _values(codes, exponents[page, :, place]).to(dtype)
-                else:
-                    rows[at] = pages[page, :, place]
+                rows[at] = _held_rows(pages, exponents, page, slice(None), place).to(dtype)
         return out[0], out[1]
     lib = _need_native()
     key, value = (torch.empty(shape, dtype=dtype, device=device) for shape in shapes)
@@ -400,18 +467,19 @@ def _check_attention(query, key_pages, lengths, page_ptr, window, bias_table, ma
                      bidirectional) -> None:
     heads = key_pages.size(1)
     if (bias_table is None and max_distance is None and window is None and query.dim() == 3
-            and query.size(0) == page_ptr.numel() - 1 == lengths.numel() and query.size(2) == key_pages.size(3)
-            and query.size(1) >= 1 and query.size(1) % heads == 0 and query.dtype in _DTYPES
-            and query.dtype is not E4M3 and (key_pages.dtype is query.dtype or key_pages.dtype is E4M3)
+            and query.size(0) == page_ptr.numel() - 1 == lengths.numel() and query.size(2) == _width(key_pages)
+            and query.size(1) >= 1 and query.size(1) % heads == 0 and query.dtype in _ROW_DTYPES
+            and (key_pages.dtype is query.dtype or key_pages.dtype in _CODED)
             and lengths.dtype is torch.long and lengths.dim() == 1
             and query.get_device() == lengths.get_device() == key_pages.get_device()
             and (max_length is None or max_length >= 0)):
         return
-    _require(query.ndim == 3 and query.size(0) == page_ptr.numel() - 1 and query.size(2) == key_pages.size(3)
+    _require(query.ndim == 3 and query.size(0) == page_ptr.numel() - 1 and query.size(2) == _width(key_pages)
              and query.size(1) >= 1 and query.size(1) % heads == 0, ValueError,
              "query must have shape [sequences, query heads, key width] with a multiple of the cache's heads")
-    _require(query.dtype in _DTYPES and query.dtype != E4M3 and key_pages.dtype in (query.dtype, E4M3), TypeError,
-             "query must use the dtype of the pages (float32, bfloat16 or float16 for float8_e4m3fn pages)")
+    _require(query.dtype in _ROW_DTYPES and key_pages.dtype in (query.dtype, *_CODED), TypeError,
+             "query must use the dtype of the pages (float32, bfloat16 or float16 for float8_e4m3fn and "
+             "float4_e2m1fn_x2 pages)")
     _require(query.device == key_pages.device, ValueError, "query must be on the cache's device")
     _require(lengths.dtype in _INTEGERS, TypeError, "lengths must use integers")
     _require(lengths.ndim == 1 and lengths.numel() == query.size(0), ValueError,
@@ -436,7 +504,7 @@ def _cpu_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, s
     sequences, heads_q, _ = query.shape
     heads, page_size = key_pages.size(1), key_pages.size(2)
     group = heads_q // heads
-    out = torch.zeros(sequences, heads_q, value_pages.size(3), dtype=torch.float32)
+    out = torch.zeros(sequences, heads_q, _width(value_pages), dtype=torch.float32)
     lse = torch.full((sequences, heads_q), float("-inf"))
     begins, rooms = _page_lists(page_ptr, page_idx)
     for b in range(sequences):
@@ -453,10 +521,7 @@ def _cpu_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, s
             continue
         rows = []
         for pages, exponents in ((key_pages, key_exponents), (value_pages, value_exponents)):
-            if exponents is None:
-                held = pages[mine].float()
-            else:
-                held = _values(pages.view(torch.uint8)[mine].view(E4M3), exponents[mine])
+            held = _held_rows(pages, exponents, mine).float()
             held = held.transpose(0, 1).reshape(heads, -1, held.size(-1))
             held = held[:, first - skipped * page_size:length - skipped * page_size]
             rows.append(held.repeat_interleave(group, 0))
@@ -495,7 +560,7 @@ def _attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, scale
         return out, lse if return_lse else None
     lib = _need_native()
     sequences, heads_q, _ = query.shape
-    out = torch.empty(sequences, heads_q, value_pages.size(3), dtype=query.dtype, device=query.device)
+    out = torch.empty(sequences, heads_q, _width(value_pages), dtype=query.dtype, device=query.device)
     lse = torch.empty(sequences, heads_q, dtype=torch.float32, device=query.device) if return_lse else None
     if sequences == 0:
         return out, lse

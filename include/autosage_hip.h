@@ -32,7 +32,7 @@
 extern "C" {
 #endif
 
-#define AS_ABI_VERSION 12
+#define AS_ABI_VERSION 13
 
 typedef enum as_status {
   AS_OK = 0,
@@ -48,7 +48,8 @@ enum {
   AS_DTYPE_F32 = 0,
   AS_DTYPE_BF16 = 1,
   AS_DTYPE_F16 = 2,
-  AS_DTYPE_E4M3 = 3   /* pages of a quantised key-value cache only */
+  AS_DTYPE_E4M3 = 3,  /* pages of a quantised key-value cache only */
+  AS_DTYPE_E2M1 = 5   /* the same, two numbers in a byte (4 is no type) */
 };
 
 /* Hub-row strategy for as_spmm_csr_split_f32 (no reference counterpart; the
@@ -758,12 +759,17 @@ int as_csr_position_bias_backward(const uint8_t* found, const void* grad,
  * the sequence needs so far, and page_idx more entries than page_ptr's last.
  * dtype AS_DTYPE_E4M3: 8-bit numbers with one exponent for each token and head
  * ([pages, heads, page_size], any strides); a held number is code * 2^exponent.
+ * dtype AS_DTYPE_E2M1: 4-bit numbers, two in a byte with the first in the low
+ * bits (strides in bytes, widths in numbers and even), with a byte b for each 32
+ * neighbouring numbers of a row ([pages, heads, page_size, ceil(width / 32)],
+ * contiguous in the last dimension); a held number is code * 2^(b - 127), NaN
+ * where b is 255.
  * Lists, lengths and ids are checked in the kernels: nothing outside the given
  * tensors is read or written whatever they hold. */
 typedef struct as_paged_cache {
   void* key_pages;
   void* value_pages;
-  int8_t* key_exponents;    /* NULL unless dtype is AS_DTYPE_E4M3 */
+  int8_t* key_exponents;    /* NULL unless dtype is AS_DTYPE_E4M3 or _E2M1 */
   int8_t* value_exponents;
   const int64_t* page_ptr;  /* [sequences + 1] */
   const int64_t* page_idx;  /* [page_idx_len] */
@@ -783,7 +789,7 @@ typedef struct as_paged_cache {
 
 /* Rows of new tokens into the cache.  key [tokens, heads, key_width] and value
  * [tokens, heads, value_width] of `dtype` (the cache's, or any where the cache
- * is e4m3) with strides of their first two dimensions.  Tokens token_ptr[b] ..
+ * is e4m3 or e2m1) with strides of their first two dimensions.  Tokens token_ptr[b] ..
  * token_ptr[b + 1] are those of sequence b, from its position start[b] on;
  * tokens in front of token_ptr[0], behind token_ptr[sequences] or without a
  * page leave the cache as it is.  A place that two tokens of one call are written to holds
@@ -795,7 +801,7 @@ int as_paged_cache_write(const as_paged_cache* cache, const void* key,
                          int64_t tokens, int dtype, void* stream);
 
 /* The rows of tokens as they are held, contiguous, in `dtype` (the cache's, or
- * any where the cache is e4m3; each number is rounded once).  Tokens as for
+ * any where the cache is e4m3 or e2m1; each number is rounded once).  Tokens as for
  * as_paged_cache_write; those without a sequence or a page are zeros. */
 int as_paged_cache_read(const as_paged_cache* cache, void* key, void* value,
                         const int64_t* token_ptr, const int64_t* start,
@@ -805,7 +811,7 @@ int as_paged_cache_read(const as_paged_cache* cache, void* key, void* value,
  * lengths[b] - 1, which the cache holds), over the last `window` tokens
  * (0: all).  query [sequences, heads * group, key_width] with strides of its
  * first two dimensions, out [sequences, heads * group, value_width], both of
- * `dtype` (the cache's, or any where the cache is e4m3); query head h reads key
+ * `dtype` (the cache's, or any where the cache is e4m3 or e2m1); query head h reads key
  * head h / group.  table: NULL or [buckets, heads * group] of `dtype`, added to
  * the scores by the distance to the new token.  lse: NULL or fp32 [sequences,
  * heads * group], the logarithm of the sum of the exponentials.  max_length: an
@@ -822,6 +828,48 @@ int as_paged_attention(const as_paged_cache* cache, const void* query,
                        const int32_t* borders, int both_sides,
                        int64_t max_length, int dtype, void* workspace,
                        size_t workspace_bytes, void* stream);
+
+/* Page lists that grow and shrink.  Sequence b has lengths[b] tokens in the
+ * pages table[b * table_stride + 0 ..] (room entries); change[b] < 0: its last
+ * tokens go, and pages that hold none of the others go back to the stack
+ * free_pages[0 .. *free_count) (of free_len entries), their entries becoming -1;
+ * change[b] > 0: tokens come, and the pages they need are taken from the
+ * stack's top.  All that go back go first; number k of them and number k of
+ * those taken (by sequence, then by entry) have the same place, so that a drop
+ * undoes a growth.  Sequences are served in their order while the stack holds
+ * the sum of what they need; one that is not served, or whose list has no room,
+ * keeps its length.
+ * new_lengths [sequences]; token_ptr [sequences + 1]: the sums of the positive
+ * changes; positions and slots [tokens]: of the tokens that come, their place in
+ * the sequence and page * page_size + place in the page, -1 where there is none.
+ * Nothing outside the given tensors is read or written whatever they hold. */
+int as_paged_cache_resize(int64_t* table, int64_t table_stride, int64_t room,
+                          const int64_t* lengths, const int64_t* change,
+                          int64_t* free_pages, int64_t free_len,
+                          int64_t* free_count, int64_t page_size,
+                          int64_t* new_lengths, int64_t* token_ptr,
+                          int64_t* positions, int64_t* slots,
+                          int64_t sequences, int64_t tokens, void* workspace,
+                          size_t workspace_bytes, void* stream);
+size_t as_paged_cache_resize_workspace_bytes(int64_t sequences);
+
+/* ---- Rotary positions --------------------------------------------------------
+ * No reference counterpart.
+ *
+ * Every row of query [tokens, heads, width] and key [tokens, key_heads, width]
+ * (strides of their first two dimensions; either may have no heads) has its
+ * first 2 * pairs numbers turned: pair i, (x[i], x[i + pairs]) or, interleaved,
+ * (x[2i], x[2i + 1]), by positions[token] * frequencies[i] radians (by minus
+ * that with `inverse`), times magnitude.  The rest is copied.  The results are
+ * contiguous.  Angles are reduced in 64 bits, the pairs are turned in fp32 and
+ * rounded once. */
+int as_rotary_positions(const void* query, const int64_t* query_strides,
+                        void* query_out, int64_t heads, const void* key,
+                        const int64_t* key_strides, void* key_out,
+                        int64_t key_heads, const int64_t* positions,
+                        const double* frequencies, int64_t tokens,
+                        int64_t width, int64_t pairs, int interleaved,
+                        int inverse, float magnitude, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
