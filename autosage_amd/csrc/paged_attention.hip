@@ -809,7 +809,6 @@ constexpr int64_t kSingle = 512;
 // short: 1,000 of 50 to 700 tokens 331 us, 375 with eight times the shares; 20,000
 // of up to 520, one key head, 468 and 899; 2,000 of up to 9 197 and 231.
 int64_t share_count(const as_paged_cache* c, int64_t group, int64_t window, int64_t max_length) {
-  if (c->dtype == AS_DTYPE_E2M1) return 0;
   const int64_t units = c->heads * ((group + kHeads - 1) / kHeads);
   // tokens of one sequence at most
   int64_t longest = c->page_idx_len * c->page_size;
@@ -861,10 +860,12 @@ int launch_attention(const AttentionArgs& a, const PositionMap& map, hipStream_t
   } else {
     launch_width<T, C, 256>(a, map, grid, s);
   }
-  if (const int bad = check_launch("paged_attention")) return bad;
-  if (a.shares == 0) return AS_OK;
+  return check_launch("paged_attention");
+}
+
+template <typename T>
+int launch_join(const AttentionArgs& a, float shift, hipStream_t s) {
   const int64_t rows = int64_t(a.cache.sequences) * a.cache.heads * a.group;
-  const float shift = Unit<T, C>::type::kShift;
   if (rows >= 1024) {
     paged_attention_join_kernel<T, 1>
         <<<dim3(static_cast<unsigned>((rows + kJoinWaves - 1) / kJoinWaves)), kJoinWaves * kWave, 0, s>>>(a, shift);
@@ -943,11 +944,14 @@ int as_paged_attention(const as_paged_cache* cache, const void* query, const int
   a.part_sum = reinterpret_cast<float2*>(ws + parts.sums);
   a.part_out = reinterpret_cast<float*>(ws + parts.out);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (cache->dtype == AS_DTYPE_E2M1) return launch_paged_attention_e2m1(a, map, dtype, s);
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
-    if (cache->dtype == AS_DTYPE_E4M3) return launch_attention<T, E4m3>(a, map, s);
-    return launch_attention<T, T>(a, map, s);
+    const bool coded = is_coded(cache->dtype);
+    const int bad = cache->dtype == AS_DTYPE_E2M1 ? launch_paged_attention_e2m1(a, map, dtype, s)
+                    : coded                       ? launch_attention<T, E4m3>(a, map, s)
+                                                  : launch_attention<T, T>(a, map, s);
+    if (bad != AS_OK || a.shares == 0) return bad;
+    return launch_join<T>(a, coded ? Unit<T, E4m3>::type::kShift : Unit<T, T>::type::kShift, s);
   });
 }
 

@@ -1,11 +1,30 @@
 // Attention of one new token of every sequence over pages of 4-bit numbers.
 //
-// The same sums as over other pages (paged_attention.hip); keys and values are
-// code * 2^(e - 127) with an exponent for each 32 numbers of a row.
+// The sums, shares, parts and matrix instructions are those of the other pages
+// (paged_attention.hip): the scores of 16 tokens and 16 query heads come out of the
+// first product where the second one wants the weights.  What differs is what four
+// bits make of the loads and what they take to become operands:
 //
-// One workgroup has a query head of a sequence; its four waves take turns with 64
-// tokens each.  A lane is a token for the scores, and two bytes of a row (four
-// columns) for the weighted sum, so that nothing is read twice but the queries.
+//   * a lane reads 16 bytes of a key: 32 neighbouring numbers, which share one
+//     exponent.  Products of 32 run over any order of a row's numbers, as long as the
+//     queries have it too; so the lanes of a token (g = lane / 16) take runs
+//     (j*4 + g) of 32 (16 where a row of 64 or 192 has no more for each), and step i of
+//     a run is its numbers 8i .. 8i+7.
+//   * a lane holds the columns 8n .. 8n+7 (n = lane % 16) of the values of 8 tokens, 4
+//     bytes of each.  They are brought to bf16 and turned 8 x 8 by byte permutes.
+//   * the conversion to bf16 multiplies with the exponent on the way.  A code times a
+//     power of two is a number of bf16, so that neither scores nor weights are scaled
+//     afterwards, and an exponent of NaN makes NaN.  Numbers below 2^-126 count as zeros.
+//   * queries enter in bf16 parts: one for bf16, two for fp16, three for float32, which
+//     hold all of their bits; weights in two (2^-18 of a weight), or three for float32.
+//
+// A row of 128 is 68 bytes, half of an 8-bit one, and each of its numbers costs a vector
+// instruction or so: what bounds the kernel is how many loads are on the way while they
+// run.  Hence the next tile of a wave is asked for before this one is worked on (26
+// registers), and the page ids of the one after it.
+//
+// A token's page may be any, its length may end anywhere and its pages may hold
+// anything behind it: see the other kernel.
 
 #include "paged_shares.h"
 
@@ -13,134 +32,556 @@ namespace as {
 
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ f32x4 multiply(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// Two numbers rounded to a word, and what the word holds.
+__device__ __forceinline__ uint32_t pack(float x, float y) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, bf16x2));
+}
+__device__ __forceinline__ f32x2 unpack(uint32_t w) {
+  return f32x2{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+}
+// The numbers 2i and 2i + 1 of a word of codes, times 2^(e - 127) for scale = e << 23; NaN for e = 255.
+template <int I>
+__device__ __forceinline__ uint32_t bf16_pair(uint32_t codes, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, I));
+}
+__device__ __forceinline__ float as_scale(uint32_t e) { return __uint_as_float(e << 23); }
+
+// A running maximum may stay this far below a score: weights are then at most 2^4.
+constexpr float kSlack = 4.0f * kLn2;
 __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
+// How a call reaches its rows.  kWhole: pages are a multiple of 8 tokens and rows of 32
+// numbers, so that the blocks of 8 tokens which a lane works on lie in one page each,
+// and no run passes a row's end.  kTokens: every token is looked up, and the last word
+// of a row is read where it ends with the row, and shifted.  kBytes: so it is, and words
+// are read a byte at a time, for rows of fewer than 4 bytes.
+enum Mode { kWhole, kTokens, kBytes };
+
+// Where a word (or half of one) of a row is read, and how far it is shifted then.
+struct Word {
+  int at;
+  int shift;
+};
+template <int BYTES, int MODE>
+__device__ __forceinline__ Word word_of(int at, int row_bytes) {
+  if constexpr (MODE == kWhole) return Word{at < row_bytes ? at : 0, 0};
+  if (MODE == kBytes || at >= row_bytes) return Word{at < row_bytes ? at : 0, 0};
+  const int last = row_bytes - BYTES;
+  return Word{at < last ? at : last, at < last ? 0 : 8 * (at - last)};
+}
+template <int BYTES, int MODE>
+__device__ __forceinline__ uint32_t load_word(const uint8_t* __restrict__ row, const Word& w, int row_bytes) {
+  if constexpr (MODE == kBytes) {
+    uint32_t x = 0u;
+#pragma unroll
+    for (int i = 0; i < BYTES; ++i) x |= w.at + i < row_bytes ? uint32_t(row[w.at + i]) << (8 * i) : 0u;
+    return x;
+  } else if constexpr (BYTES == 2) {
+    uint16_t x;
+    __builtin_memcpy(&x, row + w.at, 2);
+    return MODE == kWhole ? x : x >> w.shift;
+  } else {
+    uint32_t x;
+    __builtin_memcpy(&x, row + w.at, 4);
+    return MODE == kWhole ? x : x >> w.shift;
+  }
+}
+
 template <typename T>
+constexpr int kQueryParts = sizeof(T) == 4 ? 3 : (__is_same(T, Fp16) ? 2 : 1);
+template <typename T>
+constexpr int kWeightParts = sizeof(T) == 4 ? 3 : 2;
+
+constexpr int kTile = 32;  // tokens of one step of a wave
+constexpr int kOwn = 8;    // of which a lane weighs this many
+
+template <typename T, int W, int MODE>
 __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionArgs a, PositionMap map) {
+  constexpr int kKeyRun = W % 128 == 0 ? 32 : 16;  // numbers of a key in one load
+  constexpr int kKeyRuns = W / (4 * kKeyRun);
+  constexpr int kKeyWords = kKeyRun / 8;
+  constexpr int kSteps = kKeyRuns * kKeyWords;
+  constexpr int kValues = W / 16;  // columns that a lane holds
+  constexpr int kRun = kValues % 8 == 0 ? 8 : 4;  // of which neighbours
+  constexpr int kBlocks = kValues / kRun;
+  constexpr bool kShared = W > 128;  // queries in LDS: rows beyond 128 leave no registers for them
+  constexpr int kQ = kQueryParts<T>;
+  constexpr int kP = kWeightParts<T>;
+  constexpr int kOutWaves = 2;
+
   __shared__ int32_t border[kMaxBuckets + 1];
-  __shared__ float q[kMaxWidth];
-  __shared__ float wave_top[kWavesPerBlock];
-  __shared__ float wave_sum[kWavesPerBlock];
-  __shared__ float wave_out[kWavesPerBlock][kMaxWidth];
+  __shared__ ShareSums share_sums;
+  __shared__ float wave_top[kWavesPerBlock][kHeads];
+  __shared__ float wave_sum[kWavesPerBlock][kHeads];
+  __shared__ float bias[kMaxBuckets][kHeads];  // of the keys in front of the query
+  __shared__ float wave_out[kOutWaves][kHeads][W];
+  __shared__ u32x4 q_shared[kShared ? kSteps : 1][kQ][kShared ? kWave : 1];
 
   const PagedCache& c = a.cache;
-  const int heads_q = c.heads * a.group;
-  const int b = static_cast<int>(blockIdx.x / static_cast<unsigned>(heads_q));
-  const int hq = static_cast<int>(blockIdx.x) - b * heads_q;
-  const int h = hq / a.group;
   const int lane = lane_id();
+  const int n = lane & 15;
+  const int g = lane >> 4;
   const int wave = uniform_i32(wave_in_block());
-  const int key_width = c.key.width;
-  const int width = c.value.width;
+  // the heads of a share follow one another: they share its pages
+  const int units = c.heads * a.head_tiles;
+  const int share_index = static_cast<int>(blockIdx.x / static_cast<unsigned>(units));
+  const int unit = static_cast<int>(blockIdx.x) - share_index * units;
+  const int h = unit / a.head_tiles;
+  const int tile_of_heads = unit - h * a.head_tiles;
+  const int heads_q = c.heads * a.group;
+  const int head0 = h * a.group + tile_of_heads * kHeads;
+  const int heads_here = a.group - tile_of_heads * kHeads < kHeads ? a.group - tile_of_heads * kHeads : kHeads;
 
-  if (a.table != nullptr) stage_borders(border, map);
-  const T* q_row = static_cast<const T*>(a.query) + b * a.query_stride[0] + hq * a.query_stride[1];
-  for (int i = threadIdx.x; i < kMaxWidth; i += kBlock) q[i] = i < key_width ? Elem<T>::at(q_row, i) : 0.0f;
-  __syncthreads();
+  if (a.table != nullptr) {
+    stage_borders(border, map);
+    for (int i = threadIdx.x; i < map.side * kHeads; i += kBlock) {
+      const int hh = i % kHeads < heads_here ? i % kHeads : 0;
+      bias[i / kHeads][i % kHeads] =
+          Elem<T>::at(static_cast<const T*>(a.table), static_cast<int64_t>(i / kHeads) * heads_q + head0 + hh);
+    }
+  }
+  Share share{0, 1, 1, 0, share_index};
+  if (a.shares > 0) {
+    share = share_of(a, share_index, share_sums);
+    if (share.first >= share.end) return;
+  } else if (a.table != nullptr) {
+    __syncthreads();
+  }
 
-  const PageList list = page_list(c, b);
-  const Seen seen = seen_tokens(a, b, list);
-  const int64_t* pages = c.page_idx + list.begin;
   const uint8_t* key_base = static_cast<const uint8_t*>(c.key.data) + h * c.key.stride[1];
   const uint8_t* value_base = static_cast<const uint8_t*>(c.value.data) + h * c.value.stride[1];
-  const uint8_t* key_e = reinterpret_cast<const uint8_t*>(c.key.exponents) + h * c.key.exponent_stride[1];
-  const uint8_t* value_e = reinterpret_cast<const uint8_t*>(c.value.exponents) + h * c.value.exponent_stride[1];
-
-  float top = -INFINITY;
-  float sum = 0.0f;
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // columns 2 * lane, 2 * lane + 1, and those 128 further
-  for (int t0 = seen.begin + wave * kWave; t0 < seen.end; t0 += kWavesPerBlock * kWave) {
-    const int t = t0 + lane;
-    const bool in_sight = t < seen.end;
-    const int at = in_sight ? t : seen.end - 1;
-    const int entry = page_of_token(a, at);
-    const int64_t slot = at - entry * c.page_size;
-    const int64_t id = pages[entry];
-    const bool bad = id < 0 || id >= c.pages;
-    const int64_t page = bad ? 0 : id;
-    const uint8_t* row = key_base + page * c.key.stride[0] + slot * c.key.stride[2];
-    const uint8_t* row_e = key_e + page * c.key.exponent_stride[0] + slot * c.key.exponent_stride[2];
-    float score = 0.0f;
-    for (int d0 = 0; d0 < key_width; d0 += kGroup) {
-      const int d1 = d0 + kGroup < key_width ? d0 + kGroup : key_width;
-      float part = 0.0f;
-      for (int d = d0; d < d1; d += 2) {
-        float x[8];
-        pairs_to_floats(row[d / 2], x);
-        part = fmaf(x[0], q[d], part);
-        part = fmaf(x[1], q[d + 1], part);
-      }
-      score = fmaf(part, group_scale(row_e[d0 / kGroup]), score);
+  const uint8_t* key_e_base = reinterpret_cast<const uint8_t*>(c.key.exponents) + h * c.key.exponent_stride[1];
+  const uint8_t* value_e_base = reinterpret_cast<const uint8_t*>(c.value.exponents) + h * c.value.exponent_stride[1];
+  const int key_bytes = c.key.width / 2;
+  const int value_bytes = c.value.width / 2;
+  // tokens of this lane: the first of those it loads keys of (the other is 4 further), and of those it weighs
+  const int key_token = (n >> 2) * 8 + (n & 3);
+  const int own_token = g * kOwn;
+  // Words of a key and of a value, and their exponents.  A lane behind a row's end reads its beginning (or the last
+  // group's exponent): it has zeros on the queries' side, and columns that nobody asks for on the values'.
+  Word key_word[MODE == kWhole ? kKeyRuns : kSteps];
+  int key_e_at[kKeyRuns];
+#pragma unroll
+  for (int j = 0; j < kKeyRuns; ++j) {
+    const int d = (j * 4 + g) * kKeyRun;
+    key_e_at[j] = d < c.key.width ? d / kGroup : 0;
+    if constexpr (MODE == kWhole) {
+      key_word[j] = word_of<4, MODE>(d / 2, key_bytes);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kKeyWords; ++i) key_word[j * kKeyWords + i] = word_of<4, MODE>(d / 2 + 4 * i, key_bytes);
     }
-    score *= a.scale;
-    if (a.table != nullptr)
-      score += Elem<T>::at(static_cast<const T*>(a.table),
-                           static_cast<int64_t>(bucket_of_distance(border, map, seen.end - 1 - at)) * heads_q + hq);
-    if (bad) score = NAN;
-    if (!in_sight) score = -INFINITY;
-    const float next = fmaxf(top, wave_max_f32(score));
-    const float from = next == -INFINITY ? 0.0f : next;
-    const float keep = top == -INFINITY ? 0.0f : exp_of(top - from);
-    top = next;
-    const float weight = exp_of(score - from);
-    sum = sum * keep + weight;
+  }
+  Word value_word[kBlocks];
+  int value_e_at[kBlocks];
 #pragma unroll
-    for (float& x : acc) x *= keep;
-    const int count = seen.end - t0 < kWave ? seen.end - t0 : kWave;
-    for (int i = 0; i < count; ++i) {
-      const float w = bcast_f32(weight, i);
-      const int64_t p = __shfl(page, i, kWave);
-      const int64_t s = __shfl(slot, i, kWave);
-      const uint8_t* from_row = value_base + p * c.value.stride[0] + s * c.value.stride[2];
-      const uint8_t* from_e = value_e + p * c.value.exponent_stride[0] + s * c.value.exponent_stride[2];
+  for (int j = 0; j < kBlocks; ++j) {
+    const int d = (j * 16 + n) * kRun;
+    value_word[j] = word_of<kRun / 2, MODE>(d / 2, value_bytes);
+    value_e_at[j] = d < c.value.width ? d / kGroup : 0;
+  }
+
+  int64_t at = share.at;
+  for (int b = uniform_i32(share.b); b < c.sequences && at < share.end; ++b) {
+    const PageList list = page_list(c, b);
+    const Seen seen = seen_tokens(a, b, list);
+    const int pieces = a.shares > 0 ? piece_count(a, seen) : 1;
+    // pieces from .. to - 1 of this sequence are in the share
+    const int from_piece = share.first > at ? static_cast<int>(share.first - at) : 0;
+    const int to_piece = share.end < at + pieces ? static_cast<int>(share.end - at) : pieces;
+    const bool whole = from_piece == 0 && to_piece == pieces;
+    const int64_t part = static_cast<int64_t>(share_index) + b;
+    if (a.shares > 0 && unit == 0 && from_piece == 0 && threadIdx.x == 0)
+      a.plan[b] = make_int2(static_cast<int>(part),
+                            static_cast<int>((at + pieces - 1) / share.size - at / share.size) + 1);
+    at += pieces;
+    const int origin = first_token(a, seen);
+    const int base = origin + from_piece * kPiece;
+    const int begin = base > seen.begin ? base : seen.begin;
+    const int stop = a.shares > 0 ? origin + to_piece * kPiece : seen.end;
+    const int end = stop < seen.end ? stop : seen.end;
+    const int64_t* pages = c.page_idx + list.begin;
+
+    // the queries as operand B: step j*kKeyWords + i has the numbers 8i .. of run j
+    u32x4 q_own[kShared ? 1 : kSteps][kQ];
+    const auto q_of = [&](int j, int p) { return kShared ? q_shared[j][p][lane] : q_own[kShared ? 0 : j][p]; };
+    {
+      const int head = n < heads_here ? n : 0;
+      const T* q_row = static_cast<const T*>(a.query) + b * a.query_stride[0] + (head0 + head) * a.query_stride[1];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int d = 2 * lane + 128 * k;
-        if (d < width) {
-          float x[8];
-          pairs_to_floats(from_row[d / 2], x);
-          const float scale = group_scale(from_e[d / kGroup]);
-          acc[2 * k] = fmaf(w, x[0] * scale, acc[2 * k]);
-          acc[2 * k + 1] = fmaf(w, x[1] * scale, acc[2 * k + 1]);
+      for (int j = 0; j < kSteps; ++j) {
+        const int d0 = (j / kKeyWords * 4 + g) * kKeyRun + j % kKeyWords * 8;
+        float q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int d = d0 + i;
+          const float x = Elem<T>::at(q_row, d < c.key.width ? d : 0);
+          q[i] = d < c.key.width && n < heads_here ? x : 0.0f;
+        }
+#pragma unroll
+        for (int p = 0; p < kQ; ++p) {
+          u32x4 words;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            words[i] = pack(q[2 * i], q[2 * i + 1]);
+            // what the next part holds; nothing is left of an infinite number
+            const f32x2 held = unpack(words[i]);
+            q[2 * i] = finite(held[0]) ? q[2 * i] - held[0] : 0.0f;
+            q[2 * i + 1] = finite(held[1]) ? q[2 * i + 1] - held[1] : 0.0f;
+          }
+          if constexpr (!kShared) {
+            q_own[j][p] = words;
+          } else if (wave == 0) {
+            q_shared[j][p][lane] = words;
+          }
         }
       }
+      if constexpr (kShared) __syncthreads();
     }
-  }
-  sum = wave_sum_f32(sum);
-  if (lane == 0) {
-    wave_top[wave] = top;
-    wave_sum[wave] = sum;
-  }
+    f32x4 acc[kValues];
+    float top;  // of head n, the same in its four lanes
+    float sum;  // of head n and the tokens of this lane
+
+    // What a tile needs from memory.
+    struct Tile {
+      uint32_t key[2][kSteps];
+      uint32_t key_e[2][kKeyRuns];
+      uint32_t value[kBlocks][kOwn];
+      uint32_t value_e[kBlocks][kOwn];
+      uint32_t bad_tokens;  // tokens whose page is outside the cache, a bit each
+    };
+    struct Ids {
+      int64_t key[MODE == kWhole ? 1 : 2];
+      int64_t own[MODE == kWhole ? 1 : kOwn];
+    };
+    const auto is_bad = [&](int64_t id) { return id < 0 || id >= c.pages; };
+    // Blocks (or tokens) behind what is seen stand for the last one: their loads need no guard.
+    const int last = (end - 1) & ~7;
+    const auto block_of = [&](int t) { return (t & ~7) < last ? t & ~7 : last; };
+    const auto seen_token = [&](int t) { return t < end ? t : end - 1; };
+    const auto ids_of = [&](int t0) {
+      Ids ids;
+      if constexpr (MODE == kWhole) {
+        ids.key[0] = pages[page_of_token(a, block_of(t0 + key_token))];
+        ids.own[0] = pages[page_of_token(a, block_of(t0 + own_token))];
+      } else {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) wave_out[wave][2 * lane + 128 * (k / 2) + k % 2] = acc[k];
-  __syncthreads();
-  float most = wave_top[0];
+        for (int s = 0; s < 2; ++s) ids.key[s] = pages[page_of_token(a, seen_token(t0 + key_token + s * 4))];
 #pragma unroll
-  for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_top[w]);
-  const int d = threadIdx.x;
-  if (d >= width) return;
-  float total = 0.0f;
-  float x = 0.0f;
+        for (int e = 0; e < kOwn; ++e) ids.own[e] = pages[page_of_token(a, seen_token(t0 + own_token + e))];
+      }
+      return ids;
+    };
+    const auto load_key = [&](Tile& tile, int s, const uint8_t* row, const uint8_t* row_e) {
 #pragma unroll
-  for (int w = 0; w < kWavesPerBlock; ++w) {
-    const float f = wave_top[w] == -INFINITY ? 0.0f : exp_of(wave_top[w] - most);
-    total = fmaf(f, wave_sum[w], total);
-    x = fmaf(f, wave_out[w][d], x);
+      for (int j = 0; j < kKeyRuns; ++j) {
+        if constexpr (MODE == kWhole) {
+          __builtin_memcpy(&tile.key[s][j * kKeyWords], row + key_word[j].at, 4 * kKeyWords);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kKeyWords; ++i)
+            tile.key[s][j * kKeyWords + i] = load_word<4, MODE>(row, key_word[j * kKeyWords + i], key_bytes);
+        }
+        tile.key_e[s][j] = row_e[key_e_at[j]];
+      }
+    };
+    const auto load_value = [&](Tile& tile, int e, const uint8_t* row, const uint8_t* row_e) {
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) {
+        tile.value[j][e] = load_word<kRun / 2, MODE>(row, value_word[j], value_bytes);
+        tile.value_e[j][e] = row_e[value_e_at[j]];
+      }
+    };
+    const auto load_tile = [&](Tile& tile, int t0, const Ids& ids) {
+      if constexpr (MODE == kWhole) {
+        int t = block_of(t0 + key_token);
+        int slot = t - page_of_token(a, t) * c.page_size + (key_token & 7);
+        int64_t page = is_bad(ids.key[0]) ? 0 : ids.key[0];
+        const uint8_t* row = key_base + page * c.key.stride[0] + slot * c.key.stride[2];
+        const uint8_t* row_e = key_e_base + page * c.key.exponent_stride[0] + slot * c.key.exponent_stride[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+          load_key(tile, s, row + s * 4 * c.key.stride[2], row_e + s * 4 * c.key.exponent_stride[2]);
+        t = block_of(t0 + own_token);
+        slot = t - page_of_token(a, t) * c.page_size;
+        const bool bad = is_bad(ids.own[0]);
+        page = bad ? 0 : ids.own[0];
+        tile.bad_tokens = bad ? 0xffu : 0u;
+        row = value_base + page * c.value.stride[0] + slot * c.value.stride[2];
+        row_e = value_e_base + page * c.value.exponent_stride[0] + slot * c.value.exponent_stride[2];
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e)
+          load_value(tile, e, row + e * c.value.stride[2], row_e + e * c.value.exponent_stride[2]);
+      } else {
+        const auto slot_of = [&](int t) {
+          t = seen_token(t);
+          return t - page_of_token(a, t) * c.page_size;
+        };
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int64_t page = is_bad(ids.key[s]) ? 0 : ids.key[s];
+          const int slot = slot_of(t0 + key_token + s * 4);
+          load_key(tile, s, key_base + page * c.key.stride[0] + slot * c.key.stride[2],
+                   key_e_base + page * c.key.exponent_stride[0] + slot * c.key.exponent_stride[2]);
+        }
+        tile.bad_tokens = 0;
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) {
+          const bool bad = is_bad(ids.own[e]);
+          const int64_t page = bad ? 0 : ids.own[e];
+          const int slot = slot_of(t0 + own_token + e);
+          if (bad) tile.bad_tokens |= 1u << e;
+          load_value(tile, e, value_base + page * c.value.stride[0] + slot * c.value.stride[2],
+                     value_e_base + page * c.value.exponent_stride[0] + slot * c.value.exponent_stride[2]);
+        }
+      }
+    };
+
+    const auto work_on = [&](Tile& tile, int t0) {
+      f32x4 score[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        score[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+          const uint32_t w = tile.key[s][j];
+          const float scale = as_scale(tile.key_e[s][j / kKeyWords]);
+          const u32x4 k{bf16_pair<0>(w, scale), bf16_pair<1>(w, scale), bf16_pair<2>(w, scale), bf16_pair<3>(w, scale)};
+#pragma unroll
+          for (int p = 0; p < kQ; ++p) score[s] = multiply(k, q_of(j, p), score[s]);
+        }
+      }
+
+      float scores[kOwn];
+      float most = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < kOwn; ++e) scores[e] = score[e / 4][e % 4] * a.scale;
+      if (a.table != nullptr) {
+        // every token of the tile farther than the last border: one number a head
+        if (seen.end - t0 - kTile >= border[map.side - 1]) {
+          const float far = bias[map.side - 1][n];
+#pragma unroll
+          for (int e = 0; e < kOwn; ++e) scores[e] += far;
+        } else {
+#pragma unroll
+          for (int e = 0; e < kOwn; ++e) {
+            const int away = seen.end - 1 - (t0 + own_token + e);
+            scores[e] += bias[bucket_of_distance(border, map, away < 0 ? 0 : away)][n];
+          }
+        }
+      }
+      if (t0 < begin || t0 + kTile > end || __any(tile.bad_tokens != 0)) {
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) {
+          const int t = t0 + own_token + e;
+          const bool out_of_sight = t < begin || t >= end;
+          if ((tile.bad_tokens >> e) & 1) scores[e] = NAN;
+          if (out_of_sight) scores[e] = -INFINITY;
+          // a value out of sight may be anything; its weight is zero, and so has to be the product
+#pragma unroll
+          for (int j = 0; j < kBlocks; ++j) {
+            tile.value[j][e] = out_of_sight ? 0u : tile.value[j][e];
+            tile.value_e[j][e] = out_of_sight ? 127u : tile.value_e[j][e];
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kOwn; ++e) most = fmaxf(most, scores[e]);
+
+      if (__any(most > top + kSlack)) {
+        most = fmaxf(most, __shfl_xor(most, 16, 64));
+        most = fmaxf(most, __shfl_xor(most, 32, 64));
+        const float next = fmaxf(top, most);
+        const float keep = top == -INFINITY ? 0.0f : exp_of(top - next);
+        top = next;
+        sum *= keep;
+        // lane (n, g) holds the heads g*4 .. g*4+3 of its columns
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float f = __shfl(keep, g * 4 + i, 64);
+#pragma unroll
+          for (int j = 0; j < kValues; ++j) acc[j][i] *= f;
+        }
+      }
+      const float from = top == -INFINITY ? 0.0f : top;
+      float weight[kOwn];
+#pragma unroll
+      for (int e = 0; e < kOwn; ++e) {
+        weight[e] = exp_of(scores[e] - from);
+        sum += weight[e];
+      }
+      u32x4 w16[kP];
+#pragma unroll
+      for (int p = 0; p < kP; ++p) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = pack(weight[2 * i], weight[2 * i + 1]);
+          w16[p][i] = w;
+          weight[2 * i] -= unpack(w)[0];
+          weight[2 * i + 1] -= unpack(w)[1];
+        }
+      }
+
+#pragma unroll
+      for (int jb = 0; jb < kBlocks; ++jb) {
+        uint32_t words[kOwn][kRun / 2];
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) {
+          const uint32_t w = tile.value[jb][e];
+          const float scale = as_scale(tile.value_e[jb][e]);
+          words[e][0] = bf16_pair<0>(w, scale);
+          words[e][1] = bf16_pair<1>(w, scale);
+          if constexpr (kRun == 8) {
+            words[e][2] = bf16_pair<2>(w, scale);
+            words[e][3] = bf16_pair<3>(w, scale);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          u32x4 column;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            column[i] = __builtin_amdgcn_perm(words[2 * i + 1][j / 2], words[2 * i][j / 2],
+                                              j % 2 == 0 ? 0x05040100u : 0x07060302u);
+#pragma unroll
+          for (int p = 0; p < kP; ++p) acc[jb * kRun + j] = multiply(w16[p], column, acc[jb * kRun + j]);
+        }
+      }
+    };
+
+    constexpr int kStride = kWavesPerBlock * kTile;
+#pragma unroll
+    for (int j = 0; j < kValues; ++j) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    top = -INFINITY;
+    sum = 0.0f;
+    int t0 = base + wave * kTile;
+    if (t0 < end) {
+      // a tile ahead, in two sets of registers that take turns
+      Tile one;
+      Tile two;
+      Ids ids = ids_of(t0);
+      load_tile(one, t0, ids);
+      ids = ids_of(t0 + kStride);
+      for (;;) {
+        // the queries in LDS are read for every tile: kept, they would take the registers they are spared
+        if constexpr (kShared) asm volatile("" ::: "memory");
+        load_tile(two, t0 + kStride, ids);
+        ids = ids_of(t0 + 2 * kStride);
+        work_on(one, t0);
+        t0 += kStride;
+        if (t0 >= end) break;
+        if constexpr (kShared) asm volatile("" ::: "memory");
+        load_tile(one, t0 + kStride, ids);
+        ids = ids_of(t0 + 2 * kStride);
+        work_on(two, t0);
+        t0 += kStride;
+        if (t0 >= end) break;
+      }
+    }
+
+    // join the waves
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (g == 0) {
+      wave_top[wave][n] = top;
+      wave_sum[wave][n] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int hh = g * 4 + i;
+      float most = wave_top[0][hh];
+#pragma unroll
+      for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_top[w][hh]);
+      const float mine = wave_top[wave][hh];
+      const float f = mine == -INFINITY ? 0.0f : exp_of(mine - most);
+#pragma unroll
+      for (int j = 0; j < kValues; ++j) acc[j][i] *= f;
+    }
+    const auto each_out = [&](auto&& f) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < kValues; ++j)
+          acc[j][i] = f(wave_out[wave % kOutWaves][g * 4 + i][(j / kRun * 16 + n) * kRun + j % kRun], acc[j][i]);
+      }
+    };
+    // two waves hand their sums to the other two
+    const auto put = [](float& to, float x) { return to = x; };
+    if (wave >= kOutWaves) each_out(put);
+    __syncthreads();
+    if (wave < kOutWaves) {
+      each_out([](float& to, float x) { return x + to; });
+      each_out(put);
+    }
+    __syncthreads();
+    const int width = c.value.width;
+    for (int i = threadIdx.x; i < heads_here * width; i += kBlock) {
+      const int hh = i / width;
+      const int d = i - hh * width;
+      float most = wave_top[0][hh];
+#pragma unroll
+      for (int w = 1; w < kWavesPerBlock; ++w) most = fmaxf(most, wave_top[w][hh]);
+      float total = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWavesPerBlock; ++w) {
+        const float mine = wave_top[w][hh];
+        total += (mine == -INFINITY ? 0.0f : exp_of(mine - most)) * wave_sum[w][hh];
+      }
+      const float x = wave_out[0][hh][d] + wave_out[1][hh][d];
+      if (whole) {
+        const int64_t row = static_cast<int64_t>(b) * heads_q + head0 + hh;
+        const bool none = total == 0.0f;
+        static_cast<T*>(a.out)[row * width + d] = rounded<T>(seen.bad ? NAN : (none ? 0.0f : x / total));
+        if (a.lse != nullptr && d == 0)
+          a.lse[row] = seen.bad ? NAN : (none ? -INFINITY : fmaf(__builtin_amdgcn_logf(total), kLn2, most));
+      } else {
+        const int64_t row = part * heads_q + head0 + hh;
+        a.part_out[row * width + d] = x;
+        if (d == 0) a.part_sum[row] = make_float2(most, total);
+      }
+    }
+    __syncthreads();  // the next part's results go where these were
   }
-  const bool none = total == 0.0f;
-  static_cast<T*>(a.out)[static_cast<int64_t>(blockIdx.x) * width + d] =
-      rounded<T>(seen.bad ? NAN : (none ? 0.0f : x / total));
-  if (a.lse != nullptr && d == 0)
-    a.lse[blockIdx.x] = seen.bad ? NAN : (none ? -INFINITY : fmaf(__builtin_amdgcn_logf(total), kLn2, most));
+}
+
+template <typename T, int W>
+void launch_width(const AttentionArgs& a, const PositionMap& map, dim3 grid, hipStream_t s) {
+  const PagedCache& c = a.cache;
+  if (c.key.width < 8 || c.value.width < 8) {
+    paged_attention_e2m1_kernel<T, W, kBytes><<<grid, kBlock, 0, s>>>(a, map);
+  } else if (c.page_size % 8 == 0 && c.key.width % kGroup == 0 && c.value.width % kGroup == 0) {
+    paged_attention_e2m1_kernel<T, W, kWhole><<<grid, kBlock, 0, s>>>(a, map);
+  } else {
+    paged_attention_e2m1_kernel<T, W, kTokens><<<grid, kBlock, 0, s>>>(a, map);
+  }
 }
 
 }  // namespace
 
 int launch_paged_attention_e2m1(const AttentionArgs& a, const PositionMap& map, int dtype, hipStream_t s) {
+  const int width = a.cache.key.width > a.cache.value.width ? a.cache.key.width : a.cache.value.width;
+  const dim3 grid(static_cast<unsigned>((a.shares > 0 ? a.shares : a.cache.sequences) * a.cache.heads * a.head_tiles));
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
-    const dim3 grid(static_cast<unsigned>(a.cache.sequences * a.cache.heads * a.group));
-    paged_attention_e2m1_kernel<T><<<grid, kBlock, 0, s>>>(a, map);
+    if (width <= 64) {
+      launch_width<T, 64>(a, map, grid, s);
+    } else if (width <= 128) {
+      launch_width<T, 128>(a, map, grid, s);
+    } else if (width <= 192) {
+      launch_width<T, 192>(a, map, grid, s);
+    } else {
+      launch_width<T, 256>(a, map, grid, s);
+    }
     return check_launch("paged_attention");
   });
 }

@@ -28,8 +28,8 @@ struct AttentionArgs {
   float* part_out;    // [parts, heads * group, value width]
 };
 
-// Attention over pages of 4-bit numbers (paged_attention4.hip), and the join of
-// the parts that its shares leave (paged_attention.hip); dtype: of the queries.
+// Attention over pages of 4-bit numbers (paged_attention4.hip), without the join of
+// the parts that its shares leave; dtype: of the queries.
 int launch_paged_attention_e2m1(const AttentionArgs& a, const PositionMap& map, int dtype, hipStream_t s);
 
 namespace {
