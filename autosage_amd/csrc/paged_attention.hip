@@ -808,14 +808,17 @@ constexpr int64_t kSingle = 512;
 // heads, bf16: 5.5 TB/s; 5.1 in three rounds), also where sequences are many and
 // short: 1,000 of 50 to 700 tokens 331 us, 375 with eight times the shares; 20,000
 // of up to 520, one key head, 468 and 899; 2,000 of up to 9 197 and 231.
-int64_t share_count(const as_paged_cache* c, int64_t group, int64_t window, int64_t max_length) {
+// (4-bit pages: three workgroups of some kernels.)  dtype: of the queries, < 0 where it is not known yet.
+int64_t share_count(const as_paged_cache* c, const PagedCache& laid_out, int64_t group, int64_t window,
+                    int64_t max_length, int dtype) {
   const int64_t units = c->heads * ((group + kHeads - 1) / kHeads);
   // tokens of one sequence at most
   int64_t longest = c->page_idx_len * c->page_size;
   if (max_length >= 0 && max_length < longest) longest = max_length;
   if (window > 0 && window < longest) longest = window;
   if (longest <= kSingle) return 0;
-  return 512 / units < 1 ? 1 : 512 / units;
+  const int64_t all = c->dtype == AS_DTYPE_E2M1 ? paged_shares_e2m1(laid_out, dtype) : 512;
+  return all / units < 1 ? 1 : all / units;
 }
 
 struct Workspace {
@@ -888,7 +891,7 @@ size_t as_paged_attention_workspace_bytes(const as_paged_cache* cache, int64_t g
                                           int64_t max_length) {
   PagedCache c;
   if (read_paged_cache(cache, &c) != AS_OK || group < 1 || group > 65535 / c.heads) return 0;
-  return workspace_of(cache, group, share_count(cache, group, window, max_length)).bytes;
+  return workspace_of(cache, group, share_count(cache, c, group, window, max_length, -1)).bytes;
 }
 
 int as_paged_attention(const as_paged_cache* cache, const void* query, const int64_t* query_strides, void* out,
@@ -909,7 +912,7 @@ int as_paged_attention(const as_paged_cache* cache, const void* query, const int
   if (table != nullptr) {
     if (const int bad = fill_position_map(&map, borders, buckets, both_sides)) return bad;
   }
-  const int64_t shares = share_count(cache, group, window, max_length);
+  const int64_t shares = share_count(cache, a.cache, group, window, max_length, dtype);
   const Workspace parts = workspace_of(cache, group, shares);
   if (workspace_bytes < parts.bytes || (parts.bytes > 0 && workspace == nullptr))
     return fail(AS_ERR_WORKSPACE, "paged attention needs %zu workspace bytes", parts.bytes);

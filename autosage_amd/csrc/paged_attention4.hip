@@ -61,10 +61,13 @@ __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f
 
 // How a call reaches its rows.  kWhole: pages are a multiple of 8 tokens and rows of 32
 // numbers, so that the blocks of 8 tokens which a lane works on lie in one page each,
-// and no run passes a row's end.  kTokens: every token is looked up, and the last word
+// and no run passes a row's end.  kDense: besides, rows fill the kernel's width and the
+// tokens of a head follow one another, so that the rows of a block are constants
+// apart.  kTokens: every token is looked up, and the last word
 // of a row is read where it ends with the row, and shifted.  kBytes: so it is, and words
 // are read a byte at a time, for rows of fewer than 4 bytes.
-enum Mode { kWhole, kTokens, kBytes };
+enum Mode { kDense, kWhole, kTokens, kBytes };
+constexpr bool in_blocks(int mode) { return mode == kDense || mode == kWhole; }
 
 // Where a word (or half of one) of a row is read, and how far it is shifted then.
 struct Word {
@@ -73,6 +76,7 @@ struct Word {
 };
 template <int BYTES, int MODE>
 __device__ __forceinline__ Word word_of(int at, int row_bytes) {
+  if constexpr (MODE == kDense) return Word{at, 0};
   if constexpr (MODE == kWhole) return Word{at < row_bytes ? at : 0, 0};
   if (MODE == kBytes || at >= row_bytes) return Word{at < row_bytes ? at : 0, 0};
   const int last = row_bytes - BYTES;
@@ -88,24 +92,35 @@ __device__ __forceinline__ uint32_t load_word(const uint8_t* __restrict__ row, c
   } else if constexpr (BYTES == 2) {
     uint16_t x;
     __builtin_memcpy(&x, row + w.at, 2);
-    return MODE == kWhole ? x : x >> w.shift;
+    return in_blocks(MODE) ? x : x >> w.shift;
   } else {
     uint32_t x;
     __builtin_memcpy(&x, row + w.at, 4);
-    return MODE == kWhole ? x : x >> w.shift;
+    return in_blocks(MODE) ? x : x >> w.shift;
   }
 }
 
+template <int I>
+struct Constant {
+  static constexpr int value = I;
+};
 template <typename T>
 constexpr int kQueryParts = sizeof(T) == 4 ? 3 : (__is_same(T, Fp16) ? 2 : 1);
 template <typename T>
 constexpr int kWeightParts = sizeof(T) == 4 ? 3 : 2;
 
+// Workgroups of a CU: three where rows are dense and a wave needs at most 168 registers (paged_shares_e2m1 deals the
+// work out to as many).  64 sequences of up to 8,192 tokens, 8 key heads of 128, bf16: 76 us with three, 80 with two, 90
+// with four (which spill); 20 of up to 4,000 in float32 33 and 30, rows of 256 43 and 28.
+template <typename T, int W, int MODE>
+constexpr int kWavesPerSimd = MODE == kDense && (W == 64 || (W == 128 && sizeof(T) == 2)) ? 3 : (MODE == kBytes ? 1 : 2);
+
 constexpr int kTile = 32;  // tokens of one step of a wave
 constexpr int kOwn = 8;    // of which a lane weighs this many
 
-template <typename T, int W, int MODE>
-__global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionArgs a, PositionMap map) {
+// BIASED: with a table, or without one all the same.
+template <typename T, int W, int MODE, bool BIASED>
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPerSimd<T, W, MODE>))) void paged_attention_e2m1_kernel(AttentionArgs a, PositionMap map) {
   constexpr int kKeyRun = W % 128 == 0 ? 32 : 16;  // numbers of a key in one load
   constexpr int kKeyRuns = W / (4 * kKeyRun);
   constexpr int kKeyWords = kKeyRun / 8;
@@ -118,11 +133,11 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
   constexpr int kP = kWeightParts<T>;
   constexpr int kOutWaves = 2;
 
-  __shared__ int32_t border[kMaxBuckets + 1];
+  __shared__ int32_t border[BIASED ? kMaxBuckets + 1 : 1];
   __shared__ ShareSums share_sums;
   __shared__ float wave_top[kWavesPerBlock][kHeads];
   __shared__ float wave_sum[kWavesPerBlock][kHeads];
-  __shared__ float bias[kMaxBuckets][kHeads];  // of the keys in front of the query
+  __shared__ float bias[BIASED ? kMaxBuckets : 1][kHeads];  // of the keys in front of the query
   __shared__ float wave_out[kOutWaves][kHeads][W];
   __shared__ u32x4 q_shared[kShared ? kSteps : 1][kQ][kShared ? kWave : 1];
 
@@ -141,7 +156,8 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
   const int head0 = h * a.group + tile_of_heads * kHeads;
   const int heads_here = a.group - tile_of_heads * kHeads < kHeads ? a.group - tile_of_heads * kHeads : kHeads;
 
-  if (a.table != nullptr) {
+  const bool biased = BIASED && a.table != nullptr;
+  if (biased) {
     stage_borders(border, map);
     for (int i = threadIdx.x; i < map.side * kHeads; i += kBlock) {
       const int hh = i % kHeads < heads_here ? i % kHeads : 0;
@@ -153,14 +169,28 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
   if (a.shares > 0) {
     share = share_of(a, share_index, share_sums);
     if (share.first >= share.end) return;
-  } else if (a.table != nullptr) {
+  } else if (biased) {
     __syncthreads();
   }
 
+  // the queries have the scale's sign, or are multiplied with it where it is zero
+  const float scale = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+  const float q_sign = a.scale == 0.0f ? 0.0f : copysignf(1.0f, a.scale);
+  const float left = biased ? 1.0f : scale;  // what scores are still to be multiplied with
   const uint8_t* key_base = static_cast<const uint8_t*>(c.key.data) + h * c.key.stride[1];
   const uint8_t* value_base = static_cast<const uint8_t*>(c.value.data) + h * c.value.stride[1];
   const uint8_t* key_e_base = reinterpret_cast<const uint8_t*>(c.key.exponents) + h * c.key.exponent_stride[1];
   const uint8_t* value_e_base = reinterpret_cast<const uint8_t*>(c.value.exponents) + h * c.value.exponent_stride[1];
+  // from a token to the next, and (by the page's number) to a page
+  const int64_t key_step = MODE == kDense ? W / 2 : c.key.stride[2];
+  const int64_t value_step = MODE == kDense ? W / 2 : c.value.stride[2];
+  const int64_t key_e_step = MODE == kDense ? W / kGroup : c.key.exponent_stride[2];
+  const int64_t value_e_step = MODE == kDense ? W / kGroup : c.value.exponent_stride[2];
+  const auto page_offset = [](int64_t page, int64_t stride) {
+    return MODE == kDense ? static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(page)) *
+                                                 static_cast<uint32_t>(stride))
+                          : page * stride;
+  };
   const int key_bytes = c.key.width / 2;
   const int value_bytes = c.value.width / 2;
   // tokens of this lane: the first of those it loads keys of (the other is 4 further), and of those it weighs
@@ -168,13 +198,13 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
   const int own_token = g * kOwn;
   // Words of a key and of a value, and their exponents.  A lane behind a row's end reads its beginning (or the last
   // group's exponent): it has zeros on the queries' side, and columns that nobody asks for on the values'.
-  Word key_word[MODE == kWhole ? kKeyRuns : kSteps];
+  Word key_word[in_blocks(MODE) ? kKeyRuns : kSteps];
   int key_e_at[kKeyRuns];
 #pragma unroll
   for (int j = 0; j < kKeyRuns; ++j) {
     const int d = (j * 4 + g) * kKeyRun;
-    key_e_at[j] = d < c.key.width ? d / kGroup : 0;
-    if constexpr (MODE == kWhole) {
+    key_e_at[j] = MODE == kDense || d < c.key.width ? d / kGroup : 0;
+    if constexpr (in_blocks(MODE)) {
       key_word[j] = word_of<4, MODE>(d / 2, key_bytes);
     } else {
 #pragma unroll
@@ -187,7 +217,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
   for (int j = 0; j < kBlocks; ++j) {
     const int d = (j * 16 + n) * kRun;
     value_word[j] = word_of<kRun / 2, MODE>(d / 2, value_bytes);
-    value_e_at[j] = d < c.value.width ? d / kGroup : 0;
+    value_e_at[j] = MODE == kDense || d < c.value.width ? d / kGroup : 0;
   }
 
   int64_t at = share.at;
@@ -216,16 +246,26 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
     const auto q_of = [&](int j, int p) { return kShared ? q_shared[j][p][lane] : q_own[kShared ? 0 : j][p]; };
     {
       const int head = n < heads_here ? n : 0;
+      // not known to be the same for every sequence: the masks of its comparisons would be kept for all of them
+      int key_width = c.key.width;
+      asm("" : "+s"(key_width));
       const T* q_row = static_cast<const T*>(a.query) + b * a.query_stride[0] + (head0 + head) * a.query_stride[1];
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
         const int d0 = (j / kKeyWords * 4 + g) * kKeyRun + j % kKeyWords * 8;
         float q[8];
+        if constexpr (MODE == kDense) {
+          RawVec<8 * sizeof(T)> raw;
+          __builtin_memcpy(&raw, q_row + d0, sizeof(raw));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int d = d0 + i;
-          const float x = Elem<T>::at(q_row, d < c.key.width ? d : 0);
-          q[i] = d < c.key.width && n < heads_here ? x : 0.0f;
+          for (int i = 0; i < 8; ++i) q[i] = n < heads_here ? Elem<T>::get(raw.w, i) * q_sign : 0.0f;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int d = d0 + i;
+            const float x = Elem<T>::at(q_row, d < key_width ? d : 0);
+            q[i] = d < key_width && n < heads_here ? x * q_sign : 0.0f;
+          }
         }
 #pragma unroll
         for (int p = 0; p < kQ; ++p) {
@@ -252,16 +292,18 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
     float sum;  // of head n and the tokens of this lane
 
     // What a tile needs from memory.
-    struct Tile {
-      uint32_t key[2][kSteps];
-      uint32_t key_e[2][kKeyRuns];
-      uint32_t value[kBlocks][kOwn];
-      uint32_t value_e[kBlocks][kOwn];
+    struct Keys {
+      uint32_t codes[2][kSteps];
+      uint32_t e[2][kKeyRuns];
+    };
+    struct Values {
+      uint32_t codes[kBlocks][kOwn];
+      uint32_t e[kBlocks][kOwn];
       uint32_t bad_tokens;  // tokens whose page is outside the cache, a bit each
     };
     struct Ids {
-      int64_t key[MODE == kWhole ? 1 : 2];
-      int64_t own[MODE == kWhole ? 1 : kOwn];
+      int64_t key[in_blocks(MODE) ? 1 : 2];
+      int64_t own[in_blocks(MODE) ? 1 : kOwn];
     };
     const auto is_bad = [&](int64_t id) { return id < 0 || id >= c.pages; };
     // Blocks (or tokens) behind what is seen stand for the last one: their loads need no guard.
@@ -270,7 +312,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
     const auto seen_token = [&](int t) { return t < end ? t : end - 1; };
     const auto ids_of = [&](int t0) {
       Ids ids;
-      if constexpr (MODE == kWhole) {
+      if constexpr (in_blocks(MODE)) {
         ids.key[0] = pages[page_of_token(a, block_of(t0 + key_token))];
         ids.own[0] = pages[page_of_token(a, block_of(t0 + own_token))];
       } else {
@@ -281,122 +323,123 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
       }
       return ids;
     };
-    const auto load_key = [&](Tile& tile, int s, const uint8_t* row, const uint8_t* row_e) {
+    const auto load_key = [&](Keys& keys, int s, const uint8_t* row, const uint8_t* row_e) {
 #pragma unroll
       for (int j = 0; j < kKeyRuns; ++j) {
-        if constexpr (MODE == kWhole) {
-          __builtin_memcpy(&tile.key[s][j * kKeyWords], row + key_word[j].at, 4 * kKeyWords);
+        if constexpr (in_blocks(MODE)) {
+          __builtin_memcpy(&keys.codes[s][j * kKeyWords], row + key_word[j].at, 4 * kKeyWords);
         } else {
 #pragma unroll
           for (int i = 0; i < kKeyWords; ++i)
-            tile.key[s][j * kKeyWords + i] = load_word<4, MODE>(row, key_word[j * kKeyWords + i], key_bytes);
+            keys.codes[s][j * kKeyWords + i] = load_word<4, MODE>(row, key_word[j * kKeyWords + i], key_bytes);
         }
-        tile.key_e[s][j] = row_e[key_e_at[j]];
+        keys.e[s][j] = row_e[key_e_at[j]];
       }
     };
-    const auto load_value = [&](Tile& tile, int e, const uint8_t* row, const uint8_t* row_e) {
+    const auto load_value = [&](Values& values, int e, const uint8_t* row, const uint8_t* row_e) {
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j) {
-        tile.value[j][e] = load_word<kRun / 2, MODE>(row, value_word[j], value_bytes);
-        tile.value_e[j][e] = row_e[value_e_at[j]];
+        values.codes[j][e] = load_word<kRun / 2, MODE>(row, value_word[j], value_bytes);
+        values.e[j][e] = row_e[value_e_at[j]];
       }
     };
-    const auto load_tile = [&](Tile& tile, int t0, const Ids& ids) {
-      if constexpr (MODE == kWhole) {
-        int t = block_of(t0 + key_token);
-        int slot = t - page_of_token(a, t) * c.page_size + (key_token & 7);
-        int64_t page = is_bad(ids.key[0]) ? 0 : ids.key[0];
-        const uint8_t* row = key_base + page * c.key.stride[0] + slot * c.key.stride[2];
-        const uint8_t* row_e = key_e_base + page * c.key.exponent_stride[0] + slot * c.key.exponent_stride[2];
+    const auto slot_of = [&](int t) { return t - page_of_token(a, t) * c.page_size; };
+    const auto load_keys = [&](Keys& keys, int t0, const Ids& ids) {
+      if constexpr (in_blocks(MODE)) {
+        const int slot = slot_of(block_of(t0 + key_token)) + (key_token & 7);
+        const int64_t page = is_bad(ids.key[0]) ? 0 : ids.key[0];
+        const uint8_t* row = key_base + page_offset(page, c.key.stride[0]) + slot * key_step;
+        const uint8_t* row_e = key_e_base + page_offset(page, c.key.exponent_stride[0]) + slot * key_e_step;
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-          load_key(tile, s, row + s * 4 * c.key.stride[2], row_e + s * 4 * c.key.exponent_stride[2]);
-        t = block_of(t0 + own_token);
-        slot = t - page_of_token(a, t) * c.page_size;
-        const bool bad = is_bad(ids.own[0]);
-        page = bad ? 0 : ids.own[0];
-        tile.bad_tokens = bad ? 0xffu : 0u;
-        row = value_base + page * c.value.stride[0] + slot * c.value.stride[2];
-        row_e = value_e_base + page * c.value.exponent_stride[0] + slot * c.value.exponent_stride[2];
-#pragma unroll
-        for (int e = 0; e < kOwn; ++e)
-          load_value(tile, e, row + e * c.value.stride[2], row_e + e * c.value.exponent_stride[2]);
+        for (int s = 0; s < 2; ++s) load_key(keys, s, row + s * 4 * key_step, row_e + s * 4 * key_e_step);
       } else {
-        const auto slot_of = [&](int t) {
-          t = seen_token(t);
-          return t - page_of_token(a, t) * c.page_size;
-        };
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const int64_t page = is_bad(ids.key[s]) ? 0 : ids.key[s];
-          const int slot = slot_of(t0 + key_token + s * 4);
-          load_key(tile, s, key_base + page * c.key.stride[0] + slot * c.key.stride[2],
-                   key_e_base + page * c.key.exponent_stride[0] + slot * c.key.exponent_stride[2]);
+          const int slot = slot_of(seen_token(t0 + key_token + s * 4));
+          load_key(keys, s, key_base + page_offset(page, c.key.stride[0]) + slot * key_step,
+                   key_e_base + page_offset(page, c.key.exponent_stride[0]) + slot * key_e_step);
         }
-        tile.bad_tokens = 0;
+      }
+    };
+    const auto load_values = [&](Values& values, int t0, const Ids& ids) {
+      if constexpr (in_blocks(MODE)) {
+        const int slot = slot_of(block_of(t0 + own_token));
+        const bool bad = is_bad(ids.own[0]);
+        const int64_t page = bad ? 0 : ids.own[0];
+        values.bad_tokens = bad ? 0xffu : 0u;
+        const uint8_t* row = value_base + page_offset(page, c.value.stride[0]) + slot * value_step;
+        const uint8_t* row_e = value_e_base + page_offset(page, c.value.exponent_stride[0]) + slot * value_e_step;
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) load_value(values, e, row + e * value_step, row_e + e * value_e_step);
+      } else {
+        values.bad_tokens = 0;
 #pragma unroll
         for (int e = 0; e < kOwn; ++e) {
           const bool bad = is_bad(ids.own[e]);
           const int64_t page = bad ? 0 : ids.own[e];
-          const int slot = slot_of(t0 + own_token + e);
-          if (bad) tile.bad_tokens |= 1u << e;
-          load_value(tile, e, value_base + page * c.value.stride[0] + slot * c.value.stride[2],
-                     value_e_base + page * c.value.exponent_stride[0] + slot * c.value.exponent_stride[2]);
+          const int slot = slot_of(seen_token(t0 + own_token + e));
+          if (bad) values.bad_tokens |= 1u << e;
+          load_value(values, e, value_base + page_offset(page, c.value.stride[0]) + slot * value_step,
+                     value_e_base + page_offset(page, c.value.exponent_stride[0]) + slot * value_e_step);
         }
       }
     };
 
-    const auto work_on = [&](Tile& tile, int t0) {
-      f32x4 score[2];
+    const auto products = [&](const Keys& keys, f32x4 (&score)[2]) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         score[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
-          const uint32_t w = tile.key[s][j];
-          const float scale = as_scale(tile.key_e[s][j / kKeyWords]);
+          const uint32_t w = keys.codes[s][j];
+          const float scale = as_scale(keys.e[s][j / kKeyWords]);
           const u32x4 k{bf16_pair<0>(w, scale), bf16_pair<1>(w, scale), bf16_pair<2>(w, scale), bf16_pair<3>(w, scale)};
 #pragma unroll
           for (int p = 0; p < kQ; ++p) score[s] = multiply(k, q_of(j, p), score[s]);
         }
       }
-
+    };
+    const auto weigh = [&](Values& values, const f32x4 (&score)[2], int t0) {
+      // Scores, and the products that they are scale times of where there is no bias: one fused step less then for
+      // each weight, and their maximum is the scores' (scale is not negative, the queries have its sign).
       float scores[kOwn];
       float most = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < kOwn; ++e) scores[e] = score[e / 4][e % 4] * a.scale;
-      if (a.table != nullptr) {
+      for (int e = 0; e < kOwn; ++e) scores[e] = score[e / 4][e % 4];
+      if (biased) {
         // every token of the tile farther than the last border: one number a head
         if (seen.end - t0 - kTile >= border[map.side - 1]) {
           const float far = bias[map.side - 1][n];
 #pragma unroll
-          for (int e = 0; e < kOwn; ++e) scores[e] += far;
+          for (int e = 0; e < kOwn; ++e) scores[e] = fmaf(scores[e], scale, far);
         } else {
 #pragma unroll
           for (int e = 0; e < kOwn; ++e) {
             const int away = seen.end - 1 - (t0 + own_token + e);
-            scores[e] += bias[bucket_of_distance(border, map, away < 0 ? 0 : away)][n];
+            scores[e] = fmaf(scores[e], scale, bias[bucket_of_distance(border, map, away < 0 ? 0 : away)][n]);
           }
         }
       }
-      if (t0 < begin || t0 + kTile > end || __any(tile.bad_tokens != 0)) {
+      if (t0 < begin || t0 + kTile > end || __any(values.bad_tokens != 0)) {
 #pragma unroll
         for (int e = 0; e < kOwn; ++e) {
           const int t = t0 + own_token + e;
           const bool out_of_sight = t < begin || t >= end;
-          if ((tile.bad_tokens >> e) & 1) scores[e] = NAN;
+          if ((values.bad_tokens >> e) & 1) scores[e] = NAN;
           if (out_of_sight) scores[e] = -INFINITY;
           // a value out of sight may be anything; its weight is zero, and so has to be the product
 #pragma unroll
           for (int j = 0; j < kBlocks; ++j) {
-            tile.value[j][e] = out_of_sight ? 0u : tile.value[j][e];
-            tile.value_e[j][e] = out_of_sight ? 127u : tile.value_e[j][e];
+            values.codes[j][e] = out_of_sight ? 0u : values.codes[j][e];
+            values.e[j][e] = out_of_sight ? 127u : values.e[j][e];
           }
         }
       }
 #pragma unroll
       for (int e = 0; e < kOwn; ++e) most = fmaxf(most, scores[e]);
 
+      most *= left;
       if (__any(most > top + kSlack)) {
         most = fmaxf(most, __shfl_xor(most, 16, 64));
         most = fmaxf(most, __shfl_xor(most, 32, 64));
@@ -416,7 +459,7 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
       float weight[kOwn];
 #pragma unroll
       for (int e = 0; e < kOwn; ++e) {
-        weight[e] = exp_of(scores[e] - from);
+        weight[e] = exp_of(fmaf(scores[e], left, -from));
         sum += weight[e];
       }
       u32x4 w16[kP];
@@ -433,27 +476,29 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
 
 #pragma unroll
       for (int jb = 0; jb < kBlocks; ++jb) {
-        uint32_t words[kOwn][kRun / 2];
+        // two columns at a time, so that few converted numbers are held at once
+        const auto columns = [&](auto pair) {
+          constexpr int I = decltype(pair)::value;
+          uint32_t words[kOwn];
 #pragma unroll
-        for (int e = 0; e < kOwn; ++e) {
-          const uint32_t w = tile.value[jb][e];
-          const float scale = as_scale(tile.value_e[jb][e]);
-          words[e][0] = bf16_pair<0>(w, scale);
-          words[e][1] = bf16_pair<1>(w, scale);
-          if constexpr (kRun == 8) {
-            words[e][2] = bf16_pair<2>(w, scale);
-            words[e][3] = bf16_pair<3>(w, scale);
+          for (int e = 0; e < kOwn; ++e) words[e] = bf16_pair<I>(values.codes[jb][e], as_scale(values.e[jb][e]));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            u32x4 column;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              column[i] = __builtin_amdgcn_perm(words[2 * i + 1], words[2 * i], j == 0 ? 0x05040100u : 0x07060302u);
+            f32x4& to = acc[jb * kRun + 2 * I + j];
+#pragma unroll
+            for (int p = 0; p < kP; ++p) to = multiply(w16[p], column, to);
           }
-        }
-#pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-          u32x4 column;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            column[i] = __builtin_amdgcn_perm(words[2 * i + 1][j / 2], words[2 * i][j / 2],
-                                              j % 2 == 0 ? 0x05040100u : 0x07060302u);
-#pragma unroll
-          for (int p = 0; p < kP; ++p) acc[jb * kRun + j] = multiply(w16[p], column, acc[jb * kRun + j]);
+          __builtin_amdgcn_sched_barrier(0);
+        };
+        columns(Constant<0>{});
+        columns(Constant<1>{});
+        if constexpr (kRun == 8) {
+          columns(Constant<2>{});
+          columns(Constant<3>{});
         }
       }
     };
@@ -465,24 +510,24 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
     sum = 0.0f;
     int t0 = base + wave * kTile;
     if (t0 < end) {
-      // a tile ahead, in two sets of registers that take turns
-      Tile one;
-      Tile two;
+      // each kind of row takes the registers of the last tile's as soon as those are used up
+      Keys keys;
+      Values values;
       Ids ids = ids_of(t0);
-      load_tile(one, t0, ids);
+      load_keys(keys, t0, ids);
+      load_values(values, t0, ids);
       ids = ids_of(t0 + kStride);
       for (;;) {
         // the queries in LDS are read for every tile: kept, they would take the registers they are spared
         if constexpr (kShared) asm volatile("" ::: "memory");
-        load_tile(two, t0 + kStride, ids);
+        f32x4 score[2];
+        products(keys, score);
+        __builtin_amdgcn_sched_barrier(0);
+        load_keys(keys, t0 + kStride, ids);
+        weigh(values, score, t0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_values(values, t0 + kStride, ids);
         ids = ids_of(t0 + 2 * kStride);
-        work_on(one, t0);
-        t0 += kStride;
-        if (t0 >= end) break;
-        if constexpr (kShared) asm volatile("" ::: "memory");
-        load_tile(one, t0 + kStride, ids);
-        ids = ids_of(t0 + 2 * kStride);
-        work_on(two, t0);
         t0 += kStride;
         if (t0 >= end) break;
       }
@@ -554,33 +599,68 @@ __global__ __launch_bounds__(kBlock) void paged_attention_e2m1_kernel(AttentionA
   }
 }
 
+// The narrowest rows that hold both widths: what a row does not fill is loaded and multiplied all the same.
+int row_width(const PagedCache& c) {
+  const int width = c.key.width > c.value.width ? c.key.width : c.value.width;
+  return width <= 64 ? 64 : (width <= 128 ? 128 : (width <= 192 ? 192 : 256));
+}
+// Whether the rows of a tensor are those of kDense.
+bool dense(const PageTensor& t, int width) {
+  const auto near = [](int64_t stride) { return stride >= 0 && stride <= INT32_MAX; };
+  return t.width == width && t.stride[2] == width / 2 && t.exponent_stride[2] == width / kGroup && near(t.stride[0]) &&
+         near(t.exponent_stride[0]);
+}
+Mode mode_of(const PagedCache& c) {
+  if (c.key.width < 8 || c.value.width < 8) return kBytes;
+  if (c.page_size % 8 != 0 || c.key.width % kGroup != 0 || c.value.width % kGroup != 0) return kTokens;
+  return dense(c.key, row_width(c)) && dense(c.value, row_width(c)) ? kDense : kWhole;
+}
+
 template <typename T, int W>
 void launch_width(const AttentionArgs& a, const PositionMap& map, dim3 grid, hipStream_t s) {
-  const PagedCache& c = a.cache;
-  if (c.key.width < 8 || c.value.width < 8) {
-    paged_attention_e2m1_kernel<T, W, kBytes><<<grid, kBlock, 0, s>>>(a, map);
-  } else if (c.page_size % 8 == 0 && c.key.width % kGroup == 0 && c.value.width % kGroup == 0) {
-    paged_attention_e2m1_kernel<T, W, kWhole><<<grid, kBlock, 0, s>>>(a, map);
-  } else {
-    paged_attention_e2m1_kernel<T, W, kTokens><<<grid, kBlock, 0, s>>>(a, map);
+  switch (mode_of(a.cache)) {
+    case kBytes:
+      paged_attention_e2m1_kernel<T, W, kBytes, true><<<grid, kBlock, 0, s>>>(a, map);
+      break;
+    case kTokens:
+      paged_attention_e2m1_kernel<T, W, kTokens, true><<<grid, kBlock, 0, s>>>(a, map);
+      break;
+    case kWhole:
+      paged_attention_e2m1_kernel<T, W, kWhole, true><<<grid, kBlock, 0, s>>>(a, map);
+      break;
+    case kDense:
+      if (a.table == nullptr) {
+        paged_attention_e2m1_kernel<T, W, kDense, false><<<grid, kBlock, 0, s>>>(a, map);
+      } else {
+        paged_attention_e2m1_kernel<T, W, kDense, true><<<grid, kBlock, 0, s>>>(a, map);
+      }
   }
 }
 
 }  // namespace
 
+int64_t paged_shares_e2m1(const PagedCache& c, int dtype) {
+  if (mode_of(c) != kDense) return 512;
+  const int width = row_width(c);
+  return width == 64 || (width == 128 && dtype != AS_DTYPE_F32) ? 768 : 512;
+}
+
 int launch_paged_attention_e2m1(const AttentionArgs& a, const PositionMap& map, int dtype, hipStream_t s) {
-  const int width = a.cache.key.width > a.cache.value.width ? a.cache.key.width : a.cache.value.width;
   const dim3 grid(static_cast<unsigned>((a.shares > 0 ? a.shares : a.cache.sequences) * a.cache.heads * a.head_tiles));
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
-    if (width <= 64) {
-      launch_width<T, 64>(a, map, grid, s);
-    } else if (width <= 128) {
-      launch_width<T, 128>(a, map, grid, s);
-    } else if (width <= 192) {
-      launch_width<T, 192>(a, map, grid, s);
-    } else {
-      launch_width<T, 256>(a, map, grid, s);
+    switch (row_width(a.cache)) {
+      case 64:
+        launch_width<T, 64>(a, map, grid, s);
+        break;
+      case 128:
+        launch_width<T, 128>(a, map, grid, s);
+        break;
+      case 192:
+        launch_width<T, 192>(a, map, grid, s);
+        break;
+      default:
+        launch_width<T, 256>(a, map, grid, s);
     }
     return check_launch("paged_attention");
   });

@@ -28,8 +28,10 @@ struct AttentionArgs {
   float* part_out;    // [parts, heads * group, value width]
 };
 
-// Attention over pages of 4-bit numbers (paged_attention4.hip), without the join of
-// the parts that its shares leave; dtype: of the queries.
+// Pages of 4-bit numbers (paged_attention4.hip).  dtype: of the queries.  Workgroups in
+// one round (dtype < 0: of those queries that have the most); attention without the
+// join of the parts that its shares leave.
+int64_t paged_shares_e2m1(const PagedCache& c, int dtype);
 int launch_paged_attention_e2m1(const AttentionArgs& a, const PositionMap& map, int dtype, hipStream_t s);
 
 namespace {

@@ -450,3 +450,13 @@ def test_places_beyond_32_bits():
     query = torch.randn(1, heads, width, generator=gen).bfloat16()
     out, lse = autosage_amd.paged_attention(query.cuda(), k, v, ptr, idx, lengths, scale=0.1, return_lse=True, **names)
     assert_attention(out, lse, plain_attention(cache, query, 0.1), dtype=torch.bfloat16, quantised=True, lse_bound=2e-4)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 12])
+@pytest.mark.parametrize("scale", [0.0, -0.3])
+@pytest.mark.parametrize("bias", [None, (8, 20, False)])
+def test_scales_of_zero_and_below(dtype, page, scale, bias):
+    """A scale of zero gives all tokens the same weight (or the bias's), one below zero prefers small products."""
+    _attend([1, 40, 0, 700], 2, 3, 64, 64, page, dtype, scale=scale, bias=bias, seed=32)
+    _attend([1, 40, 0, 700], 2, 3, 64, 64, page, dtype, scale=scale, bias=bias, max_length=None, window=33, seed=33)
