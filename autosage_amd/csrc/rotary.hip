@@ -52,13 +52,16 @@ struct RotaryArgs {
   int64_t tokens;
   int width;
   int pairs;
-  int turning;      // units of V pairs in a row, the last of which ends with the pairs
-  Divisor units;    // those, and the units of 2V numbers that stay
-  Divisor heads;    // of queries and keys
-  Divisor by_pairs;
-  int each;         // tokens of a workgroup
+  int turning;  // units in a row that are turned, the last of which ends with the pairs
+  int units;    // those and the units that stay
+  int heads;    // of queries and keys
+  int each;     // tokens of a workgroup
+  int step;     // rows that a workgroup takes at once: a thread has one unit of a row, and that of every step-th
+  int step_tokens, step_heads;  // the same as tokens and heads
+  Divisor by_units, by_heads, by_pairs;
   float magnitude;
   float sign;
+  bool past_caches;  // what is written
 };
 
 constexpr double kPerTurn = 0.15915494309189535;  // 1 / (2 pi)
@@ -84,6 +87,18 @@ __device__ __forceinline__ RawVec<V * sizeof(T)> load_numbers(const T* from) {
   return r;
 }
 
+typedef uint32_t u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
+template <int V, typename T>
+__device__ __forceinline__ void store_numbers(T* to, const RawVec<V * sizeof(T)>& r, bool past_caches) {
+  if constexpr (V * sizeof(T) == 16) {
+    if (past_caches) {
+      __builtin_nontemporal_store(u32x4_a1{r.w[0], r.w[1], r.w[2], r.w[3]}, reinterpret_cast<u32x4_a1*>(to));
+      return;
+    }
+  }
+  __builtin_memcpy(to, &r, V * sizeof(T));
+}
+
 constexpr int kRotaryAhead = 2;  // units of a thread whose loads are under way at once
 
 template <typename T, int V, bool INTERLEAVED>
@@ -93,63 +108,66 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
   const int count = a.tokens - first < a.each ? static_cast<int>(a.tokens - first) : a.each;
   float* const cosines = angles;
   float* const sines = angles + a.each * a.pairs;
-  const int items = count * a.heads.d * a.units.d;
 
-  // a unit: V pairs from `pair` on, or numbers that stay (pair < 0), and where its two runs are read and written
-  struct Unit {
-    const T* from;
-    T* to;
-    int token;
-    int pair;
-    int one, two;
-  };
-  const auto unit_of = [&](int i) {
-    Unit u;
-    const int row = quotient(i, a.units);
-    const int k = i - row * a.units.d;
-    u.token = quotient(row, a.heads);
-    int h = row - u.token * a.heads.d;
-    const bool second = h >= a.rows[0].heads;
-    h = second ? h - a.rows[0].heads : h;
-    const int64_t t = first + u.token;
-    const int64_t at = second ? t * a.rows[1].stride[0] + h * a.rows[1].stride[1]
-                              : t * a.rows[0].stride[0] + h * a.rows[0].stride[1];
-    u.from = static_cast<const T*>(second ? a.rows[1].from : a.rows[0].from) + at;
-    u.to = static_cast<T*>(second ? a.rows[1].to : a.rows[0].to) +
-           (t * (second ? a.rows[1].heads : a.rows[0].heads) + h) * a.width;
-    // runs that would pass the end of the pairs, or of the row, end with it: what two units share is the same in both
-    if (k < a.turning) {
-      u.pair = k * V < a.pairs - V ? k * V : a.pairs - V;
-      u.one = INTERLEAVED ? 2 * u.pair : u.pair;
-      u.two = INTERLEAVED ? 2 * u.pair + V : u.pair + a.pairs;
-    } else {
-      const int d = 2 * a.pairs + (k - a.turning) * 2 * V;
-      u.pair = -1;
-      u.one = d < a.width - V ? d : a.width - V;
-      u.two = d + V < a.width - V ? d + V : a.width - V;
-    }
-    return u;
-  };
+  // A thread's unit: two runs of V numbers, a half of what is turned (or stays) apart, so that neighbouring lanes have
+  // neighbouring runs (with V = 1 and interleaved pairs, the numbers of a pair).  Runs that would pass the end end with
+  // it: what two units share is the same in both.
+  const int row0 = quotient(threadIdx.x, a.by_units);
+  const int k = static_cast<int>(threadIdx.x) - row0 * a.units + static_cast<int>(blockIdx.y) * kBlock;
+  const bool turns = k < a.turning;
+  int one;
+  int two;
+  if (!INTERLEAVED && turns) {
+    one = k * V < a.pairs - V ? k * V : a.pairs - V;
+    two = a.pairs + one;
+  } else if (V == 1 && turns) {
+    one = 2 * k;
+    two = 2 * k + 1;
+  } else {
+    const int begin = turns ? 0 : 2 * a.pairs;
+    const int last = (turns ? 2 * a.pairs : a.width) - V;
+    one = begin + (turns ? k : k - a.turning) * V;
+    two = one + (turns ? a.turning : a.units - a.turning) * V;
+    one = one < last ? one : last;
+    two = two < last ? two : last;
+  }
+  const bool idle = row0 >= a.step || k >= a.units;  // threads that are no whole row
+  int token = quotient(row0, a.by_heads);
+  int head = row0 - token * a.heads;
+  const int rounds = (count * a.heads + a.step - 1) / a.step;
 
-  for (int base = 0; base < items; base += kRotaryAhead * kBlock) {
-    Unit unit[kRotaryAhead];
-    RawVec<V * sizeof(T)> one[kRotaryAhead];
-    RawVec<V * sizeof(T)> two[kRotaryAhead];
+  for (int r = 0; r < rounds; r += kRotaryAhead) {
+    RawVec<V * sizeof(T)> x[kRotaryAhead];
+    RawVec<V * sizeof(T)> y[kRotaryAhead];
+    T* to[kRotaryAhead];
+    int at[kRotaryAhead];
 #pragma unroll
     for (int u = 0; u < kRotaryAhead; ++u) {
-      const int i = base + u * kBlock + static_cast<int>(threadIdx.x);
-      unit[u] = unit_of(i < items ? i : items - 1);
-      one[u] = load_numbers<T, V>(unit[u].from + unit[u].one);
-      two[u] = load_numbers<T, V>(unit[u].from + unit[u].two);
+      const bool second = head >= a.rows[0].heads;
+      const int h = second ? head - a.rows[0].heads : head;
+      at[u] = idle || token >= count ? -1 : token * a.pairs;
+      const int64_t t = first + (at[u] < 0 ? 0 : token);
+      const int64_t from = second ? t * a.rows[1].stride[0] + h * a.rows[1].stride[1]
+                                  : t * a.rows[0].stride[0] + h * a.rows[0].stride[1];
+      const T* row = static_cast<const T*>(second ? a.rows[1].from : a.rows[0].from) + from;
+      to[u] = static_cast<T*>(second ? a.rows[1].to : a.rows[0].to) +
+              (t * (second ? a.rows[1].heads : a.rows[0].heads) + h) * a.width;
+      x[u] = load_numbers<T, V>(row + one);
+      y[u] = load_numbers<T, V>(row + two);
+      token += a.step_tokens;
+      head += a.step_heads;
+      const bool over = head >= a.heads;
+      token += over ? 1 : 0;
+      head -= over ? a.heads : 0;
     }
-    if (base == 0) {
+    if (r == 0) {
       for (int i = threadIdx.x; i < count * a.pairs; i += kBlock) {
         const int t = quotient(i, a.by_pairs);
-        const double turns =
+        const double turned =
             static_cast<double>(a.positions[first + t]) * (a.frequencies[i - t * a.pairs] * kPerTurn);
         float s;
         float c;
-        sine_of_turns(turns, &s, &c);
+        sine_of_turns(turned, &s, &c);
         sines[i] = s * a.magnitude * a.sign;
         cosines[i] = c * a.magnitude;
       }
@@ -157,38 +175,49 @@ __global__ __launch_bounds__(kBlock) void rotary_kernel(RotaryArgs a) {
     }
 #pragma unroll
     for (int u = 0; u < kRotaryAhead; ++u) {
-      if (base + u * kBlock + static_cast<int>(threadIdx.x) >= items) break;
-      if (unit[u].pair >= 0) {
-        const int at = unit[u].token * a.pairs + unit[u].pair;
-        float x[2 * V];
+      if (at[u] < 0) continue;
+      if (turns) {
+        T turned[2 * V];
+        if constexpr (INTERLEAVED && V > 1) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          x[i] = Elem<T>::get(one[u].w, i);
-          x[V + i] = Elem<T>::get(two[u].w, i);
-        }
-        T y[2 * V];
+          for (int half = 0; half < 2; ++half) {
+            const RawVec<V * sizeof(T)>& w = half == 0 ? x[u] : y[u];
+            const int pair = at[u] + (half == 0 ? one : two) / 2;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float c = cosines[at + i];
-          const float s = sines[at + i];
-          const int p = INTERLEAVED ? 2 * i : i;
-          const int q = INTERLEAVED ? 2 * i + 1 : V + i;
-          y[p] = rounded<T>(x[p] * c - x[q] * s);
-          y[q] = rounded<T>(x[p] * s + x[q] * c);
+            for (int i = 0; i < V / 2; ++i) {
+              const float c = cosines[pair + i];
+              const float s = sines[pair + i];
+              const float p = Elem<T>::get(w.w, 2 * i);
+              const float q = Elem<T>::get(w.w, 2 * i + 1);
+              turned[half * V + 2 * i] = rounded<T>(p * c - q * s);
+              turned[half * V + 2 * i + 1] = rounded<T>(p * s + q * c);
+            }
+          }
+        } else {
+          const int pair = at[u] + (INTERLEAVED ? one / 2 : one);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float c = cosines[pair + i];
+            const float s = sines[pair + i];
+            const float p = Elem<T>::get(x[u].w, i);
+            const float q = Elem<T>::get(y[u].w, i);
+            turned[i] = rounded<T>(p * c - q * s);
+            turned[V + i] = rounded<T>(p * s + q * c);
+          }
         }
-        __builtin_memcpy(&one[u], y, V * sizeof(T));
-        __builtin_memcpy(&two[u], y + V, V * sizeof(T));
+        __builtin_memcpy(&x[u], turned, V * sizeof(T));
+        __builtin_memcpy(&y[u], turned + V, V * sizeof(T));
       }
-      __builtin_memcpy(unit[u].to + unit[u].one, &one[u], V * sizeof(T));
-      __builtin_memcpy(unit[u].to + unit[u].two, &two[u], V * sizeof(T));
+      store_numbers<V>(to[u] + one, x[u], a.past_caches);
+      store_numbers<V>(to[u] + two, y[u], a.past_caches);
     }
   }
 }
 
-// The widest runs that neither the pairs nor what stays is shorter than.
-int run_of(int pairs, int rest, int widest) {
+// The widest runs that neither what is turned (a half of it where halves are pairs) nor what stays is shorter than.
+int run_of(int turned, int rest, int widest) {
   int v = widest;
-  while (v > 1 && ((pairs > 0 && pairs < v) || (rest > 0 && rest < v))) v /= 2;
+  while (v > 1 && ((turned > 0 && turned < v) || (rest > 0 && rest < v))) v /= 2;
   return v;
 }
 
@@ -246,20 +275,33 @@ int as_rotary_positions(const void* query, const int64_t* query_strides, void* q
   a.magnitude = magnitude;
   a.sign = inverse ? -1.0f : 1.0f;
   const int rest = a.width - 2 * a.pairs;
-  const int v = run_of(a.pairs, rest, dtype == AS_DTYPE_F32 ? 4 : 8);
-  a.turning = (a.pairs + v - 1) / v;
-  a.units = divisor_of(a.turning + (rest + 2 * v - 1) / (2 * v));
-  a.heads = divisor_of(static_cast<int>(heads + key_heads));
+  const int v = run_of(interleaved ? 2 * a.pairs : a.pairs, rest, dtype == AS_DTYPE_F32 ? 4 : 8);
+  // units of two runs, or of a pair
+  const int halves = interleaved && v > 1 ? (a.pairs * 2 + v - 1) / v : 2 * ((a.pairs + v - 1) / v);
+  a.turning = (halves + 1) / 2;
+  a.units = a.turning + ((rest + v - 1) / v + 1) / 2;
+  a.heads = static_cast<int>(heads + key_heads);
+  a.step = a.units < kBlock ? kBlock / a.units : 1;
+  a.step_tokens = a.step / a.heads;
+  a.step_heads = a.step % a.heads;
+  a.by_units = divisor_of(a.units);
+  // Results go past the caches (16,384 tokens, 40 heads of 128, bf16: 61 us, 5.5 TB/s; 71 through them), but where what
+  // stays leaves runs that are no whole 64 bytes (5,000 tokens, 26 heads of 80, 32 turned, float32: 19 and 16).
+  const int run_bytes = (a.units - a.turning) * v * (dtype == AS_DTYPE_F32 ? 4 : 2);
+  a.past_caches = rest == 0 || run_bytes % 64 == 0;
+  a.by_heads = divisor_of(a.heads);
   a.by_pairs = divisor_of(a.pairs > 0 ? a.pairs : 1);
   // Tokens of a workgroup: as many as give each of its threads four units, while 512 workgroups are left and the
   // angles have room
-  const int64_t units = int64_t(a.units.d) * a.heads.d;
+  const int64_t units = int64_t(a.units) * a.heads;
   a.each = 1;
   while (a.each < 256 && a.each * units < 4 * kBlock && tokens / (2 * a.each) >= 512 &&
          2 * a.each * pairs <= kMostAngles)
     a.each *= 2;
   while (tokens / a.each > kMaxBlocksPerLaunch) a.each *= 2;  // at most 16, and 64 KB of angles
-  const dim3 grid(static_cast<unsigned>((tokens + a.each - 1) / a.each));
+  // rows of more units than threads take several workgroups
+  const dim3 grid(static_cast<unsigned>((tokens + a.each - 1) / a.each),
+                  static_cast<unsigned>((a.units + kBlock - 1) / kBlock));
   const size_t lds = static_cast<size_t>(a.each) * a.pairs * 2 * sizeof(float);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_float_element(dtype, [&](auto e) {

@@ -42,7 +42,7 @@ def _check(query, key, positions, frequencies, interleaved, magnitude=1.0, move=
 
 SHAPES = [(1, 0), (2, 1), (3, 1), (7, 3), (8, 4), (16, 8), (15, 7), (18, 9), (24, 12), (33, 5), (40, 10), (64, 32), (72, 36),
           (80, 16), (80, 9), (100, 50), (128, 64), (128, 1), (128, 31), (130, 64), (200, 99), (256, 128), (255, 100),
-          (300, 0), (1024, 512), (1001, 333)]
+          (300, 0), (1024, 512), (1001, 333), (1024, 1), (1023, 1), (1023, 511)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
