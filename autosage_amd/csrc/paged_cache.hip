@@ -245,9 +245,69 @@ __device__ __forceinline__ void read_rows(const PageTensor& from, const TokenRow
 // 4-bit numbers: a lane has 8 elements of a row (16 bytes of a 16-bit type, 4 of codes)
 // and four lanes share an exponent, so that neighbouring lanes are neighbours on both
 // sides and a group's maximum takes two shuffles.  Rows are cut at whole groups; what
-// passes a row's end counts as zeros and is not stored.
+// passes a row's end counts as zeros and is not stored.  Eight numbers are little work,
+// so what they need besides counts: a thread has one run of a row, and that of every
+// step-th, and where a token's rows lie is found once.  Keys and values of one width
+// are the rows of one list, else two.
 constexpr int kPairRun = 8;
-inline RowItems pair_items(int width) { return row_items((width + kGroup - 1) / kGroup * (kGroup / kPairRun), 1, false); }
+constexpr int kPairGroup = kGroup / kPairRun;  // lanes that share an exponent
+constexpr int64_t kNoPlace = INT64_MIN;
+struct PairOffsets {
+  int64_t codes[2][kMaxTokens];  // of keys and values; kNoPlace: none
+  int64_t exponents[2][kMaxTokens];
+};
+__device__ __forceinline__ void find_offsets(const PagedCache& c, const Places& places, int count, PairOffsets& to) {
+  if (threadIdx.x < 2 * kMaxTokens) {
+    const int token = static_cast<int>(threadIdx.x) % kMaxTokens;
+    const int kind = static_cast<int>(threadIdx.x) / kMaxTokens;
+    const PageTensor& t = kind == 0 ? c.key : c.value;
+    const int64_t page = token < count ? places.page[token] : -1;
+    const int64_t slot = token < count ? places.slot[token] : 0;
+    to.codes[kind][token] = page < 0 ? kNoPlace : page * t.stride[0] + slot * t.stride[2];
+    to.exponents[kind][token] = page * t.exponent_stride[0] + slot * t.exponent_stride[2];
+  }
+  __syncthreads();
+}
+
+struct PairRows {
+  int runs;      // lanes of a row
+  int step;      // rows that a workgroup takes at once
+  int shift;     // i / runs = i * magic >> (31 + shift)
+  uint32_t magic;
+};
+inline PairRows pair_rows(int width) {
+  const RowItems items = row_items((width + kGroup - 1) / kGroup * kPairGroup, 1, false);
+  return PairRows{items.runs, kBlock / items.runs, items.shift, items.magic};
+}
+
+// Calls f(kind, token, head, run, in the row) for the rows of `kinds` tensors, kAhead at a time: first f of all, then g.
+template <typename F, typename G>
+__device__ __forceinline__ void each_row(const PairRows& rows, int width, int heads, int log_tokens, int count, int kind,
+                                         int kinds, F&& f, G&& g) {
+  const int row0 = static_cast<int>((static_cast<uint64_t>(threadIdx.x) * rows.magic) >> (31 + rows.shift));
+  const int run = static_cast<int>(threadIdx.x) - row0 * rows.runs;
+  const int per_kind = heads << log_tokens;
+  const int all = kinds * per_kind;
+  const bool in_row = row0 < rows.step && run * kPairRun < width;
+  for (int r0 = 0; r0 < all; r0 += kAhead * rows.step) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int r = r0 + u * rows.step + row0;
+        const bool second = r >= per_kind;
+        const int at = second ? r - per_kind : r;
+        const int token = at & ((1 << log_tokens) - 1);
+        const bool live = in_row && r < all && token < count;
+        if (half == 0) {
+          f(u, second ? 1 : kind, token, at >> log_tokens, run, live);
+        } else {
+          g(u, second ? 1 : kind, token, at >> log_tokens, run, live);
+        }
+      }
+    }
+  }
+}
 
 template <typename E, int N>
 __device__ __forceinline__ RawVec<N * sizeof(E)> load_up_to(const E* from, int left) {
@@ -263,109 +323,158 @@ __device__ __forceinline__ RawVec<N * sizeof(E)> load_up_to(const E* from, int l
   return r;
 }
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// The bits of the largest magnitude of a run, as a float's: those of infinities and NaN are larger than any other's.
 template <typename T>
-__device__ __forceinline__ void write_rows_e2m1(const TokenRows& from, const PageTensor& to, const Places& places,
-                                                int64_t first, int count, int heads, const RowItems& row,
-                                                int log_tokens) {
-  constexpr int N = kPairRun;
-  const int items = (heads << log_tokens) * row.runs;
-  for (int i0 = threadIdx.x; i0 < items; i0 += kAhead * kBlock) {
-    RawVec<N * sizeof(T)> raw[kAhead];
+__device__ __forceinline__ uint32_t largest_bits(const uint32_t* w) {
+  uint32_t most = 0u;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
-#pragma unroll
-      for (uint32_t& w : raw[u].w) w = 0u;
-      if (it.head < heads && it.token < count && places.page[it.token] >= 0 && it.run * N < to.width)
-        raw[u] = load_up_to<T, N>(static_cast<const T*>(from.data) + (first + it.token) * from.stride[0] +
-                                      it.head * from.stride[1] + it.run * N, to.width - it.run * N);
+    for (int i = 0; i < kPairRun; ++i) {
+      const uint32_t x = w[i] & 0x7fffffffu;
+      most = most > x ? most : x;
     }
+    return most;
+  } else {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
-      float x[N];
-      float largest = 0.0f;
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        x[k] = Elem<T>::get(raw[u].w, k);
-        largest = fmaxf(largest, finite(x[k]) ? fabsf(x[k]) : INFINITY);
-      }
-      largest = fmaxf(largest, __shfl_xor(largest, 1, 64));
-      largest = fmaxf(largest, __shfl_xor(largest, 2, 64));
-      const bool odd = !finite(largest);
-      const int e = odd ? kNanExponent : group_exponent(largest);
-      const float scale = odd ? 0.0f : group_unscale(e);
-      uint32_t codes = 0u;
-#pragma unroll
-      for (int k = 0; k < N; ++k) x[k] = odd ? 0.0f : x[k] * scale;
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], 1.0f, 0);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], 1.0f, 1);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], 1.0f, 2);
-      codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], 1.0f, 3);
-      if (it.head < heads && it.token < count && places.page[it.token] >= 0 && it.run * N < to.width) {
-        const int64_t page = places.page[it.token];
-        const int64_t slot = places.slot[it.token];
-        uint8_t* y = static_cast<uint8_t*>(to.data) + page * to.stride[0] + it.head * to.stride[1] +
-                     slot * to.stride[2] + it.run * (N / 2);
-        if (to.width - it.run * N >= N) {
-          __builtin_memcpy(y, &codes, 4);
-        } else {
-#pragma unroll
-          for (int k = 0; k < N / 2; ++k) {
-            if (it.run * N + 2 * k < to.width) y[k] = static_cast<uint8_t>(codes >> (8 * k));
-          }
-        }
-        if (it.run % (kGroup / N) == 0)
-          reinterpret_cast<uint8_t*>(to.exponents)[page * to.exponent_stride[0] + it.head * to.exponent_stride[1] +
-                                                   slot * to.exponent_stride[2] + it.run / (kGroup / N)] =
-              static_cast<uint8_t>(e);
-      }
+    for (int i = 0; i < kPairRun / 2; ++i) {
+      const uint32_t low = w[i] & 0x7fffu;
+      const uint32_t high = (w[i] >> 16) & 0x7fffu;
+      most = most > low ? most : low;
+      most = most > high ? most : high;
     }
+    return __float_as_uint(Elem<T>::get(&most, 0));
   }
+}
+// Eight numbers over 2^(e - 127), e below 255, rounded to codes, half to even.
+template <typename T>
+__device__ __forceinline__ uint32_t to_codes(const uint32_t* w, int e) {
+  const float scale = __uint_as_float(static_cast<uint32_t>(e) << 23);  // its exponent alone counts: 0 is 2^-127
+  uint32_t codes = 0u;
+  if constexpr (sizeof(T) == 4) {
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, __uint_as_float(w[0]), __uint_as_float(w[1]), scale, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, __uint_as_float(w[2]), __uint_as_float(w[3]), scale, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, __uint_as_float(w[4]), __uint_as_float(w[5]), scale, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, __uint_as_float(w[6]), __uint_as_float(w[7]), scale, 3);
+  } else if constexpr (__is_same(T, Bf16)) {
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2, w[0]), scale, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2, w[1]), scale, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2, w[2]), scale, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2, w[3]), scale, 3);
+  } else {
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(codes, __builtin_bit_cast(f16x2, w[0]), scale, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(codes, __builtin_bit_cast(f16x2, w[1]), scale, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(codes, __builtin_bit_cast(f16x2, w[2]), scale, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(codes, __builtin_bit_cast(f16x2, w[3]), scale, 3);
+  }
+  return codes;
+}
+// What eight codes stand for, each number rounded once; NaN for e = 255.
+template <typename T>
+__device__ __forceinline__ RawVec<kPairRun * sizeof(T)> from_codes(uint32_t codes, int e) {
+  const float scale = __uint_as_float(static_cast<uint32_t>(e) << 23);
+  RawVec<kPairRun * sizeof(T)> r;
+  if constexpr (sizeof(T) == 4) {
+    const f32x2 x[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 0),
+                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 1),
+                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 2),
+                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 3)};
+    __builtin_memcpy(&r, x, sizeof(r));
+  } else if constexpr (__is_same(T, Bf16)) {
+    const bf16x2 x[4] = {__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0),
+                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1),
+                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2),
+                         __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3)};
+    __builtin_memcpy(&r, x, sizeof(r));
+  } else {
+    const f16x2 x[4] = {__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0),
+                        __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1),
+                        __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2),
+                        __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3)};
+    __builtin_memcpy(&r, x, sizeof(r));
+  }
+  return r;
+}
+
+// Rows of `kinds` tensors of one width, the first of them `kind`, into the pages.
+template <typename T>
+__device__ __forceinline__ void write_rows_e2m1(const TokenRows (&from)[2], const PagedCache& c, const PairOffsets& to,
+                                                int64_t first, int count, const PairRows& rows, int log_tokens, int kind,
+                                                int kinds) {
+  constexpr int N = kPairRun;
+  const int width = kind == 0 ? c.key.width : c.value.width;
+  RawVec<N * sizeof(T)> raw[kAhead];
+  const auto load = [&](int u, int kd, int token, int head, int run, bool live) {
+#pragma unroll
+    for (uint32_t& w : raw[u].w) w = 0u;
+    if (live && to.codes[kd][token] != kNoPlace) {
+      const int64_t at = (first + token) * (kd == 0 ? from[0].stride[0] : from[1].stride[0]) +
+                         head * (kd == 0 ? from[0].stride[1] : from[1].stride[1]) + run * N;
+      raw[u] = load_up_to<T, N>(static_cast<const T*>(kd == 0 ? from[0].data : from[1].data) + at, width - run * N);
+    }
+  };
+  const auto store = [&](int u, int kd, int token, int head, int run, bool live) {
+    uint32_t most = largest_bits<T>(raw[u].w);
+#pragma unroll
+    for (int o = 1; o < kPairGroup; o <<= 1) {
+      const uint32_t other = static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), o, 64));
+      most = most > other ? most : other;
+    }
+    const bool odd = most >= 0x7f800000u;
+    const int e = odd ? kNanExponent : group_exponent(__uint_as_float(most));
+    const uint32_t codes = odd ? 0u : to_codes<T>(raw[u].w, e);
+    if (live && to.codes[kd][token] != kNoPlace) {
+      const int64_t at = to.codes[kd][token] + head * (kd == 0 ? c.key.stride[1] : c.value.stride[1]) + run * (N / 2);
+      uint8_t* y = static_cast<uint8_t*>(kd == 0 ? c.key.data : c.value.data) + at;
+      if (width - run * N >= N) {
+        __builtin_memcpy(y, &codes, 4);
+      } else {
+#pragma unroll
+        for (int k = 0; k < N / 2; ++k) {
+          if (run * N + 2 * k < width) y[k] = static_cast<uint8_t>(codes >> (8 * k));
+        }
+      }
+      if (run % kPairGroup == 0)
+        reinterpret_cast<uint8_t*>(kd == 0 ? c.key.exponents : c.value.exponents)
+            [to.exponents[kd][token] + head * (kd == 0 ? c.key.exponent_stride[1] : c.value.exponent_stride[1]) +
+             run / kPairGroup] = static_cast<uint8_t>(e);
+    }
+  };
+  each_row(rows, width, c.heads, log_tokens, count, kind, kinds, load, store);
 }
 
 template <typename T>
-__device__ __forceinline__ void read_rows_e2m1(const PageTensor& from, const TokenRows& to, const Places& places,
-                                               int64_t first, int count, int heads, const RowItems& row,
-                                               int log_tokens) {
+__device__ __forceinline__ void read_rows_e2m1(const PagedCache& c, const TokenRows (&to)[2], const PairOffsets& from,
+                                               int64_t first, int count, const PairRows& rows, int log_tokens, int kind,
+                                               int kinds) {
   constexpr int N = kPairRun;
-  const int items = (heads << log_tokens) * row.runs;
-  for (int i0 = threadIdx.x; i0 < items; i0 += kAhead * kBlock) {
-    RawVec<4> raw[kAhead];
-    int e[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
-      raw[u].w[0] = 0u;
-      e[u] = 0;
-      if (it.head < heads && it.token < count && places.page[it.token] >= 0 && it.run * N < from.width) {
-        const int64_t page = places.page[it.token];
-        const int64_t slot = places.slot[it.token];
-        raw[u] = load_up_to<uint8_t, 4>(static_cast<const uint8_t*>(from.data) + page * from.stride[0] +
-                                            it.head * from.stride[1] + slot * from.stride[2] + it.run * (N / 2),
-                                        from.width / 2 - it.run * (N / 2));
-        e[u] = reinterpret_cast<const uint8_t*>(
-            from.exponents)[page * from.exponent_stride[0] + it.head * from.exponent_stride[1] +
-                            slot * from.exponent_stride[2] + it.run / (kGroup / N)];
-      }
+  const int width = kind == 0 ? c.key.width : c.value.width;
+  uint32_t codes[kAhead];
+  int e[kAhead];
+  const auto load = [&](int u, int kd, int token, int head, int run, bool live) {
+    codes[u] = 0u;
+    e[u] = 0;
+    if (live && from.codes[kd][token] != kNoPlace) {
+      const int64_t at = from.codes[kd][token] + head * (kd == 0 ? c.key.stride[1] : c.value.stride[1]) + run * (N / 2);
+      codes[u] = load_up_to<uint8_t, 4>(static_cast<const uint8_t*>(kd == 0 ? c.key.data : c.value.data) + at,
+                                        (width - run * N) / 2).w[0];
+      e[u] = reinterpret_cast<const uint8_t*>(kd == 0 ? c.key.exponents : c.value.exponents)
+          [from.exponents[kd][token] + head * (kd == 0 ? c.key.exponent_stride[1] : c.value.exponent_stride[1]) +
+           run / kPairGroup];
     }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const Item it = item_of(i0 + u * kBlock, row, log_tokens);
-      if (it.head >= heads || it.token >= count || it.run * N >= from.width) continue;
-      const float scale = group_scale(e[u]);
-      float x[N];
-      pairs_to_floats(raw[u].w[0], x);
-      T values[N];
-#pragma unroll
-      for (int k = 0; k < N; ++k) values[k] = rounded<T>(x[k] * scale);
-      T* y = static_cast<T*>(to.data) + (first + it.token) * to.stride[0] + it.head * to.stride[1] + it.run * N;
-      RawVec<N * sizeof(T)> r;
-      __builtin_memcpy(&r, values, sizeof(r));
-      // a row's last run may be a part of one
-      store_elements<true, N>(y, from.width - it.run * N, r);
-    }
-  }
+  };
+  const auto store = [&](int u, int kd, int token, int head, int run, bool live) {
+    if (!live) return;
+    const int64_t at = (first + token) * (kd == 0 ? to[0].stride[0] : to[1].stride[0]) +
+                       head * (kd == 0 ? to[0].stride[1] : to[1].stride[1]) + run * N;
+    // a row's last run may be a part of one
+    store_elements<true, N>(static_cast<T*>(kd == 0 ? to[0].data : to[1].data) + at, width - run * N,
+                            from_codes<T>(codes[u], e[u]));
+  };
+  each_row(rows, width, c.heads, log_tokens, count, kind, kinds, load, store);
 }
 
 struct RowShape {
@@ -402,32 +511,52 @@ __global__ __launch_bounds__(kBlock) void paged_read_kernel(PagedCache c, TokenR
   read_rows<C, T>(c.value, value, places, first, count, c.heads, shape.value, shape.log_tokens);
 }
 
+struct PairShape {
+  int log_tokens;
+  PairRows key;
+  PairRows value;
+};
+
 template <typename T>
 __global__ __launch_bounds__(kBlock) void paged_write_e2m1_kernel(PagedCache c, TokenRows key, TokenRows value,
                                                                   const int64_t* __restrict__ token_ptr,
                                                                   const int64_t* __restrict__ start, int64_t tokens,
-                                                                  RowShape shape) {
+                                                                  PairShape shape) {
   __shared__ Places places;
+  __shared__ PairOffsets offsets;
   const int64_t first = static_cast<int64_t>(blockIdx.x) << shape.log_tokens;
   const int64_t left = tokens - first;
   const int count = left < (1 << shape.log_tokens) ? static_cast<int>(left) : 1 << shape.log_tokens;
   find_places(c, token_ptr, start, first, count, places);
-  write_rows_e2m1<T>(key, c.key, places, first, count, c.heads, shape.key, shape.log_tokens);
-  write_rows_e2m1<T>(value, c.value, places, first, count, c.heads, shape.value, shape.log_tokens);
+  find_offsets(c, places, count, offsets);
+  const TokenRows rows[2] = {key, value};
+  if (c.key.width == c.value.width) {
+    write_rows_e2m1<T>(rows, c, offsets, first, count, shape.key, shape.log_tokens, 0, 2);
+  } else {
+    write_rows_e2m1<T>(rows, c, offsets, first, count, shape.key, shape.log_tokens, 0, 1);
+    write_rows_e2m1<T>(rows, c, offsets, first, count, shape.value, shape.log_tokens, 1, 1);
+  }
 }
 
 template <typename T>
 __global__ __launch_bounds__(kBlock) void paged_read_e2m1_kernel(PagedCache c, TokenRows key, TokenRows value,
-                                                                 const int64_t* __restrict__ token_ptr,
-                                                                 const int64_t* __restrict__ start, int64_t tokens,
-                                                                 RowShape shape) {
+                                                                  const int64_t* __restrict__ token_ptr,
+                                                                  const int64_t* __restrict__ start, int64_t tokens,
+                                                                  PairShape shape) {
   __shared__ Places places;
+  __shared__ PairOffsets offsets;
   const int64_t first = static_cast<int64_t>(blockIdx.x) << shape.log_tokens;
   const int64_t left = tokens - first;
   const int count = left < (1 << shape.log_tokens) ? static_cast<int>(left) : 1 << shape.log_tokens;
   find_places(c, token_ptr, start, first, count, places);
-  read_rows_e2m1<T>(c.key, key, places, first, count, c.heads, shape.key, shape.log_tokens);
-  read_rows_e2m1<T>(c.value, value, places, first, count, c.heads, shape.value, shape.log_tokens);
+  find_offsets(c, places, count, offsets);
+  const TokenRows rows[2] = {key, value};
+  if (c.key.width == c.value.width) {
+    read_rows_e2m1<T>(c, rows, offsets, first, count, shape.key, shape.log_tokens, 0, 2);
+  } else {
+    read_rows_e2m1<T>(c, rows, offsets, first, count, shape.key, shape.log_tokens, 0, 1);
+    read_rows_e2m1<T>(c, rows, offsets, first, count, shape.value, shape.log_tokens, 1, 1);
+  }
 }
 
 // Tokens of a workgroup: 16, fewer while that leaves fewer than 1,024 workgroups
@@ -438,9 +567,8 @@ RowShape row_shape(const PagedCache& c, int64_t tokens, int cache_dtype, int dty
   RowShape s{};
   const int elements = dtype == AS_DTYPE_F32 ? kElements<float> : kElements<Bf16>;
   const bool power_of_two = write && cache_dtype == AS_DTYPE_E4M3;
-  const bool pairs = cache_dtype == AS_DTYPE_E2M1;
-  s.key = pairs ? pair_items(c.key.width) : row_items(c.key.width, elements, power_of_two);
-  s.value = pairs ? pair_items(c.value.width) : row_items(c.value.width, elements, power_of_two);
+  s.key = row_items(c.key.width, elements, power_of_two);
+  s.value = row_items(c.value.width, elements, power_of_two);
   while ((2 << s.log_tokens) <= kMaxTokens && tokens >> (s.log_tokens + 1) >= 1024) ++s.log_tokens;
   return s;
 }
@@ -482,11 +610,12 @@ int as_paged_cache_write(const as_paged_cache* cache, const void* key, const int
   const TokenRows v{const_cast<void*>(value), {value_strides[0], value_strides[1]}};
   const RowShape shape = row_shape(c, tokens, cache->dtype, dtype, true);
   const dim3 grid(static_cast<unsigned>(((tokens - 1) >> shape.log_tokens) + 1));
+  const PairShape pairs{shape.log_tokens, pair_rows(c.key.width), pair_rows(c.value.width)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
     if (cache->dtype == AS_DTYPE_E2M1) {
-      paged_write_e2m1_kernel<T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
+      paged_write_e2m1_kernel<T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, pairs);
     } else if (cache->dtype == AS_DTYPE_E4M3) {
       paged_write_kernel<T, E4m3><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
     } else {
@@ -507,11 +636,12 @@ int as_paged_cache_read(const as_paged_cache* cache, void* key, void* value, con
   const TokenRows v{value, {int64_t(c.heads) * c.value.width, c.value.width}};
   const RowShape shape = row_shape(c, tokens, cache->dtype, dtype, false);
   const dim3 grid(static_cast<unsigned>(((tokens - 1) >> shape.log_tokens) + 1));
+  const PairShape pairs{shape.log_tokens, pair_rows(c.key.width), pair_rows(c.value.width)};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
     if (cache->dtype == AS_DTYPE_E2M1) {
-      paged_read_e2m1_kernel<T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
+      paged_read_e2m1_kernel<T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, pairs);
     } else if (cache->dtype == AS_DTYPE_E4M3) {
       paged_read_kernel<E4m3, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
     } else {

@@ -98,24 +98,6 @@ __device__ __forceinline__ int group_exponent(float largest) {
   if ((u & 0x7fffffu) > 0x400000u) ++e;
   return e < 0 ? 0 : e;
 }
-// 2^(e - 127), NaN for 255.
-__device__ __forceinline__ float group_scale(int e) {
-  return __uint_as_float(e == 0 ? 0x00400000u : (e == kNanExponent ? 0x7fc00000u : static_cast<uint32_t>(e) << 23));
-}
-// The 8 numbers of a word of codes, exactly.
-__device__ __forceinline__ void pairs_to_floats(uint32_t codes, float (&x)[8]) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 0);
-  const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 1);
-  const f32x2 c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 2);
-  const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, 3);
-  x[0] = a[0], x[1] = a[1], x[2] = b[0], x[3] = b[1], x[4] = c[0], x[5] = c[1], x[6] = d[0], x[7] = d[1];
-}
-// 2^(127 - e) for e < 255.
-__device__ __forceinline__ float group_unscale(int e) {
-  return __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-}
-
 template <typename T>
 __device__ __forceinline__ T rounded(float v);
 template <>

@@ -117,6 +117,10 @@ def _cpu_resize(page_table, lengths, change, free_pages, free_count, page_size: 
     return new_lengths, token_ptr, positions, slots
 
 
+def _long(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype is torch.long and t.is_contiguous() else t.to(torch.long).contiguous()
+
+
 def paged_cache_resize_impl(page_table, lengths, change, free_pages, free_count, page_size, tokens):
     page_size, tokens = int(page_size), int(tokens)
     _check(page_table, lengths, change, free_pages, free_count, page_size, tokens)
@@ -127,13 +131,13 @@ def paged_cache_resize_impl(page_table, lengths, change, free_pages, free_count,
     if not load_native():
         raise RuntimeError(f"AutoSAGE CUDA extension is unavailable: {native_load_error()}")
     lib = _native.library()
-    lengths, change = (t if t.dtype == torch.long and t.is_contiguous() else t.to(torch.long).contiguous()
-                       for t in (lengths, change))
+    lengths, change = _long(lengths), _long(change)
     sequences, room = page_table.shape
     device = page_table.device
     new_lengths = torch.empty(sequences, dtype=torch.long, device=device)
     token_ptr = torch.empty(sequences + 1, dtype=torch.long, device=device)
-    positions, slots = torch.empty(2, tokens, dtype=torch.long, device=device)
+    positions = torch.empty(tokens, dtype=torch.long, device=device)
+    slots = torch.empty(tokens, dtype=torch.long, device=device)
     # the kernel writes behind torch's back
     torch.autograd.graph.increment_version([page_table, free_pages, free_count])
     ws_bytes = lib.as_paged_cache_resize_workspace_bytes(sequences)
