@@ -146,10 +146,20 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
   const int n = lane & 15;
   const int g = lane >> 4;
   const int wave = uniform_i32(wave_in_block());
-  // the heads of a share follow one another: they share its pages
+  // The heads of a share follow one another: they share its pages.  Of two neighbouring heads the exponents of a
+  // page may share lines, so they are given to workgroups 8 apart, which the hardware gives to one of its 8 dies.
   const int units = c.heads * a.head_tiles;
-  const int share_index = static_cast<int>(blockIdx.x / static_cast<unsigned>(units));
-  const int unit = static_cast<int>(blockIdx.x) - share_index * units;
+  int block = static_cast<int>(blockIdx.x);
+  int in_pair = 0;
+  const bool paired = units % 2 == 0 && gridDim.x % 16 == 0;
+  if (paired) {
+    in_pair = (block >> 3) & 1;
+    block = ((block >> 4) << 3) + (block & 7);
+  }
+  const int unit_count = paired ? units / 2 : units;
+  const int share_index = static_cast<int>(static_cast<unsigned>(block) / static_cast<unsigned>(unit_count));
+  int unit = block - share_index * unit_count;
+  if (paired) unit = 2 * unit + in_pair;
   const int h = unit / a.head_tiles;
   const int tile_of_heads = unit - h * a.head_tiles;
   const int heads_q = c.heads * a.group;
