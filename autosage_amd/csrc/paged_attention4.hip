@@ -104,6 +104,12 @@ template <int I>
 struct Constant {
   static constexpr int value = I;
 };
+// 16 bytes at once, at any address of memory, and at a multiple of 16 in LDS.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(1), may_alias));
+typedef uint32_t u32x4_16 __attribute__((ext_vector_type(4), aligned(16), may_alias));
+__device__ __forceinline__ u32x4 load_16(const uint8_t* p) { return *reinterpret_cast<const u32x4_any*>(p); }
+__device__ __forceinline__ void store_16(uint8_t* p, u32x4 x) { *reinterpret_cast<u32x4_16*>(p) = x; }
+
 template <typename T>
 constexpr int kQueryParts = sizeof(T) == 4 ? 3 : (__is_same(T, Fp16) ? 2 : 1);
 template <typename T>
@@ -140,6 +146,12 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
   __shared__ float bias[BIASED ? kMaxBuckets : 1][kHeads];  // of the keys in front of the query
   __shared__ float wave_out[kOutWaves][kHeads][W];
   __shared__ u32x4 q_shared[kShared ? kSteps : 1][kQ][kShared ? kWave : 1];
+  // kStaged: a wave's tile on its way into registers.  Values of a block of 8 tokens, and a gap so that the four blocks
+  // of a read lie in banks of their own; exponents of the keys' tokens, then of the values'.
+  constexpr bool kStaged = MODE == kDense && W == 64;
+  constexpr int kBlockBytes = 4 * W + 32;
+  __shared__ __attribute__((aligned(16))) uint8_t staged_values[kStaged ? kWavesPerBlock : 1][kStaged ? 4 * kBlockBytes : 1];
+  __shared__ __attribute__((aligned(16))) uint8_t staged_e[kStaged ? kWavesPerBlock : 1][kStaged ? 2 * W : 1];
 
   const PagedCache& c = a.cache;
   const int lane = lane_id();
@@ -396,6 +408,78 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
       }
     };
 
+    // kStaged: loads of 16 bytes a lane, whose order is the memory's, and the turn to the lanes that use them in LDS
+    // (a few loads a tile where a lane that fetches its own takes 22, at 16 cycles of the address unit each).  64
+    // sequences of 16,384 tokens, 8 heads of 64: 136 us where direct loads take 152.  Rows of 128 have twice the work
+    // for each load: 64 sequences of 8,192 took 119 us both ways, uneven ones 77 against 75, and rows of 256 30 us
+    // against 28, so they load directly.  Lane l knows the page of block l % 4.
+    struct Staged {
+      u32x4 values;
+      u32x4 e;
+      uint32_t bad_tokens;
+    };
+    struct BlockId {
+      int64_t id;
+      int slot;
+    };
+    const auto block_id = [&](int t0) {
+      const int t = block_of(t0 + (lane & 3) * 8);
+      const int entry = page_of_token(a, t);
+      return BlockId{pages[entry], t - entry * c.page_size};
+    };
+    // (page, or -1, and slot) of a block
+    const auto page_and_slot = [&](const BlockId& b, int block) {
+      return make_int2(__shfl(is_bad(b.id) ? -1 : static_cast<int>(b.id), block, kWave), __shfl(b.slot, block, kWave));
+    };
+    const auto load_staged = [&](Staged& to, const BlockId& b) {
+      // the values of a block are 16 times 16 bytes, its exponents are 16 bytes
+      const int2 v = page_and_slot(b, lane >> 4);
+      to.values = load_16(value_base + page_offset(v.x < 0 ? 0 : v.x, c.value.stride[0]) + v.y * (W / 2) +
+                          (lane & 15) * 16);
+      const bool second = lane & 4;
+      const int2 e = page_and_slot(b, lane & 3);
+      to.e = load_16((second ? value_e_base : key_e_base) +
+                     page_offset(e.x < 0 ? 0 : e.x, second ? c.value.exponent_stride[0] : c.key.exponent_stride[0]) +
+                     e.y * (W / kGroup));
+      to.bad_tokens = page_and_slot(b, g).x < 0 ? 0xffu : 0u;
+    };
+    const auto load_dense_keys = [&](Keys& keys, const BlockId& b) {
+      const int2 p = page_and_slot(b, n >> 2);
+      const uint8_t* row = key_base + page_offset(p.x < 0 ? 0 : p.x, c.key.stride[0]) + (p.y + (n & 3)) * (W / 2);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int j = 0; j < kKeyRuns; ++j)
+          __builtin_memcpy(&keys.codes[s][j * kKeyWords], row + s * 4 * (W / 2) + key_word[j].at, 4 * kKeyWords);
+      }
+    };
+    const auto stage = [&](const Staged& from) {
+      store_16(&staged_values[wave][(lane >> 4) * kBlockBytes + (lane & 15) * 16], from.values);
+      store_16(&staged_e[wave][(lane & 7) * 16], from.e);  // lanes that have the same write the same
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    };
+    const auto unstage_keys = [&](Keys& keys) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int j = 0; j < kKeyRuns; ++j)
+          keys.e[s][j] = staged_e[wave][(key_token + 4 * s) * (W / kGroup) + key_e_at[j]];
+      }
+    };
+    const auto unstage_values = [&](Values& values) {
+#pragma unroll
+      for (int e = 0; e < kOwn; ++e) {
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j) {
+          const uint8_t* from = &staged_values[wave][g * kBlockBytes + e * (W / 2) + (j * 16 + n) * (kRun / 2)];
+          values.codes[j][e] = 0u;
+          __builtin_memcpy(&values.codes[j][e], from, kRun / 2);
+          values.e[j][e] = staged_e[wave][W + (own_token + e) * (W / kGroup) + value_e_at[j]];
+        }
+      }
+    };
+
     const auto products = [&](const Keys& keys, f32x4 (&score)[2]) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -523,23 +607,47 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
       // each kind of row takes the registers of the last tile's as soon as those are used up
       Keys keys;
       Values values;
-      Ids ids = ids_of(t0);
-      load_keys(keys, t0, ids);
-      load_values(values, t0, ids);
-      ids = ids_of(t0 + kStride);
-      for (;;) {
-        // the queries in LDS are read for every tile: kept, they would take the registers they are spared
-        if constexpr (kShared) asm volatile("" ::: "memory");
-        f32x4 score[2];
-        products(keys, score);
-        __builtin_amdgcn_sched_barrier(0);
-        load_keys(keys, t0 + kStride, ids);
-        weigh(values, score, t0);
-        __builtin_amdgcn_sched_barrier(0);
-        load_values(values, t0 + kStride, ids);
-        ids = ids_of(t0 + 2 * kStride);
-        t0 += kStride;
-        if (t0 >= end) break;
+      if constexpr (kStaged) {
+        Staged staged;
+        BlockId ids = block_id(t0);
+        load_dense_keys(keys, ids);
+        load_staged(staged, ids);
+        ids = block_id(t0 + kStride);
+        for (;;) {
+          stage(staged);
+          values.bad_tokens = staged.bad_tokens;
+          load_staged(staged, ids);
+          unstage_keys(keys);
+          f32x4 score[2];
+          products(keys, score);
+          __builtin_amdgcn_sched_barrier(0);
+          load_dense_keys(keys, ids);
+          ids = block_id(t0 + 2 * kStride);
+          unstage_values(values);
+          weigh(values, score, t0);
+          __builtin_amdgcn_sched_barrier(0);
+          t0 += kStride;
+          if (t0 >= end) break;
+        }
+      } else {
+        Ids ids = ids_of(t0);
+        load_keys(keys, t0, ids);
+        load_values(values, t0, ids);
+        ids = ids_of(t0 + kStride);
+        for (;;) {
+          // the queries in LDS are read for every tile: kept, they would take the registers they are spared
+          if constexpr (kShared) asm volatile("" ::: "memory");
+          f32x4 score[2];
+          products(keys, score);
+          __builtin_amdgcn_sched_barrier(0);
+          load_keys(keys, t0 + kStride, ids);
+          weigh(values, score, t0);
+          __builtin_amdgcn_sched_barrier(0);
+          load_values(values, t0 + kStride, ids);
+          ids = ids_of(t0 + 2 * kStride);
+          t0 += kStride;
+          if (t0 >= end) break;
+        }
       }
     }
 
