@@ -20,8 +20,15 @@
 //
 // A row of 128 is 68 bytes, half of an 8-bit one, and each of its numbers costs a vector
 // instruction or so: what bounds the kernel is how many loads are on the way while they
-// run.  Hence the next tile of a wave is asked for before this one is worked on (26
-// registers), and the page ids of the one after it.
+// run.  Hence the next tile of a wave is asked for before this one is worked on, its rows
+// taking over the registers of this one's as they are used up, and the page ids of the
+// one after it.
+//
+// Measured with the join, 8 key heads, 4 query heads each: 64 sequences of 8,192 tokens of
+// 128, bf16, 571 MB: 117 us, 4.9 TB/s (5.9 TB/s is what another 8,192 tokens each come in
+// at; the rest is launches, first loads and joins); of up to 8,192, 322 MB: 76; rows of 256,
+// 4,096 tokens: 109, 5.2 TB/s; of 64, 16,384 tokens: 132 to 136, 4.2 TB/s.  One sequence of
+// 17: 5.4 us.
 //
 // A token's page may be any, its length may end anywhere and its pages may hold
 // anything behind it: see the other kernel.
@@ -65,7 +72,8 @@ __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f
 // tokens of a head follow one another, so that the rows of a block are constants
 // apart.  kTokens: every token is looked up, and the last word
 // of a row is read where it ends with the row, and shifted.  kBytes: so it is, and words
-// are read a byte at a time, for rows of fewer than 4 bytes.
+// are read a byte at a time, for rows of fewer than 4 bytes.  64 sequences of up to 8,192
+// tokens, 8 key heads of 128, bf16: kDense 77 us, kWhole 105, kTokens 151.
 enum Mode { kDense, kWhole, kTokens, kBytes };
 constexpr bool in_blocks(int mode) { return mode == kDense || mode == kWhole; }
 

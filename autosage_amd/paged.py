@@ -8,8 +8,9 @@ be longer than the sequence needs so far (``page_ptr = arange(B + 1) * W`` makes
 a table of ``W`` entries a sequence).
 
 * ``paged_cache_write`` puts the rows of new tokens into their pages: as they
-  are, or as 8-bit numbers (``torch.float8_e4m3fn``) with one power of two for
-  each token and head;
+  are, as 8-bit numbers (``torch.float8_e4m3fn``) with one power of two for
+  each token and head, or as 4-bit ones (``torch.float4_e2m1fn_x2``) with one
+  for each 32 numbers of a row;
 * ``paged_cache_read`` gives the rows of any run of tokens back;
 * ``paged_attention`` is the attention of every sequence's last token over all
   tokens of the sequence, or over a window of the last ones.
@@ -451,10 +452,10 @@ def paged_cache_read(key_pages, value_pages, page_ptr, page_idx, token_ptr, star
     width]``: those of sequence ``b`` are its tokens from ``start[b]`` on and
     stand at ``token_ptr[b]:token_ptr[b + 1]``.  ``tokens`` is the number of
     rows of the result; rows of no sequence, and tokens without a page, are
-    zeros.  ``float8_e4m3fn`` pages give the numbers they stand for in
-    ``dtype`` (default bfloat16, which holds them exactly unless they are below
-    its smallest number; infinite where they are beyond its largest), other pages
-    their own dtype."""
+    zeros.  ``float8_e4m3fn`` and ``float4_e2m1fn_x2`` pages give the numbers they
+    stand for in ``dtype`` (default bfloat16, which holds them exactly unless they
+    are below its smallest number; infinite where they are beyond its largest),
+    other pages their own dtype."""
     return paged_cache_read_impl(key_pages, value_pages, page_ptr, page_idx, token_ptr, start, tokens, dtype,
                                  key_exponents, value_exponents)
 
@@ -611,8 +612,9 @@ def paged_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, 
 
     Scores, softmax and sums are float32 and the result is rounded once to the
     dtype of ``query``.  (Over 8-bit pages a query is multiplied with the codes,
-    so that finite numbers beyond 2^111 may give infinite scores.)  A sequence without tokens, or with scores of -inf alone,
-    gives zeros; a length beyond ``max_length`` or the sequence's pages, or a
+    so that finite numbers beyond 2^111 may give infinite scores.  On the GPU
+    numbers of 4-bit pages below 2^-126 count as zeros.)  A sequence without
+    tokens, or with scores of -inf alone, gives zeros; a length beyond ``max_length`` or the sequence's pages, or a
     page id outside the cache, gives NaN.  ``return_lse`` adds the logarithm of
     the sum of the exponentials, float32 ``[sequences, query heads]``, with which
     results over parts of a sequence can be joined."""
