@@ -75,7 +75,7 @@ def _check(query, key, positions, frequencies) -> None:
     if (query.dim() == 3 and (key is None or (key.dim() == 3 and key.dtype is query.dtype
                                               and key.size(0) == query.size(0) and key.size(2) == query.size(2)
                                               and key.device == query.device))
-            and query.is_floating_point() and query.size(2) >= 1
+            and query.is_floating_point() and query.size(2) >= 1 and not has_tangent(frequencies)
             and positions.dtype is torch.long and positions.shape == query.shape[:1]
             and frequencies.dtype is torch.float64 and frequencies.dim() == 1
             and 2 * frequencies.size(0) <= query.size(2) and not frequencies.requires_grad
@@ -98,6 +98,7 @@ def _check(query, key, positions, frequencies) -> None:
         _require(t is None or t.device == query.device, ValueError, f"{name} must be on the device of query")
     _require(not (torch.is_grad_enabled() and frequencies.requires_grad), RuntimeError,
              "rotary_positions has no gradient for frequencies")
+    _require(not has_tangent(frequencies), RuntimeError, "rotary_positions has no derivative for frequencies")
 
 
 def _cpu_turn(x, cos, sin, interleaved: bool):

@@ -148,3 +148,22 @@ def test_native_argument_checks_come_before_any_launch():
     ]:
         assert call() == status, message
         assert lib.as_last_error().startswith(message), lib.as_last_error()
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32])
+def test_frequencies_have_no_derivative(dtype):
+    query = torch.randn(3, 2, 8)
+    positions = torch.arange(3)
+    frequencies = autosage_amd.rotary_frequencies(8).to(dtype)
+
+    def turned(f):
+        return autosage_amd.rotary_positions(query, None, positions, f)[0]
+
+    with pytest.raises(RuntimeError, match="no gradient for frequencies"):
+        turned(frequencies.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="no derivative for frequencies"):
+        torch.func.jvp(turned, (frequencies,), (torch.ones_like(frequencies),))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(frequencies, torch.ones_like(frequencies))
+        with pytest.raises(RuntimeError, match="no derivative for frequencies"):
+            turned(dual)
