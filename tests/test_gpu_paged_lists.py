@@ -40,6 +40,12 @@ def test_many_tokens(sequences, room, page_size, most, spare):
     _resize(batch(sequences, room, page_size, 5, spare=spare, grow=0.8, drop=0.1, most=most), page_size)
 
 
+@pytest.mark.parametrize("sequences, room", [(9, 4000), (40, 819), (40, 820), (1024, 32), (1024, 33)])
+def test_lists_with_room_for_many_pages(sequences, room):
+    """Some of them end, while the others get a token or none."""
+    _resize(batch(sequences, room, 4, 12, spare=0.7, grow=0.4, drop=0.3, most=1), 4)
+
+
 @pytest.mark.parametrize("sequences, most", [(12, 16), (500, 3), (12, 3000)])
 def test_everything_comes_and_goes(sequences, most):
     """All sequences grow, all shrink to nothing, and the pages go round; a drop undoes a growth."""
