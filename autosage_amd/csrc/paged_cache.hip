@@ -247,27 +247,27 @@ __device__ __forceinline__ void read_rows(const PageTensor& from, const TokenRow
 // sides and a group's maximum takes two shuffles.  Rows are cut at whole groups; what
 // passes a row's end counts as zeros and is not stored.  Eight numbers are little work,
 // so what they need besides counts: a thread has one run of a row, and that of every
-// step-th, and where a token's rows lie is found once.  Keys and values of one width
-// are the rows of one list, else two.  A write goes through the tokens of a head, which
+// step-th, where a token's rows lie is found once, and a workgroup has keys or values.
+// A write goes through the tokens of a head, which
 // are neighbours in a page; a read through the heads of a token, which are neighbours
 // in the result, so that what goes past the caches fills its lines (20,245 tokens, 10
-// heads of 72, fp16: write 24 us, read 21; 30 through the tokens of a head).
+// heads of 72, fp16, read 21 us; 30 through the tokens of a head).  Keys and values in
+// workgroups of their own, whose strides are then the same for all lanes: write and
+// read 39.5 us, 42.5 where both are in one; 16 heads of 40 33 and 42.
 constexpr int kPairRun = 8;
 constexpr int kPairGroup = kGroup / kPairRun;  // lanes that share an exponent
 constexpr int64_t kNoPlace = INT64_MIN;
 struct PairOffsets {
-  int64_t codes[2][kMaxTokens];  // of keys and values; kNoPlace: none
-  int64_t exponents[2][kMaxTokens];
+  int64_t codes[kMaxTokens];  // kNoPlace: none
+  int64_t exponents[kMaxTokens];
 };
-__device__ __forceinline__ void find_offsets(const PagedCache& c, const Places& places, int count, PairOffsets& to) {
-  if (threadIdx.x < 2 * kMaxTokens) {
-    const int token = static_cast<int>(threadIdx.x) % kMaxTokens;
-    const int kind = static_cast<int>(threadIdx.x) / kMaxTokens;
-    const PageTensor& t = kind == 0 ? c.key : c.value;
+__device__ __forceinline__ void find_offsets(const PageTensor& t, const Places& places, int count, PairOffsets& to) {
+  if (threadIdx.x < kMaxTokens) {
+    const int token = static_cast<int>(threadIdx.x);
     const int64_t page = token < count ? places.page[token] : -1;
     const int64_t slot = token < count ? places.slot[token] : 0;
-    to.codes[kind][token] = page < 0 ? kNoPlace : page * t.stride[0] + slot * t.stride[2];
-    to.exponents[kind][token] = page * t.exponent_stride[0] + slot * t.exponent_stride[2];
+    to.codes[token] = page < 0 ? kNoPlace : page * t.stride[0] + slot * t.stride[2];
+    to.exponents[token] = page * t.exponent_stride[0] + slot * t.exponent_stride[2];
   }
   __syncthreads();
 }
@@ -285,24 +285,21 @@ inline PairRows pair_rows(int width, int heads, int run) {
   return PairRows{items.runs, kBlock / items.runs, items.shift, items.magic, row_items(heads, 1, false)};
 }
 
-// Calls f(u, kind, token, head, run, whether it is there) for the rows of `kinds` tensors, kPairAhead of them at a time,
-// first f of all, then g.  HEADS: the heads of a token follow one another, else the tokens of a head.
+// Calls f(u, row, token, head, run, whether it is there) for the rows of a tensor, kPairAhead of them at a time, first f
+// of all, then g.  HEADS: the heads of a token follow one another, else the tokens of a head.
 template <bool HEADS, int RUN, typename F, typename G>
-__device__ __forceinline__ void each_row(const PairRows& rows, int width, int heads, int log_tokens, int count, int kind,
-                                         int kinds, F&& f, G&& g) {
+__device__ __forceinline__ void each_row(const PairRows& rows, int width, int heads, int log_tokens, int count, F&& f,
+                                         G&& g) {
   const int row0 = static_cast<int>((static_cast<uint64_t>(threadIdx.x) * rows.magic) >> (31 + rows.shift));
   const int run = static_cast<int>(threadIdx.x) - row0 * rows.runs;
-  const int per_kind = heads << log_tokens;
-  const int all = kinds * per_kind;
+  const int all = heads << log_tokens;
   const bool in_row = row0 < rows.step && run * RUN < width;
   for (int r0 = 0; r0 < all; r0 += kPairAhead * rows.step) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
 #pragma unroll
       for (int u = 0; u < kPairAhead; ++u) {
-        const int r = r0 + u * rows.step + row0;
-        const bool second = r >= per_kind;
-        const int at = second ? r - per_kind : r;
+        const int at = r0 + u * rows.step + row0;
         int token = at & ((1 << log_tokens) - 1);
         int head = at >> log_tokens;
         if constexpr (HEADS) {
@@ -310,11 +307,11 @@ __device__ __forceinline__ void each_row(const PairRows& rows, int width, int he
                                    (31 + rows.heads.shift));
           head = at - token * heads;
         }
-        const bool live = in_row && r < all && token < count;
+        const bool live = in_row && at < all && token < count;
         if (half == 0) {
-          f(u, second ? 1 : kind, token, head, run, live);
+          f(u, at, token, head, run, live);
         } else {
-          g(u, second ? 1 : kind, token, head, run, live);
+          g(u, at, token, head, run, live);
         }
       }
     }
@@ -410,24 +407,22 @@ __device__ __forceinline__ RawVec<N * sizeof(T)> from_codes(uint32_t codes, int 
   return r;
 }
 
-// Rows of `kinds` tensors of one width, the first of them `kind`, into the pages.
 template <typename T>
-__device__ __forceinline__ void write_rows_e2m1(const TokenRows (&from)[2], const PagedCache& c, const PairOffsets& to,
-                                                int64_t first, int count, const PairRows& rows, int log_tokens, int kind,
-                                                int kinds) {
+__device__ __forceinline__ void write_rows_e2m1(const TokenRows& from, const PageTensor& t, const PairOffsets& to,
+                                                int64_t first, int count, int heads, const PairRows& rows,
+                                                int log_tokens) {
   constexpr int N = kPairRun;
-  const int width = kind == 0 ? c.key.width : c.value.width;
+  const T* const tokens = static_cast<const T*>(from.data) + first * from.stride[0];
+  uint8_t* const codes_to = static_cast<uint8_t*>(t.data);
+  uint8_t* const exponents_to = reinterpret_cast<uint8_t*>(t.exponents);
   RawVec<N * sizeof(T)> raw[kPairAhead];
-  const auto load = [&](int u, int kd, int token, int head, int run, bool live) {
+  const auto load = [&](int u, int, int token, int head, int run, bool live) {
 #pragma unroll
     for (uint32_t& w : raw[u].w) w = 0u;
-    if (live && to.codes[kd][token] != kNoPlace) {
-      const int64_t at = (first + token) * (kd == 0 ? from[0].stride[0] : from[1].stride[0]) +
-                         head * (kd == 0 ? from[0].stride[1] : from[1].stride[1]) + run * N;
-      raw[u] = load_up_to<T, N>(static_cast<const T*>(kd == 0 ? from[0].data : from[1].data) + at, width - run * N);
-    }
+    if (live && to.codes[token] != kNoPlace)
+      raw[u] = load_up_to<T, N>(tokens + token * from.stride[0] + head * from.stride[1] + run * N, t.width - run * N);
   };
-  const auto store = [&](int u, int kd, int token, int head, int run, bool live) {
+  const auto store = [&](int u, int, int token, int head, int run, bool live) {
     uint32_t most = largest_bits<T>(raw[u].w);
 #pragma unroll
     for (int o = 1; o < kPairGroup; o <<= 1) {
@@ -437,55 +432,48 @@ __device__ __forceinline__ void write_rows_e2m1(const TokenRows (&from)[2], cons
     const bool odd = most >= 0x7f800000u;
     const int e = odd ? kNanExponent : group_exponent(__uint_as_float(most));
     const uint32_t codes = odd ? 0u : to_codes<T>(raw[u].w, e);
-    if (live && to.codes[kd][token] != kNoPlace) {
-      const int64_t at = to.codes[kd][token] + head * (kd == 0 ? c.key.stride[1] : c.value.stride[1]) + run * (N / 2);
-      uint8_t* y = static_cast<uint8_t*>(kd == 0 ? c.key.data : c.value.data) + at;
-      if (width - run * N >= N) {
+    if (live && to.codes[token] != kNoPlace) {
+      uint8_t* y = codes_to + to.codes[token] + head * t.stride[1] + run * (N / 2);
+      if (t.width - run * N >= N) {
         __builtin_memcpy(y, &codes, 4);
       } else {
 #pragma unroll
         for (int k = 0; k < N / 2; ++k) {
-          if (run * N + 2 * k < width) y[k] = static_cast<uint8_t>(codes >> (8 * k));
+          if (run * N + 2 * k < t.width) y[k] = static_cast<uint8_t>(codes >> (8 * k));
         }
       }
       if (run % kPairGroup == 0)
-        reinterpret_cast<uint8_t*>(kd == 0 ? c.key.exponents : c.value.exponents)
-            [to.exponents[kd][token] + head * (kd == 0 ? c.key.exponent_stride[1] : c.value.exponent_stride[1]) +
-             run / kPairGroup] = static_cast<uint8_t>(e);
+        exponents_to[to.exponents[token] + head * t.exponent_stride[1] + run / kPairGroup] = static_cast<uint8_t>(e);
     }
   };
-  each_row<false, N>(rows, width, c.heads, log_tokens, count, kind, kinds, load, store);
+  each_row<false, N>(rows, t.width, heads, log_tokens, count, load, store);
 }
 
 template <typename T>
-__device__ __forceinline__ void read_rows_e2m1(const PagedCache& c, const TokenRows (&to)[2], const PairOffsets& from,
-                                               int64_t first, int count, const PairRows& rows, int log_tokens, int kind,
-                                               int kinds) {
+__device__ __forceinline__ void read_rows_e2m1(const PageTensor& t, const TokenRows& to, const PairOffsets& from,
+                                               int64_t first, int count, int heads, const PairRows& rows,
+                                               int log_tokens) {
   constexpr int N = kElements<T>;
-  const int width = kind == 0 ? c.key.width : c.value.width;
+  T* const tokens = static_cast<T*>(to.data) + first * to.stride[0];
+  const uint8_t* const codes_from = static_cast<const uint8_t*>(t.data);
+  const uint8_t* const exponents_from = reinterpret_cast<const uint8_t*>(t.exponents);
   uint32_t codes[kPairAhead];
   int e[kPairAhead];
-  const auto load = [&](int u, int kd, int token, int head, int run, bool live) {
+  const auto load = [&](int u, int, int token, int head, int run, bool live) {
     codes[u] = 0u;
     e[u] = 0;
-    if (live && from.codes[kd][token] != kNoPlace) {
-      const int64_t at = from.codes[kd][token] + head * (kd == 0 ? c.key.stride[1] : c.value.stride[1]) + run * (N / 2);
-      codes[u] = load_up_to<uint8_t, N / 2>(static_cast<const uint8_t*>(kd == 0 ? c.key.data : c.value.data) + at,
-                                        (width - run * N) / 2).w[0];
-      e[u] = reinterpret_cast<const uint8_t*>(kd == 0 ? c.key.exponents : c.value.exponents)
-          [from.exponents[kd][token] + head * (kd == 0 ? c.key.exponent_stride[1] : c.value.exponent_stride[1]) +
-           run / (kGroup / N)];
+    if (live && from.codes[token] != kNoPlace) {
+      codes[u] = load_up_to<uint8_t, N / 2>(codes_from + from.codes[token] + head * t.stride[1] + run * (N / 2),
+                                            (t.width - run * N) / 2).w[0];
+      e[u] = exponents_from[from.exponents[token] + head * t.exponent_stride[1] + run / (kGroup / N)];
     }
   };
-  const auto store = [&](int u, int kd, int token, int head, int run, bool live) {
+  const auto store = [&](int u, int row, int, int, int run, bool live) {
     if (!live) return;
-    const int64_t at = (first + token) * (kd == 0 ? to[0].stride[0] : to[1].stride[0]) +
-                       head * (kd == 0 ? to[0].stride[1] : to[1].stride[1]) + run * N;
-    // a row's last run may be a part of one
-    store_elements<true, N>(static_cast<T*>(kd == 0 ? to[0].data : to[1].data) + at, width - run * N,
-                            from_codes<T, N>(codes[u], e[u]));
+    // the results' rows are dense; a row's last run may be a part of one
+    store_elements<true, N>(tokens + (row * t.width + run * N), t.width - run * N, from_codes<T, N>(codes[u], e[u]));
   };
-  each_row<true, N>(rows, width, c.heads, log_tokens, count, kind, kinds, load, store);
+  each_row<true, N>(rows, t.width, heads, log_tokens, count, load, store);
 }
 
 struct RowShape {
@@ -538,15 +526,11 @@ __global__ __launch_bounds__(kBlock) void paged_write_e2m1_kernel(PagedCache c, 
   const int64_t first = static_cast<int64_t>(blockIdx.x) << shape.log_tokens;
   const int64_t left = tokens - first;
   const int count = left < (1 << shape.log_tokens) ? static_cast<int>(left) : 1 << shape.log_tokens;
+  const PageTensor t = blockIdx.y == 0 ? c.key : c.value;
+  const PairRows rows = blockIdx.y == 0 ? shape.key : shape.value;
   find_places(c, token_ptr, start, first, count, places);
-  find_offsets(c, places, count, offsets);
-  const TokenRows rows[2] = {key, value};
-  if (c.key.width == c.value.width) {
-    write_rows_e2m1<T>(rows, c, offsets, first, count, shape.key, shape.log_tokens, 0, 2);
-  } else {
-    write_rows_e2m1<T>(rows, c, offsets, first, count, shape.key, shape.log_tokens, 0, 1);
-    write_rows_e2m1<T>(rows, c, offsets, first, count, shape.value, shape.log_tokens, 1, 1);
-  }
+  find_offsets(t, places, count, offsets);
+  write_rows_e2m1<T>(blockIdx.y == 0 ? key : value, t, offsets, first, count, c.heads, rows, shape.log_tokens);
 }
 
 template <typename T>
@@ -559,28 +543,27 @@ __global__ __launch_bounds__(kBlock) void paged_read_e2m1_kernel(PagedCache c, T
   const int64_t first = static_cast<int64_t>(blockIdx.x) << shape.log_tokens;
   const int64_t left = tokens - first;
   const int count = left < (1 << shape.log_tokens) ? static_cast<int>(left) : 1 << shape.log_tokens;
+  const PageTensor t = blockIdx.y == 0 ? c.key : c.value;
+  const PairRows rows = blockIdx.y == 0 ? shape.key : shape.value;
   find_places(c, token_ptr, start, first, count, places);
-  find_offsets(c, places, count, offsets);
-  const TokenRows rows[2] = {key, value};
-  if (c.key.width == c.value.width) {
-    read_rows_e2m1<T>(c, rows, offsets, first, count, shape.key, shape.log_tokens, 0, 2);
-  } else {
-    read_rows_e2m1<T>(c, rows, offsets, first, count, shape.key, shape.log_tokens, 0, 1);
-    read_rows_e2m1<T>(c, rows, offsets, first, count, shape.value, shape.log_tokens, 1, 1);
-  }
+  find_offsets(t, places, count, offsets);
+  read_rows_e2m1<T>(t, blockIdx.y == 0 ? key : value, offsets, first, count, c.heads, rows, shape.log_tokens);
 }
 
 // Tokens of a workgroup: 16, fewer while that leaves fewer than 1,024 workgroups
 // (writes of 2,048 tokens, 8 heads of 128, bf16: 7.1 us; 7.8 with down to 256
 // workgroups, 9.0 with 4,096; of 8,192 tokens 12.7, 15.4 and 17.7; of 32,768 tokens
-// 44.6, 44.7 and 40.7; reads alike).
+// 44.6, 44.7 and 40.7; reads alike).  Of 4-bit pages fewer than 512 for keys and as many
+// for values (4 heads of 64, bf16, up to 16 x 1,700 tokens written and read: 15.0 us;
+// 21.2 with 1,024, 14.0 with 256, where 8 heads of 192 and 128 take 20.6, 24.8 and 22.2).
 RowShape row_shape(const PagedCache& c, int64_t tokens, int cache_dtype, int dtype, bool write) {
   RowShape s{};
   const int elements = dtype == AS_DTYPE_F32 ? kElements<float> : kElements<Bf16>;
   const bool power_of_two = write && cache_dtype == AS_DTYPE_E4M3;
   s.key = row_items(c.key.width, elements, power_of_two);
   s.value = row_items(c.value.width, elements, power_of_two);
-  while ((2 << s.log_tokens) <= kMaxTokens && tokens >> (s.log_tokens + 1) >= 1024) ++s.log_tokens;
+  const int64_t blocks = cache_dtype == AS_DTYPE_E2M1 ? 512 : 1024;
+  while ((2 << s.log_tokens) <= kMaxTokens && tokens >> (s.log_tokens + 1) >= blocks) ++s.log_tokens;
   return s;
 }
 
@@ -627,7 +610,7 @@ int as_paged_cache_write(const as_paged_cache* cache, const void* key, const int
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
     if (cache->dtype == AS_DTYPE_E2M1) {
-      paged_write_e2m1_kernel<T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, pairs);
+      paged_write_e2m1_kernel<T><<<dim3(grid.x, 2), kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, pairs);
     } else if (cache->dtype == AS_DTYPE_E4M3) {
       paged_write_kernel<T, E4m3><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
     } else {
@@ -654,7 +637,7 @@ int as_paged_cache_read(const as_paged_cache* cache, void* key, void* value, con
   return with_float_element(dtype, [&](auto e) {
     using T = decltype(e);
     if (cache->dtype == AS_DTYPE_E2M1) {
-      paged_read_e2m1_kernel<T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, pairs);
+      paged_read_e2m1_kernel<T><<<dim3(grid.x, 2), kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, pairs);
     } else if (cache->dtype == AS_DTYPE_E4M3) {
       paged_read_kernel<E4m3, T><<<grid, kBlock, 0, s>>>(c, k, v, token_ptr, start, tokens, shape);
     } else {
