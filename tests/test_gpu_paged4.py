@@ -88,6 +88,31 @@ def test_write_then_read(dtype, width, value_width, page):
         assert torch.equal(exponents.view(torch.uint8).cpu(), want)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("tokens, heads, width, value_width", [(3, 300, 34, 34), (40, 129, 2, 66), (1030, 1, 6, 96),
+                                                               (2051, 3, 40, 40), (8200, 2, 64, 192), (16390, 5, 32, 10)])
+def test_many_tokens_and_heads(dtype, tokens, heads, width, value_width):
+    """From one token a workgroup to all that it takes: pages and rows as on the CPU."""
+    gen = torch.Generator().manual_seed(tokens)
+    rows = [torch.randn(tokens + 2, heads, w, generator=gen).to(dtype) for w in (width, value_width)]
+    lengths = [tokens // 3, tokens - tokens // 3 - 1, 1]
+    counts = [-(-(n + 1) // 5) for n in lengths]
+    order = torch.randperm(sum(counts), generator=gen)
+    results = []
+    for device in ("cpu", "cuda"):
+        pages = [torch.zeros(sum(counts), heads, 5, w // 2, dtype=torch.uint8, device=device).view(E2M1)
+                 for w in (width, value_width)]
+        e = [torch.zeros(sum(counts), heads, 5, -(-w // 32), dtype=torch.uint8, device=device).view(E8M0)
+             for w in (width, value_width)]
+        names = dict(zip(("key_exponents", "value_exponents"), e))
+        span = [torch.tensor([0] + counts).cumsum(0), order, torch.tensor([1] + lengths).cumsum(0), torch.tensor([1, 1, 1])]
+        span = [t.to(device) for t in span]
+        autosage_amd.paged_cache_write(*(r.to(device) for r in rows), *pages, *span, **names)
+        back = autosage_amd.paged_cache_read(*pages, *span, tokens + 2, dtype=dtype, **names)
+        results.append([t.view(torch.uint8).cpu() for t in (*pages, *e)] + [t.cpu() for t in back])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 def test_the_gpu_holds_what_the_cpu_holds():
     """Random bits of float32 and all numbers of the 16-bit types, those that are not finite among them."""
     gen = torch.Generator().manual_seed(3)
