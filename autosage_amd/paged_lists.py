@@ -35,7 +35,8 @@ def _check(page_table, lengths, change, free_pages, free_count, page_size: int, 
             and lengths.dtype is torch.long and change.dtype is torch.long
             and lengths.shape == change.shape == page_table.shape[:1]
             and page_table.is_contiguous() and free_pages.is_contiguous()
-            and page_table.device == lengths.device == change.device == free_pages.device == free_count.device and page_size >= 1 and tokens >= 0
+            and page_table.device == lengths.device == change.device == free_pages.device == free_count.device
+            and page_size >= 1 and tokens >= 0
             and page_table.size(1) * page_size <= _MOST_TOKENS // 2):
         return
     for name, t in (("page_table", page_table), ("free_pages", free_pages), ("free_count", free_count)):

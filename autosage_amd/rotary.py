@@ -268,13 +268,15 @@ def rotary_positions(query, key, positions, frequencies, *, interleaved: bool = 
     sin + b cos)``.  The rest of a row stays as it is.
 
     ``query`` is ``[tokens, heads, width]`` and ``key``, which may be None, ``[tokens, key heads, width]``, of the same
-    dtype (on the GPU float32, bfloat16 or float16), and may be slices of one projection.  Pairs are ``(x[i], x[i + n])``, or with
-    ``interleaved`` ``(x[2 i], x[2 i + 1])``.  ``frequencies`` (``rotary_frequencies``) are float64; ``positions`` one integer per token, the
-    ``positions`` of ``paged_cache_resize`` or the numbers of a graph's nodes.
+    dtype (on the GPU float32, bfloat16 or float16, and a width of at most 1,024), and may be slices of one projection.
+    Pairs are ``(x[i], x[i + n])``, or with ``interleaved`` ``(x[2 i], x[2 i + 1])``.  ``frequencies``
+    (``rotary_frequencies``) are float64; ``positions`` one integer per token, the ``positions`` of
+    ``paged_cache_resize`` or the numbers of a graph's nodes.
 
     The angle is computed and reduced in float64, so that a position of a million is as exact as
-    one of ten; the pairs are turned in float32 and rounded once.  Both results are new, contiguous tensors with gradients of
-    every order, forward-mode derivatives and rules for ``torch.func``'s transforms; there is none for ``frequencies``."""
+    one of ten; the pairs are turned in float32 and rounded once.  Both results are new, contiguous tensors with
+    gradients of every order, forward-mode derivatives and rules for ``torch.func``'s transforms; a derivative for
+    ``frequencies`` is refused."""
     _check(query, key, positions, frequencies)
     interleaved, magnitude = bool(interleaved), float(magnitude)
     if not query.is_cuda:
