@@ -6,6 +6,7 @@
 #include <cstdint>
 
 #include "as_device.h"
+#include "raw_vec.h"
 
 namespace as {
 namespace {
@@ -81,12 +82,6 @@ struct Elem<Fp16> {
   __device__ static void put(Fp16* p, double v) { p->bits = bits(v); }
 };
 
-// BYTES consecutive bytes (2, 4, 8 or 16, naturally aligned) as 32-bit words;
-// a 2-byte load fills the low half of w[0].
-template <int BYTES>
-struct RawVec {
-  uint32_t w[BYTES >= 4 ? BYTES / 4 : 1];
-};
 template <int BYTES>
 __device__ __forceinline__ RawVec<BYTES> load_raw(const char* p) {
   RawVec<BYTES> r;

@@ -88,6 +88,7 @@ __device__ __forceinline__ int run_start(int d, int n, int width) {
 template <typename C, int N, int MODE>
 __device__ __forceinline__ RawVec<N * sizeof(C)> load_run(const C* __restrict__ row, int start, int width) {
   RawVec<N * sizeof(C)> r;
+  static_assert(sizeof(r) == N * sizeof(C));
   if constexpr (MODE != kNarrow) {
     __builtin_memcpy(&r, row + start, sizeof(r));
   } else {

@@ -78,6 +78,7 @@ __device__ __forceinline__ int run_start(int d, int n, int width) {
 template <int N, typename E>
 __device__ __forceinline__ RawVec<N * sizeof(E)> load_elements(const E* from, int width) {
   RawVec<N * sizeof(E)> r;
+  static_assert(sizeof(r) == N * sizeof(E));
   if (width >= N) {
     __builtin_memcpy(&r, from, sizeof(r));
   } else {
@@ -93,6 +94,7 @@ typedef uint32_t u32x4_a1 __attribute__((ext_vector_type(4), aligned(1)));
 // 6.0 TB/s; 95 through them).  What is written to the pages stays: attention reads it next.
 template <bool STREAM, int N, typename E>
 __device__ __forceinline__ void store_elements(E* to, int width, const RawVec<N * sizeof(E)>& r) {
+  static_assert(sizeof(r) == N * sizeof(E));
   if (width >= N) {
     if constexpr (STREAM) {
 #pragma unroll
@@ -318,20 +320,6 @@ __device__ __forceinline__ void each_row(const PairRows& rows, int width, int he
   }
 }
 
-template <typename E, int N>
-__device__ __forceinline__ RawVec<N * sizeof(E)> load_up_to(const E* from, int left) {
-  RawVec<N * sizeof(E)> r;
-  if (left >= N) {
-    __builtin_memcpy(&r, from, sizeof(r));
-  } else {
-    E part[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) part[i] = i < left ? from[i] : E{};
-    __builtin_memcpy(&r, part, sizeof(r));
-  }
-  return r;
-}
-
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -386,6 +374,7 @@ template <typename T, int N>
 __device__ __forceinline__ RawVec<N * sizeof(T)> from_codes(uint32_t codes, int e) {
   const float scale = __uint_as_float(static_cast<uint32_t>(e) << 23);
   RawVec<N * sizeof(T)> r;
+  static_assert(sizeof(r) == N * sizeof(T));
   if constexpr (sizeof(T) == 4) {
     static_assert(N == 4);
     const f32x2 x[2] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, scale, 0),
