@@ -239,7 +239,8 @@ SCHEMAS = {
 
 def _setup(ctx, inputs, output) -> None:
     ctx.set_materialize_grads(False)
-    ctx.save_for_backward(*inputs[2:4])
+    # as the kernel reads them, which is not how they may have been given
+    ctx.save_for_backward(*_plan(*inputs[2:4]))
     ctx.how = (*inputs[4:], *(False, 1.0, False)[len(inputs) - 4:])  # arguments that are the default may be left out
     ctx.with_key = inputs[1] is not None
 

@@ -1,0 +1,38 @@
+"""The registered operator of rotary positions on the GPU: gradients of plans that it converts."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import autosage_amd
+from tests.gpu_common import require_gpu
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    require_gpu()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("at", ["32 bits", "a column", "one for all"])
+@pytest.mark.parametrize("angles", ["64 bits", "32 bits", "a column"])
+def test_gradients_of_converted_plans(dtype, at, angles):
+    """Those of the public call, whose plan is converted once in front of both directions."""
+    gen = torch.Generator().manual_seed(1)
+    positions = torch.randint(0, 5000, (70,), generator=gen).cuda()
+    positions = {"32 bits": positions.int(), "a column": torch.stack((positions, positions + 1), 1)[:, 0],
+                 "one for all": positions[:1].expand(70)}[at]
+    f = autosage_amd.rotary_frequencies(48, device="cuda")
+    f = {"64 bits": f, "32 bits": f.float(), "a column": torch.stack((f, f / 2), 1)[:, 0]}[angles]
+    query, key = (torch.randn(70, heads, 64, generator=gen).to(dtype).cuda().requires_grad_() for heads in (6, 2))
+    grads = [torch.randn(t.shape, generator=gen).to(dtype).cuda().requires_grad_() for t in (query, key)]
+    own = torch.ops.autosage.rotary_positions(query, key, positions, f, True, 1.25)
+    want = autosage_amd.rotary_positions(query, key, positions, f, interleaved=True, magnitude=1.25)
+    found = []
+    for out in (own, want):
+        first = torch.autograd.grad(out, (query, key), grads, create_graph=True)
+        found.append((*out, *first, *torch.autograd.grad(first, grads, (query.detach(), key.detach()))))
+    assert all(torch.equal(a, b) for a, b in zip(*found))
