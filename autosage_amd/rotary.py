@@ -25,6 +25,7 @@ from .position import has_tangent
 MAX_WIDTH = 1024
 _DTYPES = {torch.float32: 0, **_native.DTYPES_16}
 _TwoStrides = ctypes.c_int64 * 2
+_NO_GRADIENT = "rotary_positions has no gradient for frequencies"
 
 
 def rotary_frequencies(dims: int, *, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
@@ -96,8 +97,7 @@ def _check(query, key, positions, frequencies) -> None:
              "frequencies must contain one entry per pair, and the pairs fit the width")
     for name, t in (("key", key), ("positions", positions), ("frequencies", frequencies)):
         _require(t is None or t.device == query.device, ValueError, f"{name} must be on the device of query")
-    _require(not (torch.is_grad_enabled() and frequencies.requires_grad), RuntimeError,
-             "rotary_positions has no gradient for frequencies")
+    _require(not (torch.is_grad_enabled() and frequencies.requires_grad), RuntimeError, _NO_GRADIENT)
     _require(not has_tangent(frequencies), RuntimeError, "rotary_positions has no derivative for frequencies")
 
 
@@ -238,6 +238,8 @@ SCHEMAS = {
 
 
 def _setup(ctx, inputs, output) -> None:
+    # the operator itself runs without a history, where nothing shows that there will be one
+    _require(not ctx.needs_input_grad[3], RuntimeError, _NO_GRADIENT)
     ctx.set_materialize_grads(False)
     # as the kernel reads them, which is not how they may have been given
     ctx.save_for_backward(*_plan(*inputs[2:4]))

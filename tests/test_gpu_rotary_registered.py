@@ -36,3 +36,15 @@ def test_gradients_of_converted_plans(dtype, at, angles):
         first = torch.autograd.grad(out, (query, key), grads, create_graph=True)
         found.append((*out, *first, *torch.autograd.grad(first, grads, (query.detach(), key.detach()))))
     assert all(torch.equal(a, b) for a, b in zip(*found))
+
+
+@pytest.mark.parametrize("trained", [False, True])
+def test_frequencies_have_no_gradient(trained):
+    query = torch.randn(70, 6, 64, device="cuda", requires_grad=trained)
+    frequencies = autosage_amd.rotary_frequencies(48, device="cuda").requires_grad_()
+    positions = torch.arange(70, device="cuda")
+    with pytest.raises(RuntimeError, match="no gradient for frequencies"):
+        torch.ops.autosage.rotary_positions(query, None, positions, frequencies)
+    with torch.no_grad():
+        out, _ = torch.ops.autosage.rotary_positions(query, None, positions, frequencies)
+    assert torch.equal(out, autosage_amd.rotary_positions(query.detach(), None, positions, frequencies.detach())[0])

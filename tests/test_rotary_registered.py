@@ -81,3 +81,18 @@ def test_positions_that_change_behind_the_call(operator):
             assert "modified by an inplace operation" in str(error)
         else:
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32])
+@pytest.mark.parametrize("trained", [False, True])
+def test_frequencies_have_no_gradient(operator, dtype, trained):
+    """Refused as by the public call, whether or not the rows are trained as well."""
+    query = torch.randn(5, 3, 8, dtype=torch.float64, requires_grad=trained)
+    frequencies = autosage_amd.rotary_frequencies(8).to(dtype).requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient for frequencies"):
+        operator(query, None, _positions("as they are"), frequencies)
+    with torch.no_grad():
+        out, _ = operator(query, None, _positions("as they are"), frequencies)
+    assert not out.requires_grad
+    out, _ = operator(query, None, _positions("as they are"), frequencies.detach())
+    assert out.requires_grad == trained
