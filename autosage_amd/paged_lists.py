@@ -176,6 +176,11 @@ def paged_cache_resize(page_table, lengths, change, free_pages, free_count, *, p
     ``rotary_positions``, and ``slots`` its page times ``page_size`` plus its place there.  Both are -1
     for padding and for sequences that are not served.
 
+    Rows stand one behind the other and sequences without a new token have none, but
+    ``paged_attention`` takes a query for every sequence: of queries that come as such rows
+    ``query[(token_ptr[1:] - 1).clamp(0, tokens - 1)]`` answers the sequences that grew, and the
+    results of all others belong to no query of theirs.
+
     ``page_table.view(-1)`` with ``page_ptr = arange(sequences + 1) * page_table.size(1)`` are the
     page lists of the cache's other calls."""
     return paged_cache_resize_impl(page_table, lengths, change, free_pages, free_count, page_size, tokens)
