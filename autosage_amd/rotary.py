@@ -204,6 +204,10 @@ class _RotaryTransformed(torch.autograd.Function):
     @staticmethod
     def vmap(info, in_dims, *inputs):
         rows, rest = inputs[:2], inputs[2:]
+        if info.batch_size == 0:
+            none = [None if x is None else (x.expand(0, *x.shape) if d is None else x.movedim(d, 0)).clone()
+                    for x, d in zip(rows, in_dims)]
+            return tuple(none), tuple(None if x is None else 0 for x in none)
         if in_dims[2] is None and in_dims[3] is None:
             # the batch's heads side by side
             flat = [x if d is None else x.movedim(d, 1).flatten(1, 2) for x, d in zip(rows, in_dims)]

@@ -48,3 +48,11 @@ def test_frequencies_have_no_gradient(trained):
     with torch.no_grad():
         out, _ = torch.ops.autosage.rotary_positions(query, None, positions, frequencies)
     assert torch.equal(out, autosage_amd.rotary_positions(query.detach(), None, positions, frequencies.detach())[0])
+
+
+def test_batches_of_none():
+    query, positions = torch.randn(0, 7, 3, 24, device="cuda"), torch.zeros(0, 7, dtype=torch.long, device="cuda")
+    f, one = autosage_amd.rotary_frequencies(16, device="cuda"), torch.randn(7, 3, 24, device="cuda")
+    rows = torch.vmap(lambda q: autosage_amd.rotary_positions(q, None, torch.arange(7, device="cuda"), f)[0])(query)
+    places = torch.vmap(lambda p: autosage_amd.rotary_positions(one, one, p, f))(positions)
+    assert rows.shape == (0, 7, 3, 24) and all(t.shape == (0, 7, 3, 24) and t.is_cuda for t in places)
