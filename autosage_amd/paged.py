@@ -399,7 +399,9 @@ def paged_cache_write(key, value, key_pages, value_pages, page_ptr, page_idx, to
     power of two for each 32 neighbouring numbers of a row, the smallest that brings the largest of
     them to 6; the numbers divided by it are rounded to 0, 1/2, 1, 3/2, 2, 3, 4 or 6, half to
     the even code. A number is off by at most a fifth of itself, or a quarter of its group's power
-    of two where that is more. A group with a number that is not finite is NaN as a whole.
+    of two where that is more. That may pass the largest number of a type: what is 57,344 or more
+    may be held as 65,536, which a read in float16 gives as infinity (and 2.98e38, 3.5 * 2^126, as 2^128, infinite
+    in every type and in the attention). A group with a number that is not finite is NaN as a whole.
 
     A token whose place has no page is not written.  Two tokens of one call must
     not share a place (``AUTOSAGE_VALIDATE=1`` checks it, with the lists)."""
