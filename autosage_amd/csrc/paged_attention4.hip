@@ -77,18 +77,22 @@ __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f
 enum Mode { kDense, kWhole, kTokens, kBytes };
 constexpr bool in_blocks(int mode) { return mode == kDense || mode == kWhole; }
 
-// Where a word (or half of one) of a row is read, and how far it is shifted then.
+// Where a word (or half of one) of a row is read, and which of its bytes are the word's: those that lie behind the row
+// count as zeros, for whatever is read in their place may stand for an infinite number, which a query's zero makes NaN.
 struct Word {
   int at;
-  int shift;
+  uint32_t bytes;  // as the byte permute has them: 0x0c is a zero
 };
+constexpr uint32_t kAllBytes = 0x03020100u;
+constexpr uint32_t kNoBytes = 0x0c0c0c0cu;
 template <int BYTES, int MODE>
 __device__ __forceinline__ Word word_of(int at, int row_bytes) {
-  if constexpr (MODE == kDense) return Word{at, 0};
-  if constexpr (MODE == kWhole) return Word{at < row_bytes ? at : 0, 0};
-  if (MODE == kBytes || at >= row_bytes) return Word{at < row_bytes ? at : 0, 0};
+  if constexpr (MODE == kDense || MODE == kBytes) return Word{at, kAllBytes};
+  if constexpr (MODE == kWhole) return Word{at < row_bytes ? at : 0, kAllBytes};
   const int last = row_bytes - BYTES;
-  return Word{at < last ? at : last, at < last ? 0 : 8 * (at - last)};
+  if (at <= last) return Word{at, kAllBytes};
+  const uint32_t over = at < row_bytes ? 8 * (at - last) : 32;
+  return Word{last, static_cast<uint32_t>(((uint64_t(kNoBytes) << 32) | kAllBytes) >> over)};
 }
 template <int BYTES, int MODE>
 __device__ __forceinline__ uint32_t load_word(const uint8_t* __restrict__ row, const Word& w, int row_bytes) {
@@ -100,11 +104,11 @@ __device__ __forceinline__ uint32_t load_word(const uint8_t* __restrict__ row, c
   } else if constexpr (BYTES == 2) {
     uint16_t x;
     __builtin_memcpy(&x, row + w.at, 2);
-    return in_blocks(MODE) ? x : x >> w.shift;
+    return in_blocks(MODE) ? x : __builtin_amdgcn_perm(0u, x, w.bytes);
   } else {
     uint32_t x;
     __builtin_memcpy(&x, row + w.at, 4);
-    return in_blocks(MODE) ? x : x >> w.shift;
+    return in_blocks(MODE) ? x : __builtin_amdgcn_perm(0u, x, w.bytes);
   }
 }
 
@@ -226,13 +230,16 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
   // tokens of this lane: the first of those it loads keys of (the other is 4 further), and of those it weighs
   const int key_token = (n >> 2) * 8 + (n & 3);
   const int own_token = g * kOwn;
-  // Words of a key and of a value, and their exponents.  A lane behind a row's end reads its beginning (or the last
-  // group's exponent): it has zeros on the queries' side, and columns that nobody asks for on the values'.
+  // Words of a key and of a value, and their exponents.  A lane behind a row's end reads its beginning: it has zeros on
+  // the queries' side (and codes of zero here, or an exponent that leaves them finite), and columns that nobody asks for
+  // on the values'.
   Word key_word[in_blocks(MODE) ? kKeyRuns : kSteps];
   int key_e_at[kKeyRuns];
+  bool key_there[kKeyRuns];
 #pragma unroll
   for (int j = 0; j < kKeyRuns; ++j) {
     const int d = (j * 4 + g) * kKeyRun;
+    key_there[j] = d < c.key.width;
     key_e_at[j] = MODE == kDense || d < c.key.width ? d / kGroup : 0;
     if constexpr (in_blocks(MODE)) {
       key_word[j] = word_of<4, MODE>(d / 2, key_bytes);
@@ -495,7 +502,8 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
           const uint32_t w = keys.codes[s][j];
-          const float scale = as_scale(keys.e[s][j / kKeyWords]);
+          const uint32_t e = keys.e[s][j / kKeyWords];
+          const float scale = as_scale(MODE == kWhole && !key_there[j / kKeyWords] ? 127u : e);
           const u32x4 k{bf16_pair<0>(w, scale), bf16_pair<1>(w, scale), bf16_pair<2>(w, scale), bf16_pair<3>(w, scale)};
 #pragma unroll
           for (int p = 0; p < kQ; ++p) score[s] = multiply(k, q_of(j, p), score[s]);
