@@ -77,38 +77,47 @@ __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f
 enum Mode { kDense, kWhole, kTokens, kBytes };
 constexpr bool in_blocks(int mode) { return mode == kDense || mode == kWhole; }
 
-// Where a word (or half of one) of a row is read, and which of its bytes are the word's: those that lie behind the row
-// count as zeros, for whatever is read in their place may stand for an infinite number, which a query's zero makes NaN.
+// Where a word (or half of one) of a row is read, and how far it is shifted then.
 struct Word {
   int at;
-  uint32_t bytes;  // as the byte permute has them: 0x0c is a zero
+  int shift;
 };
-constexpr uint32_t kAllBytes = 0x03020100u;
-constexpr uint32_t kNoBytes = 0x0c0c0c0cu;
 template <int BYTES, int MODE>
 __device__ __forceinline__ Word word_of(int at, int row_bytes) {
-  if constexpr (MODE == kDense || MODE == kBytes) return Word{at, kAllBytes};
-  if constexpr (MODE == kWhole) return Word{at < row_bytes ? at : 0, kAllBytes};
+  if constexpr (MODE == kDense || MODE == kBytes) return Word{at, 0};
+  if (MODE == kWhole || at >= row_bytes) return Word{at < row_bytes ? at : 0, 0};
   const int last = row_bytes - BYTES;
-  if (at <= last) return Word{at, kAllBytes};
-  const uint32_t over = at < row_bytes ? 8 * (at - last) : 32;
-  return Word{last, static_cast<uint32_t>(((uint64_t(kNoBytes) << 32) | kAllBytes) >> over)};
+  return Word{at < last ? at : last, at < last ? 0 : 8 * (at - last)};
+}
+// The same for a byte permute, of a key's words: those behind the row are zeros, for whatever is read in their place may
+// stand for an infinite number, which a query's zero makes NaN.  (Nobody asks for such columns of a value.)
+struct KeyWord {
+  int at;
+  uint32_t bytes;  // 0x0c is a zero
+};
+template <int MODE>
+__device__ __forceinline__ KeyWord key_word_of(int at, int row_bytes) {
+  constexpr uint32_t kAll = 0x03020100u;
+  constexpr uint32_t kNone = 0x0c0c0c0cu;
+  const Word w = word_of<4, MODE>(at, row_bytes);
+  if (MODE != kTokens) return KeyWord{w.at, kAll};
+  return KeyWord{w.at, at < row_bytes ? static_cast<uint32_t>(((uint64_t(kNone) << 32) | kAll) >> w.shift) : kNone};
 }
 template <int BYTES, int MODE>
-__device__ __forceinline__ uint32_t load_word(const uint8_t* __restrict__ row, const Word& w, int row_bytes) {
+__device__ __forceinline__ uint32_t load_word(const uint8_t* __restrict__ row, int at, int row_bytes) {
   if constexpr (MODE == kBytes) {
     uint32_t x = 0u;
 #pragma unroll
-    for (int i = 0; i < BYTES; ++i) x |= w.at + i < row_bytes ? uint32_t(row[w.at + i]) << (8 * i) : 0u;
+    for (int i = 0; i < BYTES; ++i) x |= at + i < row_bytes ? uint32_t(row[at + i]) << (8 * i) : 0u;
     return x;
   } else if constexpr (BYTES == 2) {
     uint16_t x;
-    __builtin_memcpy(&x, row + w.at, 2);
-    return in_blocks(MODE) ? x : __builtin_amdgcn_perm(0u, x, w.bytes);
+    __builtin_memcpy(&x, row + at, 2);
+    return x;
   } else {
     uint32_t x;
-    __builtin_memcpy(&x, row + w.at, 4);
-    return in_blocks(MODE) ? x : __builtin_amdgcn_perm(0u, x, w.bytes);
+    __builtin_memcpy(&x, row + at, 4);
+    return x;
   }
 }
 
@@ -233,7 +242,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
   // Words of a key and of a value, and their exponents.  A lane behind a row's end reads its beginning: it has zeros on
   // the queries' side (and codes of zero here, or an exponent that leaves them finite), and columns that nobody asks for
   // on the values'.
-  Word key_word[in_blocks(MODE) ? kKeyRuns : kSteps];
+  KeyWord key_word[in_blocks(MODE) ? kKeyRuns : kSteps];
   int key_e_at[kKeyRuns];
   bool key_there[kKeyRuns];
 #pragma unroll
@@ -242,10 +251,10 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
     key_there[j] = d < c.key.width;
     key_e_at[j] = MODE == kDense || d < c.key.width ? d / kGroup : 0;
     if constexpr (in_blocks(MODE)) {
-      key_word[j] = word_of<4, MODE>(d / 2, key_bytes);
+      key_word[j] = key_word_of<MODE>(d / 2, key_bytes);
     } else {
 #pragma unroll
-      for (int i = 0; i < kKeyWords; ++i) key_word[j * kKeyWords + i] = word_of<4, MODE>(d / 2 + 4 * i, key_bytes);
+      for (int i = 0; i < kKeyWords; ++i) key_word[j * kKeyWords + i] = key_word_of<MODE>(d / 2 + 4 * i, key_bytes);
     }
   }
   Word value_word[kBlocks];
@@ -368,7 +377,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
         } else {
 #pragma unroll
           for (int i = 0; i < kKeyWords; ++i)
-            keys.codes[s][j * kKeyWords + i] = load_word<4, MODE>(row, key_word[j * kKeyWords + i], key_bytes);
+            keys.codes[s][j * kKeyWords + i] = load_word<4, MODE>(row, key_word[j * kKeyWords + i].at, key_bytes);
         }
         keys.e[s][j] = row_e[key_e_at[j]];
       }
@@ -376,7 +385,8 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
     const auto load_value = [&](Values& values, int e, const uint8_t* row, const uint8_t* row_e) {
 #pragma unroll
       for (int j = 0; j < kBlocks; ++j) {
-        values.codes[j][e] = load_word<kRun / 2, MODE>(row, value_word[j], value_bytes);
+        const uint32_t x = load_word<kRun / 2, MODE>(row, value_word[j].at, value_bytes);
+        values.codes[j][e] = MODE == kTokens ? x >> value_word[j].shift : x;
         values.e[j][e] = row_e[value_e_at[j]];
       }
     };
@@ -501,7 +511,9 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
         score[s] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < kSteps; ++j) {
-          const uint32_t w = keys.codes[s][j];
+          // where it is used: in front of that it would be waited for
+          uint32_t w = keys.codes[s][j];
+          if constexpr (MODE == kTokens) w = __builtin_amdgcn_perm(0u, w, key_word[j].bytes);
           const uint32_t e = keys.e[s][j / kKeyWords];
           const float scale = as_scale(MODE == kWhole && !key_there[j / kKeyWords] ? 127u : e);
           const u32x4 k{bf16_pair<0>(w, scale), bf16_pair<1>(w, scale), bf16_pair<2>(w, scale), bf16_pair<3>(w, scale)};
