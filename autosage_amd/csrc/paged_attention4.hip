@@ -16,7 +16,9 @@
 //     power of two is a number of bf16, so that neither scores nor weights are scaled
 //     afterwards, and an exponent of NaN makes NaN.  Numbers below 2^-126 count as zeros.
 //   * queries enter in bf16 parts: one for bf16, two for fp16, three for float32, which
-//     hold all of their bits; weights in two (2^-18 of a weight), or three for float32.
+//     hold all of their bits and have one sign; weights in two (2^-18 of a weight), or
+//     three for float32.  So a key that is held as 2^128 makes an infinite score, and such
+//     a value NaN.
 //
 // A row of 128 is 68 bytes, half of an 8-bit one, and each of its numbers costs a vector
 // instruction or so: what bounds the kernel is how many loads are on the way while they
@@ -54,6 +56,18 @@ __device__ __forceinline__ uint32_t pack(float x, float y) {
 }
 __device__ __forceinline__ f32x2 unpack(uint32_t w) {
   return f32x2{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+}
+// The same cut to the word's bits (a NaN has its highest bit set after any product, and stays one).
+__device__ __forceinline__ uint32_t cut(float x, float y) {
+  return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+}
+// What is left of x for the next part.  All parts have to make one infinity of a number that is held as 2^128: so they are
+// cut, which leaves the rest with x's sign, and where nothing is left, or x is infinite itself, the rest is 2^-40 of the
+// first part (a zero only for a zero, and for queries below 2^-86).
+constexpr float kLeast = 1.0f / (1024.0f * 1024.0f * 1024.0f * 1024.0f);
+__device__ __forceinline__ float next_part(float x, float held, float least) {
+  const float rest = x - held;
+  return __builtin_islessgreater(rest, 0.0f) ? rest : least;
 }
 // The numbers 2i and 2i + 1 of a word of codes, times 2^(e - 127) for scale = e << 23; NaN for e = 255.
 template <int I>
@@ -313,16 +327,17 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
             q[i] = d < key_width && n < heads_here ? x * q_sign : 0.0f;
           }
         }
+        f32x2 least[4];
 #pragma unroll
         for (int p = 0; p < kQ; ++p) {
           u32x4 words;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            words[i] = pack(q[2 * i], q[2 * i + 1]);
-            // what the next part holds; nothing is left of an infinite number
+            words[i] = kQ == 1 ? pack(q[2 * i], q[2 * i + 1]) : cut(q[2 * i], q[2 * i + 1]);
             const f32x2 held = unpack(words[i]);
-            q[2 * i] = finite(held[0]) ? q[2 * i] - held[0] : 0.0f;
-            q[2 * i + 1] = finite(held[1]) ? q[2 * i + 1] - held[1] : 0.0f;
+            if (p == 0) least[i] = f32x2{held[0] * kLeast, held[1] * kLeast};
+            q[2 * i] = next_part(q[2 * i], held[0], least[i][0]);
+            q[2 * i + 1] = next_part(q[2 * i + 1], held[1], least[i][1]);
           }
           if constexpr (!kShared) {
             q_own[j][p] = words;

@@ -401,7 +401,7 @@ def paged_cache_write(key, value, key_pages, value_pages, page_ptr, page_idx, to
     the even code. A number is off by at most a fifth of itself, or a quarter of its group's power
     of two where that is more. That may pass the largest number of a type: what is 57,344 or more
     may be held as 65,536, which a read in float16 gives as infinity (and 2.98e38, 3.5 * 2^126, as 2^128, infinite
-    in every type and in the attention). A group with a number that is not finite is NaN as a whole.
+    in every type). A group with a number that is not finite is NaN as a whole.
 
     A token whose place has no page is not written.  Two tokens of one call must
     not share a place (``AUTOSAGE_VALIDATE=1`` checks it, with the lists)."""
@@ -615,7 +615,8 @@ def paged_attention(query, key_pages, value_pages, page_ptr, page_idx, lengths, 
     Scores, softmax and sums are float32 and the result is rounded once to the
     dtype of ``query``.  (Over 8-bit pages a query is multiplied with the codes,
     so that finite numbers beyond 2^111 may give infinite scores.  On the GPU
-    numbers of 4-bit pages below 2^-126 count as zeros.)  A sequence without
+    numbers of 4-bit pages below 2^-126 count as zeros, as weights below it do, and a value
+    that is held as 2^128 makes NaN of its column where the CPU makes an infinity.)  A sequence without
     tokens, or with scores of -inf alone, gives zeros; a length beyond ``max_length`` or the sequence's pages, or a
     page id outside the cache, gives NaN.  ``return_lse`` adds the logarithm of
     the sum of the exponentials, float32 ``[sequences, query heads]``, with which

@@ -1,5 +1,6 @@
 """Attention over 4-bit pages that hold infinite numbers (what is written from 3.5 * 2^126 on), against the CPU composition:
-a score of -inf takes no weight, one of +inf makes its head NaN, and an infinite value makes its column infinite."""
+a score of -inf takes no weight, one of +inf makes its head NaN, and an infinite value makes its column infinite (NaN on the
+GPU), and all others stay as they are.  Queries next to their type's largest number stay finite."""
 
 from __future__ import annotations
 
@@ -12,7 +13,7 @@ from tests.paged4_common import E2M1, E8M0
 
 pytestmark = pytest.mark.gpu
 
-DTYPES = [torch.bfloat16]
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 HUGE = 3.2e38  # held as 2^128
 # rows that fill the kernel's width, whole groups, parts of groups, parts of words, rows of single bytes
 WIDTHS = [64, 128, 256, 32, 96, 160, 40, 72, 34, 130, 200, 6]
@@ -82,3 +83,66 @@ def test_keys_whose_score_is_minus_infinity(dtype, page, width):
     want = _check(held, query, scale=0.1)
     assert want.isfinite().all() and not want[2, 2:].any() and want[2, :2].any()
     _check(held, query, scale=0.1, max_length=300)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 12])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_keys_whose_score_is_infinite(dtype, page, width):
+    """Numbers of the query that fill one part of it (0.5), two or three (1/3), or are negative; a query's zero makes NaN."""
+    held = Held([40, 300], 2, width, 64, page, seed=width)
+    query = torch.randn(2, 8, width, generator=held.gen)
+    # heads 0 to 3 have the first key head: +inf, -inf, -inf, NaN
+    for head, first in enumerate((-0.5, 0.5, 1.0 / 3.0, 0.0)):
+        query[:, head, 0] = first
+    held.rows[0][5, 0, 0] = -HUGE
+    held.rows[0][77, 0, 0] = -HUGE
+    want = _check(held, query.to(dtype), scale=0.1)
+    assert want[:, [0, 3]].isnan().all() and want[:, [1, 2, 4, 5, 6, 7]].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [16, 12])
+@pytest.mark.parametrize("width", WIDTHS)
+def test_infinite_values(dtype, page, width):
+    held = Held([40, 300], 2, 64, width, page, seed=width)
+    query = torch.randn(2, 4, 64, generator=held.gen).to(dtype)
+    plain, _ = held.attend(query, "cuda", scale=0.1)
+    spoilt = list(held.rows)
+    for sign in (1, -1):
+        held.rows = [spoilt[0], spoilt[1].clone()]
+        held.rows[1][7, 1, width - 1] = sign * HUGE  # the other numbers of its group become zeros
+        out, lse = held.attend(query, "cuda", scale=0.1)
+        want, want_lse = held.attend(query, "cpu", scale=0.1)
+        assert torch.equal(out.isfinite(), want.isfinite()) and not want[0, 2:, width - 1].isfinite().any()
+        assert int((~want.isfinite()).sum()) == 2 and torch.allclose(lse, want_lse, rtol=2.0**-20, atol=2e-4)
+        assert torch.equal(out[1], plain[1]) and torch.equal(out[0, :2], plain[0, :2])
+        keep = want.isfinite()
+        assert torch.allclose(out[keep].double(), want[keep].double(), rtol=torch.finfo(dtype).eps, atol=8 * 2.0**-16)
+
+
+@pytest.mark.parametrize("page", [16, 12])
+@pytest.mark.parametrize("width", [64, 128, 96, 40, 256])
+def test_the_largest_queries_stay_finite(page, width):
+    """Numbers that bf16 would round to infinity, times keys of some 2^-122."""
+    held = Held([40, 300], 2, width, 64, page, seed=width)
+    held.rows[0][:, :, :32] *= 2.0**-122
+    query = torch.randn(2, 4, width, generator=held.gen)
+    query[:, :, :32] = 0.0
+    query[:, :, 3], query[:, :, 7] = torch.finfo(torch.float32).max, -3.4e38
+    want = _check(held, query, scale=0.02)
+    assert want.isfinite().all()
+
+
+@pytest.mark.parametrize("width", [64, 40, 200])
+@pytest.mark.parametrize("dtype, bits", [(torch.float32, 0x7F800001), (torch.float32, -1), (torch.float16, 0x7C01),
+                                         (torch.bfloat16, 0x7F81)])
+def test_every_nan_of_a_query_stays_one(dtype, bits, width):
+    """Also one whose only bits are those that a shorter type has not."""
+    held = Held([40, 300], 1, width, 64, 16, seed=width)
+    query = torch.randn(2, 3, width, generator=held.gen).to(dtype)
+    query.view(torch.int32 if dtype == torch.float32 else torch.int16)[0, 1, 9] = bits
+    assert query.isnan().sum() == 1
+    out, lse = held.attend(query, "cuda", scale=0.1)
+    assert out[0, 1].isnan().all() and lse[0, 1].isnan()
+    assert int(out.isnan().sum()) == 64 and int(lse.isnan().sum()) == 1
