@@ -522,7 +522,8 @@ paged_attention_kernel(AttentionArgs a, PositionMap map) {
       if (__any(most > top + kSlack)) {
         most = fmaxf(most, __shfl_xor(most, 16, 64));
         most = fmaxf(most, __shfl_xor(most, 32, 64));
-        const float next = fmaxf(top, most);
+        // each head decides for itself, so that its result does not depend on the others'
+        const float next = most > top + kSlack ? most : top;
         const float keep = top == -INFINITY ? 0.0f : exp_of(top - next);
         top = next;
         sum *= keep;

@@ -580,7 +580,8 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(kWavesPe
       if (__any(most > top + kSlack)) {
         most = fmaxf(most, __shfl_xor(most, 16, 64));
         most = fmaxf(most, __shfl_xor(most, 32, 64));
-        const float next = fmaxf(top, most);
+        // each head decides for itself, so that its result does not depend on the others'
+        const float next = most > top + kSlack ? most : top;
         const float keep = top == -INFINITY ? 0.0f : exp_of(top - next);
         top = next;
         sum *= keep;
