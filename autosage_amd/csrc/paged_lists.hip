@@ -441,6 +441,15 @@ int as_paged_cache_resize(int64_t* table, int64_t table_stride, int64_t room, co
   if (workspace_bytes < bytes || (bytes > 0 && workspace == nullptr))
     return fail(AS_ERR_WORKSPACE, "page lists need %zu workspace bytes", bytes);
   if (!aligned(workspace, 8)) return fail(AS_ERR_INVALID_ARGUMENT, "the workspace must be 8-byte aligned");
+  // later launches read lengths and changes again
+  for (const int64_t* const from : {lengths, change}) {
+    const auto apart = [&](const int64_t* to, int64_t count, int64_t read) {
+      return count == 0 || read == 0 || to + count <= from || from + read <= to;
+    };
+    if (!apart(new_lengths, sequences, sequences) || !apart(token_ptr, sequences + 1, sequences) ||
+        !apart(positions, tokens, sequences) || !apart(slots, tokens, sequences))
+      return fail(AS_ERR_INVALID_ARGUMENT, "the results must lie apart from lengths and change");
+  }
   int64_t* const ws = static_cast<int64_t*>(workspace);
   const int tiles = static_cast<int>(tiles_of(sequences));
   ListArgs a{};

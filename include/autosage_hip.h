@@ -842,6 +842,7 @@ int as_paged_attention(const as_paged_cache* cache, const void* query,
  * new_lengths [sequences]; token_ptr [sequences + 1]: the sums of the positive
  * changes; positions and slots [tokens]: of the tokens that come, their place in
  * the sequence and page * page_size + place in the page, -1 where there is none.
+ * These results lie apart from lengths and change.
  * Nothing outside the given tensors is read or written whatever they hold. */
 int as_paged_cache_resize(int64_t* table, int64_t table_stride, int64_t room,
                           const int64_t* lengths, const int64_t* change,
