@@ -88,12 +88,14 @@ __device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f
 // of a row is read where it ends with the row, and shifted.  kBytes: so it is, and words
 // are read a byte at a time, for rows of fewer than 4 bytes.
 //
-// 64 sequences of up to 8,192 tokens, 8 key heads, bf16: kDense, rows of 128, 77 us on a floor of 64, by
-// memory.  kWhole, rows of 96, 99 on 48: addresses that are no constants apart and columns that are not there
-// are 28M vector instructions instead of 23M (45 us of the ALUs), and leave registers for two workgroups a CU and not
-// three.  kTokens, rows of 80 in pages of 16 143 on 40, of 128 in pages of 12 152 on 64: a lane's 10 tokens looked up one by
-// one and shifted words are 50M (82 us) and 2.9M loads for 1.7M (75 us of the address units).  Of the two conditions
-// that lead there the page's is the one that a block of 8 tokens needs; rows of parts of 32 in pages of 8 only share the mode.
+// 64 sequences of up to 8,192 tokens, 8 key heads, bf16.  kDense, rows of 128: 79 us on a floor
+// of 64, bound by memory.  kWhole, rows of 96: 99 on 48; addresses that are no constants apart
+// and columns that are not there make 28M vector instructions of 23M (46 us of the ALUs), and
+// leave registers for two workgroups a CU, not three.  kTokens, rows of 80 in pages of 16: 144
+// on 40, of 128 in pages of 12: 152 on 64; ten tokens a lane that are looked up one by one, and
+// shifted words, make 50M (82 us) and 2.9M loads of 1.7M (75 us of the address units).  Of the
+// two conditions that lead there a block of 8 tokens needs the page's alone: rows that are no
+// multiple of 32 in pages of 8 only share the mode.
 enum Mode { kDense, kWhole, kTokens, kBytes };
 constexpr bool in_blocks(int mode) { return mode == kDense || mode == kWhole; }
 
